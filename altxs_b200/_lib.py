@@ -16,6 +16,7 @@ ALTXS_OK = 0
 ALTXS_EINVAL, ALTXS_ENOSPC, ALTXS_ENOTSUP, ALTXS_ECUDA, ALTXS_ENOMEM = -22, -28, -95, -5, -12
 ST_OVERFLOW, ST_BAD_SYMBOL, ST_BAD_TOTAL, ST_NONFINITE, ST_TIMEOUT, ST_BAD_POS = 1, 2, 4, 8, 16, 32
 CDF_FIXED, CDF_REF = 0, 1
+F32, BF16, F16 = 0, 1, 2
 STEP_LOGITS, STEP_ENCODE, STEP_DECODE = 0, 1, 2
 
 EXPORTS = (
@@ -36,9 +37,10 @@ EXPORTS = (
     "altxs_create", "altxs_load_weights", "altxs_set_adapters", "altxs_set_ttt", "altxs_set_segment",
     "altxs_streams_init", "altxs_step_encode", "altxs_step_decode", "altxs_ttt_boundary", "altxs_flush",
     "altxs_begin_decode", "altxs_get_status", "altxs_ctx_words_per_stream", "altxs_destroy",
+    "altxs_rope", "altxs_paged_append", "altxs_paged_attention_workspace_bytes", "altxs_paged_attention",
 )
 KERNEL_CLASSES = ("embed", "prenorm", "linear", "qkv_post", "attn_partial", "attn_merge", "post_attn",
-                  "final_norm", "cdf_code", "coder", "ttt", "fused_step")
+                  "final_norm", "cdf_code", "coder", "ttt", "fused_step", "rope", "paged")
 
 
 class AcState(C.Structure):
@@ -111,6 +113,23 @@ class TttHparams(C.Structure):
 class DenseWeights(C.Structure):
     _fields_ = [("emb", C.c_void_p), ("qkv", C.c_void_p), ("o", C.c_void_p), ("up", C.c_void_p),
                 ("down", C.c_void_p)]
+
+
+class RotaryTables(C.Structure):
+    _fields_ = [("cos", C.c_void_p), ("sin", C.c_void_p), ("positions", C.c_int64), ("dims", C.c_int32),
+                ("interleaved", C.c_int32)]
+
+
+class PagedKv(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("page_stride", C.c_int64), ("token_stride", C.c_int64),
+                ("head_stride", C.c_int64), ("dtype", C.c_int32), ("page_size", C.c_int32), ("n_pages", C.c_int32),
+                ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32)]
+
+
+class Chunks(C.Structure):
+    _fields_ = [("q_start", C.c_void_p), ("kv_len", C.c_void_p), ("page_table", C.c_void_p),
+                ("table_stride", C.c_int64), ("n_seqs", C.c_int32), ("n_tokens", C.c_int32),
+                ("max_new", C.c_int32), ("max_kv", C.c_int32), ("total_kv", C.c_int64), ("status", C.c_void_p)]
 
 
 class Batch(C.Structure):
@@ -202,6 +221,13 @@ def lib():
             "altxs_get_status": (C.c_int, [vp, vp]),
             "altxs_ctx_words_per_stream": (i64, [vp]),
             "altxs_destroy": (None, [vp]),
+            "altxs_rope": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(RotaryTables), vp, C.c_int, vp, i64,
+                                     vp, i64, vp, vp]),
+            "altxs_paged_append": (C.c_int, [C.POINTER(PagedKv), C.POINTER(Chunks), C.POINTER(RotaryTables), vp, vp,
+                                             i64, vp, i64, C.c_int, vp, i64, vp, i64, vp]),
+            "altxs_paged_attention_workspace_bytes": (i64, [C.POINTER(PagedKv), C.POINTER(Chunks), C.c_int, C.c_int]),
+            "altxs_paged_attention": (C.c_int, [C.POINTER(PagedKv), C.POINTER(Chunks), C.c_int, C.c_float, C.c_int, vp,
+                                                i64, vp, i64, vp, vp, i64, vp]),
             "altxs_full_workspace_bytes": (i64, [C.POINTER(ModelDesc), C.c_int]),
             "altxs_full_loss_grad": (C.c_int, [C.POINTER(ModelDesc), C.POINTER(Weights), C.POINTER(DenseWeights), vp,
                                                C.c_int, C.c_int, vp, vp, vp, i64, vp]),

@@ -21,6 +21,8 @@ enum KernelClass : int {
     kKCoder,
     kKTtt,
     kKFused,
+    kKRope,
+    kKPaged,
     kKNumClasses
 };
 

@@ -484,6 +484,104 @@ int altxs_params_anchor(int64_t n, float *p, const float *w0, const float *pull,
 int altxs_split_params(const altxs_model_desc *desc, const float *params, const altxs_split_planes *planes,
                        altxs_stream_t stream);
 
+/* ---- paged key/value cache ----------------------------------------------------
+ * A cache of fixed-size pages for streams of different lengths: a page holds
+ * page_size positions of one sequence, a page table per sequence says which
+ * page holds which block of positions, so a stream occupies what it has coded
+ * instead of a whole ring (altxs_batch.kv).  Three calls work on it: the
+ * rotary positions on their own, the append of new tokens (keys rotated on the
+ * way), and the attention of those tokens over everything cached.  The
+ * reference keeps one contiguous static cache per stream and runs its
+ * encoder's 64-symbol windows over it (StaticACEngine, altxs
+ * src/xsa_ttt/incremental.py:203-1218, run_window :1268-1290; GPT.static_extend,
+ * model.py:1617-1781).
+ *
+ * Types: activations and cache share one type, fp32, bf16 or fp16; sums, the
+ * softmax and the rotation are fp32 and rounded once at the end.  Data errors
+ * never fault: a position or a page out of range sets ALTXS_ST_BAD_POS in the
+ * caller's status word (a device word, NULL = not wanted), the access is
+ * skipped, and what depends on it is said at each call. */
+#define ALTXS_F32 0
+#define ALTXS_BF16 1
+#define ALTXS_F16 2
+
+/* cos/sin of position x frequency.  A pair (a, b) of channels becomes
+ * (a cos + b sin, b cos - a sin), the sense of the engine's step (the
+ * reference's apply_rotary_emb, model.py); interleaved pairs are channels (2j, 2j+1), else
+ * (j, j + dims/2); channels from dims on pass through.  A table whose entries
+ * carry a common amplitude factor (long-context scaling) is applied as it is. */
+typedef struct altxs_rotary {
+    const float *cos, *sin; /* device [positions][dims/2], 16-byte aligned */
+    int64_t positions;
+    int32_t dims; /* even, <= head_dim */
+    int32_t interleaved;
+} altxs_rotary;
+
+/* y = R(pos) x on [n_tokens][n_heads] heads (head h of a token at column
+ * h*head_dim; row strides ldx, ldy in elements; x == y with ldx == ldy rotates
+ * in place, any other overlap is not allowed).  backward: the product with the
+ * transpose of R, i.e. dx from dy.  pos: device [n_tokens].  head_dim even, at
+ * most 512.  A token whose position is outside the table gets NaN. */
+int altxs_rope(int dtype, int n_tokens, int n_heads, int head_dim, const altxs_rotary *r, const int64_t *pos,
+               int backward, const void *x, int64_t ldx, void *y, int64_t ldy, uint32_t *status,
+               altxs_stream_t stream);
+
+/* Pages of keys and values: position slot t, head g of page p starts at
+ * p*page_stride + t*token_stride + g*head_stride elements from k (and v);
+ * channels are contiguous.  16-byte aligned, strides multiples of 16 bytes, so
+ * both [page][slot][head][channel] and [page][head][slot][channel] pools, and
+ * pools that interleave k and v, are addressed as they lie.  page_size >= 1;
+ * head_dim 32, 64 or 128 (else ALTXS_ENOTSUP). */
+typedef struct altxs_paged_kv {
+    void *k, *v;
+    int64_t page_stride, token_stride, head_stride;
+    int32_t dtype, page_size, n_pages, n_kv_heads, head_dim;
+} altxs_paged_kv;
+
+/* The new tokens of a batch of sequences.  Sequence s owns rows q_start[s] ..
+ * q_start[s+1] of the token arrays; they are the last of its kv_len[s]
+ * positions (kv_len counts them).  Entry b of its page-table row holds
+ * positions b*page_size ..; entries of blocks that no new token sees are not
+ * read.  max_new and max_kv bound the device lengths on the host side; a
+ * sequence outside its bounds (or with rows outside [0, n_tokens)) sets
+ * ALTXS_ST_BAD_POS and is left out. */
+typedef struct altxs_chunks {
+    const int32_t *q_start;    /* device [n_seqs + 1] */
+    const int32_t *kv_len;     /* device [n_seqs] */
+    const int32_t *page_table; /* device [n_seqs][table_stride] */
+    int64_t table_stride;      /* entries; table_stride * page_size >= max_kv */
+    int32_t n_seqs, n_tokens, max_new, max_kv;
+    int64_t total_kv; /* bound on the sum of kv_len (sizes the workspace); 0 = n_seqs * max_kv */
+    uint32_t *status; /* device word or NULL */
+} altxs_chunks;
+
+/* Writes the new tokens' keys (rotated when r is given) and values to their
+ * pages and, with q, the rotated queries of n_heads heads to q_out (q_out == q
+ * with equal strides rotates in place).  k, v: [n_tokens] rows of n_kv_heads
+ * heads.  pos: device [n_tokens] rotary positions, NULL = the cache positions.
+ * A token with a negative cache position or a page out of range is not
+ * stored; one whose rotary position is outside the table is not stored and
+ * its query row becomes NaN. */
+int altxs_paged_append(const altxs_paged_kv *kv, const altxs_chunks *c, const altxs_rotary *r, const int64_t *pos,
+                       const void *k, int64_t ldk, const void *v, int64_t ldv, int n_heads, const void *q,
+                       int64_t ldq, void *q_out, int64_t ldqo, altxs_stream_t stream);
+
+/* out[i][h] = sum_j softmax_j(scale * q[i][h] . K_j) V_j over the cached
+ * positions j of token i's sequence with j <= pos(i) and, with window > 0,
+ * j > pos(i) - window; query head h reads key/value head h / (n_heads /
+ * n_kv_heads).  A token that sees nothing (negative position) gets zeros.
+ * lse: optional device [n_heads][n_tokens], log2 of each row's sum of
+ * 2^(scale * log2(e) * q . K) (-inf for a row that sees nothing).  Positions on
+ * a page out of range (ALTXS_ST_BAD_POS) count as unseen.  A row's result does
+ * not depend on the other sequences of the call.  The workspace (16-byte
+ * aligned) must be zeroed before its first use; a call leaves it ready for the
+ * next one on the same stream, of any shape it is large enough for. */
+int64_t altxs_paged_attention_workspace_bytes(const altxs_paged_kv *kv, const altxs_chunks *c, int n_heads,
+                                              int window);
+int altxs_paged_attention(const altxs_paged_kv *kv, const altxs_chunks *c, int n_heads, float scale, int window,
+                          const void *q, int64_t ldq, void *out, int64_t ldo, float *lse, void *workspace,
+                          int64_t workspace_bytes, altxs_stream_t stream);
+
 /* ---- runtime context ----------------------------------------------------------
  * A handle over the calls above for callers that want the engine's state kept
  * for them: the reference's compress_full_sha_incremental /
@@ -605,7 +703,8 @@ int altxs_profile(int enable);
  * n_classes, the summed duration ms[c] and launch count counts[c].  Classes:
  * 0 embed, 1 prenorm, 2 mixed-bit linear, 3 qkv post, 4 attention partials,
  * 5 attention merge, 6 post-attention, 7 final norm, 8 logits->CDF->coder,
- * 9 standalone coder, 10 test-time LoRA.  Returns the number of pairs read. */
+ * 9 standalone coder, 10 test-time LoRA, 11 fused step, 12 rotary positions
+ * and paged append, 13 paged attention.  Returns the number of pairs read. */
 int altxs_profile_read(int n_classes, double *ms, int64_t *counts);
 
 /* Restrict recording to the classes whose bit is set in mask (bit c = class

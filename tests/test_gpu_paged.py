@@ -1,0 +1,554 @@
+"""Paged cache on the GPU: rotary positions, append and attention of new tokens
+against plain restatements in 64 bits.
+
+Tolerances, from the arithmetic: a value rounded once to b significand bits is
+within 2^-b of it relatively.  The rotation is two fp32 products and a sum of
+values of size |x|, then one rounding: 2^-22 |x|max (fp32), 2^-8 (bf16), 2^-11
+(fp16) of |x|max sqrt(2).  The attention's output is a mean of V rows: fp32
+scores of up to ~40 (log2 units) carry 40 x 2^-21 from products kept to 22 bits
+and the exponential's 2^-22, so 4e-5 |V|max covers p's relative error; in 16
+bits p is rounded once (2^-9, 2^-12) and the result once more, and q, k, v are
+the inputs' own: 2^-8 and 2^-11 of |V|max with half as much again for the
+scores.  The row sums' log2 is fp32: 4e-5 absolute.
+"""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from altxs_b200 import _lib, paged
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda")
+DT = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+ROT_TOL = {"f32": 2.0 ** -22, "bf16": 2.0 ** -8, "f16": 2.0 ** -11}
+ATT_TOL = {"f32": 4e-5, "bf16": 1.5 * 2.0 ** -8, "f16": 1.5 * 2.0 ** -11}
+LSE_TOL = 4e-5
+
+
+def _gen(seed):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    return g
+
+
+def _rand(g, *shape):
+    return torch.randn(*shape, generator=g, device=DEV)
+
+
+def _rot_ref(x, cos, sin, pos, il, backward=False):
+    """The rotation pair by pair in 64 bits, as matrices [[c, s], [-s, c]] (transposed backward)."""
+    x = x.double().clone()
+    d = 2 * cos.shape[1]
+    c, s = cos.double()[pos][:, None], sin.double()[pos][:, None]
+    if backward:
+        s = -s
+    j = torch.arange(d // 2, device=x.device)
+    ia, ib = (2 * j, 2 * j + 1) if il else (j, j + d // 2)
+    a, b = x[..., ia].clone(), x[..., ib].clone()
+    x[..., ia], x[..., ib] = c * a + s * b, c * b - s * a
+    return x
+
+
+def _table(n, dims):
+    return paged.rope_table(n, dims, device=DEV)
+
+
+# ---- rotary positions ----------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("il", [False, True])
+@pytest.mark.parametrize("T,H,hd,dims,lead", [(1, 1, 2, 2, 0), (1, 3, 32, 8, 0), (7, 5, 64, 16, 64), (130, 8, 128, 128, 3),
+                                               (33, 2, 96, 48, 0), (5, 1, 512, 512, 8), (300, 1, 64, 0, 0), (3, 7, 30, 14, 1)])
+def test_rope_forward_and_backward(dtype, il, T, H, hd, dims, lead):
+    g = _gen(T * 31 + hd)
+    cos, sin = _table(5000, dims)
+    rot = paged.Rotary(cos, sin, il)
+    wide = _rand(g, T, lead + H * hd + 5).to(DT[dtype])
+    x = wide[:, lead:lead + H * hd].unflatten(1, (H, hd))
+    pos = torch.randint(0, 5000, (T,), generator=g, device=DEV)
+    for back, f in ((False, paged.rope), (True, paged.rope_backward)):
+        want = _rot_ref(x, cos, sin, pos, il, back)
+        y = f(x, rot, pos)
+        err = (y.double() - want).abs().max().item()
+        assert err <= ROT_TOL[dtype] * math.sqrt(2) * x.abs().max().item()
+    assert torch.equal(y[..., dims:], x[..., dims:])
+    # in place through the same strided view: same bits, and nothing outside the view changes
+    keep, y = wide.clone(), paged.rope(x, rot, pos)
+    paged.rope(x, rot, pos, out=x)
+    assert torch.equal(x, y)
+    assert torch.equal(wide[:, :lead], keep[:, :lead]) and torch.equal(wide[:, lead + H * hd:], keep[:, lead + H * hd:])
+    rot.check_status()
+
+
+@pytest.mark.parametrize("il", [False, True])
+def test_rope_backward_is_the_gradient(il):
+    """Against differences: the loss sum(c * rope(x)) changes by <rope_backward(c), e> along every e
+    (the map is linear, so the quotient is exact up to rounding)."""
+    g = _gen(3)
+    cos, sin = _table(100, 12)
+    rot = paged.Rotary(cos, sin, il)
+    x, c = _rand(g, 2, 1, 16), _rand(g, 2, 1, 16)
+    pos = torch.tensor([17, 99], device=DEV)
+    grad = paged.rope_backward(c, rot, pos)
+    base = (c * paged.rope(x, rot, pos)).double().sum()
+    for i in range(x.numel()):
+        e = torch.zeros_like(x)
+        e.view(-1)[i] = 1.0
+        diff = (c * paged.rope(x + e, rot, pos)).double().sum() - base
+        assert abs(diff.item() - grad.reshape(-1)[i].item()) < 32 * 2.0 ** -21
+    xg = x.double().requires_grad_()
+    (_autograd_rot(xg, cos, sin, pos, il) * c).sum().backward()
+    assert (xg.grad - grad).abs().max().item() < 2.0 ** -20
+
+
+def _autograd_rot(x, cos, sin, pos, il):
+    d = 2 * cos.shape[1]
+    c, s = cos.double()[pos][:, None], sin.double()[pos][:, None]
+    a, b = (x[..., 0:d:2], x[..., 1:d:2]) if il else (x[..., :d // 2], x[..., d // 2:d])
+    u, v = a * c + b * s, b * c - a * s
+    r = torch.stack((u, v), -1).flatten(-2) if il else torch.cat((u, v), -1)
+    return torch.cat((r, x[..., d:]), -1)
+
+
+def test_rope_position_outside_the_table():
+    cos, sin = _table(10, 16)
+    rot = paged.Rotary(cos, sin)
+    x = _rand(_gen(1), 4, 2, 32)
+    y = paged.rope(x, rot, torch.tensor([0, 10, -1, 9], device=DEV))
+    assert torch.isnan(y[1:3]).all() and torch.isfinite(y[[0, 3]]).all()
+    with pytest.raises(RuntimeError, match="status 0x20"):
+        rot.check_status()
+    rot.check_status()
+
+
+def test_rope_matches_the_engine_tables():
+    """The engine's own tables and sense: the step's rotation of a head."""
+    from altxs_b200.config import c3_config
+    from altxs_b200.lora import rope_tables
+
+    cfg = c3_config()
+    cos, sin = (torch.from_numpy(a).to(DEV) for a in rope_tables(cfg, 64))
+    x = _rand(_gen(2), 3, cfg.num_heads, cfg.head_dim)
+    pos = torch.tensor([0, 5, 63], device=DEV)
+    y = paged.rope(x, paged.Rotary(cos, sin), pos)
+    h = cfg.rope_dims // 2
+    x1, x2, c, s = x[..., :h], x[..., h:2 * h], cos[pos][:, None], sin[pos][:, None]
+    want = torch.cat((x1 * c + x2 * s, x1 * -s + x2 * c, x[..., 2 * h:]), -1)
+    assert (y - want).abs().max().item() < 1e-6
+
+
+# ---- a batch of sequences over a paged cache --------------------------------------
+
+
+class Batch:
+    """Random sequences in a random page order; unheld pages and slots past a
+    sequence's length hold NaN."""
+
+    def __init__(self, dtype, hd, Hkv, P, news, kvs, seed=0, layout="nhd", spare=2):
+        g = _gen(seed)
+        blocks = [-(-max(k, 0) // P) for k in kvs]
+        n_pages = sum(blocks) + spare
+        perm = torch.randperm(n_pages, generator=g, device=DEV).tolist()
+        cols = max(1, max(blocks))
+        table = np.full((len(kvs), cols), 0x7ffffff0, dtype=np.int32)
+        at = 0
+        for s, b in enumerate(blocks):
+            table[s, :b] = perm[at:at + b]
+            at += b
+        shape = (n_pages, P, Hkv, hd) if layout == "nhd" else (n_pages, Hkv, P, hd)
+        if layout == "pair":  # keys and values of a page side by side
+            both = torch.full((n_pages, 2, P, Hkv, hd), float("nan"), dtype=DT[dtype], device=DEV)
+            k, v = both[:, 0], both[:, 1]
+        else:
+            k, v = (torch.full(shape, float("nan"), dtype=DT[dtype], device=DEV) for _ in range(2))
+            if layout == "hnd":
+                k, v = k.transpose(1, 2), v.transpose(1, 2)
+        self.K = [_rand(g, max(L, 0), Hkv, hd).to(DT[dtype]) for L in kvs]
+        self.V = [_rand(g, max(L, 0), Hkv, hd).to(DT[dtype]) for L in kvs]
+        self.table, self.P, self.news, self.kvs, self.dtype, self.hd, self.Hkv = table, P, news, kvs, dtype, hd, Hkv
+        self.cache = paged.PagedKV(k, v)
+        for s in range(len(kvs)):
+            self.fill(s, 0, kvs[s])
+        self.q_start = torch.tensor(np.concatenate(([0], np.cumsum(news))), dtype=torch.int32, device=DEV)
+        self.kv_len = torch.tensor(kvs, dtype=torch.int32, device=DEV)
+        self.tab = torch.from_numpy(table).to(DEV)
+        self.chunks = self.make_chunks()
+
+    def slots(self, s, p0, p1):
+        pos = torch.arange(p0, p1, device=DEV)
+        return self.tab_of(s)[pos // self.P].long(), pos % self.P
+
+    def tab_of(self, s):
+        return torch.from_numpy(self.table[s]).to(DEV)
+
+    def fill(self, s, p0, p1):
+        if p1 > p0:
+            page, slot = self.slots(s, p0, p1)
+            self.cache.k[page, slot], self.cache.v[page, slot] = self.K[s][p0:p1], self.V[s][p0:p1]
+
+    def make_chunks(self, **kw):
+        kw = {"max_new": max(self.news), "max_kv": max(1, max(self.kvs)), **kw}
+        return paged.Chunks(self.q_start, self.kv_len, self.tab, **kw)
+
+    def ref(self, q, scale, window):
+        """Row by row over the keys a row sees, 64 bits; (out, lse in log2 units)."""
+        T, H, hd = q.shape
+        out = torch.zeros(T, H, hd, dtype=torch.float64, device=DEV)
+        lse = torch.full((H, T), -math.inf, dtype=torch.float64, device=DEV)
+        t = 0
+        for s, (n, L) in enumerate(zip(self.news, self.kvs)):
+            K, V = (x[s].double().repeat_interleave(H // self.Hkv, 1) for x in (self.K, self.V))
+            for i in range(n):
+                p = L - n + i
+                if p >= 0:
+                    lo = max(0, p - window + 1) if window else 0
+                    x = torch.einsum("hd,jhd->hj", q[t].double(), K[lo:p + 1]) * scale
+                    lse[:, t] = torch.logsumexp(x, 1) / math.log(2)
+                    out[t] = torch.einsum("hj,jhd->hd", torch.softmax(x, 1), V[lo:p + 1])
+                t += 1
+        return out, lse
+
+
+def _check(b, q, window=0, scale=None, cache=None):
+    scale = q.shape[2] ** -0.5 if scale is None else scale
+    out, lse = b.cache.attend(b.chunks, q, scale=scale, window=window, return_lse=True)
+    want, wl = b.ref(q, scale, window)
+    vmax = max([v.abs().max().item() for v in b.V if v.numel()] + [1.0])
+    assert torch.isfinite(out).all()
+    assert (out.double() - want).abs().max().item() <= ATT_TOL[b.dtype] * vmax
+    seen = torch.isfinite(wl)
+    assert torch.equal(torch.isneginf(lse), ~seen)
+    if seen.any():
+        assert (lse.double() - wl)[seen].abs().max().item() <= LSE_TOL
+    b.cache.check_status()
+    return out, lse
+
+
+# every head size and type against group sizes, page sizes, lengths around tiles and splits
+ONE = [([1], [1]), ([1, 1, 1], [2, 17, 33]), ([1] * 5, [255, 256, 257, 640, 1]), ([1, 1], [4097, 511]),
+       ([1, 0, 1], [100, 37, 0])]
+FEW = [([2], [2]), ([3, 5], [3, 300]), ([4, 1, 7], [259, 1, 1030]), ([5], [2])]
+MANY = [([17], [17]), ([64, 33], [64, 500]), ([130, 1, 129], [130, 77, 1000]), ([300], [1300]), ([40], [10]),
+        ([257, 2, 128], [257, 2, 385])]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("kind", ["one", "few", "many"])
+def test_attention_matches_float64(dtype, hd, kind):
+    cases = {"one": ONE, "few": FEW, "many": MANY}[kind]
+    for i, (news, kvs) in enumerate(cases):
+        Hkv, G = [(1, 1), (2, 4), (3, 3), (1, 16), (4, 1), (2, 8)][i]
+        P = [16, 1, 24, 64, 7, 128][(i + hd // 32) % 6]
+        for window in (0, [1, 5, 64, 300][i % 4]):
+            b = Batch(dtype, hd, Hkv, P, news, kvs, seed=i, layout=["nhd", "hnd", "pair"][i % 3])
+            q = (2.0 * _rand(_gen(9 + i), sum(news), Hkv * G, hd)).to(DT[dtype])
+            _check(b, q, window=window)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attention_of_peaked_and_growing_scores(dtype):
+    """Scores that rise along the keys (the running maximum moves at every tile) and rows
+    dominated by one key."""
+    b = Batch(dtype, 64, 2, 32, [1, 40], [700, 700], seed=4)
+    for s in range(2):
+        ramp = torch.linspace(-3, 3, b.kvs[s], device=DEV)[:, None, None]
+        b.K[s] = (torch.ones(b.kvs[s], 2, 64, device=DEV) * ramp).to(DT[dtype])
+        b.fill(s, 0, b.kvs[s])
+    q = torch.full((41, 4, 64), 1.0, device=DEV).to(DT[dtype])
+    _check(b, q, scale=0.25)
+    _check(b, q, scale=-0.25)
+    _check(b, q, scale=0.0)
+
+
+def test_attention_rows_do_not_depend_on_the_batch():
+    """Every sequence alone gives the bits it has in the batch (16- and 32-bit types,
+    one, few and many new tokens)."""
+    for dtype in ("f32", "bf16"):
+        news, kvs = [1, 3, 70, 1, 200], [900, 40, 333, 2500, 1000]
+        b = Batch(dtype, 64, 2, 16, news, kvs, seed=5)
+        q = (2.0 * _rand(_gen(6), sum(news), 8, 64)).to(DT[dtype])
+        out, lse = b.cache.attend(b.chunks, q, return_lse=True, window=0)
+        again = b.cache.attend(b.chunks, q)
+        assert torch.equal(out, again)
+        t = 0
+        for s, n in enumerate(news):
+            c = paged.Chunks(torch.tensor([0, n], dtype=torch.int32, device=DEV), b.kv_len[s:s + 1], b.tab[s:s + 1],
+                             max_new=n, max_kv=kvs[s])
+            o, l1 = b.cache.attend(c, q[t:t + n], return_lse=True)
+            assert torch.equal(o, out[t:t + n]) and torch.equal(l1, lse[:, t:t + n])
+            t += n
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_attention_ignores_what_its_mask_hides(dtype):
+    """NaN and infinities in keys and values that a row does not see (later tokens of its own
+    chunk, keys before its window) do not reach it."""
+    for n, G in ((1, 2), (4, 2), (64, 2)):
+        L, w = 300, 100
+        b = Batch(dtype, 64, 2, 16, [n], [L], seed=7)
+        q = (2.0 * _rand(_gen(8), n, 2 * G, 64)).to(DT[dtype])
+        want, _ = b.ref(q, 0.125, w)
+        bad_k, bad_v = float("nan"), float("inf")
+        page, slot = b.slots(0, 0, L - n + 1 - w)  # before every window
+        b.cache.k[page, slot], b.cache.v[page, slot] = bad_k, bad_v
+        if n > 1:  # the last token's key and value: only the last row sees them
+            page, slot = b.slots(0, L - 1, L)
+            b.cache.k[page, slot], b.cache.v[page, slot] = bad_v, bad_k
+        out = b.cache.attend(b.chunks, q, window=w)
+        rows = slice(0, max(1, n - 1))
+        assert torch.isfinite(out[rows]).all()
+        vmax = b.V[0].abs().max().item()
+        assert (out[rows].double() - want[rows]).abs().max().item() <= ATT_TOL[dtype] * vmax
+        if n > 1:
+            assert torch.isnan(out[-1]).any()
+
+
+def test_attention_table_entries_before_the_window_are_not_read():
+    b = Batch("bf16", 64, 2, 16, [1, 20], [400, 400], seed=11)
+    q = _rand(_gen(12), 21, 4, 64).bfloat16()
+    want = b.cache.attend(b.chunks, q, window=50)
+    b.tab[0, : (400 - 50) // 16] = -1
+    b.tab[1, : (400 - 20 - 50) // 16] = 1 << 30
+    assert torch.equal(b.cache.attend(b.chunks, q, window=50), want)
+    b.cache.check_status()
+
+
+@pytest.mark.parametrize("n", [1, 30])
+def test_attention_page_out_of_range_is_unseen_and_reported(n):
+    b = Batch("f32", 64, 1, 16, [n], [200], seed=13)
+    q = _rand(_gen(14), n, 2, 64)
+    b.tab[0, 3] = 1 << 28  # positions 48 .. 63
+    out = b.cache.attend(b.chunks, q)
+    keep = torch.cat((torch.arange(48), torch.arange(64, 200))).to(DEV)
+    for i in range(n):
+        k = keep[keep <= 200 - n + i]
+        for h in range(2):
+            p = torch.softmax(b.K[0][k, 0].double() @ q[i, h].double() / 8, 0)
+            assert ((p @ b.V[0][k, 0].double()) - out[i, h]).abs().max().item() < 1e-4
+    with pytest.raises(RuntimeError, match="status 0x20"):
+        b.cache.check_status()
+
+
+def test_attention_lengths_outside_their_bounds_are_left_out():
+    b = Batch("f32", 32, 1, 16, [1, 1, 1], [50, 60, 70], seed=15)
+    q = _rand(_gen(16), 3, 1, 32)
+    want, _ = b.ref(q, 32 ** -0.5, 0)
+    out = torch.full_like(q, 7.0)
+    b.cache.attend(b.make_chunks(max_kv=60), q, out=out)  # the third is longer than its bound
+    assert (out[:2].double() - want[:2]).abs().max().item() < 1e-4 and (out[2] == 7.0).all()
+    with pytest.raises(RuntimeError, match="status"):
+        b.cache.check_status()
+
+
+def test_attention_far_offsets():
+    """Pages whose element offset passes 2^32."""
+    P, Hkv, hd = 64, 8, 128
+    per = P * Hkv * hd
+    n_pages = (1 << 32) // per + 20
+    k = torch.empty(n_pages, P, Hkv, hd, dtype=torch.bfloat16, device=DEV)
+    v = torch.empty_like(k)
+    b = Batch("bf16", hd, Hkv, P, [1, 40], [300, 200], seed=17)
+    tab = torch.full_like(b.tab, -1)
+    at = n_pages - 12
+    for s in range(2):
+        for blk in range(-(-b.kvs[s] // P)):
+            src = int(b.table[s, blk])
+            k[at], v[at] = b.cache.k[src], b.cache.v[src]
+            tab[s, blk] = at
+            at += 1
+    q = (2.0 * _rand(_gen(18), 41, 16, hd)).bfloat16()
+    want, wl = b.cache.attend(b.chunks, q, return_lse=True)
+    far = paged.PagedKV(k, v)
+    c = paged.Chunks(b.q_start, b.kv_len, tab, max_new=40, max_kv=300)
+    out, lse = far.attend(c, q, return_lse=True)
+    assert torch.equal(out, want) and torch.equal(lse, wl)
+    # and the append reaches them
+    kn, vn = _rand(_gen(1), 41, Hkv, hd).bfloat16(), _rand(_gen(2), 41, Hkv, hd).bfloat16()
+    far.append(c, kn, vn)
+    pos = torch.arange(160, 200, device=DEV)
+    assert torch.equal(k[tab[1][pos // P].long(), pos % P], kn[1:])
+    far.check_status()
+
+
+def test_attention_on_a_side_stream_and_strided_rows():
+    b = Batch("f32", 64, 2, 16, [1, 30], [600, 90], seed=19)
+    wide = _rand(_gen(20), 31, 5 * 64 + 4)
+    q = wide[:, 4:4 + 4 * 64].unflatten(1, (4, 64))
+    want, _ = b.ref(q, 0.125, 0)
+    buf = torch.zeros(31, 6 * 64, device=DEV)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        b.cache.attend(b.chunks, q, out=buf[:, 64:320].unflatten(1, (4, 64)))
+    s.synchronize()
+    assert (buf[:, 64:320].unflatten(1, (4, 64)).double() - want).abs().max().item() < 1e-4
+    assert (buf[:, :64] == 0).all() and (buf[:, 320:] == 0).all()
+
+
+def test_attention_in_a_cuda_graph():
+    b = Batch("bf16", 64, 2, 16, [1, 1], [600, 90], seed=21)
+    q = _rand(_gen(22), 2, 4, 64).bfloat16()
+    want = b.cache.attend(b.chunks, q)
+    out = torch.zeros_like(want)
+    g = torch.cuda.CUDAGraph()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        b.cache.attend(b.chunks, q, out=out)
+        s.synchronize()
+        out.zero_()
+        with torch.cuda.graph(g, stream=s):
+            b.cache.attend(b.chunks, q, out=out)
+    for _ in range(3):
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
+# ---- append -------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("hd,dims,il,P,layout", [(32, 8, False, 16, "nhd"), (64, 16, False, 7, "hnd"), (128, 128, True, 64, "nhd"),
+                                                  (64, 64, True, 1, "pair"), (128, 6, False, 24, "hnd")])
+def test_append_writes_pages_and_rotates(dtype, hd, dims, il, P, layout):
+    news, kvs = [1, 0, 5, 90, 33], [40, 12, 5, 300, 64]
+    b = Batch(dtype, hd, 2, P, news, kvs, seed=hd + dims, layout=layout)
+    g, T, H = _gen(5), sum(news), 6
+    cos, sin = _table(512, dims)
+    rot = paged.Rotary(cos, sin, il)
+    rows = _rand(g, T, (H + 4) * hd).to(DT[dtype])
+    q, k, v = (x.unflatten(1, (-1, hd)) for x in rows.split([H * hd, 2 * hd, 2 * hd], 1))
+    k0, v0 = b.cache.k.clone(), b.cache.v.clone()
+    qr = b.cache.append(b.chunks, k, v, rotary=rot, q=q)
+    pos = torch.cat([torch.arange(L - n, L) for n, L in zip(news, kvs)]).to(DEV)
+    assert torch.equal(qr, paged.rope(q, rot, pos))
+    assert (qr.double() - _rot_ref(q, cos, sin, pos, il)).abs().max().item() <= \
+        ROT_TOL[dtype] * math.sqrt(2) * q.abs().max().item()
+    kr, t = paged.rope(k, rot, pos), 0
+    for s, (n, L) in enumerate(zip(news, kvs)):
+        if n:
+            page, slot = b.slots(s, L - n, L)
+            k0[page, slot], v0[page, slot] = kr[t:t + n], v[t:t + n]
+        t += n
+    bits = lambda x: x.contiguous().view(torch.int32 if dtype == "f32" else torch.int16)  # noqa: E731
+    assert torch.equal(bits(b.cache.k), bits(k0)) and torch.equal(bits(b.cache.v), bits(v0))  # and nothing else
+    # given positions, queries in place, and no rotation at all
+    other = torch.randint(0, 512, (T,), generator=g, device=DEV)
+    want = paged.rope(q, rot, other)
+    b.cache.append(b.chunks, k, v, rotary=rot, q=q, positions=other, q_out=q)
+    assert torch.equal(q, want)
+    b.cache.append(b.chunks, k, v)
+    page, slot = b.slots(3, 210, 300)
+    assert torch.equal(b.cache.k[page, slot], k[6:96])
+    b.cache.check_status()
+
+
+def test_append_skips_and_reports_what_has_no_place():
+    b = Batch("f32", 32, 1, 16, [2, 3, 1], [30, 2, 20], seed=2)  # the second has one token too many
+    cos, sin = _table(25, 16)
+    rot = paged.Rotary(cos, sin)
+    b.tab[2, 1] = b.cache.k.shape[0]  # position 19's page does not exist
+    k, v, q = (_rand(_gen(i), 6, 1, 32) for i in (1, 2, 3))
+    before = b.cache.k.clone()
+    qr = b.cache.append(b.chunks, k, v, rotary=rot, q=q)
+    assert torch.isnan(qr[:2]).all()   # positions 28, 29 are outside the table
+    assert torch.isnan(qr[2]).all()    # position -1
+    assert torch.isfinite(qr[3:]).all()
+    page, slot = b.slots(1, 0, 2)
+    before[page, slot] = paged.rope(k[3:5], rot, torch.tensor([0, 1], device=DEV))
+    assert torch.equal(torch.nan_to_num(b.cache.k, 9.0), torch.nan_to_num(before, 9.0))
+    with pytest.raises(RuntimeError, match="status 0x20"):
+        b.cache.check_status()
+
+
+def test_chunked_appends_and_attention_equal_one_pass():
+    """A sequence fed in pieces of 1, 7, 64 and 28 tokens gives what one piece of 100 gives
+    (each against the 64-bit reference)."""
+    g, hd, H, Hkv = _gen(31), 64, 4, 2
+    k, v, q = _rand(g, 100, Hkv, hd), _rand(g, 100, Hkv, hd), 2 * _rand(g, 100, H, hd)
+    cos, sin = _table(128, 16)
+    rot = paged.Rotary(cos, sin)
+    outs = []
+    for pieces in ([100], [1, 7, 64, 28]):
+        cache = paged.PagedKV.empty(12, 16, Hkv, hd)
+        alloc = paged.PageAllocator(1, 12, 16, 128, DEV)
+        t, ys = 0, []
+        for n in pieces:
+            c = alloc.extend([n])
+            qr = cache.append(c, k[t:t + n], v[t:t + n], rotary=rot, q=q[t:t + n])
+            ys.append(cache.attend(c, qr))
+            t += n
+        outs.append(torch.cat(ys))
+        cache.check_status()
+    pos = torch.arange(100, device=DEV)
+    kr, qr = _rot_ref(k, cos, sin, pos, False), _rot_ref(q, cos, sin, pos, False)
+    x = torch.einsum("ihd,jhd->hij", qr, kr.repeat_interleave(2, 1)) / 8
+    x.masked_fill_(torch.ones(100, 100, dtype=torch.bool, device=DEV).triu(1), -math.inf)
+    want = torch.einsum("hij,jhd->ihd", torch.softmax(x, 2), v.double().repeat_interleave(2, 1))
+    for o in outs:
+        assert (o.double() - want).abs().max().item() <= ATT_TOL["f32"] * v.abs().max().item()
+
+
+# ---- refusals ------------------------------------------------------------------
+
+
+def test_refusals():
+    b = Batch("f32", 64, 2, 16, [1], [40], seed=1)
+    q = _rand(_gen(1), 1, 4, 64)
+    cos, sin = _table(64, 16)
+    rot = paged.Rotary(cos, sin)
+    with pytest.raises(ValueError):
+        b.cache.attend(b.chunks, q.double())
+    with pytest.raises(ValueError):
+        b.cache.attend(b.chunks, q[:, :3])            # heads not a multiple
+    with pytest.raises(ValueError):
+        b.cache.attend(b.chunks, q.cpu())
+    with pytest.raises(ValueError):
+        b.cache.attend(b.chunks, _rand(_gen(1), 4, 1, 64).transpose(0, 1)[:, ::2])  # heads apart
+    with pytest.raises(RuntimeError):
+        b.cache.attend(b.chunks, q, window=-1)
+    with pytest.raises(RuntimeError):                  # rows not on 16 bytes
+        b.cache.attend(b.chunks, _rand(_gen(1), 260)[1:257].view(1, 4, 64))
+    with pytest.raises(ValueError):
+        b.cache.append(b.chunks, q, q)                 # wrong head count
+    with pytest.raises(ValueError):
+        paged.PagedKV(b.cache.k, b.cache.v.half())
+    with pytest.raises(ValueError):
+        paged.Rotary(cos.half(), sin.half())
+    with pytest.raises(RuntimeError):
+        paged.rope(_rand(_gen(1), 1, 1, 8), rot, torch.zeros(1, dtype=torch.int64, device=DEV))  # dims > head
+    with pytest.raises(ValueError):
+        paged.rope(q, rot, torch.zeros(1, dtype=torch.int32, device=DEV))
+    with pytest.raises(RuntimeError):                  # head size without a kernel
+        p = paged.PagedKV.empty(2, 16, 1, 96)
+        p.attend(b.chunks, _rand(_gen(1), 1, 1, 96))
+    with pytest.raises(ValueError):
+        b.cache.attend(b.make_chunks(max_kv=500), q)   # the table is shorter
+    # nothing to do is not an error
+    c0 = paged.Chunks(torch.zeros(2, dtype=torch.int32, device=DEV), b.kv_len, b.tab, max_new=0, max_kv=40)
+    assert b.cache.attend(c0, q[:0]).shape == (0, 4, 64)
+    assert b.cache.append(c0, q[:0, :2], q[:0, :2]) is None
+    assert paged.rope(q[:0], rot, torch.zeros(0, dtype=torch.int64, device=DEV)).shape == (0, 4, 64)
+    b.cache.check_status()
+
+
+def test_short_workspace_is_refused():
+    import ctypes
+
+    b = Batch("f32", 64, 2, 16, [1], [4000], seed=1)
+    q = _rand(_gen(1), 1, 4, 64)
+    L = _lib.lib()
+    b.cache._chunks(b.chunks, 1)
+    need = L.altxs_paged_attention_workspace_bytes(b.cache._ref, b.chunks._ref, 4, 0)
+    rc = L.altxs_paged_attention(b.cache._ref, b.chunks._ref, 4, ctypes.c_float(0.1), 0, q.data_ptr(), 256, q.data_ptr(), 256,
+                                 None, None, need - 1, None)
+    assert rc == _lib.ALTXS_ENOSPC

@@ -1,0 +1,139 @@
+"""CPU checks of the paged cache: argument validation runs before any CUDA call,
+the page allocator is plain host code, and the rotary tables follow their rules."""
+
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from altxs_b200 import _lib, paged
+
+
+def _kv(**kw):
+    d = dict(k=4096, v=8192, page_stride=16 * 2 * 64, token_stride=2 * 64, head_stride=64, dtype=_lib.F32,
+             page_size=16, n_pages=4, n_kv_heads=2, head_dim=64)
+    return _lib.PagedKv(**{**d, **kw})
+
+
+def _ch(**kw):
+    d = dict(q_start=4096, kv_len=4096, page_table=4096, table_stride=4, n_seqs=1, n_tokens=1, max_new=1, max_kv=40)
+    return _lib.Chunks(**{**d, **kw})
+
+
+def _attend(kv, ch, H=4, window=0, ldq=256, ws=0, nbytes=0):
+    return _lib.lib().altxs_paged_attention(C.byref(kv), C.byref(ch), H, 0.1, window, 4096, ldq, 4096, 256, None, ws,
+                                            nbytes, None)
+
+
+@pytest.mark.parametrize("kv,ch,kw,code", [
+    (dict(head_dim=48), {}, {}, _lib.ALTXS_ENOTSUP), (dict(dtype=3), {}, {}, _lib.ALTXS_EINVAL),
+    (dict(page_size=0), {}, {}, _lib.ALTXS_EINVAL), (dict(k=4097), {}, {}, _lib.ALTXS_EINVAL),
+    (dict(token_stride=130), {}, {}, _lib.ALTXS_EINVAL), (dict(token_stride=32), {}, {}, _lib.ALTXS_EINVAL),
+    (dict(dtype=_lib.F16, head_stride=68), {}, {}, _lib.ALTXS_EINVAL), (dict(n_kv_heads=0), {}, {}, _lib.ALTXS_EINVAL),
+    ({}, dict(max_kv=65), {}, _lib.ALTXS_EINVAL), ({}, dict(n_seqs=-1), {}, _lib.ALTXS_EINVAL),
+    ({}, dict(max_new=-1), {}, _lib.ALTXS_EINVAL), ({}, dict(q_start=None), {}, _lib.ALTXS_EINVAL),
+    ({}, {}, dict(H=5), _lib.ALTXS_EINVAL), ({}, {}, dict(H=0), _lib.ALTXS_EINVAL),
+    ({}, {}, dict(window=-1), _lib.ALTXS_EINVAL), ({}, {}, dict(ldq=255), _lib.ALTXS_EINVAL),
+    ({}, {}, dict(ldq=258), _lib.ALTXS_EINVAL), ({}, dict(n_seqs=0), {}, 0), ({}, dict(n_tokens=0), {}, 0)])
+def test_attention_refuses_before_touching_the_device(kv, ch, kw, code):
+    assert _attend(_kv(**kv), _ch(**ch), **kw) == code
+
+
+def test_workspace_sizes():
+    L = _lib.lib()
+    f = lambda kv, ch, H=4, w=0: L.altxs_paged_attention_workspace_bytes(C.byref(kv), C.byref(ch), H, w)  # noqa: E731
+    assert f(_kv(head_dim=48), _ch()) == -1 and f(_kv(), _ch(), H=3) == -1 and f(_kv(), _ch(), w=-1) == -1
+    long = _ch(n_seqs=64, n_tokens=64, max_kv=100000, table_stride=10000)
+    assert f(_kv(), long) >= f(_kv(), _ch()) >= 0
+    # a window and a known total bound it
+    assert f(_kv(), long, w=512) <= f(_kv(), long)
+    some = _ch(n_seqs=64, n_tokens=64, max_kv=100000, table_stride=10000, total_kv=200000)
+    assert f(_kv(), some) <= f(_kv(), long)
+
+
+def test_rope_and_append_refuse_before_touching_the_device():
+    L = _lib.lib()
+    r = _lib.RotaryTables(cos=4096, sin=4096, positions=10, dims=16, interleaved=0)
+
+    def rope(dtype=0, T=1, H=2, hd=64, r=r, pos=4096, x=4096, ldx=128, y=8192, ldy=128):
+        return L.altxs_rope(dtype, T, H, hd, C.byref(r), pos, 0, x, ldx, y, ldy, None, None)
+
+    bad = lambda **kw: _lib.RotaryTables(**{**dict(cos=4096, sin=4096, positions=10, dims=16, interleaved=0), **kw})  # noqa: E731
+    assert rope(dtype=7) == _lib.ALTXS_EINVAL and rope(hd=63) == _lib.ALTXS_EINVAL
+    assert rope(hd=514, ldx=2000, ldy=2000) == _lib.ALTXS_ENOTSUP
+    assert rope(ldx=127) == _lib.ALTXS_EINVAL and rope(pos=None) == _lib.ALTXS_EINVAL
+    assert rope(x=4097) == _lib.ALTXS_EINVAL and rope(x=8192, ldx=256) == _lib.ALTXS_EINVAL
+    assert rope(r=bad(dims=66)) == _lib.ALTXS_EINVAL and rope(r=bad(dims=15)) == _lib.ALTXS_EINVAL
+    assert rope(r=bad(cos=4100)) == _lib.ALTXS_EINVAL and rope(r=bad(sin=None)) == _lib.ALTXS_EINVAL
+    assert rope(T=0) == 0 and rope(H=0, ldx=0, ldy=0) == 0
+
+    def append(kv=_kv(), ch=_ch(), ldk=128, H=4, q=4096, ldq=256, qo=8192, ldqo=256, r=r, k=4096):
+        return L.altxs_paged_append(C.byref(kv), C.byref(ch), C.byref(r), None, k, ldk, 8192, 128, H, q, ldq, qo, ldqo,
+                                    None)
+
+    assert append(kv=_kv(head_dim=16)) == _lib.ALTXS_ENOTSUP and append(ldk=127) == _lib.ALTXS_EINVAL
+    assert append(ldq=255) == _lib.ALTXS_EINVAL and append(qo=None) == _lib.ALTXS_EINVAL
+    assert append(qo=4096, ldqo=512) == _lib.ALTXS_EINVAL and append(k=None) == _lib.ALTXS_EINVAL
+    assert append(k=4098) == _lib.ALTXS_EINVAL and append(r=bad(dims=128)) == _lib.ALTXS_EINVAL
+    assert append(ch=_ch(n_tokens=0)) == 0
+
+
+def test_page_allocator():
+    a = paged.PageAllocator(3, 6, 4, 20, "cpu")
+    c = a.extend([5, 0, 1])
+    assert c.q_start.tolist() == [0, 5, 5, 6] and c.kv_len.tolist() == [5, 0, 1]
+    assert c.struct.max_new == 5 and c.struct.max_kv == 5 and c.struct.total_kv == 6
+    held = [p for p in a.table.ravel() if p >= 0]
+    assert len(set(held)) == 3 and len(a.free) == 3 and (a.table[1] == -1).all()
+    a.extend([3, 0, 0])  # fills the second page: no new one
+    assert len(a.free) == 3 and a.len.tolist() == [8, 0, 1]
+    before = a.table.copy()
+    with pytest.raises(RuntimeError, match="out of pages"):
+        a.extend([4, 12, 0])
+    with pytest.raises(ValueError, match="max_kv"):
+        a.extend([13, 0, 0])
+    with pytest.raises(ValueError):
+        a.extend([1, 1])
+    assert (a.table == before).all() and a.len.tolist() == [8, 0, 1]
+    a.extend([9, 0, 0])  # 17 tokens: five pages
+    # window 6: the next token (position 17) sees 12 ..: pages of 0-3, 4-7, 8-11 come back
+    assert a.trim(0, 6) == 3 and a.trim(0, 6) == 0 and (a.table[0, :3] == -1).all() and (a.table[0, 3:5] >= 0).all()
+    a.release(0)
+    assert a.len[0] == 0 and len(a.free) == 5 and sorted(a.free + [int(a.table[2, 0])]) == list(range(6))
+
+
+def test_rope_table_rules():
+    n, d, base = 300, 32, 1e4
+    p, j = np.arange(n)[:, None], np.arange(0, d, 2)
+    w = base ** (-j / d)
+
+    def close(t, w, amp=1.0):
+        cos, sin = t
+        return max(np.abs(cos.double().numpy() - amp * np.cos(p * w)).max(),
+                   np.abs(sin.double().numpy() - amp * np.sin(p * w)).max()) < 2.0 ** -23
+
+    assert close(paged.rope_table(n, d, base, device="cpu"), w)
+    assert close(paged.rope_table(n, d, base, scaling="linear", factor=4.0, device="cpu"), w / 4)
+    wb = (base * 4.0 ** (d / (d - 2))) ** (-j / d)
+    assert wb[0] == 1.0 and abs(wb[-1] * 4 / w[-1] - 1) < 1e-12
+    assert close(paged.rope_table(n, d, base, scaling="base", factor=4.0, device="cpu"), wb)
+    t = 2048
+    turns = t * w / (2 * math.pi)
+    wp = np.where(turns > 32, w, np.where(turns < 1, w / 8, 0))
+    ramp = (turns - 1) / 31
+    mid = (turns <= 32) & (turns >= 1)
+    wp[mid] = (w * (ramp + (1 - ramp) / 8))[mid]
+    amp = 0.1 * math.log(8.0) + 1
+    assert close(paged.rope_table(n, d, base, scaling="parts", factor=8.0, trained=t, device="cpu"), wp, amp)
+    assert paged.rope_table(0, 16, device="cpu")[0].shape == (0, 8)
+    assert torch.equal(paged.rope_table(5, 2, scaling="base", factor=2.0, device="cpu")[0],
+                       paged.rope_table(5, 2, device="cpu")[0])
+    for kw in (dict(scaling="parts", factor=2.0), dict(scaling="x"), dict(factor=0.5)):
+        with pytest.raises(ValueError):
+            paged.rope_table(4, 16, device="cpu", **kw)
+    with pytest.raises(ValueError):
+        paged.rope_table(4, 15, device="cpu")
