@@ -1,17 +1,565 @@
-// Attention of new tokens over a paged key/value cache.
+// Attention of a few new tokens over a paged key/value cache: the rows of one
+// key/value head (its query heads times the sequence's new tokens) fit one
+// 16-row MMA tile.
 //
-// One warp per (token, head): the lanes share the channels, keys one at a time
-// with a running maximum and sum (o = o 2^(m - m') + p v), fp32 throughout.
+// Every cached key and value is read once and serves at most 16 rows, so HBM
+// bounds it (8 flops a byte at 16 rows in 16 bits against the card's 260).  A
+// sequence's visible keys are cut into splits (split_keys: a function of their
+// number alone, so a row's bits do not depend on the batch); an item is one
+// split of one key/value head, taken by a block of four warps.  Each warp
+// streams 8 KB chunks (keys and values of CK positions) through its own three
+// slots with 16-byte asynchronous copies, gathering rows through the page
+// table (a page may end anywhere in a chunk; rows past the end are filled with
+// zeros), two chunks in flight while one is computed; there is no block-wide
+// barrier until the four warps' partial rows meet.  Per chunk a warp forms
+// S = Q K^T, the online softmax and O += P V as 16-row mma.sync fragments: the
+// 16-bit types in m16n8k16 with fp32 sums, fp32 as three tf32 products of
+// hi/lo halves (22 significant bits).  The tcgen05 tile would be at least 128
+// rows for at most 16 real ones and is not what bounds this kernel.
+//
+// A split's rows go to the workspace as (m, l, o); the block that finishes the
+// last split of a (sequence, head) joins them in split order.
+#include <algorithm>
+#include <type_traits>
+
 #include "paged.cuh"
 #include "prof.cuh"
 
 namespace altxs {
 namespace {
 
+constexpr int kWarps = 4;
+constexpr int kSlots = 3;
+constexpr int kChunkBytes = 8192;  // keys and values of one chunk
+constexpr int kMaxRows = 16;
+constexpr int kSplitCap = 64;    // splits of a sequence at most
+constexpr int kSplitUnit = 256;  // keys
+constexpr unsigned kAll = 0xffffffffu;
+
+__host__ __device__ inline int split_keys(int keys) {
+    const int u = kSplitUnit * kSplitCap;
+    return kSplitUnit * (keys > u ? (keys + u - 1) / u : 1);
+}
+__host__ __device__ inline int split_count(int keys) {
+    const int k = split_keys(keys);
+    return keys > k ? (keys + k - 1) / k : 1;
+}
+
+struct FewArgs {
+    PagedAttnArgs a;
+    int G;
+    int64_t max_items;  // partial slots in the workspace
+    uint32_t *cnt;      // [n_seqs * Hkv], zero between calls
+    float *part;        // [max_items][rows][HD + 2]
+    int part_rows;
+};
+
+// Items of the sequences before each group of `per` sequences.
+struct ItemScan {
+    int before[kWarps * 32 + 1];
+    int per;
+};
+
+__device__ __forceinline__ int few_splits(const FewArgs &f, const Seq &q) {
+    if (q.n <= 0 || q.n * f.G > kMaxRows) return 0;
+    return split_count(max(0, q.L - first_seen(q.n, q.L, f.a.window)));
+}
+
+__device__ __forceinline__ void scan_items(const FewArgs &f, ItemScan &sc) {
+    const int n = f.a.c.n_seqs, per = (n + kWarps * 32 - 1) / (kWarps * 32);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int sum = 0;
+    for (int s = tid * per; s < min(n, (tid + 1) * per); ++s)
+        sum += few_splits(f, blockIdx.x == 0 ? load_seq_report(f.a.c, s) : load_seq(f.a.c, s));
+    sum *= f.a.kv.n_kv_heads;
+    int inc = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(kAll, inc, o);
+        if (lane >= o) inc += v;
+    }
+    __shared__ int wsum[kWarps];
+    if (lane == 31) wsum[warp] = inc;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) inc += wsum[w];
+    sc.before[tid + 1] = inc;
+    if (tid == 0) sc.before[0] = 0, sc.per = per;
+    __syncthreads();
+}
+
+__device__ __forceinline__ uint32_t f2u(float x) { return __float_as_uint(x); }
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+template <int TRANS>
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t *r) {
+    if (TRANS)
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+    else
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void lds128(uint32_t addr, uint32_t *r) {
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ void mma16(float *d, const uint32_t *a, uint32_t b0, uint32_t b1) {
+    if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_tf32(float *d, const uint32_t *a, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// x = hi + lo + O(2^-22 x), both read by the tensor cores to 11 significant bits:
+// hi is x rounded half up there, lo the exact rest rounded by the same addition.
+// (An infinity becomes NaN: inf - inf.)
+__device__ __forceinline__ void split_tf32(uint32_t x, uint32_t &hi, uint32_t &lo) {
+    hi = (x + 0x1000u) & 0xffffe000u;
+    lo = f2u(__fsub_rn(__uint_as_float(x), __uint_as_float(hi))) + 0x1000u;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+}
+
+template <typename T, int HD>
+struct Few {
+    static constexpr int ES = sizeof(T), RB = HD * ES;        // bytes of a row
+    static constexpr int CK = kChunkBytes / (2 * RB);         // positions of a chunk
+    static constexpr int NC = RB / 16;                        // 16-byte pieces of a row
+    static constexpr int NK = CK / 8, NO = HD / 8;            // score and output column tiles
+    static constexpr bool F32 = ES == 4;
+    static constexpr int QS = F32 ? HD / 8 : HD / 16;         // k steps of Q K^T
+    // piece c of position k in shared memory: conflict-free for the reads below
+    static __device__ __forceinline__ uint32_t at(int k, int c) {
+        const int sw = F32 ? (k & 6) ^ ((k & 1) << 2) : NC >= 8 ? k & 7 : (k >> 1) & 3;
+        return k * RB + ((c ^ sw) << 4);
+    }
+};
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kWarps * 32, 2) k_paged_few(FewArgs f) {
+    using F = Few<T, HD>;
+    constexpr int CK = F::CK, NC = F::NC, NK = F::NK, NO = F::NO;
+    extern __shared__ __align__(1024) unsigned char few_smem[];
+    __shared__ ItemScan sc;
+    __shared__ uint64_t seen_sh[kWarps][kSlots];  // positions of a slot's chunk that exist
+    __shared__ float ml_sh[kWarps][kMaxRows][2];
+    __shared__ int last_sh, odd_sh;
+    const PagedAttnArgs &a = f.a;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane >> 2, j = lane & 3;
+    const int Hkv = a.kv.n_kv_heads, G = f.G, P = a.kv.page_size;
+    const int pshift = (P & (P - 1)) == 0 ? 31 - __clz(P) : -1;
+    const float c2 = __fmul_rn(a.scale, kLog2e);
+    const uint32_t ring = smem_u32(few_smem) + warp * kSlots * kChunkBytes;
+    scan_items(f, sc);
+    const int total = sc.before[kWarps * 32];
+
+    for (int item = blockIdx.x; item < total; item += gridDim.x) {
+        // item -> sequence, split, head (heads fastest: they share the rows' DRAM pages)
+        int lo = 0, hi = kWarps * 32;
+        while (hi - lo > 1) {
+            const int m = (lo + hi) >> 1;
+            if (sc.before[m] <= item) lo = m; else hi = m;
+        }
+        int s = lo * sc.per, local = item - sc.before[lo];
+        Seq q = load_seq(a.c, s);
+        for (int w; s < a.c.n_seqs - 1 && local >= (w = few_splits(f, q) * Hkv); q = load_seq(a.c, ++s)) local -= w;
+        const int g = local % Hkv, split = local / Hkv;
+        const int R = q.n * G, kfirst = first_seen(q.n, q.L, a.window), keys = max(0, q.L - kfirst);
+        const int nsplit = split_count(keys), slen = split_keys(keys);
+        const int k0 = kfirst + split * slen, k1 = min(q.L, k0 + slen);
+        const int nchunk = k1 > k0 ? (k1 - k0 + CK - 1) / CK : 0;
+        const int p0 = q.L - q.n;  // position of the first new token
+        // positions [all0, all1) are seen by every row
+        const int all1 = p0 + 1, all0 = a.window > 0 ? q.L - a.window : 0;
+        const char *kb = static_cast<const char *>(a.kv.k) + (int64_t)g * a.kv.head_stride * F::ES;
+        const char *vb = static_cast<const char *>(a.kv.v) + (int64_t)g * a.kv.head_stride * F::ES;
+        const int32_t *table = a.c.page_table + s * a.c.table_stride;
+        if (threadIdx.x == 0) odd_sh = 0;
+
+        auto block_of = [&](int k) { return pshift >= 0 ? k >> pshift : k / P; };
+        constexpr int KL = (CK + 31) / 32;  // positions a lane looks up per chunk
+        int pg[KL];
+        auto fetch_pages = [&](int ci) {
+#pragma unroll
+            for (int r = 0; r < KL; ++r) {
+                const int kc = r * 32 + lane, k = k0 + ci * CK + kc;
+                pg[r] = kc < CK && k < k1 && ci < nchunk ? __ldg(table + block_of(k)) : -1;
+            }
+        };
+        auto issue = [&](int ci, int slot) {  // chunk ci into a slot; pg holds its pages
+            uint64_t seen = 0;
+            int64_t off[KL];
+#pragma unroll
+            for (int r = 0; r < KL; ++r) {
+                const int k = k0 + ci * CK + r * 32 + lane;
+                const bool in = pg[r] >= 0 && pg[r] < a.kv.n_pages;
+                if (!in && k < k1 && r * 32 + lane < CK) set_status(a.c.status, ALTXS_ST_BAD_POS);
+                const int b = block_of(k);
+                off[r] = in ? ((int64_t)pg[r] * a.kv.page_stride + (int64_t)(k - b * P) * a.kv.token_stride) * F::ES : -1;
+                seen |= (uint64_t)__ballot_sync(kAll, in) << (32 * r);
+            }
+            if (lane == 0) seen_sh[warp][slot] = seen;
+            const uint32_t dst = ring + slot * kChunkBytes;
+#pragma unroll
+            for (int i = 0; i < CK * NC / 32; ++i) {
+                const int p = i * 32 + lane, k = p / NC, c = p % NC;
+                const int64_t o = __shfl_sync(kAll, off[CK > 32 ? (i * 32 / NC) / 32 : 0], k & 31);
+                const int64_t src = (o < 0 ? 0 : o) + c * 16;
+                const uint32_t bytes = o < 0 ? 0u : 16u, d = dst + F::at(k, c);
+                cp_async16(d, kb + src, bytes);
+                cp_async16(d + kChunkBytes / 2, vb + src, bytes);
+            }
+        };
+
+        // the first chunks are on their way before the queries are read
+        int next = warp;
+        fetch_pages(next);
+#pragma unroll
+        for (int i = 0; i < kSlots - 1; ++i) {
+            if (next < nchunk) issue(next, i);
+            cp_commit();
+            next += kWarps;
+            fetch_pages(next);
+        }
+        // Q fragments: rows quad, quad + 8 (row r = token r / G, head r % G of the group)
+        uint32_t qa[F::QS][F::F32 ? 8 : 4];
+        int rpos[2];
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+            const int r = quad + 8 * hh, i = r / G, h = g * G + r - i * G;
+            rpos[hh] = r < R ? p0 + i : -1;
+            const T *qp = static_cast<const T *>(a.q) + (int64_t)(q.q0 + i) * a.ldq + (int64_t)h * HD;
+            if constexpr (F::F32) {
+#pragma unroll
+                for (int kk = 0; kk < HD / 16; ++kk) {  // channels 16 kk + 4 j ..: two k steps of (j, j + 4)
+                    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (r < R) x = *reinterpret_cast<const float4 *>(qp + 16 * kk + 4 * j);
+                    split_tf32(f2u(x.x), qa[2 * kk][hh], qa[2 * kk][4 + hh]);
+                    split_tf32(f2u(x.y), qa[2 * kk][2 + hh], qa[2 * kk][6 + hh]);
+                    split_tf32(f2u(x.z), qa[2 * kk + 1][hh], qa[2 * kk + 1][4 + hh]);
+                    split_tf32(f2u(x.w), qa[2 * kk + 1][2 + hh], qa[2 * kk + 1][6 + hh]);
+                }
+            } else {
+#pragma unroll
+                for (int kk = 0; kk < HD / 16; ++kk) {
+                    qa[kk][hh] = r < R ? *reinterpret_cast<const uint32_t *>(qp + 16 * kk + 2 * j) : 0u;
+                    qa[kk][2 + hh] = r < R ? *reinterpret_cast<const uint32_t *>(qp + 16 * kk + 8 + 2 * j) : 0u;
+                }
+            }
+        }
+        float o[NO][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int t = 0; t < NO; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.0f;
+        __syncthreads();  // odd_sh is clear
+
+        int slot = 0;
+        for (int ci = warp; ci < nchunk; ci += kWarps) {
+            cp_wait<kSlots - 2>();
+            __syncwarp();  // the chunk has landed for every lane, and the slot before it has been read
+            if (next < nchunk) issue(next, slot == 0 ? kSlots - 1 : slot - 1);
+            cp_commit();
+            next += kWarps;
+            fetch_pages(next);
+            const uint32_t kt = ring + slot * kChunkBytes, vt = kt + kChunkBytes / 2;
+            const uint64_t have = seen_sh[warp][slot];
+            // S = Q K^T
+            float sacc[NK][4];
+#pragma unroll
+            for (int t = 0; t < NK; ++t) sacc[t][0] = sacc[t][1] = sacc[t][2] = sacc[t][3] = 0.0f;
+            if constexpr (F::F32) {
+#pragma unroll
+                for (int t = 0; t < NK; ++t)
+#pragma unroll
+                    for (int kk = 0; kk < HD / 16; ++kk) {
+                        uint32_t x[4], hi[4], lo[4];
+                        lds128(kt + F::at(8 * t + quad, 4 * kk + j), x);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) split_tf32(x[e], hi[e], lo[e]);
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            mma_tf32(sacc[t], qa[2 * kk + e] + 4, hi[2 * e], hi[2 * e + 1]);
+                            mma_tf32(sacc[t], qa[2 * kk + e], lo[2 * e], lo[2 * e + 1]);
+                            mma_tf32(sacc[t], qa[2 * kk + e], hi[2 * e], hi[2 * e + 1]);
+                        }
+                    }
+            } else {
+#pragma unroll
+                for (int t = 0; t < NK; t += 2)
+#pragma unroll
+                    for (int kk = 0; kk < HD / 16; ++kk) {
+                        uint32_t b[4];
+                        ldsm4<0>(kt + F::at(8 * t + (lane & 7) + ((lane >> 4) << 3), 2 * kk + ((lane >> 3) & 1)), b);
+                        mma16<T>(sacc[t], qa[kk], b[0], b[1]);
+                        mma16<T>(sacc[t + 1], qa[kk], b[2], b[3]);
+                    }
+            }
+            // scale, mask, running maximum
+            const int kc = k0 + ci * CK;
+            const bool whole = kc >= all0 && kc + CK <= min(all1, k1) &&
+                               have == (CK == 64 ? ~0ull : (1ull << (CK & 63)) - 1);
+            float mx[2] = {m[0], m[1]};
+#pragma unroll
+            for (int t = 0; t < NK; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int kl = 8 * t + 2 * j + (e & 1), k = kc + kl, hh = e >> 1;
+                    float x = __fmul_rn(sacc[t][e], c2);
+                    if (!whole)
+                        x = k <= rpos[hh] && (a.window == 0 || k > rpos[hh] - a.window) && ((have >> kl) & 1) ? x : -INFINITY;
+                    sacc[t][e] = x;
+                    mx[hh] = fmaxf(mx[hh], x);
+                }
+            float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+                mx[hh] = fmaxf(mx[hh], __shfl_xor_sync(kAll, mx[hh], 1));
+                mx[hh] = fmaxf(mx[hh], __shfl_xor_sync(kAll, mx[hh], 2));
+                const float base = mx[hh] == -INFINITY ? 0.0f : mx[hh];  // nothing seen yet: every p is 2^-inf = 0
+                const float fold = ex2(__fsub_rn(m[hh], base));
+                m[hh] = mx[hh];
+                mx[hh] = base;
+                l[hh] = __fmul_rn(l[hh], fold);
+#pragma unroll
+                for (int t = 0; t < NO; ++t) {
+                    o[t][2 * hh] = __fmul_rn(o[t][2 * hh], fold);
+                    o[t][2 * hh + 1] = __fmul_rn(o[t][2 * hh + 1], fold);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < NK; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    sacc[t][e] = ex2(__fsub_rn(sacc[t][e], mx[e >> 1]));
+                    sum[e >> 1] = __fadd_rn(sum[e >> 1], sacc[t][e]);
+                }
+            l[0] = __fadd_rn(l[0], sum[0]);
+            l[1] = __fadd_rn(l[1], sum[1]);
+            // Some rows do not see some of these values: one that is not finite must not meet
+            // their p = 0.  It becomes 0 here and is added to the rows that see it at the end.
+            if (!whole && q.n > 1) {
+                bool odd = false;
+#pragma unroll
+                for (int i = 0; i < CK * NC / 32; ++i) {
+                    const uint32_t d = vt + (i * 32 + lane) * 16;
+                    uint32_t w[4];
+                    lds128(d, w);
+                    bool bad = false;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if constexpr (F::F32) {
+                            if ((w[e] & 0x7f800000u) == 0x7f800000u) w[e] = 0, bad = true;
+                        } else {
+                            constexpr uint32_t X = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+                            if ((w[e] & X) == X) w[e] &= 0xffff0000u, bad = true;
+                            if (((w[e] >> 16) & X) == X) w[e] &= 0xffffu, bad = true;
+                        }
+                    }
+                    if (bad) {
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(d), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                        odd = true;
+                    }
+                }
+                if (odd) odd_sh = 1;
+                __syncwarp();
+            }
+            // O += P V
+            if constexpr (F::F32) {
+#pragma unroll
+                for (int t = 0; t < NK; ++t) {
+                    // k index j is position 8 t + 2 j, j + 4 is 8 t + 2 j + 1 (how the scores lie)
+                    uint32_t ph[4], pl[4];
+                    split_tf32(f2u(sacc[t][0]), ph[0], pl[0]);
+                    split_tf32(f2u(sacc[t][2]), ph[1], pl[1]);
+                    split_tf32(f2u(sacc[t][1]), ph[2], pl[2]);
+                    split_tf32(f2u(sacc[t][3]), ph[3], pl[3]);
+#pragma unroll
+                    for (int b = 0; b < HD / 32; ++b) {  // column quad of tile 4 b + e is channel 32 b + 4 quad + e
+                        uint32_t x[4], y[4];
+                        lds128(vt + F::at(8 * t + 2 * j, 8 * b + quad), x);
+                        lds128(vt + F::at(8 * t + 2 * j + 1, 8 * b + quad), y);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            uint32_t xh, xl, yh, yl;
+                            split_tf32(x[e], xh, xl);
+                            split_tf32(y[e], yh, yl);
+                            mma_tf32(o[4 * b + e], pl, xh, yh);
+                            mma_tf32(o[4 * b + e], ph, xl, yl);
+                            mma_tf32(o[4 * b + e], ph, xh, yh);
+                        }
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int t = 0; t < NK; t += 2) {
+                    const uint32_t pa[4] = {pack2<T>(sacc[t][0], sacc[t][1]), pack2<T>(sacc[t][2], sacc[t][3]),
+                                            pack2<T>(sacc[t + 1][0], sacc[t + 1][1]), pack2<T>(sacc[t + 1][2], sacc[t + 1][3])};
+#pragma unroll
+                    for (int n = 0; n < NO; n += 2) {
+                        uint32_t b[4];
+                        ldsm4<1>(vt + F::at(8 * t + (lane & 15), n + (lane >> 4)), b);
+                        mma16<T>(o[n], pa, b[0], b[1]);
+                        mma16<T>(o[n + 1], pa, b[2], b[3]);
+                    }
+                }
+            }
+            slot = slot == kSlots - 1 ? 0 : slot + 1;
+        }
+        cp_wait<0>();
+        __syncthreads();  // every warp is done with its slots: they take the warps' rows [warp][row][HD]
+        float *rows = reinterpret_cast<float *>(few_smem);
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+            l[hh] = __fadd_rn(l[hh], __shfl_xor_sync(kAll, l[hh], 1));
+            l[hh] = __fadd_rn(l[hh], __shfl_xor_sync(kAll, l[hh], 2));
+            const int r = quad + 8 * hh;
+            if (r >= R) continue;
+            if (j == 0) ml_sh[warp][r][0] = m[hh], ml_sh[warp][r][1] = l[hh];
+            float *y = rows + (warp * kMaxRows + r) * HD;
+            if constexpr (F::F32) {
+#pragma unroll
+                for (int b = 0; b < HD / 32; ++b)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)  // channels 32 b + 8 j + 4 e ..
+                        *reinterpret_cast<float4 *>(y + 32 * b + 8 * j + 4 * e) =
+                            make_float4(o[4 * b][2 * hh + e], o[4 * b + 1][2 * hh + e], o[4 * b + 2][2 * hh + e], o[4 * b + 3][2 * hh + e]);
+            } else {
+#pragma unroll
+                for (int t = 0; t < NO; ++t)
+                    *reinterpret_cast<float2 *>(y + 8 * t + 2 * j) = make_float2(o[t][2 * hh], o[t][2 * hh + 1]);
+            }
+        }
+        __syncthreads();
+        // join the four warps in order; one thread per (row, four channels)
+        const int64_t pbase = (int64_t)(item - split * Hkv - g) * f.part_rows;  // first split's rows; Hkv items a split
+        for (int i = threadIdx.x; i < R * (HD / 4); i += kWarps * 32) {
+            const int r = i / (HD / 4), c = (i % (HD / 4)) * 4;
+            float M = -INFINITY, lt = 0.0f, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) M = fmaxf(M, ml_sh[w][r][0]);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float sc2 = M == -INFINITY ? 0.0f : ex2(__fsub_rn(ml_sh[w][r][0], M));
+                const float4 x = *reinterpret_cast<const float4 *>(rows + (w * kMaxRows + r) * HD + c);
+                lt = __fmaf_rn(ml_sh[w][r][1], sc2, lt);
+                y[0] = __fmaf_rn(x.x, sc2, y[0]), y[1] = __fmaf_rn(x.y, sc2, y[1]);
+                y[2] = __fmaf_rn(x.z, sc2, y[2]), y[3] = __fmaf_rn(x.w, sc2, y[3]);
+            }
+            if (odd_sh) {  // values that are not finite, from the positions that only some rows see
+                const int pos = p0 + r / G;
+                for (int k = k0; k < k1; ++k) {
+                    if (k >= all0 && k < all1) continue;
+                    if (k > pos || (a.window > 0 && k <= pos - a.window)) continue;
+                    const int b = block_of(k), page = __ldg(table + b);
+                    if (page < 0 || page >= a.kv.n_pages) continue;
+                    const T *v = reinterpret_cast<const T *>(vb) + (int64_t)page * a.kv.page_stride +
+                                 (int64_t)(k - b * P) * a.kv.token_stride + c;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (!isfinite(to_f(v[e]))) y[e] = __fadd_rn(y[e], to_f(v[e]));
+                }
+            }
+            if (nsplit == 1) {
+                const int tok = q.q0 + r / G, h = g * G + r % G;
+                const float inv = M == -INFINITY ? 0.0f : __frcp_rn(lt);
+                Vec<T, 4> out;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) out.e[e] = from_f<T>(__fmul_rn(y[e], inv));
+                *reinterpret_cast<Vec<T, 4> *>(static_cast<T *>(a.out) + (int64_t)tok * a.ldo + (int64_t)h * HD + c) = out;
+                if (a.lse && c == 0)
+                    a.lse[(int64_t)h * a.c.n_tokens + tok] = M == -INFINITY ? -INFINITY : __fadd_rn(M, log2f(lt));
+            } else if (item < f.max_items) {
+                float *p = f.part + ((int64_t)item * f.part_rows + r) * (HD + 4);
+                __stcg(reinterpret_cast<float4 *>(p + c), make_float4(y[0], y[1], y[2], y[3]));
+                if (c == 0) __stcg(reinterpret_cast<float2 *>(p + HD), make_float2(M, lt));
+            } else if (i == 0) {  // the lengths' sum is above its bound
+                set_status(a.c.status, ALTXS_ST_BAD_POS);
+            }
+        }
+        if (nsplit > 1) {
+            __threadfence();
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                uint32_t *cnt = f.cnt + (int64_t)s * Hkv + g;
+                const bool last = atomicAdd(cnt, 1u) == (uint32_t)nsplit - 1;
+                if (last) *cnt = 0;
+                __threadfence();
+                last_sh = last;
+            }
+            __syncthreads();
+            if (last_sh && item - (int64_t)split * Hkv + (int64_t)(nsplit - 1) * Hkv < f.max_items) {
+                // join the splits in order; the rows' maxima and sums first, in shared memory
+                float *ms = rows;  // [nsplit][R] weights, then [R] 1 / sum
+                const float *p0s = f.part + pbase * (HD + 4) + (int64_t)g * f.part_rows * (HD + 4);
+                const int64_t ps = (int64_t)Hkv * f.part_rows * (HD + 4);  // one split to the next
+                for (int r = threadIdx.x; r < R; r += kWarps * 32) {
+                    float M = -INFINITY, lt = 0.0f;
+                    for (int t = 0; t < nsplit; ++t) M = fmaxf(M, __ldcg(p0s + t * ps + r * (HD + 4) + HD));
+                    for (int t = 0; t < nsplit; ++t) {
+                        const float2 x = __ldcg(reinterpret_cast<const float2 *>(p0s + t * ps + r * (HD + 4) + HD));
+                        const float w = M == -INFINITY ? 0.0f : ex2(__fsub_rn(x.x, M));
+                        ms[t * R + r] = w;
+                        lt = __fmaf_rn(x.y, w, lt);
+                    }
+                    ms[nsplit * R + r] = M == -INFINITY ? 0.0f : __frcp_rn(lt);
+                    if (a.lse)
+                        a.lse[(int64_t)(g * G + r % G) * a.c.n_tokens + q.q0 + r / G] =
+                            M == -INFINITY ? -INFINITY : __fadd_rn(M, log2f(lt));
+                }
+                __syncthreads();
+                for (int i = threadIdx.x; i < R * (HD / 4); i += kWarps * 32) {
+                    const int r = i / (HD / 4), c = (i % (HD / 4)) * 4;
+                    float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+                    for (int t = 0; t < nsplit; ++t) {
+                        const float4 x = __ldcg(reinterpret_cast<const float4 *>(p0s + t * ps + r * (HD + 4) + c));
+                        const float w = ms[t * R + r];
+                        y[0] = __fmaf_rn(x.x, w, y[0]), y[1] = __fmaf_rn(x.y, w, y[1]);
+                        y[2] = __fmaf_rn(x.z, w, y[2]), y[3] = __fmaf_rn(x.w, w, y[3]);
+                    }
+                    const float inv = ms[nsplit * R + r];
+                    Vec<T, 4> out;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) out.e[e] = from_f<T>(__fmul_rn(y[e], inv));
+                    *reinterpret_cast<Vec<T, 4> *>(static_cast<T *>(a.out) + (int64_t)(q.q0 + r / G) * a.ldo +
+                                                   (int64_t)(g * G + r % G) * HD + c) = out;
+                }
+            }
+        }
+        __syncthreads();  // before the slots and the shared words are used again
+    }
+}
+
+// One warp per (token, head) of the sequences with more rows than the kernel
+// above takes: keys one at a time with a running maximum and sum.
 template <typename T, int HD>
 __global__ void __launch_bounds__(128) k_paged_rows(PagedAttnArgs a) {
     constexpr int E = HD / 32;
     const Seq s = load_seq_report(a.c, blockIdx.x);
+    if (s.n * (a.H / a.kv.n_kv_heads) <= kMaxRows) return;
     const int h = blockIdx.y, g = h / (a.H / a.kv.n_kv_heads), lane = threadIdx.x & 31;
     const float c2 = __fmul_rn(a.scale, kLog2e);
     for (int i = blockIdx.z * 4 + (threadIdx.x >> 5); i < s.n; i += gridDim.z * 4) {
@@ -48,24 +596,82 @@ __global__ void __launch_bounds__(128) k_paged_rows(PagedAttnArgs a) {
     }
 }
 
+// Workspace: arrival counters (zero between calls: a call's last arrivals reset
+// them), then partial rows.
+constexpr int64_t kCounters = 65536;  // more than these are cleared by the call that needs them
+
+struct Plan {
+    bool few, many;       // which kernels the host's bounds allow work for
+    int64_t items;        // few: bound on the items
+    int part_rows;
+    int64_t cnt_bytes, bytes;
+};
+Plan plan_of(const altxs_paged_kv &kv, const altxs_chunks &c, int H, int window) {
+    Plan p{};
+    const int G = H / kv.n_kv_heads;
+    const int64_t n = c.n_seqs;
+    if (n == 0 || c.max_new == 0) return p;
+    const bool same = c.n_tokens == n * c.max_new;  // every sequence has max_new tokens
+    p.many = (int64_t)c.max_new * G > kMaxRows;
+    p.few = G <= kMaxRows && (!p.many || !same);
+    const int64_t keys = window > 0 ? std::min<int64_t>(c.max_kv, (int64_t)window + c.max_new - 1) : c.max_kv;
+    int64_t total = n * keys;
+    if (c.total_kv > 0) total = std::min(total, c.total_kv);
+    const bool split = split_count((int)keys) > 1;
+    p.items = (split ? total / kSplitUnit + n : n) * kv.n_kv_heads;
+    p.part_rows = (int)std::min<int64_t>(kMaxRows, (int64_t)c.max_new * G);
+    p.cnt_bytes = align_up(4 * std::max(kCounters, n * kv.n_kv_heads), 256);
+    if (p.few && split) p.bytes = p.cnt_bytes + p.items * p.part_rows * (kv.head_dim + 4) * 4;
+    return p;
+}
+
+int sm_count() {
+    static int sms[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+    if (!sms[dev]) cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev);
+    return sms[dev] > 0 ? sms[dev] : 148;
+}
+
+template <typename T, int HD>
+int launch(const PagedAttnArgs &a, const Plan &p, cudaStream_t st) {
+    if (p.few) {
+        constexpr int smem = kWarps * kSlots * kChunkBytes;
+        FewArgs f{a, a.H / a.kv.n_kv_heads, 0, nullptr, nullptr, p.part_rows};
+        if (p.bytes > 0) {
+            f.max_items = p.items;
+            f.cnt = static_cast<uint32_t *>(a.ws);
+            f.part = reinterpret_cast<float *>(static_cast<unsigned char *>(a.ws) + p.cnt_bytes);
+            if ((int64_t)a.c.n_seqs * a.kv.n_kv_heads > kCounters &&
+                cudaMemsetAsync(f.cnt, 0, p.cnt_bytes, st) != cudaSuccess)
+                return ALTXS_ECUDA;
+        }
+        if (cudaFuncSetAttribute(k_paged_few<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+            return ALTXS_ECUDA;
+        const unsigned grid = (unsigned)std::min<int64_t>(p.items, 2 * sm_count());
+        ALTXS_LAUNCH(kKPaged, st, k_paged_few<T, HD><<<grid, kWarps * 32, smem, st>>>(f));
+    }
+    if (p.many) {
+        const dim3 grid(a.c.n_seqs, a.H, (unsigned)std::min(256, (a.c.max_new + 3) / 4));
+        ALTXS_LAUNCH(kKPaged, st, k_paged_rows<T, HD><<<grid, 128, 0, st>>>(a));
+    }
+    return ALTXS_OK;
+}
 template <typename T>
-void go(const PagedAttnArgs &a, cudaStream_t st) {
-    const dim3 grid(a.c.n_seqs, a.H, (unsigned)min(256, (a.c.max_new + 3) / 4));
-    if (a.kv.head_dim == 32) k_paged_rows<T, 32><<<grid, 128, 0, st>>>(a);
-    else if (a.kv.head_dim == 64) k_paged_rows<T, 64><<<grid, 128, 0, st>>>(a);
-    else k_paged_rows<T, 128><<<grid, 128, 0, st>>>(a);
+int launch(const PagedAttnArgs &a, const Plan &p, cudaStream_t st) {
+    return a.kv.head_dim == 32 ? launch<T, 32>(a, p, st) : a.kv.head_dim == 64 ? launch<T, 64>(a, p, st) : launch<T, 128>(a, p, st);
 }
 
 }  // namespace
 
-int64_t paged_attention_ws(const altxs_paged_kv &, const altxs_chunks &, int, int) { return 0; }
+int64_t paged_attention_ws(const altxs_paged_kv &kv, const altxs_chunks &c, int H, int window) {
+    return plan_of(kv, c, H, window).bytes;
+}
 
 int launch_paged_attention(const PagedAttnArgs &a, cudaStream_t st) {
-    if (a.c.max_new == 0) return ALTXS_OK;
-    if (a.kv.dtype == ALTXS_F32) ALTXS_LAUNCH(kKPaged, st, go<float>(a, st));
-    else if (a.kv.dtype == ALTXS_BF16) ALTXS_LAUNCH(kKPaged, st, go<__nv_bfloat16>(a, st));
-    else ALTXS_LAUNCH(kKPaged, st, go<__half>(a, st));
-    return ALTXS_OK;
+    const Plan p = plan_of(a.kv, a.c, a.H, a.window);
+    if (a.kv.dtype == ALTXS_F32) return launch<float>(a, p, st);
+    return a.kv.dtype == ALTXS_BF16 ? launch<__nv_bfloat16>(a, p, st) : launch<__half>(a, p, st);
 }
 
 }  // namespace altxs
