@@ -72,6 +72,16 @@ struct PagedAttnArgs {
     int64_t ws_bytes;
 };
 int64_t paged_attention_ws(const altxs_paged_kv &kv, const altxs_chunks &c, int H, int window);
+// The tensor-core kernel for many rows (16-bit types): bounds on its items and
+// partial slots from the host's bounds on the lengths.
+struct ManyPlan {
+    int64_t items, slots, slot_bytes;
+    int rows;  // rows of a slot
+};
+ManyPlan paged_many_plan(const altxs_paged_kv &kv, const altxs_chunks &c, int H, int window);
+int launch_paged_many(const PagedAttnArgs &a, const ManyPlan &p, int min_rows, uint32_t *cnt, float *part, int sms,
+                      cudaStream_t stream);
+int set_wait_limit_paged(uint32_t limit);
 int launch_paged_attention(const PagedAttnArgs &a, cudaStream_t stream);
 
 }  // namespace altxs

@@ -20,6 +20,7 @@
 // A split's rows go to the workspace as (m, l, o); the block that finishes the
 // last split of a (sequence, head) joins them in split order.
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "paged.cuh"
@@ -160,7 +161,7 @@ struct Few {
 };
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(kWarps * 32, 2) k_paged_few(FewArgs f) {
+__global__ void __launch_bounds__(kWarps * 32, 2) k_paged_few(const __grid_constant__ FewArgs f) {
     using F = Few<T, HD>;
     constexpr int CK = F::CK, NC = F::NC, NK = F::NK, NO = F::NO;
     extern __shared__ __align__(1024) unsigned char few_smem[];
@@ -604,7 +605,8 @@ struct Plan {
     bool few, many;       // which kernels the host's bounds allow work for
     int64_t items;        // few: bound on the items
     int part_rows;
-    int64_t cnt_bytes, bytes;
+    ManyPlan mp;
+    int64_t few_cnt, many_cnt, bytes;  // counters' bytes (both lists), then the partial rows, shared
 };
 Plan plan_of(const altxs_paged_kv &kv, const altxs_chunks &c, int H, int window) {
     Plan p{};
@@ -615,13 +617,19 @@ Plan plan_of(const altxs_paged_kv &kv, const altxs_chunks &c, int H, int window)
     p.many = (int64_t)c.max_new * G > kMaxRows;
     p.few = G <= kMaxRows && (!p.many || !same);
     const int64_t keys = window > 0 ? std::min<int64_t>(c.max_kv, (int64_t)window + c.max_new - 1) : c.max_kv;
-    int64_t total = n * keys;
+    int64_t total = n * keys, part = 0;
     if (c.total_kv > 0) total = std::min(total, c.total_kv);
     const bool split = split_count((int)keys) > 1;
     p.items = (split ? total / kSplitUnit + n : n) * kv.n_kv_heads;
     p.part_rows = (int)std::min<int64_t>(kMaxRows, (int64_t)c.max_new * G);
-    p.cnt_bytes = align_up(4 * std::max(kCounters, n * kv.n_kv_heads), 256);
-    if (p.few && split) p.bytes = p.cnt_bytes + p.items * p.part_rows * (kv.head_dim + 4) * 4;
+    if (p.few && split) part = p.items * p.part_rows * (kv.head_dim + 4) * 4;
+    if (p.many && kv.dtype != ALTXS_F32) {
+        p.mp = paged_many_plan(kv, c, H, window);
+        part = std::max(part, p.mp.slots * p.mp.slot_bytes);
+    }
+    p.few_cnt = align_up(4 * std::max(kCounters, n * kv.n_kv_heads), 256);
+    p.many_cnt = align_up(4 * std::max(kCounters, p.mp.slots), 256);
+    if (part > 0) p.bytes = p.few_cnt + p.many_cnt + part;
     return p;
 }
 
@@ -635,25 +643,38 @@ int sm_count() {
 
 template <typename T, int HD>
 int launch(const PagedAttnArgs &a, const Plan &p, cudaStream_t st) {
+    unsigned char *ws = static_cast<unsigned char *>(a.ws);
+    uint32_t *few_cnt = nullptr, *many_cnt = nullptr;
+    float *part = nullptr;
+    if (p.bytes > 0) {
+        few_cnt = reinterpret_cast<uint32_t *>(ws);
+        many_cnt = reinterpret_cast<uint32_t *>(ws + p.few_cnt);
+        part = reinterpret_cast<float *>(ws + p.few_cnt + p.many_cnt);
+        if ((p.few_cnt > 4 * kCounters || p.many_cnt > 4 * kCounters) &&
+            cudaMemsetAsync(ws, 0, p.few_cnt + p.many_cnt, st) != cudaSuccess)
+            return ALTXS_ECUDA;
+    }
     if (p.few) {
         constexpr int smem = kWarps * kSlots * kChunkBytes;
-        FewArgs f{a, a.H / a.kv.n_kv_heads, 0, nullptr, nullptr, p.part_rows};
-        if (p.bytes > 0) {
-            f.max_items = p.items;
-            f.cnt = static_cast<uint32_t *>(a.ws);
-            f.part = reinterpret_cast<float *>(static_cast<unsigned char *>(a.ws) + p.cnt_bytes);
-            if ((int64_t)a.c.n_seqs * a.kv.n_kv_heads > kCounters &&
-                cudaMemsetAsync(f.cnt, 0, p.cnt_bytes, st) != cudaSuccess)
+        static std::atomic<uint64_t> set{0};  // devices whose shared-memory limit is raised
+        int dev = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess) return ALTXS_ECUDA;
+        if (dev >= 64 || !((set.load() >> dev) & 1)) {
+            if (cudaFuncSetAttribute(k_paged_few<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
                 return ALTXS_ECUDA;
+            if (dev < 64) set.fetch_or(1ull << dev);
         }
-        if (cudaFuncSetAttribute(k_paged_few<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-            return ALTXS_ECUDA;
+        const FewArgs f{a, a.H / a.kv.n_kv_heads, p.bytes > 0 ? p.items : 0, few_cnt, part, p.part_rows};
         const unsigned grid = (unsigned)std::min<int64_t>(p.items, 2 * sm_count());
         ALTXS_LAUNCH(kKPaged, st, k_paged_few<T, HD><<<grid, kWarps * 32, smem, st>>>(f));
     }
     if (p.many) {
-        const dim3 grid(a.c.n_seqs, a.H, (unsigned)std::min(256, (a.c.max_new + 3) / 4));
-        ALTXS_LAUNCH(kKPaged, st, k_paged_rows<T, HD><<<grid, 128, 0, st>>>(a));
+        if constexpr (sizeof(T) == 2) {
+            return launch_paged_many(a, p.mp, kMaxRows + 1, many_cnt, part, sm_count(), st);
+        } else {
+            const dim3 grid(a.c.n_seqs, a.H, (unsigned)std::min(256, (a.c.max_new + 3) / 4));
+            ALTXS_LAUNCH(kKPaged, st, k_paged_rows<T, HD><<<grid, 128, 0, st>>>(a));
+        }
     }
     return ALTXS_OK;
 }

@@ -1,0 +1,800 @@
+// Attention of many new tokens over a paged key/value cache (16-bit types) on
+// the tensor cores, the scores never leaving the SM.
+//
+// The rows of one key/value head (its G query heads x the sequence's new
+// tokens, row = token * G + head) are cut into blocks of 256; an item is one
+// split of one block's visible key tiles (128 positions each), taken by a
+// persistent block of 12 warps:
+//   warps 0-3, 4-7  softmax groups 0 and 1, one score row per thread;
+//   warp 8          issues the MMAs: S = Q K^T into a group's tensor-memory
+//                   score columns, then (P written over S) O += P V, P read
+//                   from tensor memory, V as it lies (MN-major);
+//   warps 9-11      gather key and value rows through the page table with
+//                   16-byte asynchronous copies into a ring of tiles, rows
+//                   that no position of the block needs filled with zeros.
+// With more than 128 rows each group owns 128 of them and every key tile
+// serves both; with at most 128 the two groups share the rows and take even
+// and odd key tiles, and group 0 joins both outputs at the end.  Either way
+// the MMA warp alternates between the groups, so one group's softmax runs
+// under the other's MMAs.
+//
+// Softmax: x = s scale log2(e) in fp32, p = 2^(x - m) rounded once to the
+// 16-bit type, the sum from the unrounded p.  m follows the running maximum
+// only when that grows by more than 2^8: until then p <= 256 is as exact, and
+// O (fp32, in tensor memory) is not touched.
+//
+// Splits of a block go to the workspace as (m, l, O); the item that arrives
+// last joins them in split order.  Tiles, blocks and splits are functions of
+// the sequence's own lengths, so a row's bits do not depend on the batch.
+//
+// Every wait is bounded: one that gives up stops the block's roles, which let
+// their copies and MMAs finish, and sets ALTXS_ST_TIMEOUT.
+#include <algorithm>
+#include <atomic>
+#include <type_traits>
+
+#include "paged.cuh"
+#include "prof.cuh"
+#include "tcgen05.cuh"
+
+namespace altxs {
+namespace {
+
+constexpr int kTile = 128;       // positions per key tile
+constexpr int kBlockRows = 256;  // rows per item
+constexpr int kMmaWarp = 8, kProducers = 3;
+constexpr int kScan = 128;  // sequences are counted in this many groups
+constexpr int kMostItems = 1184;  // of a sequence that is split (8 waves)
+constexpr int kThreadsTc = (kMmaWarp + 1 + kProducers) * 32;
+constexpr int kMaskRing = 16;  // key tiles (and items) the producers can be ahead of the softmax, at most
+constexpr unsigned kAll = 0xffffffffu;
+constexpr float kLazy = 8.0f;
+
+template <int HD>
+struct Tc {
+    static constexpr int RowB = HD * 2;
+    static constexpr int Halves = HD > 64 ? 2 : 1;      // 64-channel halves of a tile, 16 KB each
+    static constexpr int TileB = Halves * kTile * 128;  // HD 32 leaves half of each 128-byte row unused
+    static constexpr int Slots = HD > 64 ? 5 : 12;
+    static constexpr int Lag = HD > 64 ? 3 : HD > 32 ? 6 : 8;  // tiles a producer has in flight behind the newest
+    static constexpr int Smem = 2 * TileB + Slots * TileB + 1024;
+    static constexpr uint32_t ColS = 0, ColO = 2 * kTile;  // group i: S at 128 i, O at 256 + HD i
+    static_assert(Smem + 2048 <= 227 * 1024, "shared memory (with the static part)");
+};
+
+// one sequence's share of the work
+struct Shape {
+    int R, blocks, nsplit;
+};
+__host__ __device__ inline int tiles_of(int keys) { return (keys + kTile - 1) / kTile; }
+// Splits of every block of a sequence: enough items to fill the 148 SMs in whole
+// waves by itself, at least 8 key tiles each (a split costs about 1.5 tiles' time).
+__host__ __device__ inline int many_splits(int items, int nt) {
+    constexpr int kSms = 148;
+    int most = nt / 8 < 16 ? nt / 8 : 16;
+    if (items >= 4 * kSms || most < 2) return 1;
+    int best = 1;
+    float cost = 3e38f;
+    for (int ns = 1; ns <= most && (ns == 1 || items * ns <= kMostItems); ++ns) {
+        const float c = (float)((items * ns + kSms - 1) / kSms) * ((float)nt / (float)ns + 1.5f);
+        if (c < cost * 0.99f) cost = c, best = ns;
+    }
+    return best;
+}
+
+struct ManyArgs {
+    PagedAttnArgs a;
+    int G, min_rows;    // sequences with at least min_rows rows are this kernel's
+    int64_t max_slots;  // partial slots in the workspace (one per item of a split sequence)
+    uint32_t *cnt;      // [max_slots], zero between calls
+    float *part;        // [max_slots][part_rows * (HD + 2)]
+    int part_rows;
+};
+
+__device__ __forceinline__ Shape shape_of(const ManyArgs &f, const Seq &q) {
+    Shape w{0, 0, 0};
+    if (q.n <= 0 || q.n * f.G < f.min_rows) return w;
+    w.R = q.n * f.G;
+    w.blocks = (w.R + kBlockRows - 1) / kBlockRows;
+    // the longest block: the last 256 rows' keys
+    const int rows = min(w.R, kBlockRows), toks = (rows + f.G - 1) / f.G;
+    const int keys = f.a.window > 0 ? min(q.L, f.a.window + toks - 1) : q.L;
+    w.nsplit = many_splits(w.blocks * f.a.kv.n_kv_heads, tiles_of(max(keys, 0)));
+    return w;
+}
+
+struct Scan {
+    int before[kScan + 1], slots[kScan + 1];  // items, and items of split sequences, before each group
+    int per;
+};
+
+struct Item {
+    Seq q;
+    int s, g, nsplit, split;
+    int r0, rows;        // rows of the block
+    int lo, t0, t1, hi;  // positions lo + 128 t of key tiles t0 .. t1 of this split; the block sees [lo, hi)
+    bool two;            // two row tiles (both groups over every key tile)
+    int slot;            // partial slot of the block's split 0
+};
+
+__device__ __forceinline__ Item locate(const ManyArgs &f, const Scan &sc, int item) {
+    int lo = 0, hi = kScan;
+    while (hi - lo > 1) {
+        const int m = (lo + hi) >> 1;
+        if (sc.before[m] <= item) lo = m; else hi = m;
+    }
+    Item it;
+    const int Hkv = f.a.kv.n_kv_heads;
+    it.s = lo * sc.per;
+    int local = item - sc.before[lo], slot = sc.slots[lo];
+    it.q = load_seq(f.a.c, it.s);
+    Shape w = shape_of(f, it.q);
+    for (int n; it.s < f.a.c.n_seqs - 1 && local >= (n = w.blocks * w.nsplit * Hkv); w = shape_of(f, it.q)) {
+        local -= n;
+        if (w.nsplit > 1) slot += n;
+        it.q = load_seq(f.a.c, ++it.s);
+    }
+    it.nsplit = w.nsplit;
+    it.split = local % w.nsplit;
+    it.slot = slot + local - it.split;
+    local /= w.nsplit;
+    it.g = local % Hkv;
+    const int blk = w.blocks - 1 - local / Hkv;  // the longest blocks first
+    it.r0 = blk * kBlockRows;
+    it.rows = min(w.R - it.r0, kBlockRows);
+    it.two = it.rows > kTile;
+    const int p0 = it.q.L - it.q.n, i0 = it.r0 / f.G, i1 = (it.r0 + it.rows - 1) / f.G;
+    it.hi = max(0, p0 + i1 + 1);
+    it.lo = f.a.window > 0 ? max(0, p0 + i0 - f.a.window + 1) : 0;
+    const int nt = tiles_of(max(0, it.hi - it.lo)), per = (nt + it.nsplit - 1) / it.nsplit;
+    it.t0 = min(nt, it.split * per);
+    it.t1 = min(nt, it.t0 + per);
+    return it;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void sts16(uint32_t addr, uint4 v) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+}
+template <typename T>
+constexpr uint32_t idesc(int n, int bmn) {  // kind::f16, fp32 sums, M = 128, A K-major
+    const uint32_t fmt = std::is_same<T, __half>::value ? 0u : 1u;
+    return (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)bmn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+// D += A B with A (rows = lanes, two 16-bit values per column) in tensor memory
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(id), "r"(accumulate)
+        : "memory");
+}
+#define ALTXS_R32(v) \
+    "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), \
+    "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), \
+    "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), \
+    "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+__device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t *v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        ALTXS_R32(v)
+        : "memory");
+}
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// 32 columns without waiting; tc_wait_ld, then tc_tie32 before the values are used
+__device__ __forceinline__ void tc_ld32_nowait(uint32_t taddr, float *f) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+#pragma unroll
+    for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_tie32(float *f) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 8)
+        asm volatile("" : "+f"(f[i]), "+f"(f[i + 1]), "+f"(f[i + 2]), "+f"(f[i + 3]), "+f"(f[i + 4]), "+f"(f[i + 5]),
+                          "+f"(f[i + 6]), "+f"(f[i + 7])::"memory");
+}
+
+// The values of channel `dim` that are not finite, over the positions [lo, hi) that a
+// row at `pos` sees (the tiles that only some rows see hold 0 in their place).
+template <typename T>
+__device__ __noinline__ float odd_term(const PagedAttnArgs &a, int s, int g, int pos, int lo, int hi, int dim) {
+    float y = 0.0f;
+    for (int k = max(lo, a.window > 0 ? pos - a.window + 1 : 0); k < min(hi, pos + 1); ++k) {
+        const int b = k / a.kv.page_size, page = __ldg(a.c.page_table + s * a.c.table_stride + b);
+        if (page < 0 || page >= a.kv.n_pages) continue;
+        const float v = to_f(static_cast<const T *>(a.kv.v)[page * a.kv.page_stride +
+                                                           (int64_t)(k - b * a.kv.page_size) * a.kv.token_stride +
+                                                           g * a.kv.head_stride + dim]);
+        if (!isfinite(v)) y = __fadd_rn(y, v);
+    }
+    return y;
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kThreadsTc, 1) k_paged_many(const __grid_constant__ ManyArgs f) {
+    using C = Tc<HD>;
+    extern __shared__ unsigned char pm_smem_raw[];
+    __shared__ __align__(8) uint64_t full[C::Slots], empty[C::Slots], s_full[2], p_full[2], o_done[2], q_full, drainb;
+    __shared__ Scan sc;
+    __shared__ uint32_t tmem_sh, kmask[kMaskRing][4], odd_sh[kMaskRing][kProducers];
+    __shared__ int2 wsum[kScan / 32];
+    __shared__ int last_sh, stop_sh;
+    __shared__ volatile int abort_sh;
+    const PagedAttnArgs &a = f.a;
+    const uint32_t raw_s = smem_u32(pm_smem_raw);
+    const uint32_t sq = raw_s + ((1024u - (raw_s & 1023u)) & 1023u), ring = sq + 2 * C::TileB;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int s = 0; s < C::Slots; ++s) {
+            mbar_init(&full[s], kProducers);
+            mbar_init(&empty[s], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 4);
+            mbar_init(&o_done[i], 1);
+        }
+        mbar_init(&q_full, 8);
+        mbar_init(&drainb, 1);
+        abort_sh = 0;
+        fence_mbar_init();
+    }
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_sh)), "r"(512u)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (warp < kScan / 32) {  // items of the sequences before each thread's group of them
+        const int n = a.c.n_seqs, per = (n + kScan - 1) / kScan;
+        int sum = 0, cut = 0;
+        for (int s = tid * per; s < min(n, (tid + 1) * per); ++s) {
+            const Shape w = shape_of(f, blockIdx.x == 0 ? load_seq_report(a.c, s) : load_seq(a.c, s));
+            const int k = w.blocks * w.nsplit * a.kv.n_kv_heads;
+            sum += k;
+            if (w.nsplit > 1) cut += k;
+        }
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(kAll, sum, o), u = __shfl_up_sync(kAll, cut, o);
+            if (lane >= o) sum += v, cut += u;
+        }
+        if (lane == 31) wsum[warp] = make_int2(sum, cut);
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        for (int w = 0; w < warp; ++w) sum += wsum[w].x, cut += wsum[w].y;
+        sc.before[tid + 1] = sum, sc.slots[tid + 1] = cut;
+        if (tid == 0) sc.before[0] = sc.slots[0] = 0, sc.per = per;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_sh;
+    const int total = sc.before[kScan];
+
+    if (warp > kMmaWarp) {
+        // ---- producers ----
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        const int pw = warp - kMmaWarp - 1;
+        constexpr int NC = C::RowB / 16, KPI = 32 / NC;  // 16-byte pieces of a row, rows per warp copy
+        const int P = a.kv.page_size, pshift = (P & (P - 1)) == 0 ? 31 - __clz(P) : -1;
+        auto block_of = [&](int k) { return pshift >= 0 ? k >> pshift : k / P; };
+        // Warp pw copies the 8-row groups pw, pw + 3, .. of every tile: at most 6 of 16.
+        constexpr int kGroups = (kTile / 8 + kProducers - 1) / kProducers;
+        uint32_t n = 0, kt = 0, live = 0;  // slots, key tiles and items with tiles so far
+        uint32_t done = 0;                 // slots published
+        bool ok = true;
+        // a published slot needs its values checked when only some rows see them
+        uint32_t check = 0;                // bit (slot n & 31): check before publishing
+        uint32_t odd_of = 0;
+        auto publish = [&](uint32_t m) {   // slot number m has landed (this warp's share)
+            const uint32_t base = ring + (m % C::Slots) * C::TileB;
+            if ((check >> (m & 31)) & 1) {
+                bool odd = false;
+                for (int i = 0; i < kGroups; ++i) {
+                    const int grp = pw + i * kProducers;
+                    if (grp >= kTile / 8) break;
+#pragma unroll
+                    for (int e = 0; e < 8 / KPI; ++e) {
+                        const int r = grp * 8 + e * KPI + lane / NC, c = lane % NC;
+                        const uint32_t d = base + (c >> 3) * (kTile * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                        uint4 v = lds16(d);
+                        uint32_t *w = reinterpret_cast<uint32_t *>(&v);
+                        bool bad = false;
+                        constexpr uint32_t X = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            if ((w[u] & X) == X) w[u] &= 0xffff0000u, bad = true;
+                            if (((w[u] >> 16) & X) == X) w[u] &= 0xffffu, bad = true;
+                        }
+                        if (bad) sts16(d, v), odd = true;
+                    }
+                }
+                check &= ~(1u << (m & 31));
+                if (__any_sync(kAll, odd) && lane == 0) odd_sh[odd_of % kMaskRing][pw] = 1;
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[m % C::Slots]);
+        };
+        for (int item = blockIdx.x; item < total && ok; item += gridDim.x) {
+            const Item it = locate(f, sc, item);
+            if (it.t0 == it.t1) continue;
+            const int p0 = it.q.L - it.q.n, i0 = it.r0 / f.G, i1 = (it.r0 + it.rows - 1) / f.G;
+            const int32_t *table = a.c.page_table + it.s * a.c.table_stride;
+            const char *kbase = static_cast<const char *>(a.kv.k) + (int64_t)it.g * a.kv.head_stride * 2;
+            const char *vbase = static_cast<const char *>(a.kv.v) + (int64_t)it.g * a.kv.head_stride * 2;
+            // the slots still on their way belong to the previous item: publish them under its flag
+            if (check != 0) {
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+                while (done < n) publish(done++);
+            }
+            odd_of = live++;
+            if (lane == 0) odd_sh[odd_of % kMaskRing][pw] = 0;
+            for (int t = it.t0; t < it.t1 && ok; ++t) {
+                const int kb = it.lo + t * kTile;
+                // offsets of this warp's rows: lane 8 i' + r holds row r of its i'-th group (two rounds)
+                int64_t off[2];
+                uint32_t seen[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int grp = pw + (4 * e + lane / 8) * kProducers, k = kb + grp * 8 + lane % 8;
+                    const bool want = grp < kTile / 8 && k < it.hi;
+                    const int b = want ? block_of(k) : 0, page = want ? __ldg(table + b) : -1;
+                    const bool in = page >= 0 && page < a.kv.n_pages;
+                    if (want && !in) set_status(a.c.status, ALTXS_ST_BAD_POS);
+                    off[e] = in ? ((int64_t)page * a.kv.page_stride + (int64_t)(k - b * P) * a.kv.token_stride) * 2 : -1;
+                    seen[e] = __ballot_sync(kAll, in);
+                }
+                if (lane < kGroups) {  // which rows exist, for the softmax
+                    const int grp = pw + lane * kProducers;
+                    if (grp < kTile / 8)
+                        reinterpret_cast<uint8_t *>(kmask[kt % kMaskRing])[grp] = (uint8_t)(seen[lane / 4] >> (8 * (lane % 4)));
+                }
+                ++kt;
+                // every row of the block sees the whole tile?
+                const bool whole = kb + kTile <= p0 + i0 + 1 && (a.window == 0 || kb > p0 + i1 - a.window);
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv, ++n) {
+                    const uint32_t s = n % C::Slots;
+                    if (n >= C::Slots) {
+                        // let what has landed go out before blocking on a slot that waits for it
+                        bool free_now = mbar_try_wait(&empty[s], ((n / C::Slots) - 1) & 1);
+                        if (!__all_sync(kAll, free_now)) {
+                            asm volatile("cp.async.wait_group 0;" ::: "memory");
+                            while (done < n) publish(done++);
+                            ok = __all_sync(kAll, !abort_sh && mbar_wait_bounded(&empty[s], ((n / C::Slots) - 1) & 1, wait_limit()));
+                            if (!ok) break;
+                        }
+                    }
+                    const char *src0 = kv ? vbase : kbase;
+                    const uint32_t dst = ring + s * C::TileB;
+#pragma unroll
+                    for (int i = 0; i < kGroups; ++i) {
+                        const int grp = pw + i * kProducers;
+                        if (grp < kTile / 8) {
+#pragma unroll
+                            for (int e = 0; e < 8 / KPI; ++e) {
+                                const int r8 = e * KPI + lane / NC, r = grp * 8 + r8, c = lane % NC;
+                                const int64_t o = __shfl_sync(kAll, off[i / 4], (i % 4) * 8 + r8);
+                                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                                                 dst + (c >> 3) * (kTile * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)),
+                                             "l"(src0 + (o < 0 ? 0 : o) + c * 16), "r"(o < 0 ? 0u : 16u)
+                                             : "memory");
+                            }
+                        }
+                    }
+                    asm volatile("cp.async.commit_group;" ::: "memory");
+                    if (kv && !whole && i1 > i0) check |= 1u << (n & 31);
+                    if (n - done >= C::Lag) {
+                        asm volatile("cp.async.wait_group %0;" ::"n"(C::Lag) : "memory");
+                        publish(done++);
+                    }
+                }
+            }
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        while (done < n) publish(done++);
+        if (!ok) abort_sh = 1;
+    } else if (warp == kMmaWarp) {
+        // ---- MMA issuer ----
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (lane == 0) {
+            uint32_t n = 0, items = 0, jobs[2] = {0, 0};  // slots and items so far; PV jobs issued per group
+            bool ok = true;
+            for (int item = blockIdx.x; item < total && ok; item += gridDim.x) {
+                const Item it = locate(f, sc, item);
+                const int nt = it.t1 - it.t0;
+                if (nt == 0) continue;
+                ok = mbar_wait_bounded(&q_full, items & 1, wait_limit());
+                ++items;
+                const int T2 = it.two ? 2 * nt : nt;  // jobs: (group t & 1, tile t / 2 or t)
+                for (int t = 0; t < T2 + 2 && ok && !abort_sh; ++t) {
+                    const int i = t & 1;
+                    if (t >= 2) {  // O_i += P V of job t - 2
+                        const int j = it.two ? (t - 2) / 2 : t - 2;
+                        const uint32_t v = n + 2 * j + 1, s = v % C::Slots;
+                        if (!mbar_wait_bounded(&full[s], (v / C::Slots) & 1, wait_limit()) ||
+                            !mbar_wait_bounded(&p_full[i], jobs[i] & 1, wait_limit())) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint32_t vb = ring + s * C::TileB;
+#pragma unroll
+                        for (int kk = 0; kk < kTile / 16; ++kk)
+                            tc_mma_ts(tmem + C::ColO + HD * i, tmem + C::ColS + kTile * i + 8 * kk,
+                                      sw128_desc(vb + kk * 2048, kTile * 128), idesc<T>(HD, 1), t >= 4 || kk != 0);
+                        tc_commit(&o_done[i]);
+                        ++jobs[i];
+                        if (!it.two || i == 1) tc_commit(&empty[s]);
+                    }
+                    if (t < T2) {  // S_i = Q K^T of job t
+                        const int j = it.two ? t / 2 : t;
+                        const uint32_t k = n + 2 * j, s = k % C::Slots;
+                        if (!mbar_wait_bounded(&full[s], (k / C::Slots) & 1, wait_limit())) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint32_t kb = ring + s * C::TileB, qb = sq + (it.two ? i * C::TileB : 0);
+#pragma unroll
+                        for (int kk = 0; kk < HD / 16; ++kk) {
+                            const uint32_t o = (kk >> 2) * (kTile * 128) + (kk & 3) * 32;
+                            tc_mma(tmem + C::ColS + kTile * i, sw128_desc(qb + o, 16), sw128_desc(kb + o, 16),
+                                   idesc<T>(kTile, 0), kk != 0);
+                        }
+                        tc_commit(&s_full[i]);
+                        if (!it.two || i == 1) tc_commit(&empty[s]);
+                    }
+                }
+                n += 2 * nt;
+                ok = ok && !abort_sh;
+            }
+            if (!ok) abort_sh = 1;
+            tc_commit(&drainb);  // every MMA has completed before the block can exit
+            mbar_wait_bounded(&drainb, 0, kWaitLimit);
+        }
+        __syncwarp();
+    } else {
+        // ---- softmax ----
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        const int grp = warp >> 2, row = (warp & 3) * 32 + lane;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem + lanes + C::ColS + kTile * grp, to = tmem + lanes + C::ColO + HD * grp;
+        // a negative scale turns the queries round instead; a scale of 0 stays above it (-inf marks the unseen)
+        const float c2 = fmaxf(__fmul_rn(fabsf(a.scale), kLog2e), 1.17549435e-38f);
+        // group 1's (m, l) on their way to group 0, in the second query tile's place
+        float2 *ml = reinterpret_cast<float2 *>(pm_smem_raw + (sq - raw_s) + C::TileB);
+        const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+        uint32_t job = 0, kt = 0, live = 0;
+        bool ok = true;
+        for (int item = blockIdx.x; item < total; item += gridDim.x) {
+            const Item it = locate(f, sc, item);
+            const int nt = it.t1 - it.t0, p0 = it.q.L - it.q.n;
+            // this thread's row of the block (rows past the end follow the last one and are not stored)
+            const int r_own = it.two ? grp * kTile + row : row;
+            const int r = it.r0 + min(r_own, it.rows - 1), tok = r / f.G, h = it.g * f.G + r - tok * f.G;
+            const int pos = p0 + tok;
+            const bool mine = r_own < it.rows;
+            float m = -INFINITY, l = 0.0f;
+            uint32_t njob = 0;  // jobs of this group in this item
+            if (nt > 0) {
+                if (it.two || grp == 0) {  // the row's query
+                    const uint4 *qp = reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) +
+                                                                     (int64_t)(it.q.q0 + tok) * a.ldq + (int64_t)h * HD);
+                    const uint32_t d = sq + (it.two ? grp * C::TileB : 0) + row * 128;
+#pragma unroll
+                    for (int c = 0; c < HD / 8; ++c) {
+                        uint4 v = __ldg(qp + c);
+                        v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
+                        sts16(d + (c >> 3) * (kTile * 128) + (((c & 7) ^ (row & 7)) << 4), v);
+                    }
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&q_full);
+                // positions that all of this warp's rows see: from the first row's and the last row's
+                const int ra = it.r0 + min(it.two ? grp * kTile + (warp & 3) * 32 : (warp & 3) * 32, it.rows - 1);
+                const int rb = it.r0 + min(it.two ? grp * kTile + (warp & 3) * 32 + 31 : (warp & 3) * 32 + 31, it.rows - 1);
+                const int pa = p0 + ra / f.G, pb = p0 + rb / f.G;
+                for (int j = it.two ? 0 : grp; j < nt && ok; j += it.two ? 1 : 2) {
+                    const int kb = it.lo + (it.t0 + j) * kTile;
+                    ok = __all_sync(kAll, !abort_sh && mbar_wait_bounded(&s_full[grp], job & 1, wait_limit()));
+                    if (!ok) break;
+                    tc_fence_after();
+                    float x[kTile];
+#pragma unroll
+                    for (int c = 0; c < kTile; c += 32) tc_ld32_nowait(ts + c, x + c);
+                    const uint32_t *km = kmask[(kt + j) % kMaskRing];
+                    const uint32_t m0 = km[0], m1 = km[1], m2 = km[2], m3 = km[3];
+                    tc_wait_ld();
+#pragma unroll
+                    for (int c = 0; c < kTile; c += 32) tc_tie32(x + c);
+                    const bool whole = kb + kTile <= pa + 1 && (a.window == 0 || kb > pb - a.window) &&
+                                       (m0 & m1 & m2 & m3) == kAll;
+                    if (!whole) {
+                        const int first = a.window > 0 ? max(0, pos - a.window + 1 - kb) : 0, last = pos - kb;
+#pragma unroll
+                        for (int u = 0; u < kTile; ++u) {
+                            const uint32_t mk = u < 32 ? m0 : u < 64 ? m1 : u < 96 ? m2 : m3;
+                            if (u < first || u > last || !((mk >> (u & 31)) & 1)) x[u] = -INFINITY;
+                        }
+                    }
+                    float mx = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+                    for (int u = 0; u < kTile; u += 4) {
+                        mx = fmaxf(mx, fmaxf(x[u], x[u + 1]));
+                        mx1 = fmaxf(mx1, fmaxf(x[u + 2], x[u + 3]));
+                    }
+                    mx = fmaxf(mx, mx1);
+                    mx = mx == -INFINITY ? mx : __fmul_rn(mx, c2);
+                    const bool grow = mx > __fadd_rn(m, kLazy) || (m == -INFINITY && mx > m);
+                    if (__any_sync(kAll, grow)) {
+                        const float mn = grow ? mx : m;
+                        const float fold = m == -INFINITY ? 0.0f : grow ? ex2(__fsub_rn(m, mn)) : 1.0f;
+                        l = __fmul_rn(l, fold);
+                        m = mn;
+                        if (njob > 0) {  // O of the jobs so far, once the last of them is complete
+                            ok = __all_sync(kAll, mbar_wait_bounded(&o_done[grp], (job - 1) & 1, wait_limit()));
+                            if (!ok) break;
+                            tc_fence_after();
+#pragma unroll
+                            for (int c = 0; c < HD; c += 32) {
+                                float v[32];
+                                tc_ld32(to + c, v);
+                                uint32_t w[32];
+#pragma unroll
+                                for (int u = 0; u < 32; ++u) w[u] = __float_as_uint(__fmul_rn(v[u], fold));
+                                tc_st32(to + c, w);
+                            }
+                            tc_wait_st();
+                        }
+                    }
+                    const float base = m == -INFINITY ? 0.0f : m;
+                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int c = 0; c < kTile; c += 64) {
+                        uint32_t w[32];
+#pragma unroll
+                        for (int u = 0; u < 64; u += 2) {
+                            const float e0 = ex2(__fmaf_rn(x[c + u], c2, -base)), e1 = ex2(__fmaf_rn(x[c + u + 1], c2, -base));
+                            sum[u & 2] = __fadd_rn(sum[u & 2], e0);
+                            sum[(u & 2) + 1] = __fadd_rn(sum[(u & 2) + 1], e1);
+                            w[u / 2] = pack2<T>(e0, e1);
+                        }
+                        tc_st32(ts + c / 2, w);
+                    }
+                    l = __fadd_rn(l, __fadd_rn(__fadd_rn(sum[0], sum[1]), __fadd_rn(sum[2], sum[3])));
+                    tc_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[grp]);
+                    ++job;
+                    ++njob;
+                }
+                kt += nt;
+                if (ok && njob > 0) {
+                    ok = __all_sync(kAll, mbar_wait_bounded(&o_done[grp], (job - 1) & 1, wait_limit()));
+                    tc_fence_after();
+                }
+            }
+            if (!ok) abort_sh = 1;
+            // ---- the item's rows: group 0 joins group 1's when they shared them ----
+            if (!it.two && grp == 1) ml[row] = make_float2(m, l);
+            tc_fence_before();
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            tc_fence_after();
+            ok = !abort_sh;
+            if (ok && (it.two || grp == 0)) {
+                float f0 = 1.0f, f1 = 0.0f;
+                const bool other = !it.two && nt > 1;  // group 1 had tiles
+                if (other) {
+                    const float2 o1 = ml[row];
+                    const float m1 = o1.x, M = fmaxf(m, m1);
+                    f0 = m == -INFINITY ? 0.0f : ex2(__fsub_rn(m, M));
+                    f1 = m1 == -INFINITY ? 0.0f : ex2(__fsub_rn(m1, M));
+                    l = __fmaf_rn(o1.y, f1, __fmul_rn(l, f0));
+                    m = M;
+                }
+                bool odd = false;
+                if (nt > 0)
+#pragma unroll
+                    for (int e = 0; e < kProducers; ++e) odd = odd || odd_sh[live % kMaskRing][e] != 0;
+                const bool fin = it.nsplit == 1;
+                const float inv = m == -INFINITY ? 0.0f : __frcp_rn(l), w0 = fin ? __fmul_rn(f0, inv) : f0,
+                            w1 = fin ? __fmul_rn(f1, inv) : f1;
+                const bool room = it.slot + it.nsplit <= f.max_slots;
+                float4 *pp = reinterpret_cast<float4 *>(f.part + (int64_t)(it.slot + it.split) * f.part_rows * (HD + 2));
+                T *yp = static_cast<T *>(a.out) + (int64_t)(it.q.q0 + tok) * a.ldo + (int64_t)h * HD;
+#pragma unroll
+                for (int c = 0; c < HD; c += 32) {
+                    float v[32];
+                    if (nt > 0) {
+                        tc_ld32(to + c, v);
+#pragma unroll
+                        for (int u = 0; u < 32; ++u) v[u] = __fmul_rn(v[u], w0);
+                        if (other) {
+                            float v1[32];
+                            tc_ld32(to + HD + c, v1);
+#pragma unroll
+                            for (int u = 0; u < 32; ++u) v[u] = __fmaf_rn(v1[u], w1, v[u]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < 32; ++u) v[u] = 0.0f;
+                    }
+                    if (fin) {
+                        if (mine)
+#pragma unroll
+                            for (int u = 0; u < 32; u += 8) {
+                                uint4 y;
+                                y.x = pack2<T>(v[u], v[u + 1]), y.y = pack2<T>(v[u + 2], v[u + 3]);
+                                y.z = pack2<T>(v[u + 4], v[u + 5]), y.w = pack2<T>(v[u + 6], v[u + 7]);
+                                *reinterpret_cast<uint4 *>(yp + c + u) = y;
+                            }
+                    } else if (room) {
+#pragma unroll
+                        for (int u = 0; u < 32; u += 4)
+                            __stcg(pp + (c + u) / 4 * f.part_rows + r_own, make_float4(v[u], v[u + 1], v[u + 2], v[u + 3]));
+                    }
+                }
+                if (fin) {
+                    if (mine && a.lse)
+                        a.lse[(int64_t)h * a.c.n_tokens + it.q.q0 + tok] = m == -INFINITY ? -INFINITY : __fadd_rn(m, log2f(l));
+                } else if (room) {
+                    __stcg(reinterpret_cast<float2 *>(pp + HD / 4 * f.part_rows) + r_own, make_float2(m, l));
+                } else if (tid == 0) {
+                    set_status(a.c.status, ALTXS_ST_BAD_POS);
+                }
+                if (odd && mine)
+                    for (int c = 0; c < HD; ++c) {
+                        const float y = odd_term<T>(a, it.s, it.g, pos, it.lo + it.t0 * kTile, it.lo + it.t1 * kTile, c);
+                        if (y == 0.0f) continue;
+                        if (fin) yp[c] = from_f<T>(y);
+                        else if (room) __stcg(reinterpret_cast<float *>(pp + c / 4 * f.part_rows + r_own) + c % 4, y);
+                    }
+            }
+            if (nt > 0) ++live;
+            if (it.nsplit > 1) {  // the same barriers on every path
+                __threadfence();
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                if (tid == 0) {
+                    last_sh = 0;
+                    if (it.slot + it.nsplit <= f.max_slots) {
+                        uint32_t *cnt = f.cnt + it.slot;
+                        last_sh = atomicAdd(cnt, 1u) == (uint32_t)it.nsplit - 1;
+                        if (last_sh) *cnt = 0;
+                    }
+                    __threadfence();
+                }
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                if (last_sh && tid < it.rows) {  // thread = row of the block
+                    const int64_t ps = (int64_t)f.part_rows * (HD + 2);
+                    const float *p = f.part + it.slot * ps;
+                    const int rr = it.r0 + tid, tk = rr / f.G, hh = it.g * f.G + rr - tk * f.G;
+                    float M = -INFINITY, lt = 0.0f;
+                    for (int t = 0; t < it.nsplit; ++t)
+                        M = fmaxf(M, __ldcg(reinterpret_cast<const float2 *>(p + t * ps + (int64_t)HD * f.part_rows) + tid).x);
+                    float w[16];
+#pragma unroll
+                    for (int t = 0; t < 16; ++t) {
+                        w[t] = 0.0f;
+                        if (t < it.nsplit) {
+                            const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p + t * ps + (int64_t)HD * f.part_rows) + tid);
+                            w[t] = M == -INFINITY ? 0.0f : ex2(__fsub_rn(ml.x, M));
+                            lt = __fmaf_rn(ml.y, w[t], lt);
+                        }
+                    }
+                    const float inv = M == -INFINITY ? 0.0f : __frcp_rn(lt);
+                    T *yp = static_cast<T *>(a.out) + (int64_t)(it.q.q0 + tk) * a.ldo + (int64_t)hh * HD;
+                    for (int c = 0; c < HD; c += 8) {
+                        float y[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int t = 0; t < 16; ++t)
+                            if (t < it.nsplit) {
+                                const float4 *pt = reinterpret_cast<const float4 *>(p + t * ps) + (int64_t)(c / 4) * f.part_rows + tid;
+                                const float4 v0 = __ldcg(pt), v1 = __ldcg(pt + f.part_rows);
+                                y[0] = __fmaf_rn(v0.x, w[t], y[0]), y[1] = __fmaf_rn(v0.y, w[t], y[1]);
+                                y[2] = __fmaf_rn(v0.z, w[t], y[2]), y[3] = __fmaf_rn(v0.w, w[t], y[3]);
+                                y[4] = __fmaf_rn(v1.x, w[t], y[4]), y[5] = __fmaf_rn(v1.y, w[t], y[5]);
+                                y[6] = __fmaf_rn(v1.z, w[t], y[6]), y[7] = __fmaf_rn(v1.w, w[t], y[7]);
+                            }
+                        uint4 o;
+                        o.x = pack2<T>(y[0] * inv, y[1] * inv), o.y = pack2<T>(y[2] * inv, y[3] * inv);
+                        o.z = pack2<T>(y[4] * inv, y[5] * inv), o.w = pack2<T>(y[6] * inv, y[7] * inv);
+                        *reinterpret_cast<uint4 *>(yp + c) = o;
+                    }
+                    if (a.lse) a.lse[(int64_t)hh * a.c.n_tokens + it.q.q0 + tk] = M == -INFINITY ? -INFINITY : __fadd_rn(M, log2f(lt));
+                }
+            }
+            // the next item's queries overwrite this one's, and its first products the outputs
+            if (tid == 0) stop_sh = abort_sh;
+            tc_fence_before();
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            tc_fence_after();
+            if (stop_sh) break;
+        }
+        if (abort_sh && tid == 0) set_status(a.c.status, ALTXS_ST_TIMEOUT);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+template <typename T, int HD>
+int launch(const ManyArgs &f, unsigned grid, cudaStream_t st) {
+    static std::atomic<uint64_t> set{0};  // devices whose shared-memory limit is raised
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return ALTXS_ECUDA;
+    if (dev >= 64 || !((set.load() >> dev) & 1)) {
+        if (cudaFuncSetAttribute(k_paged_many<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tc<HD>::Smem) != cudaSuccess)
+            return ALTXS_ECUDA;
+        if (dev < 64) set.fetch_or(1ull << dev);
+    }
+    ALTXS_LAUNCH(kKPaged, st, k_paged_many<T, HD><<<grid, kThreadsTc, Tc<HD>::Smem, st>>>(f));
+    return ALTXS_OK;
+}
+template <typename T>
+int launch(const ManyArgs &f, unsigned grid, cudaStream_t st) {
+    const int hd = f.a.kv.head_dim;
+    return hd == 32 ? launch<T, 32>(f, grid, st) : hd == 64 ? launch<T, 64>(f, grid, st) : launch<T, 128>(f, grid, st);
+}
+
+}  // namespace
+
+ManyPlan paged_many_plan(const altxs_paged_kv &kv, const altxs_chunks &c, int H, int window) {
+    ManyPlan p{};
+    const int G = H / kv.n_kv_heads;
+    const int64_t blocks = (int64_t)c.n_tokens * G / kBlockRows + c.n_seqs;
+    const int64_t keys = window > 0 ? std::min<int64_t>(c.max_kv, (int64_t)window + kBlockRows) : c.max_kv;
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(16, tiles_of((int)keys) / 8));
+    p.items = blocks * kv.n_kv_heads * most;
+    p.rows = (int64_t)c.max_new * G <= kTile ? kTile : kBlockRows;
+    if (most > 1) p.slots = std::min<int64_t>(p.items, (int64_t)c.n_seqs * kMostItems);
+    p.slot_bytes = (int64_t)p.rows * (kv.head_dim + 2) * 4;
+    return p;
+}
+
+int launch_paged_many(const PagedAttnArgs &a, const ManyPlan &p, int min_rows, uint32_t *cnt, float *part, int sms,
+                      cudaStream_t st) {
+    const ManyArgs f{a, a.H / a.kv.n_kv_heads, min_rows, p.slots, cnt, part, p.rows};
+    const unsigned grid = (unsigned)std::min<int64_t>(p.items, sms);
+    return a.kv.dtype == ALTXS_BF16 ? launch<__nv_bfloat16>(f, grid, st) : launch<__half>(f, grid, st);
+}
+
+int set_wait_limit_paged(uint32_t limit) {
+    return cudaMemcpyToSymbol(g_wait_limit, &limit, sizeof(limit)) == cudaSuccess ? ALTXS_OK : ALTXS_ECUDA;
+}
+
+}  // namespace altxs

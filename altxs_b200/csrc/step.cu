@@ -15,6 +15,7 @@
 
 #include "coder.cuh"
 #include "flash.cuh"
+#include "paged.cuh"
 #include "model.cuh"
 #include "prof.cuh"
 #include "qmm.cuh"
@@ -1344,6 +1345,7 @@ extern "C" {
 int altxs_set_wait_limit(uint32_t limit) {
     if (cudaMemcpyToSymbol(g_wait_limit, &limit, sizeof(limit)) != cudaSuccess) return ALTXS_ECUDA;
     if (altxs::set_wait_limit_flash(limit) != ALTXS_OK) return ALTXS_ECUDA;
+    if (altxs::set_wait_limit_paged(limit) != ALTXS_OK) return ALTXS_ECUDA;
     return altxs::set_wait_limit_tc(limit);
 }
 
