@@ -554,49 +554,6 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_paged_few(const __grid_const
     }
 }
 
-// One warp per (token, head) of the sequences with more rows than the kernel
-// above takes: keys one at a time with a running maximum and sum.
-template <typename T, int HD>
-__global__ void __launch_bounds__(128) k_paged_rows(PagedAttnArgs a) {
-    constexpr int E = HD / 32;
-    const Seq s = load_seq_report(a.c, blockIdx.x);
-    if (s.n * (a.H / a.kv.n_kv_heads) <= kMaxRows) return;
-    const int h = blockIdx.y, g = h / (a.H / a.kv.n_kv_heads), lane = threadIdx.x & 31;
-    const float c2 = __fmul_rn(a.scale, kLog2e);
-    for (int i = blockIdx.z * 4 + (threadIdx.x >> 5); i < s.n; i += gridDim.z * 4) {
-        const T *q = static_cast<const T *>(a.q) + (int64_t)(s.q0 + i) * a.ldq + (int64_t)h * HD + lane * E;
-        float x[E], o[E], m = -INFINITY, l = 0.0f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = __fmul_rn(to_f(q[e]), c2), o[e] = 0.0f;
-        const int pos = s.L - s.n + i;
-        for (int j = a.window > 0 ? max(0, pos - a.window + 1) : 0; j <= pos; ++j) {
-            const int page = a.c.page_table[blockIdx.x * a.c.table_stride + j / a.kv.page_size];
-            if (page < 0 || page >= a.kv.n_pages) {
-                if (lane == 0) set_status(a.c.status, ALTXS_ST_BAD_POS);
-                continue;
-            }
-            const int64_t at = page * a.kv.page_stride + (int64_t)(j % a.kv.page_size) * a.kv.token_stride +
-                               g * a.kv.head_stride + lane * E;
-            float d = 0.0f;
-#pragma unroll
-            for (int e = 0; e < E; ++e) d = __fmaf_rn(x[e], to_f(static_cast<const T *>(a.kv.k)[at + e]), d);
-            d = warp_sum(d);
-            const float mn = fmaxf(m, d), f = m == -INFINITY ? 0.0f : exp2f(__fsub_rn(m, mn));
-            const float p = d == -INFINITY ? 0.0f : exp2f(__fsub_rn(d, mn));
-            l = __fmaf_rn(l, f, p);
-            m = mn;
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-                o[e] = __fmaf_rn(o[e], f, __fmul_rn(p, to_f(static_cast<const T *>(a.kv.v)[at + e])));
-        }
-        T *y = static_cast<T *>(a.out) + (int64_t)(s.q0 + i) * a.ldo + (int64_t)h * HD + lane * E;
-#pragma unroll
-        for (int e = 0; e < E; ++e) y[e] = from_f<T>(m == -INFINITY ? 0.0f : __fdiv_rn(o[e], l));
-        if (a.lse && lane == 0)
-            a.lse[(int64_t)h * a.c.n_tokens + s.q0 + i] = m == -INFINITY ? -INFINITY : __fadd_rn(m, log2f(l));
-    }
-}
-
 // Workspace: arrival counters (zero between calls: a call's last arrivals reset
 // them), then partial rows.
 constexpr int64_t kCounters = 65536;  // more than these are cleared by the call that needs them
@@ -623,7 +580,7 @@ Plan plan_of(const altxs_paged_kv &kv, const altxs_chunks &c, int H, int window)
     p.items = (split ? total / kSplitUnit + n : n) * kv.n_kv_heads;
     p.part_rows = (int)std::min<int64_t>(kMaxRows, (int64_t)c.max_new * G);
     if (p.few && split) part = p.items * p.part_rows * (kv.head_dim + 4) * 4;
-    if (p.many && kv.dtype != ALTXS_F32) {
+    if (p.many) {
         p.mp = paged_many_plan(kv, c, H, window);
         part = std::max(part, p.mp.slots * p.mp.slot_bytes);
     }
@@ -668,14 +625,7 @@ int launch(const PagedAttnArgs &a, const Plan &p, cudaStream_t st) {
         const unsigned grid = (unsigned)std::min<int64_t>(p.items, 2 * sm_count());
         ALTXS_LAUNCH(kKPaged, st, k_paged_few<T, HD><<<grid, kWarps * 32, smem, st>>>(f));
     }
-    if (p.many) {
-        if constexpr (sizeof(T) == 2) {
-            return launch_paged_many(a, p.mp, kMaxRows + 1, many_cnt, part, sm_count(), st);
-        } else {
-            const dim3 grid(a.c.n_seqs, a.H, (unsigned)std::min(256, (a.c.max_new + 3) / 4));
-            ALTXS_LAUNCH(kKPaged, st, k_paged_rows<T, HD><<<grid, 128, 0, st>>>(a));
-        }
-    }
+    if (p.many) return launch_paged_many(a, p.mp, kMaxRows + 1, many_cnt, part, sm_count(), st);
     return ALTXS_OK;
 }
 template <typename T>

@@ -1,27 +1,38 @@
-// Attention of many new tokens over a paged key/value cache (16-bit types) on
-// the tensor cores, the scores never leaving the SM.
+// Attention of many new tokens over a paged key/value cache on the tensor
+// cores, the scores never leaving the SM.
 //
 // The rows of one key/value head (its G query heads x the sequence's new
-// tokens, row = token * G + head) are cut into blocks of 256; an item is one
-// split of one block's visible key tiles (128 positions each), taken by a
-// persistent block of 12 warps:
+// tokens, row = token * G + head) are cut into blocks of 256 (fp32 with 128
+// channels: 128); an item is one split of one block's visible key tiles (128
+// positions each; there: 64), taken by a persistent block of warps:
 //   warps 0-3, 4-7  softmax groups 0 and 1, one score row per thread;
 //   warp 8          issues the MMAs: S = Q K^T into a group's tensor-memory
 //                   score columns, then (P written over S) O += P V, P read
 //                   from tensor memory, V as it lies (MN-major);
-//   warps 9-11      gather key and value rows through the page table with
-//                   16-byte asynchronous copies into a ring of tiles, rows
-//                   that no position of the block needs filled with zeros.
+//   the rest        gather key and value rows through the page table into a
+//                   ring of tiles, rows that no position of the block needs
+//                   filled with zeros.
 // With more than 128 rows each group owns 128 of them and every key tile
 // serves both; with at most 128 the two groups share the rows and take even
 // and odd key tiles, and group 0 joins both outputs at the end.  Either way
 // the MMA warp alternates between the groups, so one group's softmax runs
 // under the other's MMAs.
 //
-// Softmax: x = s scale log2(e) in fp32, p = 2^(x - m) rounded once to the
-// 16-bit type, the sum from the unrounded p.  m follows the running maximum
-// only when that grows by more than 2^8: until then p <= 256 is as exact, and
-// O (fp32, in tensor memory) is not touched.
+// Softmax: x = s scale log2(e) in fp32, p = 2^(x - m), the sum from the
+// unrounded p.  m follows the running maximum only when that grows by more
+// than 2^8: until then p <= 256 is as exact, and O (fp32, in tensor memory) is
+// not touched.
+//
+// 16-bit types: the tiles are the cache's own rows (16-byte asynchronous
+// copies), p is rounded once to the type.
+// fp32: every operand is a pair of fp16 planes, hi = fp16(v 2^a) and lo =
+// fp16(v 2^a - hi), a power of two per query row, per key tile and (running)
+// for the values that puts the largest magnitude at 2^14: hi + lo keeps 22
+// significant bits of everything within 2^-18 of that magnitude, and 2^-40 of
+// it below.  A product is hi hi + hi lo + lo hi with fp32 sums.  Three fp16
+// products instead of six with bf16 planes or three at half the rate with
+// tf32; the producer warps hold a tile's rows in registers, agree on its
+// exponent and write the planes.
 //
 // Splits of a block go to the workspace as (m, l, O); the item that arrives
 // last joins them in split order.  Tiles, blocks and splits are functions of
@@ -40,33 +51,43 @@
 namespace altxs {
 namespace {
 
-constexpr int kTile = 128;       // positions per key tile
-constexpr int kBlockRows = 256;  // rows per item
-constexpr int kMmaWarp = 8, kProducers = 3;
-constexpr int kScan = 128;  // sequences are counted in this many groups
+constexpr int kMmaWarp = 8;
+constexpr int kScan = 64;         // sequences are counted in this many groups
 constexpr int kMostItems = 1184;  // of a sequence that is split (8 waves)
-constexpr int kThreadsTc = (kMmaWarp + 1 + kProducers) * 32;
-constexpr int kMaskRing = 16;  // key tiles (and items) the producers can be ahead of the softmax, at most
+constexpr int kMaskRing = 16;     // key tiles (and items) the producers can be ahead of the softmax, at most
 constexpr unsigned kAll = 0xffffffffu;
 constexpr float kLazy = 8.0f;
 
-template <int HD>
+template <typename T, int HD>
 struct Tc {
-    static constexpr int RowB = HD * 2;
-    static constexpr int Halves = HD > 64 ? 2 : 1;      // 64-channel halves of a tile, 16 KB each
-    static constexpr int TileB = Halves * kTile * 128;  // HD 32 leaves half of each 128-byte row unused
-    static constexpr int Slots = HD > 64 ? 5 : 12;
+    static constexpr bool F32 = sizeof(T) == 4;
+    static constexpr int KT = F32 && HD > 64 ? 64 : 128;     // positions per key tile
+    static constexpr int Rows = F32 && HD > 64 ? 128 : 256;  // rows per item
+    static constexpr int Planes = F32 ? 2 : 1;
+    static constexpr int Halves = HD > 64 ? 2 : 1;           // 64-channel halves of a plane
+    static constexpr int PlaneB = Halves * KT * 128;         // HD 32 leaves half of each 128-byte row unused
+    static constexpr int TileB = Planes * PlaneB;
+    static constexpr int QPlaneB = Halves * 128 * 128, QTileB = Planes * QPlaneB;  // 128 rows
+    static constexpr int Producers = F32 ? 7 : 3;
+    static constexpr int Threads = (kMmaWarp + 1 + Producers) * 32;
+    // registers: (8 warps x RegS + the others x RegP) x 32 = Threads x 168 (16 bits) or 128 (fp32)
+    static constexpr int RegS = F32 ? 168 : 208, RegP = 88;
+    static_assert(256 * RegS + (Threads - 256) * RegP == Threads * (F32 ? 128 : 168), "register split");
+    static constexpr int Slots = F32 || HD > 64 ? 5 : 12;
     static constexpr int Lag = HD > 64 ? 3 : HD > 32 ? 6 : 8;  // tiles a producer has in flight behind the newest
-    static constexpr int Smem = 2 * TileB + Slots * TileB + 1024;
-    static constexpr uint32_t ColS = 0, ColO = 2 * kTile;  // group i: S at 128 i, O at 256 + HD i
+    static constexpr int Smem = Rows / 128 * QTileB + Slots * TileB + 1024;
+    static constexpr uint32_t ColS = 0, ColO = 2 * 128;  // group i: S at KT i, O at 256 + HD i
     static_assert(Smem + 2048 <= 227 * 1024, "shared memory (with the static part)");
 };
+// the same two numbers for the host and the item arithmetic
+__host__ __device__ inline int tile_keys(int dtype, int hd) { return dtype == ALTXS_F32 && hd > 64 ? 64 : 128; }
+__host__ __device__ inline int block_rows(int dtype, int hd) { return dtype == ALTXS_F32 && hd > 64 ? 128 : 256; }
 
 // one sequence's share of the work
 struct Shape {
     int R, blocks, nsplit;
 };
-__host__ __device__ inline int tiles_of(int keys) { return (keys + kTile - 1) / kTile; }
+__host__ __device__ inline int tiles_of(int keys, int kt) { return (keys + kt - 1) / kt; }
 // Splits of every block of a sequence: enough items to fill the 148 SMs in whole
 // waves by itself, at least 8 key tiles each (a split costs about 1.5 tiles' time).
 __host__ __device__ inline int many_splits(int items, int nt) {
@@ -91,15 +112,16 @@ struct ManyArgs {
     int part_rows;
 };
 
+template <class C>
 __device__ __forceinline__ Shape shape_of(const ManyArgs &f, const Seq &q) {
     Shape w{0, 0, 0};
     if (q.n <= 0 || q.n * f.G < f.min_rows) return w;
     w.R = q.n * f.G;
-    w.blocks = (w.R + kBlockRows - 1) / kBlockRows;
-    // the longest block: the last 256 rows' keys
-    const int rows = min(w.R, kBlockRows), toks = (rows + f.G - 1) / f.G;
+    w.blocks = (w.R + C::Rows - 1) / C::Rows;
+    // the longest block: the last rows' keys
+    const int rows = min(w.R, C::Rows), toks = (rows + f.G - 1) / f.G;
     const int keys = f.a.window > 0 ? min(q.L, f.a.window + toks - 1) : q.L;
-    w.nsplit = many_splits(w.blocks * f.a.kv.n_kv_heads, tiles_of(max(keys, 0)));
+    w.nsplit = many_splits(w.blocks * f.a.kv.n_kv_heads, tiles_of(max(keys, 0), C::KT));
     return w;
 }
 
@@ -112,11 +134,12 @@ struct Item {
     Seq q;
     int s, g, nsplit, split;
     int r0, rows;        // rows of the block
-    int lo, t0, t1, hi;  // positions lo + 128 t of key tiles t0 .. t1 of this split; the block sees [lo, hi)
+    int lo, t0, t1, hi;  // positions lo + KT t of key tiles t0 .. t1 of this split; the block sees [lo, hi)
     bool two;            // two row tiles (both groups over every key tile)
     int slot;            // partial slot of the block's split 0
 };
 
+template <class C>
 __device__ __forceinline__ Item locate(const ManyArgs &f, const Scan &sc, int item) {
     int lo = 0, hi = kScan;
     while (hi - lo > 1) {
@@ -128,8 +151,8 @@ __device__ __forceinline__ Item locate(const ManyArgs &f, const Scan &sc, int it
     it.s = lo * sc.per;
     int local = item - sc.before[lo], slot = sc.slots[lo];
     it.q = load_seq(f.a.c, it.s);
-    Shape w = shape_of(f, it.q);
-    for (int n; it.s < f.a.c.n_seqs - 1 && local >= (n = w.blocks * w.nsplit * Hkv); w = shape_of(f, it.q)) {
+    Shape w = shape_of<C>(f, it.q);
+    for (int n; it.s < f.a.c.n_seqs - 1 && local >= (n = w.blocks * w.nsplit * Hkv); w = shape_of<C>(f, it.q)) {
         local -= n;
         if (w.nsplit > 1) slot += n;
         it.q = load_seq(f.a.c, ++it.s);
@@ -140,13 +163,13 @@ __device__ __forceinline__ Item locate(const ManyArgs &f, const Scan &sc, int it
     local /= w.nsplit;
     it.g = local % Hkv;
     const int blk = w.blocks - 1 - local / Hkv;  // the longest blocks first
-    it.r0 = blk * kBlockRows;
-    it.rows = min(w.R - it.r0, kBlockRows);
-    it.two = it.rows > kTile;
+    it.r0 = blk * C::Rows;
+    it.rows = min(w.R - it.r0, C::Rows);
+    it.two = it.rows > 128;
     const int p0 = it.q.L - it.q.n, i0 = it.r0 / f.G, i1 = (it.r0 + it.rows - 1) / f.G;
     it.hi = max(0, p0 + i1 + 1);
     it.lo = f.a.window > 0 ? max(0, p0 + i0 - f.a.window + 1) : 0;
-    const int nt = tiles_of(max(0, it.hi - it.lo)), per = (nt + it.nsplit - 1) / it.nsplit;
+    const int nt = tiles_of(max(0, it.hi - it.lo), C::KT), per = (nt + it.nsplit - 1) / it.nsplit;
     it.t0 = min(nt, it.split * per);
     it.t1 = min(nt, it.t0 + per);
     return it;
@@ -176,8 +199,8 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     }
 }
 template <typename T>
-constexpr uint32_t idesc(int n, int bmn) {  // kind::f16, fp32 sums, M = 128, A K-major
-    const uint32_t fmt = std::is_same<T, __half>::value ? 0u : 1u;
+constexpr uint32_t idesc(int n, int bmn) {  // kind::f16 (bf16, or fp16: fp32's planes too), fp32 sums, M = 128, A K-major
+    const uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     return (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)bmn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
 // D += A B with A (rows = lanes, two 16-bit values per column) in tensor memory
@@ -198,6 +221,13 @@ __device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t *v) {
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
         "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
         ALTXS_R32(v)
+        : "memory");
+}
+__device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t *v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+        "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
         : "memory");
 }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -223,6 +253,32 @@ __device__ __forceinline__ void tc_tie32(float *f) {
                           "+f"(f[i + 6]), "+f"(f[i + 7])::"memory");
 }
 
+// 8 consecutive values to dst (16- or 32-byte aligned)
+template <typename T>
+__device__ __forceinline__ void store8(T *dst, const float *v) {
+    if constexpr (sizeof(T) == 4) {
+        reinterpret_cast<float4 *>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4 *>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+        *reinterpret_cast<uint4 *>(dst) = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+    }
+}
+// fp16 planes of two values
+__device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t &lo) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(__fsub_rn(a, f.x), __fsub_rn(b, f.y));
+    hi = *reinterpret_cast<const uint32_t *>(&h);
+    lo = *reinterpret_cast<const uint32_t *>(&l);
+}
+// Exponent e of the largest finite magnitude (its bits), within +-100: 2^(14 - e) scales it to 2^14 ..
+__device__ __forceinline__ int exp_of(uint32_t bits) { return min(max((int)(bits >> 23) - 127, -100), 100); }
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((127 + e) << 23); }
+__device__ __forceinline__ uint32_t finite_abs(float x) {
+    const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
+    return b < 0x7f800000u ? b : 0u;
+}
+
 // The values of channel `dim` that are not finite, over the positions [lo, hi) that a
 // row at `pos` sees (the tiles that only some rows see hold 0 in their place).
 template <typename T>
@@ -240,22 +296,29 @@ __device__ __noinline__ float odd_term(const PagedAttnArgs &a, int s, int g, int
 }
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(kThreadsTc, 1) k_paged_many(const __grid_constant__ ManyArgs f) {
-    using C = Tc<HD>;
+__global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __grid_constant__ ManyArgs f) {
+    using C = Tc<T, HD>;
+    constexpr int KT = C::KT;
+    constexpr bool F32 = C::F32;
     extern __shared__ unsigned char pm_smem_raw[];
     __shared__ __align__(8) uint64_t full[C::Slots], empty[C::Slots], s_full[2], p_full[2], o_done[2], q_full, drainb;
     __shared__ Scan sc;
-    __shared__ uint32_t tmem_sh, kmask[kMaskRing][4], odd_sh[kMaskRing][kProducers];
+    // by key tile: which positions exist (4 to a byte), and (fp32) the exponents of its keys and of the values so far
+    __shared__ __align__(16) uint8_t kmask[kMaskRing][KT / 4];
+    __shared__ int kv_exp[F32 ? kMaskRing : 1][2];
+    __shared__ uint32_t wmax[F32 ? 2 : 1][8];  // (fp32) the producers' maxima, bit 31: a wait gave up
+    __shared__ uint32_t tmem_sh;
+    __shared__ uint8_t odd_sh[kMaskRing][8];
     __shared__ int2 wsum[kScan / 32];
     __shared__ int last_sh, stop_sh;
     __shared__ volatile int abort_sh;
     const PagedAttnArgs &a = f.a;
     const uint32_t raw_s = smem_u32(pm_smem_raw);
-    const uint32_t sq = raw_s + ((1024u - (raw_s & 1023u)) & 1023u), ring = sq + 2 * C::TileB;
+    const uint32_t sq = raw_s + ((1024u - (raw_s & 1023u)) & 1023u), ring = sq + C::Rows / 128 * C::QTileB;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int s = 0; s < C::Slots; ++s) {
-            mbar_init(&full[s], kProducers);
+            mbar_init(&full[s], C::Producers);
             mbar_init(&empty[s], 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -277,7 +340,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) k_paged_many(const __grid_const
         const int n = a.c.n_seqs, per = (n + kScan - 1) / kScan;
         int sum = 0, cut = 0;
         for (int s = tid * per; s < min(n, (tid + 1) * per); ++s) {
-            const Shape w = shape_of(f, blockIdx.x == 0 ? load_seq_report(a.c, s) : load_seq(a.c, s));
+            const Shape w = shape_of<C>(f, blockIdx.x == 0 ? load_seq_report(a.c, s) : load_seq(a.c, s));
             const int k = w.blocks * w.nsplit * a.kv.n_kv_heads;
             sum += k;
             if (w.nsplit > 1) cut += k;
@@ -288,7 +351,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) k_paged_many(const __grid_const
             if (lane >= o) sum += v, cut += u;
         }
         if (lane == 31) wsum[warp] = make_int2(sum, cut);
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+        asm volatile("bar.sync 1, %0;" ::"n"(kScan) : "memory");
         for (int w = 0; w < warp; ++w) sum += wsum[w].x, cut += wsum[w].y;
         sc.before[tid + 1] = sum, sc.slots[tid + 1] = cut;
         if (tid == 0) sc.before[0] = sc.slots[0] = 0, sc.per = per;
@@ -301,16 +364,17 @@ __global__ void __launch_bounds__(kThreadsTc, 1) k_paged_many(const __grid_const
 
     if (warp > kMmaWarp) {
         // ---- producers ----
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::RegP));
         const int pw = warp - kMmaWarp - 1;
-        constexpr int NC = C::RowB / 16, KPI = 32 / NC;  // 16-byte pieces of a row, rows per warp copy
         const int P = a.kv.page_size, pshift = (P & (P - 1)) == 0 ? 31 - __clz(P) : -1;
         auto block_of = [&](int k) { return pshift >= 0 ? k >> pshift : k / P; };
-        // Warp pw copies the 8-row groups pw, pw + 3, .. of every tile: at most 6 of 16.
-        constexpr int kGroups = (kTile / 8 + kProducers - 1) / kProducers;
         uint32_t n = 0, kt = 0, live = 0;  // slots, key tiles and items with tiles so far
-        uint32_t done = 0;                 // slots published
         bool ok = true;
+        if constexpr (!F32) {
+        constexpr int NC = HD / 8, KPI = 32 / NC;  // 16-byte pieces of a row, rows per warp copy
+        // Warp pw copies the 8-row groups pw, pw + 3, .. of every tile: at most 6 of 16.
+        constexpr int kGroups = (KT / 8 + C::Producers - 1) / C::Producers;
+        uint32_t done = 0;                 // slots published
         // a published slot needs its values checked when only some rows see them
         uint32_t check = 0;                // bit (slot n & 31): check before publishing
         uint32_t odd_of = 0;
@@ -319,12 +383,12 @@ __global__ void __launch_bounds__(kThreadsTc, 1) k_paged_many(const __grid_const
             if ((check >> (m & 31)) & 1) {
                 bool odd = false;
                 for (int i = 0; i < kGroups; ++i) {
-                    const int grp = pw + i * kProducers;
-                    if (grp >= kTile / 8) break;
+                    const int grp = pw + i * C::Producers;
+                    if (grp >= KT / 8) break;
 #pragma unroll
                     for (int e = 0; e < 8 / KPI; ++e) {
                         const int r = grp * 8 + e * KPI + lane / NC, c = lane % NC;
-                        const uint32_t d = base + (c >> 3) * (kTile * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                        const uint32_t d = base + (c >> 3) * (KT * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
                         uint4 v = lds16(d);
                         uint32_t *w = reinterpret_cast<uint32_t *>(&v);
                         bool bad = false;
@@ -345,7 +409,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) k_paged_many(const __grid_const
             if (lane == 0) mbar_arrive(&full[m % C::Slots]);
         };
         for (int item = blockIdx.x; item < total && ok; item += gridDim.x) {
-            const Item it = locate(f, sc, item);
+            const Item it = locate<C>(f, sc, item);
             if (it.t0 == it.t1) continue;
             const int p0 = it.q.L - it.q.n, i0 = it.r0 / f.G, i1 = (it.r0 + it.rows - 1) / f.G;
             const int32_t *table = a.c.page_table + it.s * a.c.table_stride;
@@ -359,14 +423,14 @@ __global__ void __launch_bounds__(kThreadsTc, 1) k_paged_many(const __grid_const
             odd_of = live++;
             if (lane == 0) odd_sh[odd_of % kMaskRing][pw] = 0;
             for (int t = it.t0; t < it.t1 && ok; ++t) {
-                const int kb = it.lo + t * kTile;
+                const int kb = it.lo + t * KT;
                 // offsets of this warp's rows: lane 8 i' + r holds row r of its i'-th group (two rounds)
                 int64_t off[2];
                 uint32_t seen[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const int grp = pw + (4 * e + lane / 8) * kProducers, k = kb + grp * 8 + lane % 8;
-                    const bool want = grp < kTile / 8 && k < it.hi;
+                    const int grp = pw + (4 * e + lane / 8) * C::Producers, k = kb + grp * 8 + lane % 8;
+                    const bool want = grp < KT / 8 && k < it.hi;
                     const int b = want ? block_of(k) : 0, page = want ? __ldg(table + b) : -1;
                     const bool in = page >= 0 && page < a.kv.n_pages;
                     if (want && !in) set_status(a.c.status, ALTXS_ST_BAD_POS);
@@ -374,13 +438,15 @@ __global__ void __launch_bounds__(kThreadsTc, 1) k_paged_many(const __grid_const
                     seen[e] = __ballot_sync(kAll, in);
                 }
                 if (lane < kGroups) {  // which rows exist, for the softmax
-                    const int grp = pw + lane * kProducers;
-                    if (grp < kTile / 8)
-                        reinterpret_cast<uint8_t *>(kmask[kt % kMaskRing])[grp] = (uint8_t)(seen[lane / 4] >> (8 * (lane % 4)));
+                    const int grp = pw + lane * C::Producers;
+                    const uint32_t sb = seen[lane / 4] >> (8 * (lane % 4));
+                    if (grp < KT / 8)
+                        *reinterpret_cast<uint16_t *>(&kmask[kt % kMaskRing][2 * grp]) =
+                            (uint16_t)(((sb >> 4) & 15) << 8 | (sb & 15));
                 }
                 ++kt;
                 // every row of the block sees the whole tile?
-                const bool whole = kb + kTile <= p0 + i0 + 1 && (a.window == 0 || kb > p0 + i1 - a.window);
+                const bool whole = kb + KT <= p0 + i0 + 1 && (a.window == 0 || kb > p0 + i1 - a.window);
 #pragma unroll
                 for (int kv = 0; kv < 2; ++kv, ++n) {
                     const uint32_t s = n % C::Slots;
@@ -398,14 +464,14 @@ __global__ void __launch_bounds__(kThreadsTc, 1) k_paged_many(const __grid_const
                     const uint32_t dst = ring + s * C::TileB;
 #pragma unroll
                     for (int i = 0; i < kGroups; ++i) {
-                        const int grp = pw + i * kProducers;
-                        if (grp < kTile / 8) {
+                        const int grp = pw + i * C::Producers;
+                        if (grp < KT / 8) {
 #pragma unroll
                             for (int e = 0; e < 8 / KPI; ++e) {
                                 const int r8 = e * KPI + lane / NC, r = grp * 8 + r8, c = lane % NC;
                                 const int64_t o = __shfl_sync(kAll, off[i / 4], (i % 4) * 8 + r8);
                                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                                                 dst + (c >> 3) * (kTile * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)),
+                                                 dst + (c >> 3) * (KT * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)),
                                              "l"(src0 + (o < 0 ? 0 : o) + c * 16), "r"(o < 0 ? 0u : 16u)
                                              : "memory");
                             }
@@ -422,15 +488,117 @@ __global__ void __launch_bounds__(kThreadsTc, 1) k_paged_many(const __grid_const
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         while (done < n) publish(done++);
+        } else {
+            // fp32: units of 2 KB (64 chunks of 8 channels); warp pw takes units pw, pw + 7, ..
+            // Per tile: load the unit rows to registers, agree on the tile's largest
+            // magnitude, write the scaled planes.
+            constexpr int CR = HD / 8, UR = 64 / CR, Units = KT / UR, UW = (Units + C::Producers - 1) / C::Producers;
+            static_assert(UW * UR <= 32, "one page look-up per lane");
+            for (int item = blockIdx.x; item < total && ok; item += gridDim.x) {
+                const Item it = locate<C>(f, sc, item);
+                if (it.t0 == it.t1) continue;
+                const int p0 = it.q.L - it.q.n, i0 = it.r0 / f.G, i1 = (it.r0 + it.rows - 1) / f.G;
+                const int32_t *table = a.c.page_table + it.s * a.c.table_stride;
+                const float *kbase = static_cast<const float *>(a.kv.k) + (int64_t)it.g * a.kv.head_stride;
+                const float *vbase = static_cast<const float *>(a.kv.v) + (int64_t)it.g * a.kv.head_stride;
+                const uint32_t me = live++ % kMaskRing;
+                if (lane == 0) odd_sh[me][pw] = 0;
+                int ve = -100;  // exponent of the item's values so far
+                for (int t = it.t0; t < it.t1 && ok; ++t, ++kt) {
+                    const int kb = it.lo + t * KT;
+                    // lane: row lane % UR of this warp's unit lane / UR
+                    const int un = pw + lane / UR * C::Producers, k = kb + un * UR + lane % UR;
+                    const bool want = lane < UW * UR && un < Units && k < it.hi;
+                    const int b = want ? block_of(k) : 0, page = want ? __ldg(table + b) : -1;
+                    const bool in = page >= 0 && page < a.kv.n_pages;
+                    if (want && !in) set_status(a.c.status, ALTXS_ST_BAD_POS);
+                    const int64_t off = in ? (int64_t)page * a.kv.page_stride + (int64_t)(k - b * P) * a.kv.token_stride : -1;
+                    const uint32_t seen = __ballot_sync(kAll, in);
+                    if (lane % 4 == 0 && lane < UW * UR && un < Units)
+                        kmask[kt % kMaskRing][(un * UR + lane % UR) / 4] = (uint8_t)((seen >> lane) & 15);
+                    const bool whole = kb + KT <= p0 + i0 + 1 && (a.window == 0 || kb > p0 + i1 - a.window);
+#pragma unroll
+                    for (int kv = 0; kv < 2; ++kv, ++n) {
+                        const float *src0 = kv ? vbase : kbase;
+                        float4 x[UW][2][2];
+                        uint32_t mx = 0;
+#pragma unroll
+                        for (int i = 0; i < UW; ++i)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const int q = e * 32 + lane;  // chunk of the unit: row q / CR, channels 8 (q % CR) ..
+                                const int64_t o = __shfl_sync(kAll, off, i * UR + q / CR);
+                                x[i][e][0] = x[i][e][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                                if (pw + i * C::Producers < Units && o >= 0) {
+                                    const float4 *src = reinterpret_cast<const float4 *>(src0 + o + q % CR * 8);
+                                    x[i][e][0] = __ldg(src), x[i][e][1] = __ldg(src + 1);
+                                }
+                            }
+                        const uint32_t s = n % C::Slots;
+                        if (n >= C::Slots)
+                            ok = __all_sync(kAll, !abort_sh && mbar_wait_bounded(&empty[s], ((n / C::Slots) - 1) & 1, wait_limit()));
+                        bool odd = false;
+#pragma unroll
+                        for (int i = 0; i < UW; ++i)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                float4 &v = x[i][e >> 1][e & 1];
+                                float *w = reinterpret_cast<float *>(&v);
+#pragma unroll
+                                for (int u = 0; u < 4; ++u) {
+                                    mx = max(mx, finite_abs(w[u]));
+                                    if (kv && !whole && i1 > i0 && !isfinite(w[u])) w[u] = 0.0f, odd = true;
+                                }
+                            }
+                        mx = __reduce_max_sync(kAll, mx);
+                        if (lane == 0) wmax[n & 1][pw] = mx | (ok ? 0u : 0x80000000u);
+                        if (kv && __any_sync(kAll, odd) && lane == 0) odd_sh[me][pw] = 1;
+                        asm volatile("bar.sync 2, %0;" ::"n"(C::Producers * 32) : "memory");
+                        mx = 0;
+#pragma unroll
+                        for (int w = 0; w < C::Producers; ++w) {
+                            const uint32_t o = wmax[n & 1][w];
+                            ok = ok && !(o >> 31);
+                            mx = max(mx, o & 0x7fffffffu);
+                        }
+                        if (!ok) break;  // every producer warp sees the same words
+                        int ex = exp_of(mx);
+                        if (kv) ex = ve = max(ve, ex);
+                        if (pw == 0 && lane == 0) kv_exp[kt % kMaskRing][kv] = ex;
+                        const float scale = pow2(14 - ex);
+                        const uint32_t dst = ring + s * C::TileB;
+#pragma unroll
+                        for (int i = 0; i < UW; ++i)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const int q = e * 32 + lane, r = (pw + i * C::Producers) * UR + q / CR, c = q % CR;
+                                if (pw + i * C::Producers >= Units) continue;
+                                uint4 hi, lo;
+                                const float4 v0 = x[i][e][0], v1 = x[i][e][1];
+                                split2(v0.x * scale, v0.y * scale, hi.x, lo.x);
+                                split2(v0.z * scale, v0.w * scale, hi.y, lo.y);
+                                split2(v1.x * scale, v1.y * scale, hi.z, lo.z);
+                                split2(v1.z * scale, v1.w * scale, hi.w, lo.w);
+                                const uint32_t d = dst + (c >> 3) * (KT * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                                sts16(d, hi);
+                                sts16(d + C::PlaneB, lo);
+                            }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&full[s]);
+                    }
+                }
+            }
+        }
         if (!ok) abort_sh = 1;
     } else if (warp == kMmaWarp) {
         // ---- MMA issuer ----
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::RegP));
         if (lane == 0) {
             uint32_t n = 0, items = 0, jobs[2] = {0, 0};  // slots and items so far; PV jobs issued per group
             bool ok = true;
             for (int item = blockIdx.x; item < total && ok; item += gridDim.x) {
-                const Item it = locate(f, sc, item);
+                const Item it = locate<C>(f, sc, item);
                 const int nt = it.t1 - it.t0;
                 if (nt == 0) continue;
                 ok = mbar_wait_bounded(&q_full, items & 1, wait_limit());
@@ -449,9 +617,15 @@ __global__ void __launch_bounds__(kThreadsTc, 1) k_paged_many(const __grid_const
                         tc_fence_after();
                         const uint32_t vb = ring + s * C::TileB;
 #pragma unroll
-                        for (int kk = 0; kk < kTile / 16; ++kk)
-                            tc_mma_ts(tmem + C::ColO + HD * i, tmem + C::ColS + kTile * i + 8 * kk,
-                                      sw128_desc(vb + kk * 2048, kTile * 128), idesc<T>(HD, 1), t >= 4 || kk != 0);
+                        for (int kk = 0; kk < KT / 16; ++kk) {
+                            const uint32_t d = tmem + C::ColO + HD * i, p = tmem + C::ColS + KT * i + 8 * kk;
+                            const uint64_t vh = sw128_desc(vb + kk * 2048, KT * 128);
+                            tc_mma_ts(d, p, vh, idesc<T>(HD, 1), t >= 4 || kk != 0);
+                            if constexpr (F32) {
+                                tc_mma_ts(d, p, sw128_desc(vb + C::PlaneB + kk * 2048, KT * 128), idesc<T>(HD, 1), 1u);
+                                tc_mma_ts(d, p + KT / 2, vh, idesc<T>(HD, 1), 1u);
+                            }
+                        }
                         tc_commit(&o_done[i]);
                         ++jobs[i];
                         if (!it.two || i == 1) tc_commit(&empty[s]);
@@ -464,12 +638,17 @@ __global__ void __launch_bounds__(kThreadsTc, 1) k_paged_many(const __grid_const
                             break;
                         }
                         tc_fence_after();
-                        const uint32_t kb = ring + s * C::TileB, qb = sq + (it.two ? i * C::TileB : 0);
+                        const uint32_t kb = ring + s * C::TileB, qb = sq + (it.two ? i * C::QTileB : 0);
+                        const uint32_t d = tmem + C::ColS + KT * i;
 #pragma unroll
                         for (int kk = 0; kk < HD / 16; ++kk) {
-                            const uint32_t o = (kk >> 2) * (kTile * 128) + (kk & 3) * 32;
-                            tc_mma(tmem + C::ColS + kTile * i, sw128_desc(qb + o, 16), sw128_desc(kb + o, 16),
-                                   idesc<T>(kTile, 0), kk != 0);
+                            const uint32_t oq = (kk >> 2) * (128 * 128) + (kk & 3) * 32, ok2 = (kk >> 2) * (KT * 128) + (kk & 3) * 32;
+                            const uint64_t qh = sw128_desc(qb + oq, 16), kh = sw128_desc(kb + ok2, 16);
+                            tc_mma(d, qh, kh, idesc<T>(KT, 0), kk != 0);
+                            if constexpr (F32) {
+                                tc_mma(d, qh, sw128_desc(kb + C::PlaneB + ok2, 16), idesc<T>(KT, 0), 1u);
+                                tc_mma(d, sw128_desc(qb + C::QPlaneB + oq, 16), kh, idesc<T>(KT, 0), 1u);
+                            }
                         }
                         tc_commit(&s_full[i]);
                         if (!it.two || i == 1) tc_commit(&empty[s]);
@@ -485,83 +664,126 @@ __global__ void __launch_bounds__(kThreadsTc, 1) k_paged_many(const __grid_const
         __syncwarp();
     } else {
         // ---- softmax ----
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::RegS));
         const int grp = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t ts = tmem + lanes + C::ColS + kTile * grp, to = tmem + lanes + C::ColO + HD * grp;
+        const uint32_t ts = tmem + lanes + C::ColS + KT * grp, to = tmem + lanes + C::ColO + HD * grp;
         // a negative scale turns the queries round instead; a scale of 0 stays above it (-inf marks the unseen)
         const float c2 = fmaxf(__fmul_rn(fabsf(a.scale), kLog2e), 1.17549435e-38f);
-        // group 1's (m, l) on their way to group 0, in the second query tile's place
-        float2 *ml = reinterpret_cast<float2 *>(pm_smem_raw + (sq - raw_s) + C::TileB);
+        // fp32's p carries 2^6 (it is 2^14 at most), so that what it loses below 2^-24 is far from the sum
+        constexpr float kBias = F32 ? 6.0f : 0.0f;
         const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
         uint32_t job = 0, kt = 0, live = 0;
         bool ok = true;
         for (int item = blockIdx.x; item < total; item += gridDim.x) {
-            const Item it = locate(f, sc, item);
+            const Item it = locate<C>(f, sc, item);
             const int nt = it.t1 - it.t0, p0 = it.q.L - it.q.n;
             // this thread's row of the block (rows past the end follow the last one and are not stored)
-            const int r_own = it.two ? grp * kTile + row : row;
+            const int r_own = it.two ? grp * 128 + row : row;
             const int r = it.r0 + min(r_own, it.rows - 1), tok = r / f.G, h = it.g * f.G + r - tok * f.G;
             const int pos = p0 + tok;
             const bool mine = r_own < it.rows;
-            float m = -INFINITY, l = 0.0f;
+            float m = -INFINITY, l = 0.0f, cf = c2;  // cf: score to log2 units (fp32: times the tile's and the row's scales)
+            int qe = 0, ve = -100;                    // fp32: exponents of the row's query and of O's values
             uint32_t njob = 0;  // jobs of this group in this item
             if (nt > 0) {
-                if (it.two || grp == 0) {  // the row's query
-                    const uint4 *qp = reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) +
-                                                                     (int64_t)(it.q.q0 + tok) * a.ldq + (int64_t)h * HD);
-                    const uint32_t d = sq + (it.two ? grp * C::TileB : 0) + row * 128;
+                const T *qp = static_cast<const T *>(a.q) + (int64_t)(it.q.q0 + tok) * a.ldq + (int64_t)h * HD;
+                const uint32_t d = sq + (it.two ? grp * C::QTileB : 0) + row * 128;
+                if constexpr (F32) {
+                    uint32_t mq = 0;
+#pragma unroll 8
+                    for (int c = 0; c < HD; c += 4) {
+                        const float4 v = __ldg(reinterpret_cast<const float4 *>(qp + c));
+                        mq = max(max(mq, max(finite_abs(v.x), finite_abs(v.y))), max(finite_abs(v.z), finite_abs(v.w)));
+                    }
+                    qe = exp_of(mq);
+                    if (it.two || grp == 0) {
+                        const float sc1 = a.scale < 0.0f ? -pow2(14 - qe) : pow2(14 - qe);
+#pragma unroll 4
+                        for (int c = 0; c < HD / 8; ++c) {
+                            const float4 v0 = __ldg(reinterpret_cast<const float4 *>(qp + 8 * c)),
+                                         v1 = __ldg(reinterpret_cast<const float4 *>(qp + 8 * c + 4));
+                            uint4 hi, lo;
+                            split2(v0.x * sc1, v0.y * sc1, hi.x, lo.x);
+                            split2(v0.z * sc1, v0.w * sc1, hi.y, lo.y);
+                            split2(v1.x * sc1, v1.y * sc1, hi.z, lo.z);
+                            split2(v1.z * sc1, v1.w * sc1, hi.w, lo.w);
+                            const uint32_t dd = d + (c >> 3) * (128 * 128) + (((c & 7) ^ (row & 7)) << 4);
+                            sts16(dd, hi);
+                            sts16(dd + C::QPlaneB, lo);
+                        }
+                    }
+                } else if (it.two || grp == 0) {  // the row's query
 #pragma unroll
                     for (int c = 0; c < HD / 8; ++c) {
-                        uint4 v = __ldg(qp + c);
+                        uint4 v = __ldg(reinterpret_cast<const uint4 *>(qp) + c);
                         v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
-                        sts16(d + (c >> 3) * (kTile * 128) + (((c & 7) ^ (row & 7)) << 4), v);
+                        sts16(d + (c >> 3) * (128 * 128) + (((c & 7) ^ (row & 7)) << 4), v);
                     }
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&q_full);
                 // positions that all of this warp's rows see: from the first row's and the last row's
-                const int ra = it.r0 + min(it.two ? grp * kTile + (warp & 3) * 32 : (warp & 3) * 32, it.rows - 1);
-                const int rb = it.r0 + min(it.two ? grp * kTile + (warp & 3) * 32 + 31 : (warp & 3) * 32 + 31, it.rows - 1);
+                const int ra = it.r0 + min(it.two ? grp * 128 + (warp & 3) * 32 : (warp & 3) * 32, it.rows - 1);
+                const int rb = it.r0 + min(it.two ? grp * 128 + (warp & 3) * 32 + 31 : (warp & 3) * 32 + 31, it.rows - 1);
                 const int pa = p0 + ra / f.G, pb = p0 + rb / f.G;
                 for (int j = it.two ? 0 : grp; j < nt && ok; j += it.two ? 1 : 2) {
-                    const int kb = it.lo + (it.t0 + j) * kTile;
+                    const int kb = it.lo + (it.t0 + j) * KT;
                     ok = __all_sync(kAll, !abort_sh && mbar_wait_bounded(&s_full[grp], job & 1, wait_limit()));
                     if (!ok) break;
                     tc_fence_after();
-                    float x[kTile];
+                    float x[KT];
 #pragma unroll
-                    for (int c = 0; c < kTile; c += 32) tc_ld32_nowait(ts + c, x + c);
-                    const uint32_t *km = kmask[(kt + j) % kMaskRing];
-                    const uint32_t m0 = km[0], m1 = km[1], m2 = km[2], m3 = km[3];
+                    for (int c = 0; c < KT; c += 32) tc_ld32_nowait(ts + c, x + c);
+                    uint32_t km[KT / 16];  // 4 positions to a byte
+#pragma unroll
+                    for (int c = 0; c < KT / 16; ++c) km[c] = reinterpret_cast<const uint32_t *>(kmask[(kt + j) % kMaskRing])[c];
                     tc_wait_ld();
 #pragma unroll
-                    for (int c = 0; c < kTile; c += 32) tc_tie32(x + c);
-                    const bool whole = kb + kTile <= pa + 1 && (a.window == 0 || kb > pb - a.window) &&
-                                       (m0 & m1 & m2 & m3) == kAll;
+                    for (int c = 0; c < KT; c += 32) tc_tie32(x + c);
+                    uint32_t have = 0x0f0f0f0fu;
+#pragma unroll
+                    for (int c = 0; c < KT / 16; ++c) have &= km[c];
+                    const bool whole = kb + KT <= pa + 1 && (a.window == 0 || kb > pb - a.window) && have == 0x0f0f0f0fu;
                     if (!whole) {
                         const int first = a.window > 0 ? max(0, pos - a.window + 1 - kb) : 0, last = pos - kb;
 #pragma unroll
-                        for (int u = 0; u < kTile; ++u) {
-                            const uint32_t mk = u < 32 ? m0 : u < 64 ? m1 : u < 96 ? m2 : m3;
-                            if (u < first || u > last || !((mk >> (u & 31)) & 1)) x[u] = -INFINITY;
+                        for (int u = 0; u < KT; ++u) {
+                            const uint32_t bit = 1u << (8 * (u / 4 % 4) + u % 4);
+                            if (u < first || u > last || !(km[u / 16] & bit)) x[u] = -INFINITY;
                         }
                     }
                     float mx = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
-                    for (int u = 0; u < kTile; u += 4) {
+                    for (int u = 0; u < KT; u += 4) {
                         mx = fmaxf(mx, fmaxf(x[u], x[u + 1]));
                         mx1 = fmaxf(mx1, fmaxf(x[u + 2], x[u + 3]));
                     }
                     mx = fmaxf(mx, mx1);
-                    mx = mx == -INFINITY ? mx : __fmul_rn(mx, c2);
+                    if constexpr (F32) {
+                        const int ke = kv_exp[(kt + j) % kMaskRing][0];
+                        cf = fmaxf(__fmul_rn(__fmul_rn(c2, pow2(qe - 14)), pow2(ke - 14)), 1.17549435e-38f);
+                    }
+                    mx = mx == -INFINITY ? mx : __fmul_rn(mx, cf);
                     const bool grow = mx > __fadd_rn(m, kLazy) || (m == -INFINITY && mx > m);
-                    if (__any_sync(kAll, grow)) {
+                    int vt = 0;  // fp32: exponent of this tile's values
+                    if constexpr (F32) {
+                        const uint32_t v = 2 * (kt + j) + 1;  // the values' slot: their exponent comes with them
+                        ok = __all_sync(kAll, mbar_wait_bounded(&full[v % C::Slots], (v / C::Slots) & 1, wait_limit()));
+                        if (!ok) break;
+                        vt = kv_exp[(kt + j) % kMaskRing][1];
+                        if (njob == 0) ve = vt;
+                    }
+                    if (__any_sync(kAll, grow) || (F32 && vt != ve)) {
                         const float mn = grow ? mx : m;
-                        const float fold = m == -INFINITY ? 0.0f : grow ? ex2(__fsub_rn(m, mn)) : 1.0f;
+                        float fold = m == -INFINITY ? 0.0f : grow ? ex2(__fsub_rn(m, mn)) : 1.0f;
                         l = __fmul_rn(l, fold);
                         m = mn;
+                        if constexpr (F32) {  // O in the units of the larger values
+                            fold = __fmul_rn(fold, pow2(max(ve - vt, -126)));
+                            ve = vt;
+                        }
                         if (njob > 0) {  // O of the jobs so far, once the last of them is complete
                             ok = __all_sync(kAll, mbar_wait_bounded(&o_done[grp], (job - 1) & 1, wait_limit()));
                             if (!ok) break;
@@ -578,19 +800,21 @@ __global__ void __launch_bounds__(kThreadsTc, 1) k_paged_many(const __grid_const
                             tc_wait_st();
                         }
                     }
-                    const float base = m == -INFINITY ? 0.0f : m;
+                    const float base = m == -INFINITY ? 0.0f : __fsub_rn(m, kBias);
                     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int c = 0; c < kTile; c += 64) {
-                        uint32_t w[32];
+                    for (int c = 0; c < KT; c += 32) {
+                        uint32_t w[16], wl[F32 ? 16 : 1];
 #pragma unroll
-                        for (int u = 0; u < 64; u += 2) {
-                            const float e0 = ex2(__fmaf_rn(x[c + u], c2, -base)), e1 = ex2(__fmaf_rn(x[c + u + 1], c2, -base));
+                        for (int u = 0; u < 32; u += 2) {
+                            const float e0 = ex2(__fmaf_rn(x[c + u], cf, -base)), e1 = ex2(__fmaf_rn(x[c + u + 1], cf, -base));
                             sum[u & 2] = __fadd_rn(sum[u & 2], e0);
                             sum[(u & 2) + 1] = __fadd_rn(sum[(u & 2) + 1], e1);
-                            w[u / 2] = pack2<T>(e0, e1);
+                            if constexpr (F32) split2(e0, e1, w[u / 2], wl[u / 2]);
+                            else w[u / 2] = pack2<T>(e0, e1);
                         }
-                        tc_st32(ts + c / 2, w);
+                        tc_st16(ts + c / 2, w);
+                        if constexpr (F32) tc_st16(ts + KT / 2 + c / 2, wl);
                     }
                     l = __fadd_rn(l, __fadd_rn(__fadd_rn(sum[0], sum[1]), __fadd_rn(sum[2], sum[3])));
                     tc_wait_st();
@@ -608,7 +832,12 @@ __global__ void __launch_bounds__(kThreadsTc, 1) k_paged_many(const __grid_const
             }
             if (!ok) abort_sh = 1;
             // ---- the item's rows: group 0 joins group 1's when they shared them ----
-            if (!it.two && grp == 1) ml[row] = make_float2(m, l);
+            if (!it.two && grp == 1 && ok && nt > 1) {  // in the score columns, which are free
+                uint32_t w[32] = {};
+                w[0] = __float_as_uint(m), w[1] = __float_as_uint(l), w[2] = __float_as_uint(pow2(ve));
+                tc_st32(ts, w);
+                tc_wait_st();
+            }
             tc_fence_before();
             asm volatile("bar.sync 1, 256;" ::: "memory");
             tc_fence_after();
@@ -617,17 +846,20 @@ __global__ void __launch_bounds__(kThreadsTc, 1) k_paged_many(const __grid_const
                 float f0 = 1.0f, f1 = 0.0f;
                 const bool other = !it.two && nt > 1;  // group 1 had tiles
                 if (other) {
-                    const float2 o1 = ml[row];
-                    const float m1 = o1.x, M = fmaxf(m, m1);
+                    float o1[32];
+                    tc_ld32(ts + KT, o1);
+                    const float m1 = o1[0], M = fmaxf(m, m1);
                     f0 = m == -INFINITY ? 0.0f : ex2(__fsub_rn(m, M));
                     f1 = m1 == -INFINITY ? 0.0f : ex2(__fsub_rn(m1, M));
-                    l = __fmaf_rn(o1.y, f1, __fmul_rn(l, f0));
+                    l = __fmaf_rn(o1[1], f1, __fmul_rn(l, f0));
                     m = M;
+                    if constexpr (F32) f1 = __fmul_rn(__fmul_rn(f1, o1[2]), pow2(-14));
                 }
+                if constexpr (F32) f0 = __fmul_rn(__fmul_rn(f0, pow2(ve)), pow2(-14));
                 bool odd = false;
                 if (nt > 0)
 #pragma unroll
-                    for (int e = 0; e < kProducers; ++e) odd = odd || odd_sh[live % kMaskRing][e] != 0;
+                    for (int e = 0; e < C::Producers; ++e) odd = odd || odd_sh[live % kMaskRing][e] != 0;
                 const bool fin = it.nsplit == 1;
                 const float inv = m == -INFINITY ? 0.0f : __frcp_rn(l), w0 = fin ? __fmul_rn(f0, inv) : f0,
                             w1 = fin ? __fmul_rn(f1, inv) : f1;
@@ -654,12 +886,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) k_paged_many(const __grid_const
                     if (fin) {
                         if (mine)
 #pragma unroll
-                            for (int u = 0; u < 32; u += 8) {
-                                uint4 y;
-                                y.x = pack2<T>(v[u], v[u + 1]), y.y = pack2<T>(v[u + 2], v[u + 3]);
-                                y.z = pack2<T>(v[u + 4], v[u + 5]), y.w = pack2<T>(v[u + 6], v[u + 7]);
-                                *reinterpret_cast<uint4 *>(yp + c + u) = y;
-                            }
+                            for (int u = 0; u < 32; u += 8) store8<T>(yp + c + u, v + u);
                     } else if (room) {
 #pragma unroll
                         for (int u = 0; u < 32; u += 4)
@@ -668,7 +895,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) k_paged_many(const __grid_const
                 }
                 if (fin) {
                     if (mine && a.lse)
-                        a.lse[(int64_t)h * a.c.n_tokens + it.q.q0 + tok] = m == -INFINITY ? -INFINITY : __fadd_rn(m, log2f(l));
+                        a.lse[(int64_t)h * a.c.n_tokens + it.q.q0 + tok] = m == -INFINITY ? -INFINITY : __fadd_rn(m, __fsub_rn(log2f(l), kBias));
                 } else if (room) {
                     __stcg(reinterpret_cast<float2 *>(pp + HD / 4 * f.part_rows) + r_own, make_float2(m, l));
                 } else if (tid == 0) {
@@ -676,7 +903,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) k_paged_many(const __grid_const
                 }
                 if (odd && mine)
                     for (int c = 0; c < HD; ++c) {
-                        const float y = odd_term<T>(a, it.s, it.g, pos, it.lo + it.t0 * kTile, it.lo + it.t1 * kTile, c);
+                        const float y = odd_term<T>(a, it.s, it.g, pos, it.lo + it.t0 * KT, it.lo + it.t1 * KT, c);
                         if (y == 0.0f) continue;
                         if (fin) yp[c] = from_f<T>(y);
                         else if (room) __stcg(reinterpret_cast<float *>(pp + c / 4 * f.part_rows + r_own) + c % 4, y);
@@ -727,12 +954,11 @@ __global__ void __launch_bounds__(kThreadsTc, 1) k_paged_many(const __grid_const
                                 y[4] = __fmaf_rn(v1.x, w[t], y[4]), y[5] = __fmaf_rn(v1.y, w[t], y[5]);
                                 y[6] = __fmaf_rn(v1.z, w[t], y[6]), y[7] = __fmaf_rn(v1.w, w[t], y[7]);
                             }
-                        uint4 o;
-                        o.x = pack2<T>(y[0] * inv, y[1] * inv), o.y = pack2<T>(y[2] * inv, y[3] * inv);
-                        o.z = pack2<T>(y[4] * inv, y[5] * inv), o.w = pack2<T>(y[6] * inv, y[7] * inv);
-                        *reinterpret_cast<uint4 *>(yp + c) = o;
+#pragma unroll
+                        for (int u = 0; u < 8; ++u) y[u] = __fmul_rn(y[u], inv);
+                        store8<T>(yp + c, y);
                     }
-                    if (a.lse) a.lse[(int64_t)hh * a.c.n_tokens + it.q.q0 + tk] = M == -INFINITY ? -INFINITY : __fadd_rn(M, log2f(lt));
+                    if (a.lse) a.lse[(int64_t)hh * a.c.n_tokens + it.q.q0 + tk] = M == -INFINITY ? -INFINITY : __fadd_rn(M, __fsub_rn(log2f(lt), kBias));
                 }
             }
             // the next item's queries overwrite this one's, and its first products the outputs
@@ -758,11 +984,11 @@ int launch(const ManyArgs &f, unsigned grid, cudaStream_t st) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return ALTXS_ECUDA;
     if (dev >= 64 || !((set.load() >> dev) & 1)) {
-        if (cudaFuncSetAttribute(k_paged_many<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tc<HD>::Smem) != cudaSuccess)
+        if (cudaFuncSetAttribute(k_paged_many<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tc<T, HD>::Smem) != cudaSuccess)
             return ALTXS_ECUDA;
         if (dev < 64) set.fetch_or(1ull << dev);
     }
-    ALTXS_LAUNCH(kKPaged, st, k_paged_many<T, HD><<<grid, kThreadsTc, Tc<HD>::Smem, st>>>(f));
+    ALTXS_LAUNCH(kKPaged, st, k_paged_many<T, HD><<<grid, Tc<T, HD>::Threads, Tc<T, HD>::Smem, st>>>(f));
     return ALTXS_OK;
 }
 template <typename T>
@@ -776,11 +1002,12 @@ int launch(const ManyArgs &f, unsigned grid, cudaStream_t st) {
 ManyPlan paged_many_plan(const altxs_paged_kv &kv, const altxs_chunks &c, int H, int window) {
     ManyPlan p{};
     const int G = H / kv.n_kv_heads;
-    const int64_t blocks = (int64_t)c.n_tokens * G / kBlockRows + c.n_seqs;
-    const int64_t keys = window > 0 ? std::min<int64_t>(c.max_kv, (int64_t)window + kBlockRows) : c.max_kv;
-    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(16, tiles_of((int)keys) / 8));
+    const int rows = block_rows(kv.dtype, kv.head_dim);
+    const int64_t blocks = (int64_t)c.n_tokens * G / rows + c.n_seqs;
+    const int64_t keys = window > 0 ? std::min<int64_t>(c.max_kv, (int64_t)window + rows) : c.max_kv;
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(16, tiles_of((int)keys, tile_keys(kv.dtype, kv.head_dim)) / 8));
     p.items = blocks * kv.n_kv_heads * most;
-    p.rows = (int64_t)c.max_new * G <= kTile ? kTile : kBlockRows;
+    p.rows = (int64_t)c.max_new * G <= 128 ? 128 : rows;
     if (most > 1) p.slots = std::min<int64_t>(p.items, (int64_t)c.n_seqs * kMostItems);
     p.slot_bytes = (int64_t)p.rows * (kv.head_dim + 2) * 4;
     return p;
@@ -790,6 +1017,7 @@ int launch_paged_many(const PagedAttnArgs &a, const ManyPlan &p, int min_rows, u
                       cudaStream_t st) {
     const ManyArgs f{a, a.H / a.kv.n_kv_heads, min_rows, p.slots, cnt, part, p.rows};
     const unsigned grid = (unsigned)std::min<int64_t>(p.items, sms);
+    if (a.kv.dtype == ALTXS_F32) return launch<float>(f, grid, st);
     return a.kv.dtype == ALTXS_BF16 ? launch<__nv_bfloat16>(f, grid, st) : launch<__half>(f, grid, st);
 }
 
