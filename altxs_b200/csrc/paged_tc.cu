@@ -54,6 +54,7 @@ namespace {
 constexpr int kMmaWarp = 8;
 constexpr int kScan = 64;         // sequences are counted in this many groups
 constexpr int kMostItems = 1184;  // of a sequence that is split (8 waves)
+constexpr int kMostSplits = 16;
 constexpr int kMaskRing = 16;     // key tiles (and items) the producers can be ahead of the softmax, at most
 constexpr unsigned kAll = 0xffffffffu;
 constexpr float kLazy = 8.0f;
@@ -73,10 +74,14 @@ struct Tc {
     // registers: (8 warps x RegS + the others x RegP) x 32 = Threads x 168 (16 bits) or 128 (fp32)
     static constexpr int RegS = F32 ? 168 : 208, RegP = 88;
     static_assert(256 * RegS + (Threads - 256) * RegP == Threads * (F32 ? 128 : 168), "register split");
-    static constexpr int Slots = F32 || HD > 64 ? 5 : 12;
+    static constexpr int Slots = F32 ? 3 : HD > 64 ? 5 : 12;
+    static constexpr int StageB = F32 ? KT * HD * 4 : 0;  // fp32: a tile's raw rows, one stage for keys and one for values
     static constexpr int Lag = HD > 64 ? 3 : HD > 32 ? 6 : 8;  // tiles a producer has in flight behind the newest
-    static constexpr int Smem = Rows / 128 * QTileB + Slots * TileB + 1024;
-    static constexpr uint32_t ColS = 0, ColO = 2 * 128;  // group i: S at KT i, O at 256 + HD i
+    static constexpr int Smem = Rows / 128 * QTileB + Slots * TileB + 2 * StageB + 1024;
+    // Tensor memory of group i: S at KT i, O at 256 + HD i.  fp32 up to 64 channels keeps the small products
+    // (hi lo + lo hi) apart at 256 + HD (2 + i): a sum loses least when it meets O's magnitude least often.
+    static constexpr bool Apart = F32 && HD <= 64;
+    static constexpr uint32_t ColS = 0, ColO = 2 * 128;
     static_assert(Smem + 2048 <= 227 * 1024, "shared memory (with the static part)");
 };
 // the same two numbers for the host and the item arithmetic
@@ -92,13 +97,14 @@ __host__ __device__ inline int tiles_of(int keys, int kt) { return (keys + kt - 
 // waves by itself, at least 8 key tiles each (a split costs about 1.5 tiles' time).
 __host__ __device__ inline int many_splits(int items, int nt) {
     constexpr int kSms = 148;
-    int most = nt / 8 < 16 ? nt / 8 : 16;
-    if (items >= 4 * kSms || most < 2) return 1;
+    const int most = nt / 8;
     int best = 1;
+    if (items >= 4 * kSms || most < 2) return 1;
     float cost = 3e38f;
-    for (int ns = 1; ns <= most && (ns == 1 || items * ns <= kMostItems); ++ns) {
-        const float c = (float)((items * ns + kSms - 1) / kSms) * ((float)nt / (float)ns + 1.5f);
-        if (c < cost * 0.99f) cost = c, best = ns;
+#pragma unroll
+    for (int ns = 1; ns <= kMostSplits; ++ns) {  // unrolled: the divisors are constants
+        const float c = (float)((items * ns + kSms - 1) / kSms) * ((float)nt * (1.0f / (float)ns) + 1.5f);
+        if (ns <= most && (ns == 1 || items * ns <= kMostItems) && c < cost * 0.99f) cost = c, best = ns;
     }
     return best;
 }
@@ -182,6 +188,9 @@ __device__ __forceinline__ float ex2(float x) {
 }
 __device__ __forceinline__ void sts16(uint32_t addr, uint4 v) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ void sts8(uint32_t addr, uint2 v) {
+    asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(v.x), "r"(v.y) : "memory");
 }
 __device__ __forceinline__ uint4 lds16(uint32_t addr) {
     uint4 v;
@@ -316,6 +325,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
     const uint32_t raw_s = smem_u32(pm_smem_raw);
     const uint32_t sq = raw_s + ((1024u - (raw_s & 1023u)) & 1023u), ring = sq + C::Rows / 128 * C::QTileB;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t limit = wait_limit();
     if (tid == 0) {
         for (int s = 0; s < C::Slots; ++s) {
             mbar_init(&full[s], C::Producers);
@@ -456,7 +466,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                         if (!__all_sync(kAll, free_now)) {
                             asm volatile("cp.async.wait_group 0;" ::: "memory");
                             while (done < n) publish(done++);
-                            ok = __all_sync(kAll, !abort_sh && mbar_wait_bounded(&empty[s], ((n / C::Slots) - 1) & 1, wait_limit()));
+                            ok = __all_sync(kAll, !abort_sh && mbar_wait_bounded(&empty[s], ((n / C::Slots) - 1) & 1, limit));
                             if (!ok) break;
                         }
                     }
@@ -489,106 +499,156 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         while (done < n) publish(done++);
         } else {
-            // fp32: units of 2 KB (64 chunks of 8 channels); warp pw takes units pw, pw + 7, ..
-            // Per tile: load the unit rows to registers, agree on the tile's largest
-            // magnitude, write the scaled planes.
-            constexpr int CR = HD / 8, UR = 64 / CR, Units = KT / UR, UW = (Units + C::Producers - 1) / C::Producers;
+            // fp32: units of 2 KB, 16-byte pieces; warp pw takes units pw, pw + 7, ..  Per tile: copy
+            // the unit rows to the raw stage one tile ahead (each lane its own pieces, so its own
+            // copies are all it waits for), agree on the tile's largest magnitude, write the planes.
+            constexpr int CR = HD / 4, UR = 128 / CR, Units = KT / UR, UW = (Units + C::Producers - 1) / C::Producers;
             static_assert(UW * UR <= 32, "one page look-up per lane");
-            for (int item = blockIdx.x; item < total && ok; item += gridDim.x) {
-                const Item it = locate<C>(f, sc, item);
-                if (it.t0 == it.t1) continue;
-                const int p0 = it.q.L - it.q.n, i0 = it.r0 / f.G, i1 = (it.r0 + it.rows - 1) / f.G;
-                const int32_t *table = a.c.page_table + it.s * a.c.table_stride;
-                const float *kbase = static_cast<const float *>(a.kv.k) + (int64_t)it.g * a.kv.head_stride;
-                const float *vbase = static_cast<const float *>(a.kv.v) + (int64_t)it.g * a.kv.head_stride;
-                const uint32_t me = live++ % kMaskRing;
-                if (lane == 0) odd_sh[me][pw] = 0;
-                int ve = -100;  // exponent of the item's values so far
-                for (int t = it.t0; t < it.t1 && ok; ++t, ++kt) {
-                    const int kb = it.lo + t * KT;
-                    // lane: row lane % UR of this warp's unit lane / UR
-                    const int un = pw + lane / UR * C::Producers, k = kb + un * UR + lane % UR;
-                    const bool want = lane < UW * UR && un < Units && k < it.hi;
-                    const int b = want ? block_of(k) : 0, page = want ? __ldg(table + b) : -1;
-                    const bool in = page >= 0 && page < a.kv.n_pages;
-                    if (want && !in) set_status(a.c.status, ALTXS_ST_BAD_POS);
-                    const int64_t off = in ? (int64_t)page * a.kv.page_stride + (int64_t)(k - b * P) * a.kv.token_stride : -1;
-                    const uint32_t seen = __ballot_sync(kAll, in);
+            const uint32_t raw = ring + C::Slots * C::TileB;
+            int item = (int)blockIdx.x - (int)gridDim.x, t = 0, ve = -100;
+            Item it;
+            it.t1 = 0;
+            // the tile being copied: its row offsets, and for its conversion later
+            int64_t off = -1;
+            uint32_t seen = 0;
+            bool whole = true, fresh = false, more = true;
+            auto advance = [&]() {  // to the next tile
+                ++t;
+                fresh = false;
+                while (t >= it.t1) {
+                    item += gridDim.x;
+                    if (item >= total) {
+                        more = false;
+                        return;
+                    }
+                    it = locate<C>(f, sc, item);
+                    t = it.t0;
+                    fresh = true;
+                }
+                const int kb = it.lo + t * KT, p0 = it.q.L - it.q.n, i0 = it.r0 / f.G, i1 = (it.r0 + it.rows - 1) / f.G;
+                // lane: row lane % UR of this warp's unit lane / UR
+                const int un = pw + lane / UR * C::Producers, k = kb + un * UR + lane % UR;
+                const bool want = lane < UW * UR && un < Units && k < it.hi;
+                const int b = want ? block_of(k) : 0;
+                const int page = want ? __ldg(a.c.page_table + it.s * a.c.table_stride + b) : -1;
+                const bool in = page >= 0 && page < a.kv.n_pages;
+                if (want && !in) set_status(a.c.status, ALTXS_ST_BAD_POS);
+                off = in ? ((int64_t)page * a.kv.page_stride + (int64_t)(k - b * P) * a.kv.token_stride +
+                            (int64_t)it.g * a.kv.head_stride) * 4 : -1;
+                seen = __ballot_sync(kAll, in);
+                whole = (kb + KT <= p0 + i0 + 1 && (a.window == 0 || kb > p0 + i1 - a.window)) || i1 == i0;
+            };
+            auto copy = [&](int kv) {
+                if (more) {
+                    const char *src0 = static_cast<const char *>(kv ? a.kv.v : a.kv.k);
+#pragma unroll
+                    for (int i = 0; i < UW; ++i) {
+                        const int un = pw + i * C::Producers;
+                        if (un >= Units) break;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int q = e * 32 + lane;  // piece of the unit: row q / CR, channels 4 (q % CR) ..
+                            const int64_t o = __shfl_sync(kAll, off, i * UR + q / CR);
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(raw + kv * C::StageB + un * 2048 + q * 16),
+                                         "l"(src0 + (o < 0 ? 0 : o) + q % CR * 16), "r"(o < 0 ? 0u : 16u)
+                                         : "memory");
+                        }
+                    }
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
+            advance();
+            copy(0);
+            copy(1);
+            while (more && ok) {
+                if (fresh) {
+                    ve = -100;  // exponent of the item's values so far
+                    if (lane == 0) odd_sh[live % kMaskRing][pw] = 0;
+                    ++live;
+                }
+                const uint32_t me = (live - 1) % kMaskRing;
+                const bool check = !whole;
+                {
+                    const int un = pw + lane / UR * C::Producers;
                     if (lane % 4 == 0 && lane < UW * UR && un < Units)
                         kmask[kt % kMaskRing][(un * UR + lane % UR) / 4] = (uint8_t)((seen >> lane) & 15);
-                    const bool whole = kb + KT <= p0 + i0 + 1 && (a.window == 0 || kb > p0 + i1 - a.window);
+                }
+                advance();
 #pragma unroll
-                    for (int kv = 0; kv < 2; ++kv, ++n) {
-                        const float *src0 = kv ? vbase : kbase;
-                        float4 x[UW][2][2];
+                for (int kv = 0; kv < 2; ++kv, ++n) {
+                    asm volatile("cp.async.wait_group 1;" ::: "memory");
+                    float4 x[UW][4];
+                    float mf = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < UW; ++i) {
+                        if (pw + i * C::Producers >= Units) break;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint4 w = lds16(raw + kv * C::StageB + (pw + i * C::Producers) * 2048 + (e * 32 + lane) * 16);
+                            x[i][e] = make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
+                            mf = fmaxf(mf, fmaxf(fmaxf(fabsf(x[i][e].x), fabsf(x[i][e].y)), fmaxf(fabsf(x[i][e].z), fabsf(x[i][e].w))));
+                        }
+                    }
+                    copy(kv);  // the next tile's, into the stage just read
+                    if ((kv && check) || __any_sync(kAll, mf == INFINITY)) {  // the largest finite magnitude; odd values
+                        bool odd = false;
                         uint32_t mx = 0;
 #pragma unroll
-                        for (int i = 0; i < UW; ++i)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const int q = e * 32 + lane;  // chunk of the unit: row q / CR, channels 8 (q % CR) ..
-                                const int64_t o = __shfl_sync(kAll, off, i * UR + q / CR);
-                                x[i][e][0] = x[i][e][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                                if (pw + i * C::Producers < Units && o >= 0) {
-                                    const float4 *src = reinterpret_cast<const float4 *>(src0 + o + q % CR * 8);
-                                    x[i][e][0] = __ldg(src), x[i][e][1] = __ldg(src + 1);
-                                }
-                            }
-                        const uint32_t s = n % C::Slots;
-                        if (n >= C::Slots)
-                            ok = __all_sync(kAll, !abort_sh && mbar_wait_bounded(&empty[s], ((n / C::Slots) - 1) & 1, wait_limit()));
-                        bool odd = false;
-#pragma unroll
-                        for (int i = 0; i < UW; ++i)
+                        for (int i = 0; i < UW; ++i) {
+                            if (pw + i * C::Producers >= Units) break;
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
-                                float4 &v = x[i][e >> 1][e & 1];
-                                float *w = reinterpret_cast<float *>(&v);
+                                float *w = reinterpret_cast<float *>(&x[i][e]);
 #pragma unroll
                                 for (int u = 0; u < 4; ++u) {
                                     mx = max(mx, finite_abs(w[u]));
-                                    if (kv && !whole && i1 > i0 && !isfinite(w[u])) w[u] = 0.0f, odd = true;
+                                    if (kv && check && !isfinite(w[u])) w[u] = 0.0f, odd = true;
                                 }
                             }
-                        mx = __reduce_max_sync(kAll, mx);
-                        if (lane == 0) wmax[n & 1][pw] = mx | (ok ? 0u : 0x80000000u);
-                        if (kv && __any_sync(kAll, odd) && lane == 0) odd_sh[me][pw] = 1;
-                        asm volatile("bar.sync 2, %0;" ::"n"(C::Producers * 32) : "memory");
-                        mx = 0;
-#pragma unroll
-                        for (int w = 0; w < C::Producers; ++w) {
-                            const uint32_t o = wmax[n & 1][w];
-                            ok = ok && !(o >> 31);
-                            mx = max(mx, o & 0x7fffffffu);
                         }
-                        if (!ok) break;  // every producer warp sees the same words
-                        int ex = exp_of(mx);
-                        if (kv) ex = ve = max(ve, ex);
-                        if (pw == 0 && lane == 0) kv_exp[kt % kMaskRing][kv] = ex;
-                        const float scale = pow2(14 - ex);
-                        const uint32_t dst = ring + s * C::TileB;
-#pragma unroll
-                        for (int i = 0; i < UW; ++i)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const int q = e * 32 + lane, r = (pw + i * C::Producers) * UR + q / CR, c = q % CR;
-                                if (pw + i * C::Producers >= Units) continue;
-                                uint4 hi, lo;
-                                const float4 v0 = x[i][e][0], v1 = x[i][e][1];
-                                split2(v0.x * scale, v0.y * scale, hi.x, lo.x);
-                                split2(v0.z * scale, v0.w * scale, hi.y, lo.y);
-                                split2(v1.x * scale, v1.y * scale, hi.z, lo.z);
-                                split2(v1.z * scale, v1.w * scale, hi.w, lo.w);
-                                const uint32_t d = dst + (c >> 3) * (KT * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-                                sts16(d, hi);
-                                sts16(d + C::PlaneB, lo);
-                            }
-                        fence_proxy_async_smem();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&full[s]);
+                        mf = __uint_as_float(mx);
+                        if (__any_sync(kAll, odd) && lane == 0) odd_sh[me][pw] = 1;
                     }
+                    const uint32_t s = n % C::Slots;
+                    if (n >= C::Slots)
+                        ok = __all_sync(kAll, !abort_sh && mbar_wait_bounded(&empty[s], ((n / C::Slots) - 1) & 1, limit));
+                    const uint32_t wm = __reduce_max_sync(kAll, __float_as_uint(mf));
+                    if (lane == 0) wmax[n & 1][pw] = wm | (ok ? 0u : 0x80000000u);
+                    asm volatile("bar.sync 2, %0;" ::"n"(C::Producers * 32) : "memory");
+                    uint32_t mx = 0;
+#pragma unroll
+                    for (int w = 0; w < C::Producers; ++w) {
+                        const uint32_t o = wmax[n & 1][w];
+                        ok = ok && !(o >> 31);
+                        mx = max(mx, o & 0x7fffffffu);
+                    }
+                    if (!ok) break;  // every producer warp sees the same words
+                    int ex = exp_of(mx);
+                    if (kv) ex = ve = max(ve, ex);
+                    if (pw == 0 && lane == 0) kv_exp[kt % kMaskRing][kv] = ex;
+                    const float scale = pow2(14 - ex);
+                    const uint32_t dst = ring + s * C::TileB;
+#pragma unroll
+                    for (int i = 0; i < UW; ++i) {
+                        if (pw + i * C::Producers >= Units) break;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int q = e * 32 + lane, r = (pw + i * C::Producers) * UR + q / CR, c4 = q % CR, c = c4 >> 1;
+                            uint2 hi, lo;
+                            split2(x[i][e].x * scale, x[i][e].y * scale, hi.x, lo.x);
+                            split2(x[i][e].z * scale, x[i][e].w * scale, hi.y, lo.y);
+                            const uint32_t d = dst + (c >> 3) * (KT * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4) + (c4 & 1) * 8;
+                            sts8(d, hi);
+                            sts8(d + C::PlaneB, lo);
+                        }
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&full[s]);
                 }
+                ++kt;
             }
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
         }
         if (!ok) abort_sh = 1;
     } else if (warp == kMmaWarp) {
@@ -601,7 +661,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                 const Item it = locate<C>(f, sc, item);
                 const int nt = it.t1 - it.t0;
                 if (nt == 0) continue;
-                ok = mbar_wait_bounded(&q_full, items & 1, wait_limit());
+                ok = mbar_wait_bounded(&q_full, items & 1, limit);
                 ++items;
                 const int T2 = it.two ? 2 * nt : nt;  // jobs: (group t & 1, tile t / 2 or t)
                 for (int t = 0; t < T2 + 2 && ok && !abort_sh; ++t) {
@@ -609,23 +669,26 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                     if (t >= 2) {  // O_i += P V of job t - 2
                         const int j = it.two ? (t - 2) / 2 : t - 2;
                         const uint32_t v = n + 2 * j + 1, s = v % C::Slots;
-                        if (!mbar_wait_bounded(&full[s], (v / C::Slots) & 1, wait_limit()) ||
-                            !mbar_wait_bounded(&p_full[i], jobs[i] & 1, wait_limit())) {
+                        if (!mbar_wait_bounded(&full[s], (v / C::Slots) & 1, limit) ||
+                            !mbar_wait_bounded(&p_full[i], jobs[i] & 1, limit)) {
                             ok = false;
                             break;
                         }
                         tc_fence_after();
                         const uint32_t vb = ring + s * C::TileB;
+                        const uint32_t d = tmem + C::ColO + HD * i, p = tmem + C::ColS + KT * i, first = t >= 4;
+                        if constexpr (F32) {
+                            const uint32_t dl = d + (C::Apart ? 2 * HD : 0);
 #pragma unroll
-                        for (int kk = 0; kk < KT / 16; ++kk) {
-                            const uint32_t d = tmem + C::ColO + HD * i, p = tmem + C::ColS + KT * i + 8 * kk;
-                            const uint64_t vh = sw128_desc(vb + kk * 2048, KT * 128);
-                            tc_mma_ts(d, p, vh, idesc<T>(HD, 1), t >= 4 || kk != 0);
-                            if constexpr (F32) {
-                                tc_mma_ts(d, p, sw128_desc(vb + C::PlaneB + kk * 2048, KT * 128), idesc<T>(HD, 1), 1u);
-                                tc_mma_ts(d, p + KT / 2, vh, idesc<T>(HD, 1), 1u);
+                            for (int kk = 0; kk < KT / 16; ++kk) {
+                                tc_mma_ts(dl, p + 8 * kk, sw128_desc(vb + C::PlaneB + kk * 2048, KT * 128), idesc<T>(HD, 1), first | kk);
+                                tc_mma_ts(dl, p + KT / 2 + 8 * kk, sw128_desc(vb + kk * 2048, KT * 128), idesc<T>(HD, 1), 1u);
                             }
                         }
+#pragma unroll
+                        for (int kk = 0; kk < KT / 16; ++kk)
+                            tc_mma_ts(d, p + 8 * kk, sw128_desc(vb + kk * 2048, KT * 128), idesc<T>(HD, 1),
+                                      (F32 && !C::Apart) ? 1u : first | kk);
                         tc_commit(&o_done[i]);
                         ++jobs[i];
                         if (!it.two || i == 1) tc_commit(&empty[s]);
@@ -633,23 +696,24 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                     if (t < T2) {  // S_i = Q K^T of job t
                         const int j = it.two ? t / 2 : t;
                         const uint32_t k = n + 2 * j, s = k % C::Slots;
-                        if (!mbar_wait_bounded(&full[s], (k / C::Slots) & 1, wait_limit())) {
+                        if (!mbar_wait_bounded(&full[s], (k / C::Slots) & 1, limit)) {
                             ok = false;
                             break;
                         }
                         tc_fence_after();
                         const uint32_t kb = ring + s * C::TileB, qb = sq + (it.two ? i * C::QTileB : 0);
                         const uint32_t d = tmem + C::ColS + KT * i;
+                        auto qd = [&](int kk, int pl) { return sw128_desc(qb + pl * C::QPlaneB + (kk >> 2) * (128 * 128) + (kk & 3) * 32, 16); };
+                        auto kd = [&](int kk, int pl) { return sw128_desc(kb + pl * C::PlaneB + (kk >> 2) * (KT * 128) + (kk & 3) * 32, 16); };
+                        if constexpr (F32) {  // the small products first, while the sum is small
 #pragma unroll
-                        for (int kk = 0; kk < HD / 16; ++kk) {
-                            const uint32_t oq = (kk >> 2) * (128 * 128) + (kk & 3) * 32, ok2 = (kk >> 2) * (KT * 128) + (kk & 3) * 32;
-                            const uint64_t qh = sw128_desc(qb + oq, 16), kh = sw128_desc(kb + ok2, 16);
-                            tc_mma(d, qh, kh, idesc<T>(KT, 0), kk != 0);
-                            if constexpr (F32) {
-                                tc_mma(d, qh, sw128_desc(kb + C::PlaneB + ok2, 16), idesc<T>(KT, 0), 1u);
-                                tc_mma(d, sw128_desc(qb + C::QPlaneB + oq, 16), kh, idesc<T>(KT, 0), 1u);
+                            for (int kk = 0; kk < HD / 16; ++kk) {
+                                tc_mma(d, qd(kk, 0), kd(kk, 1), idesc<T>(KT, 0), kk != 0);
+                                tc_mma(d, qd(kk, 1), kd(kk, 0), idesc<T>(KT, 0), 1u);
                             }
                         }
+#pragma unroll
+                        for (int kk = 0; kk < HD / 16; ++kk) tc_mma(d, qd(kk, 0), kd(kk, 0), idesc<T>(KT, 0), F32 || kk != 0);
                         tc_commit(&s_full[i]);
                         if (!it.two || i == 1) tc_commit(&empty[s]);
                     }
@@ -672,6 +736,15 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
         const float c2 = fmaxf(__fmul_rn(fabsf(a.scale), kLog2e), 1.17549435e-38f);
         // fp32's p carries 2^6 (it is 2^14 at most), so that what it loses below 2^-24 is far from the sum
         constexpr float kBias = F32 ? 6.0f : 0.0f;
+        auto load_o = [](uint32_t at, float *v) {  // 32 columns of an output
+            tc_ld32(at, v);
+            if constexpr (C::Apart) {
+                float u[32];
+                tc_ld32(at + 2 * HD, u);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = __fadd_rn(v[i], u[i]);
+            }
+        };
         const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
         uint32_t job = 0, kt = 0, live = 0;
         bool ok = true;
@@ -730,7 +803,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                 const int pa = p0 + ra / f.G, pb = p0 + rb / f.G;
                 for (int j = it.two ? 0 : grp; j < nt && ok; j += it.two ? 1 : 2) {
                     const int kb = it.lo + (it.t0 + j) * KT;
-                    ok = __all_sync(kAll, !abort_sh && mbar_wait_bounded(&s_full[grp], job & 1, wait_limit()));
+                    ok = __all_sync(kAll, !abort_sh && mbar_wait_bounded(&s_full[grp], job & 1, limit));
                     if (!ok) break;
                     tc_fence_after();
                     float x[KT];
@@ -770,7 +843,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                     int vt = 0;  // fp32: exponent of this tile's values
                     if constexpr (F32) {
                         const uint32_t v = 2 * (kt + j) + 1;  // the values' slot: their exponent comes with them
-                        ok = __all_sync(kAll, mbar_wait_bounded(&full[v % C::Slots], (v / C::Slots) & 1, wait_limit()));
+                        ok = __all_sync(kAll, mbar_wait_bounded(&full[v % C::Slots], (v / C::Slots) & 1, limit));
                         if (!ok) break;
                         vt = kv_exp[(kt + j) % kMaskRing][1];
                         if (njob == 0) ve = vt;
@@ -785,17 +858,18 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                             ve = vt;
                         }
                         if (njob > 0) {  // O of the jobs so far, once the last of them is complete
-                            ok = __all_sync(kAll, mbar_wait_bounded(&o_done[grp], (job - 1) & 1, wait_limit()));
+                            ok = __all_sync(kAll, mbar_wait_bounded(&o_done[grp], (job - 1) & 1, limit));
                             if (!ok) break;
                             tc_fence_after();
 #pragma unroll
-                            for (int c = 0; c < HD; c += 32) {
+                            for (int c = 0; c < HD * (C::Apart ? 2 : 1); c += 32) {
+                                const uint32_t at = to + (c < HD ? c : c + HD);
                                 float v[32];
-                                tc_ld32(to + c, v);
+                                tc_ld32(at, v);
                                 uint32_t w[32];
 #pragma unroll
                                 for (int u = 0; u < 32; ++u) w[u] = __float_as_uint(__fmul_rn(v[u], fold));
-                                tc_st32(to + c, w);
+                                tc_st32(at, w);
                             }
                             tc_wait_st();
                         }
@@ -826,7 +900,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                 }
                 kt += nt;
                 if (ok && njob > 0) {
-                    ok = __all_sync(kAll, mbar_wait_bounded(&o_done[grp], (job - 1) & 1, wait_limit()));
+                    ok = __all_sync(kAll, mbar_wait_bounded(&o_done[grp], (job - 1) & 1, limit));
                     tc_fence_after();
                 }
             }
@@ -870,12 +944,12 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                 for (int c = 0; c < HD; c += 32) {
                     float v[32];
                     if (nt > 0) {
-                        tc_ld32(to + c, v);
+                        load_o(to + c, v);
 #pragma unroll
                         for (int u = 0; u < 32; ++u) v[u] = __fmul_rn(v[u], w0);
                         if (other) {
                             float v1[32];
-                            tc_ld32(to + HD + c, v1);
+                            load_o(to + HD + c, v1);
 #pragma unroll
                             for (int u = 0; u < 32; ++u) v[u] = __fmaf_rn(v1[u], w1, v[u]);
                         }
