@@ -52,10 +52,10 @@ namespace altxs {
 namespace {
 
 constexpr int kMmaWarp = 8;
-constexpr int kScan = 64;         // sequences are counted in this many groups
-constexpr int kMostItems = 1184;  // of a sequence that is split (8 waves)
+constexpr int kScan = 64;        // sequences are counted in this many groups
+constexpr int kCached = 48;       // up to this many sequences' shares are kept in shared memory
+constexpr int kMostItems = 1184;  // splits of one sequence
 constexpr int kMostSplits = 16;
-constexpr int kMaskRing = 16;     // key tiles (and items) the producers can be ahead of the softmax, at most
 constexpr unsigned kAll = 0xffffffffu;
 constexpr float kLazy = 8.0f;
 
@@ -72,10 +72,11 @@ struct Tc {
     static constexpr int Producers = F32 ? 7 : 3;
     static constexpr int Threads = (kMmaWarp + 1 + Producers) * 32;
     // registers: (8 warps x RegS + the others x RegP) x 32 = Threads x 168 (16 bits) or 128 (fp32)
-    static constexpr int RegS = F32 ? 168 : 208, RegP = 88;
+    static constexpr int RegS = F32 ? 192 : 208, RegP = F32 ? 64 : 88;
     static_assert(256 * RegS + (Threads - 256) * RegP == Threads * (F32 ? 128 : 168), "register split");
-    static constexpr int Slots = F32 ? 3 : HD > 64 ? 5 : 12;
+    static constexpr int Slots = F32 ? 3 : HD > 64 ? 5 : 11;
     static constexpr int StageB = F32 ? KT * HD * 4 : 0;  // fp32: a tile's raw rows, one stage for keys and one for values
+    static constexpr int Ring = Slots > 8 ? 16 : 8;  // key tiles (and items) the producers are ahead of the softmax, at most
     static constexpr int Lag = HD > 64 ? 3 : HD > 32 ? 6 : 8;  // tiles a producer has in flight behind the newest
     static constexpr int Smem = Rows / 128 * QTileB + Slots * TileB + 2 * StageB + 1024;
     // Tensor memory of group i: S at KT i, O at 256 + HD i.  fp32 up to 64 channels keeps the small products
@@ -88,25 +89,32 @@ struct Tc {
 __host__ __device__ inline int tile_keys(int dtype, int hd) { return dtype == ALTXS_F32 && hd > 64 ? 64 : 128; }
 __host__ __device__ inline int block_rows(int dtype, int hd) { return dtype == ALTXS_F32 && hd > 64 ? 128 : 256; }
 
-// one sequence's share of the work
+// One sequence's share of the work: its (block, head) pairs, longest blocks
+// first; the first `whole` of them are one item each, the others nsplit items.
 struct Shape {
-    int R, blocks, nsplit;
+    int pairs, whole, nsplit;
+    __host__ __device__ int items() const { return whole + (pairs - whole) * nsplit; }
 };
 __host__ __device__ inline int tiles_of(int keys, int kt) { return (keys + kt - 1) / kt; }
-// Splits of every block of a sequence: enough items to fill the 148 SMs in whole
-// waves by itself, at least 8 key tiles each (a split costs about 1.5 tiles' time).
-__host__ __device__ inline int many_splits(int items, int nt) {
+// A sequence by itself fills the 148 SMs in whole waves; the pairs of the last,
+// partly filled wave are cut so that they spread over all SMs, at least 8 key
+// tiles to a split (a split costs about 4.5 tiles' time, a whole item 1.5) and
+// only for a twentieth or more of the sequence's time.
+__host__ __device__ inline void split_rule(Shape &w, int nt) {
     constexpr int kSms = 148;
-    const int most = nt / 8;
-    int best = 1;
-    if (items >= 4 * kSms || most < 2) return 1;
-    float cost = 3e38f;
+    const int waves = w.pairs / kSms, rest = w.pairs - waves * kSms, most = nt / 8;
+    w.whole = w.pairs;
+    w.nsplit = 1;
+    if (rest == 0 || most < 2) return;
+    float cost = (float)nt + 1.5f;
+    const float gain = 0.05f * cost * (float)(waves + 1);
+    cost -= gain;
 #pragma unroll
-    for (int ns = 1; ns <= kMostSplits; ++ns) {  // unrolled: the divisors are constants
-        const float c = (float)((items * ns + kSms - 1) / kSms) * ((float)nt * (1.0f / (float)ns) + 1.5f);
-        if (ns <= most && (ns == 1 || items * ns <= kMostItems) && c < cost * 0.99f) cost = c, best = ns;
+    for (int ns = 2; ns <= kMostSplits; ++ns) {  // unrolled: the divisors are constants
+        const float c = (float)((rest * ns + kSms - 1) / kSms) * ((float)nt * (1.0f / (float)ns) + 4.5f);
+        if (ns <= most && rest * ns <= kMostItems && c < cost) cost = c, w.nsplit = ns;
     }
-    return best;
+    if (w.nsplit > 1) w.whole = waves * kSms;
 }
 
 struct ManyArgs {
@@ -120,20 +128,22 @@ struct ManyArgs {
 
 template <class C>
 __device__ __forceinline__ Shape shape_of(const ManyArgs &f, const Seq &q) {
-    Shape w{0, 0, 0};
+    Shape w{0, 0, 1};
     if (q.n <= 0 || q.n * f.G < f.min_rows) return w;
-    w.R = q.n * f.G;
-    w.blocks = (w.R + C::Rows - 1) / C::Rows;
+    const int R = q.n * f.G;
+    w.pairs = (R + C::Rows - 1) / C::Rows * f.a.kv.n_kv_heads;
     // the longest block: the last rows' keys
-    const int rows = min(w.R, C::Rows), toks = (rows + f.G - 1) / f.G;
+    const int toks = (min(R, C::Rows) + f.G - 1) / f.G;
     const int keys = f.a.window > 0 ? min(q.L, f.a.window + toks - 1) : q.L;
-    w.nsplit = many_splits(w.blocks * f.a.kv.n_kv_heads, tiles_of(max(keys, 0), C::KT));
+    split_rule(w, tiles_of(max(keys, 0), C::KT));
     return w;
 }
 
 struct Scan {
-    int before[kScan + 1], slots[kScan + 1];  // items, and items of split sequences, before each group
+    int before[kScan + 1], slots[kScan + 1];  // items, and partial slots, before each group of sequences
     int per;
+    // up to kCached sequences: each one's rows (q0, n, L) and its share (whole << 5 | nsplit)
+    int4 seq[kCached];
 };
 
 struct Item {
@@ -156,21 +166,33 @@ __device__ __forceinline__ Item locate(const ManyArgs &f, const Scan &sc, int it
     const int Hkv = f.a.kv.n_kv_heads;
     it.s = lo * sc.per;
     int local = item - sc.before[lo], slot = sc.slots[lo];
-    it.q = load_seq(f.a.c, it.s);
-    Shape w = shape_of<C>(f, it.q);
-    for (int n; it.s < f.a.c.n_seqs - 1 && local >= (n = w.blocks * w.nsplit * Hkv); w = shape_of<C>(f, it.q)) {
-        local -= n;
-        if (w.nsplit > 1) slot += n;
-        it.q = load_seq(f.a.c, ++it.s);
+    Shape w;
+    if (f.a.c.n_seqs <= kCached) {
+        const int4 v = sc.seq[lo];
+        it.q = Seq{v.x, v.y, v.z};
+        w.whole = v.w >> 5, w.nsplit = v.w & 31;
+    } else {
+        it.q = load_seq(f.a.c, it.s);
+        w = shape_of<C>(f, it.q);
+        for (int n; it.s < f.a.c.n_seqs - 1 && local >= (n = w.items()); w = shape_of<C>(f, it.q)) {
+            local -= n;
+            slot += n - w.whole;
+            it.q = load_seq(f.a.c, ++it.s);
+        }
     }
-    it.nsplit = w.nsplit;
-    it.split = local % w.nsplit;
-    it.slot = slot + local - it.split;
-    local /= w.nsplit;
-    it.g = local % Hkv;
-    const int blk = w.blocks - 1 - local / Hkv;  // the longest blocks first
+    const int R = it.q.n * f.G;
+    it.nsplit = 1, it.split = 0, it.slot = 0;
+    if (local >= w.whole && w.nsplit > 1) {
+        const int r = local - w.whole, pr = r / w.nsplit;
+        it.nsplit = w.nsplit;
+        it.split = r - pr * w.nsplit;
+        it.slot = slot + r - it.split;
+        local = w.whole + pr;
+    }
+    const int bd = local / Hkv, blk = (R + C::Rows - 1) / C::Rows - 1 - bd;  // the longest blocks first
+    it.g = local - bd * Hkv;
     it.r0 = blk * C::Rows;
-    it.rows = min(w.R - it.r0, C::Rows);
+    it.rows = min(R - it.r0, C::Rows);
     it.two = it.rows > 128;
     const int p0 = it.q.L - it.q.n, i0 = it.r0 / f.G, i1 = (it.r0 + it.rows - 1) / f.G;
     it.hi = max(0, p0 + i1 + 1);
@@ -197,6 +219,11 @@ __device__ __forceinline__ uint4 lds16(uint32_t addr) {
     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
     return v;
 }
+__device__ __forceinline__ float4 lds_f4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
     if constexpr (std::is_same<T, __half>::value) {
@@ -212,12 +239,25 @@ constexpr uint32_t idesc(int n, int bmn) {  // kind::f16 (bf16, or fp16: fp32's 
     const uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     return (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)bmn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
-// D += A B with A (rows = lanes, two 16-bit values per column) in tensor memory
-__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+// Matrix descriptors of 128-byte-swizzled tiles: the upper word is the same for
+// all of them (8-row groups every 1024 bytes), the lower one holds the address
+// and, for MN-major tiles, the distance of 64-channel halves; offsets are added
+// in units of 16 bytes.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo) { return (saddr >> 4) | (lbo >> 4) << 16; }
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t accumulate) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-        "r"(a), "l"(b), "r"(id), "r"(accumulate)
+        "{\n .reg .pred p;\n .reg .b64 a, b;\n setp.ne.b32 p, %5, 0;\n mov.b64 a, {%1, %3};\n mov.b64 b, {%2, %3};\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(kDescHi), "r"(id), "r"(accumulate)
+        : "memory");
+}
+// D += A B with A (rows = lanes, two 16-bit values per column) in tensor memory
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t accumulate) {
+    asm volatile(
+        "{\n .reg .pred p;\n .reg .b64 b;\n setp.ne.b32 p, %5, 0;\n mov.b64 b, {%2, %3};\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(kDescHi), "r"(id), "r"(accumulate)
         : "memory");
 }
 #define ALTXS_R32(v) \
@@ -313,11 +353,11 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
     __shared__ __align__(8) uint64_t full[C::Slots], empty[C::Slots], s_full[2], p_full[2], o_done[2], q_full, drainb;
     __shared__ Scan sc;
     // by key tile: which positions exist (4 to a byte), and (fp32) the exponents of its keys and of the values so far
-    __shared__ __align__(16) uint8_t kmask[kMaskRing][KT / 4];
-    __shared__ int kv_exp[F32 ? kMaskRing : 1][2];
+    __shared__ __align__(16) uint8_t kmask[C::Ring][KT / 4];
+    __shared__ int kv_exp[F32 ? C::Ring : 1][2];
     __shared__ uint32_t wmax[F32 ? 2 : 1][8];  // (fp32) the producers' maxima, bit 31: a wait gave up
     __shared__ uint32_t tmem_sh;
-    __shared__ uint8_t odd_sh[kMaskRing][8];
+    __shared__ uint8_t odd_sh[C::Ring][8];
     __shared__ int2 wsum[kScan / 32];
     __shared__ int last_sh, stop_sh;
     __shared__ volatile int abort_sh;
@@ -350,10 +390,11 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
         const int n = a.c.n_seqs, per = (n + kScan - 1) / kScan;
         int sum = 0, cut = 0;
         for (int s = tid * per; s < min(n, (tid + 1) * per); ++s) {
-            const Shape w = shape_of<C>(f, blockIdx.x == 0 ? load_seq_report(a.c, s) : load_seq(a.c, s));
-            const int k = w.blocks * w.nsplit * a.kv.n_kv_heads;
-            sum += k;
-            if (w.nsplit > 1) cut += k;
+            const Seq q = blockIdx.x == 0 ? load_seq_report(a.c, s) : load_seq(a.c, s);
+            const Shape w = shape_of<C>(f, q);
+            sum += w.items();
+            if (w.nsplit > 1) cut += w.items() - w.whole;
+            if (n <= kCached) sc.seq[s] = make_int4(q.q0, q.n, q.L, w.whole << 5 | w.nsplit);
         }
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -412,7 +453,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                     }
                 }
                 check &= ~(1u << (m & 31));
-                if (__any_sync(kAll, odd) && lane == 0) odd_sh[odd_of % kMaskRing][pw] = 1;
+                if (__any_sync(kAll, odd) && lane == 0) odd_sh[odd_of % C::Ring][pw] = 1;
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -431,7 +472,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                 while (done < n) publish(done++);
             }
             odd_of = live++;
-            if (lane == 0) odd_sh[odd_of % kMaskRing][pw] = 0;
+            if (lane == 0) odd_sh[odd_of % C::Ring][pw] = 0;
             for (int t = it.t0; t < it.t1 && ok; ++t) {
                 const int kb = it.lo + t * KT;
                 // offsets of this warp's rows: lane 8 i' + r holds row r of its i'-th group (two rounds)
@@ -451,7 +492,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                     const int grp = pw + lane * C::Producers;
                     const uint32_t sb = seen[lane / 4] >> (8 * (lane % 4));
                     if (grp < KT / 8)
-                        *reinterpret_cast<uint16_t *>(&kmask[kt % kMaskRing][2 * grp]) =
+                        *reinterpret_cast<uint16_t *>(&kmask[kt % C::Ring][2 * grp]) =
                             (uint16_t)(((sb >> 4) & 15) << 8 | (sb & 15));
                 }
                 ++kt;
@@ -563,48 +604,47 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
             while (more && ok) {
                 if (fresh) {
                     ve = -100;  // exponent of the item's values so far
-                    if (lane == 0) odd_sh[live % kMaskRing][pw] = 0;
+                    if (lane == 0) odd_sh[live % C::Ring][pw] = 0;
                     ++live;
                 }
-                const uint32_t me = (live - 1) % kMaskRing;
+                const uint32_t me = (live - 1) % C::Ring;
                 const bool check = !whole;
                 {
                     const int un = pw + lane / UR * C::Producers;
                     if (lane % 4 == 0 && lane < UW * UR && un < Units)
-                        kmask[kt % kMaskRing][(un * UR + lane % UR) / 4] = (uint8_t)((seen >> lane) & 15);
+                        kmask[kt % C::Ring][(un * UR + lane % UR) / 4] = (uint8_t)((seen >> lane) & 15);
                 }
                 advance();
 #pragma unroll
                 for (int kv = 0; kv < 2; ++kv, ++n) {
                     asm volatile("cp.async.wait_group 1;" ::: "memory");
-                    float4 x[UW][4];
+                    const uint32_t stage = raw + kv * C::StageB + lane * 16;
                     float mf = 0.0f;
 #pragma unroll
                     for (int i = 0; i < UW; ++i) {
                         if (pw + i * C::Producers >= Units) break;
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const uint4 w = lds16(raw + kv * C::StageB + (pw + i * C::Producers) * 2048 + (e * 32 + lane) * 16);
-                            x[i][e] = make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
-                            mf = fmaxf(mf, fmaxf(fmaxf(fabsf(x[i][e].x), fabsf(x[i][e].y)), fmaxf(fabsf(x[i][e].z), fabsf(x[i][e].w))));
+                            const float4 x = lds_f4(stage + (pw + i * C::Producers) * 2048 + e * 512);
+                            mf = fmaxf(mf, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
                         }
                     }
-                    copy(kv);  // the next tile's, into the stage just read
                     if ((kv && check) || __any_sync(kAll, mf == INFINITY)) {  // the largest finite magnitude; odd values
                         bool odd = false;
                         uint32_t mx = 0;
+                        for (int i = 0; i < UW * 4; ++i) {
+                            const int un = pw + i / 4 * C::Producers;
+                            if (un >= Units) break;
+                            const uint32_t at = stage + un * 2048 + i % 4 * 512;
+                            float4 x = lds_f4(at);
+                            float *w = reinterpret_cast<float *>(&x);
+                            bool bad = false;
 #pragma unroll
-                        for (int i = 0; i < UW; ++i) {
-                            if (pw + i * C::Producers >= Units) break;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                float *w = reinterpret_cast<float *>(&x[i][e]);
-#pragma unroll
-                                for (int u = 0; u < 4; ++u) {
-                                    mx = max(mx, finite_abs(w[u]));
-                                    if (kv && check && !isfinite(w[u])) w[u] = 0.0f, odd = true;
-                                }
+                            for (int u = 0; u < 4; ++u) {
+                                mx = max(mx, finite_abs(w[u]));
+                                if (kv && check && !isfinite(w[u])) w[u] = 0.0f, bad = true;
                             }
+                            if (bad) sts16(at, make_uint4(__float_as_uint(x.x), __float_as_uint(x.y), __float_as_uint(x.z), __float_as_uint(x.w))), odd = true;
                         }
                         mf = __uint_as_float(mx);
                         if (__any_sync(kAll, odd) && lane == 0) odd_sh[me][pw] = 1;
@@ -625,7 +665,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                     if (!ok) break;  // every producer warp sees the same words
                     int ex = exp_of(mx);
                     if (kv) ex = ve = max(ve, ex);
-                    if (pw == 0 && lane == 0) kv_exp[kt % kMaskRing][kv] = ex;
+                    if (pw == 0 && lane == 0) kv_exp[kt % C::Ring][kv] = ex;
                     const float scale = pow2(14 - ex);
                     const uint32_t dst = ring + s * C::TileB;
 #pragma unroll
@@ -634,14 +674,16 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const int q = e * 32 + lane, r = (pw + i * C::Producers) * UR + q / CR, c4 = q % CR, c = c4 >> 1;
+                            const float4 x = lds_f4(stage + (pw + i * C::Producers) * 2048 + e * 512);
                             uint2 hi, lo;
-                            split2(x[i][e].x * scale, x[i][e].y * scale, hi.x, lo.x);
-                            split2(x[i][e].z * scale, x[i][e].w * scale, hi.y, lo.y);
+                            split2(x.x * scale, x.y * scale, hi.x, lo.x);
+                            split2(x.z * scale, x.w * scale, hi.y, lo.y);
                             const uint32_t d = dst + (c >> 3) * (KT * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4) + (c4 & 1) * 8;
                             sts8(d, hi);
                             sts8(d + C::PlaneB, lo);
                         }
                     }
+                    copy(kv);  // the next tile's, into the stage just read
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&full[s]);
@@ -655,7 +697,15 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
         // ---- MMA issuer ----
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::RegP));
         if (lane == 0) {
-            uint32_t n = 0, items = 0, jobs[2] = {0, 0};  // slots and items so far; PV jobs issued per group
+            uint32_t items = 0, pph[2] = {0, 0};  // items so far; p_full's parity per group
+            // keys take slots 0, 2, 4, .. and values 1, 3, 5, .. of the ring's sequence
+            uint32_t ks = 0, kph = 0, vs = 1, vph = 0;
+            auto step = [](uint32_t &s, uint32_t &ph) {
+                s += 2;
+                if (s >= C::Slots) s -= C::Slots, ph ^= 1;
+            };
+            constexpr uint32_t kTileD = C::TileB >> 4, kPlaneD = C::PlaneB >> 4, kQPlaneD = C::QPlaneB >> 4;
+            const uint32_t ringk = desc_lo(ring, 16), ringv = desc_lo(ring, KT * 128), q0d = desc_lo(sq, 16);
             bool ok = true;
             for (int item = blockIdx.x; item < total && ok; item += gridDim.x) {
                 const Item it = locate<C>(f, sc, item);
@@ -666,59 +716,59 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                 const int T2 = it.two ? 2 * nt : nt;  // jobs: (group t & 1, tile t / 2 or t)
                 for (int t = 0; t < T2 + 2 && ok && !abort_sh; ++t) {
                     const int i = t & 1;
+                    const bool last = !it.two || i == 1;  // the tile's last use
+                    const uint32_t sc0 = tmem + C::ColS + KT * i;
                     if (t >= 2) {  // O_i += P V of job t - 2
-                        const int j = it.two ? (t - 2) / 2 : t - 2;
-                        const uint32_t v = n + 2 * j + 1, s = v % C::Slots;
-                        if (!mbar_wait_bounded(&full[s], (v / C::Slots) & 1, limit) ||
-                            !mbar_wait_bounded(&p_full[i], jobs[i] & 1, limit)) {
+                        if (!mbar_wait_bounded(&full[vs], vph, limit) || !mbar_wait_bounded(&p_full[i], pph[i], limit)) {
                             ok = false;
                             break;
                         }
+                        pph[i] ^= 1;
                         tc_fence_after();
-                        const uint32_t vb = ring + s * C::TileB;
-                        const uint32_t d = tmem + C::ColO + HD * i, p = tmem + C::ColS + KT * i, first = t >= 4;
+                        const uint32_t vb = ringv + vs * kTileD, d = tmem + C::ColO + HD * i, more = t >= 4;
                         if constexpr (F32) {
                             const uint32_t dl = d + (C::Apart ? 2 * HD : 0);
 #pragma unroll
                             for (int kk = 0; kk < KT / 16; ++kk) {
-                                tc_mma_ts(dl, p + 8 * kk, sw128_desc(vb + C::PlaneB + kk * 2048, KT * 128), idesc<T>(HD, 1), first | kk);
-                                tc_mma_ts(dl, p + KT / 2 + 8 * kk, sw128_desc(vb + kk * 2048, KT * 128), idesc<T>(HD, 1), 1u);
+                                mma_ts(dl, sc0 + 8 * kk, vb + kPlaneD + kk * 128, idesc<T>(HD, 1), kk ? 1u : more);
+                                mma_ts(dl, sc0 + KT / 2 + 8 * kk, vb + kk * 128, idesc<T>(HD, 1), 1u);
                             }
                         }
 #pragma unroll
                         for (int kk = 0; kk < KT / 16; ++kk)
-                            tc_mma_ts(d, p + 8 * kk, sw128_desc(vb + kk * 2048, KT * 128), idesc<T>(HD, 1),
-                                      (F32 && !C::Apart) ? 1u : first | kk);
+                            mma_ts(d, sc0 + 8 * kk, vb + kk * 128, idesc<T>(HD, 1), kk || (F32 && !C::Apart) ? 1u : more);
                         tc_commit(&o_done[i]);
-                        ++jobs[i];
-                        if (!it.two || i == 1) tc_commit(&empty[s]);
+                        if (last) {
+                            tc_commit(&empty[vs]);
+                            step(vs, vph);
+                        }
                     }
                     if (t < T2) {  // S_i = Q K^T of job t
-                        const int j = it.two ? t / 2 : t;
-                        const uint32_t k = n + 2 * j, s = k % C::Slots;
-                        if (!mbar_wait_bounded(&full[s], (k / C::Slots) & 1, limit)) {
+                        if (!mbar_wait_bounded(&full[ks], kph, limit)) {
                             ok = false;
                             break;
                         }
                         tc_fence_after();
-                        const uint32_t kb = ring + s * C::TileB, qb = sq + (it.two ? i * C::QTileB : 0);
-                        const uint32_t d = tmem + C::ColS + KT * i;
-                        auto qd = [&](int kk, int pl) { return sw128_desc(qb + pl * C::QPlaneB + (kk >> 2) * (128 * 128) + (kk & 3) * 32, 16); };
-                        auto kd = [&](int kk, int pl) { return sw128_desc(kb + pl * C::PlaneB + (kk >> 2) * (KT * 128) + (kk & 3) * 32, 16); };
+                        const uint32_t kb = ringk + ks * kTileD, qb = q0d + (it.two && i ? C::QTileB >> 4 : 0);
+                        // channels 16 kk ..: 32 bytes along a row, 64 channels to a half
+                        auto at = [](int kk, int half) { return (uint32_t)((kk >> 2) * (half >> 4) + (kk & 3) * 2); };
                         if constexpr (F32) {  // the small products first, while the sum is small
 #pragma unroll
                             for (int kk = 0; kk < HD / 16; ++kk) {
-                                tc_mma(d, qd(kk, 0), kd(kk, 1), idesc<T>(KT, 0), kk != 0);
-                                tc_mma(d, qd(kk, 1), kd(kk, 0), idesc<T>(KT, 0), 1u);
+                                mma_ss(sc0, qb + at(kk, 128 * 128), kb + kPlaneD + at(kk, KT * 128), idesc<T>(KT, 0), kk != 0);
+                                mma_ss(sc0, qb + kQPlaneD + at(kk, 128 * 128), kb + at(kk, KT * 128), idesc<T>(KT, 0), 1u);
                             }
                         }
 #pragma unroll
-                        for (int kk = 0; kk < HD / 16; ++kk) tc_mma(d, qd(kk, 0), kd(kk, 0), idesc<T>(KT, 0), F32 || kk != 0);
+                        for (int kk = 0; kk < HD / 16; ++kk)
+                            mma_ss(sc0, qb + at(kk, 128 * 128), kb + at(kk, KT * 128), idesc<T>(KT, 0), F32 || kk != 0);
                         tc_commit(&s_full[i]);
-                        if (!it.two || i == 1) tc_commit(&empty[s]);
+                        if (last) {
+                            tc_commit(&empty[ks]);
+                            step(ks, kph);
+                        }
                     }
                 }
-                n += 2 * nt;
                 ok = ok && !abort_sh;
             }
             if (!ok) abort_sh = 1;
@@ -811,7 +861,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                     for (int c = 0; c < KT; c += 32) tc_ld32_nowait(ts + c, x + c);
                     uint32_t km[KT / 16];  // 4 positions to a byte
 #pragma unroll
-                    for (int c = 0; c < KT / 16; ++c) km[c] = reinterpret_cast<const uint32_t *>(kmask[(kt + j) % kMaskRing])[c];
+                    for (int c = 0; c < KT / 16; ++c) km[c] = reinterpret_cast<const uint32_t *>(kmask[(kt + j) % C::Ring])[c];
                     tc_wait_ld();
 #pragma unroll
                     for (int c = 0; c < KT; c += 32) tc_tie32(x + c);
@@ -835,7 +885,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                     }
                     mx = fmaxf(mx, mx1);
                     if constexpr (F32) {
-                        const int ke = kv_exp[(kt + j) % kMaskRing][0];
+                        const int ke = kv_exp[(kt + j) % C::Ring][0];
                         cf = fmaxf(__fmul_rn(__fmul_rn(c2, pow2(qe - 14)), pow2(ke - 14)), 1.17549435e-38f);
                     }
                     mx = mx == -INFINITY ? mx : __fmul_rn(mx, cf);
@@ -845,7 +895,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                         const uint32_t v = 2 * (kt + j) + 1;  // the values' slot: their exponent comes with them
                         ok = __all_sync(kAll, mbar_wait_bounded(&full[v % C::Slots], (v / C::Slots) & 1, limit));
                         if (!ok) break;
-                        vt = kv_exp[(kt + j) % kMaskRing][1];
+                        vt = kv_exp[(kt + j) % C::Ring][1];
                         if (njob == 0) ve = vt;
                     }
                     if (__any_sync(kAll, grow) || (F32 && vt != ve)) {
@@ -933,7 +983,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                 bool odd = false;
                 if (nt > 0)
 #pragma unroll
-                    for (int e = 0; e < C::Producers; ++e) odd = odd || odd_sh[live % kMaskRing][e] != 0;
+                    for (int e = 0; e < C::Producers; ++e) odd = odd || odd_sh[live % C::Ring][e] != 0;
                 const bool fin = it.nsplit == 1;
                 const float inv = m == -INFINITY ? 0.0f : __frcp_rn(l), w0 = fin ? __fmul_rn(f0, inv) : f0,
                             w1 = fin ? __fmul_rn(f1, inv) : f1;
@@ -1004,9 +1054,9 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                     float M = -INFINITY, lt = 0.0f;
                     for (int t = 0; t < it.nsplit; ++t)
                         M = fmaxf(M, __ldcg(reinterpret_cast<const float2 *>(p + t * ps + (int64_t)HD * f.part_rows) + tid).x);
-                    float w[16];
+                    float w[kMostSplits];
 #pragma unroll
-                    for (int t = 0; t < 16; ++t) {
+                    for (int t = 0; t < kMostSplits; ++t) {
                         w[t] = 0.0f;
                         if (t < it.nsplit) {
                             const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p + t * ps + (int64_t)HD * f.part_rows) + tid);
@@ -1016,21 +1066,23 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                     }
                     const float inv = M == -INFINITY ? 0.0f : __frcp_rn(lt);
                     T *yp = static_cast<T *>(a.out) + (int64_t)(it.q.q0 + tk) * a.ldo + (int64_t)hh * HD;
-                    for (int c = 0; c < HD; c += 8) {
-                        float y[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+                    for (int c = 0; c < HD; c += 16) {
+                        float y[16] = {};
 #pragma unroll
-                        for (int t = 0; t < 16; ++t)
+                        for (int t = 0; t < kMostSplits; ++t)
                             if (t < it.nsplit) {
                                 const float4 *pt = reinterpret_cast<const float4 *>(p + t * ps) + (int64_t)(c / 4) * f.part_rows + tid;
-                                const float4 v0 = __ldcg(pt), v1 = __ldcg(pt + f.part_rows);
-                                y[0] = __fmaf_rn(v0.x, w[t], y[0]), y[1] = __fmaf_rn(v0.y, w[t], y[1]);
-                                y[2] = __fmaf_rn(v0.z, w[t], y[2]), y[3] = __fmaf_rn(v0.w, w[t], y[3]);
-                                y[4] = __fmaf_rn(v1.x, w[t], y[4]), y[5] = __fmaf_rn(v1.y, w[t], y[5]);
-                                y[6] = __fmaf_rn(v1.z, w[t], y[6]), y[7] = __fmaf_rn(v1.w, w[t], y[7]);
+#pragma unroll
+                                for (int u = 0; u < 4; ++u) {
+                                    const float4 v = __ldcg(pt + u * f.part_rows);
+                                    y[4 * u] = __fmaf_rn(v.x, w[t], y[4 * u]), y[4 * u + 1] = __fmaf_rn(v.y, w[t], y[4 * u + 1]);
+                                    y[4 * u + 2] = __fmaf_rn(v.z, w[t], y[4 * u + 2]), y[4 * u + 3] = __fmaf_rn(v.w, w[t], y[4 * u + 3]);
+                                }
                             }
 #pragma unroll
-                        for (int u = 0; u < 8; ++u) y[u] = __fmul_rn(y[u], inv);
+                        for (int u = 0; u < 16; ++u) y[u] = __fmul_rn(y[u], inv);
                         store8<T>(yp + c, y);
+                        store8<T>(yp + c + 8, y + 8);
                     }
                     if (a.lse) a.lse[(int64_t)hh * a.c.n_tokens + it.q.q0 + tk] = M == -INFINITY ? -INFINITY : __fadd_rn(M, __fsub_rn(log2f(lt), kBias));
                 }
@@ -1079,7 +1131,7 @@ ManyPlan paged_many_plan(const altxs_paged_kv &kv, const altxs_chunks &c, int H,
     const int rows = block_rows(kv.dtype, kv.head_dim);
     const int64_t blocks = (int64_t)c.n_tokens * G / rows + c.n_seqs;
     const int64_t keys = window > 0 ? std::min<int64_t>(c.max_kv, (int64_t)window + rows) : c.max_kv;
-    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(16, tiles_of((int)keys, tile_keys(kv.dtype, kv.head_dim)) / 8));
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kMostSplits, tiles_of((int)keys, tile_keys(kv.dtype, kv.head_dim)) / 8));
     p.items = blocks * kv.n_kv_heads * most;
     p.rows = (int64_t)c.max_new * G <= 128 ? 128 : rows;
     if (most > 1) p.slots = std::min<int64_t>(p.items, (int64_t)c.n_seqs * kMostItems);
