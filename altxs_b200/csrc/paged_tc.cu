@@ -243,6 +243,11 @@ constexpr uint32_t idesc(int n, int bmn) {  // kind::f16 (bf16, or fp16: fp32's 
 // all of them (8-row groups every 1024 bytes), the lower one holds the address
 // and, for MN-major tiles, the distance of 64-channel halves; offsets are added
 // in units of 16 bytes.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+    return p != 0;
+}
 __device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo) { return (saddr >> 4) | (lbo >> 4) << 16; }
 constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
 __device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t accumulate) {
@@ -696,8 +701,12 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
     } else if (warp == kMmaWarp) {
         // ---- MMA issuer ----
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::RegP));
-        if (lane == 0) {
-            uint32_t items = 0, pph[2] = {0, 0};  // items so far; p_full's parity per group
+        {
+            // The whole warp runs the loop and one lane issues, so that the operands stay in uniform
+            // registers: an issue from one lane's own control flow costs about 100 clocks each.
+            const uint32_t tm = __shfl_sync(kAll, tmem, 0);
+            const bool leader = elect_one();
+            uint32_t items = 0, pph0 = 0, pph1 = 0;  // items so far; p_full's parity per group
             // keys take slots 0, 2, 4, .. and values 1, 3, 5, .. of the ring's sequence
             uint32_t ks = 0, kph = 0, vs = 1, vph = 0;
             auto step = [](uint32_t &s, uint32_t &ph) {
@@ -709,23 +718,24 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
             bool ok = true;
             for (int item = blockIdx.x; item < total && ok; item += gridDim.x) {
                 const Item it = locate<C>(f, sc, item);
-                const int nt = it.t1 - it.t0;
+                const int nt = __shfl_sync(kAll, it.t1 - it.t0, 0);
+                const bool two = __shfl_sync(kAll, (int)it.two, 0) != 0;
                 if (nt == 0) continue;
-                ok = mbar_wait_bounded(&q_full, items & 1, limit);
+                ok = __all_sync(kAll, mbar_wait_bounded(&q_full, items & 1, limit));
                 ++items;
-                const int T2 = it.two ? 2 * nt : nt;  // jobs: (group t & 1, tile t / 2 or t)
-                for (int t = 0; t < T2 + 2 && ok && !abort_sh; ++t) {
+                const int T2 = two ? 2 * nt : nt;  // jobs: (group t & 1, tile t / 2 or t)
+                for (int t = 0; t < T2 + 2; ++t) {
                     const int i = t & 1;
-                    const bool last = !it.two || i == 1;  // the tile's last use
-                    const uint32_t sc0 = tmem + C::ColS + KT * i;
+                    const bool last = !two || i == 1;  // the tile's last use
+                    const uint32_t sc0 = tm + C::ColS + KT * i;
                     if (t >= 2) {  // O_i += P V of job t - 2
-                        if (!mbar_wait_bounded(&full[vs], vph, limit) || !mbar_wait_bounded(&p_full[i], pph[i], limit)) {
-                            ok = false;
-                            break;
-                        }
-                        pph[i] ^= 1;
+                        ok = mbar_wait_bounded(&full[vs], vph, limit) && mbar_wait_bounded(&p_full[i], i ? pph1 : pph0, limit);
+                        ok = __all_sync(kAll, ok && !abort_sh);
+                        if (!ok) break;
+                        if (i) pph1 ^= 1; else pph0 ^= 1;
                         tc_fence_after();
-                        const uint32_t vb = ringv + vs * kTileD, d = tmem + C::ColO + HD * i, more = t >= 4;
+                        const uint32_t vb = ringv + vs * kTileD, d = tm + C::ColO + HD * i, more = t >= 4;
+                        if (leader) {
                         if constexpr (F32) {
                             const uint32_t dl = d + (C::Apart ? 2 * HD : 0);
 #pragma unroll
@@ -738,20 +748,18 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                         for (int kk = 0; kk < KT / 16; ++kk)
                             mma_ts(d, sc0 + 8 * kk, vb + kk * 128, idesc<T>(HD, 1), kk || (F32 && !C::Apart) ? 1u : more);
                         tc_commit(&o_done[i]);
-                        if (last) {
-                            tc_commit(&empty[vs]);
-                            step(vs, vph);
+                        if (last) tc_commit(&empty[vs]);
                         }
+                        if (last) step(vs, vph);
                     }
                     if (t < T2) {  // S_i = Q K^T of job t
-                        if (!mbar_wait_bounded(&full[ks], kph, limit)) {
-                            ok = false;
-                            break;
-                        }
+                        ok = __all_sync(kAll, mbar_wait_bounded(&full[ks], kph, limit));
+                        if (!ok) break;
                         tc_fence_after();
-                        const uint32_t kb = ringk + ks * kTileD, qb = q0d + (it.two && i ? C::QTileB >> 4 : 0);
+                        const uint32_t kb = ringk + ks * kTileD, qb = q0d + (two && i ? C::QTileB >> 4 : 0);
                         // channels 16 kk ..: 32 bytes along a row, 64 channels to a half
                         auto at = [](int kk, int half) { return (uint32_t)((kk >> 2) * (half >> 4) + (kk & 3) * 2); };
+                        if (leader) {
                         if constexpr (F32) {  // the small products first, while the sum is small
 #pragma unroll
                             for (int kk = 0; kk < HD / 16; ++kk) {
@@ -763,17 +771,18 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                         for (int kk = 0; kk < HD / 16; ++kk)
                             mma_ss(sc0, qb + at(kk, 128 * 128), kb + at(kk, KT * 128), idesc<T>(KT, 0), F32 || kk != 0);
                         tc_commit(&s_full[i]);
-                        if (last) {
-                            tc_commit(&empty[ks]);
-                            step(ks, kph);
+                        if (last) tc_commit(&empty[ks]);
                         }
+                        if (last) step(ks, kph);
                     }
                 }
-                ok = ok && !abort_sh;
+                ok = __all_sync(kAll, ok && !abort_sh);
             }
             if (!ok) abort_sh = 1;
-            tc_commit(&drainb);  // every MMA has completed before the block can exit
-            mbar_wait_bounded(&drainb, 0, kWaitLimit);
+            if (leader) {
+                tc_commit(&drainb);  // every MMA has completed before the block can exit
+                mbar_wait_bounded(&drainb, 0, kWaitLimit);
+            }
         }
         __syncwarp();
     } else {
