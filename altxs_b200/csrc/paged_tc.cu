@@ -243,6 +243,16 @@ constexpr uint32_t idesc(int n, int bmn) {  // kind::f16 (bf16, or fp16: fp32's 
 // all of them (8-row groups every 1024 bytes), the lower one holds the address
 // and, for MN-major tiles, the distance of 64-channel halves; offsets are added
 // in units of 16 bytes.
+// whether a phase is complete, without waiting (mbar_try_wait may sleep for a while first)
+__device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
     asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
@@ -508,8 +518,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                     const uint32_t s = n % C::Slots;
                     if (n >= C::Slots) {
                         // let what has landed go out before blocking on a slot that waits for it
-                        bool free_now = mbar_try_wait(&empty[s], ((n / C::Slots) - 1) & 1);
-                        if (!__all_sync(kAll, free_now)) {
+                        if (!__all_sync(kAll, mbar_test(&empty[s], ((n / C::Slots) - 1) & 1))) {
                             asm volatile("cp.async.wait_group 0;" ::: "memory");
                             while (done < n) publish(done++);
                             ok = __all_sync(kAll, !abort_sh && mbar_wait_bounded(&empty[s], ((n / C::Slots) - 1) & 1, limit));
@@ -724,54 +733,71 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                 ok = __all_sync(kAll, mbar_wait_bounded(&q_full, items & 1, limit));
                 ++items;
                 const int T2 = two ? 2 * nt : nt;  // jobs: (group t & 1, tile t / 2 or t)
+                auto issue_pv = [&](int i, uint32_t more) {  // O_i += P V
+                    const uint32_t vb = ringv + vs * kTileD, d = tm + C::ColO + HD * i, p = tm + C::ColS + KT * i;
+                    if constexpr (F32) {
+                        const uint32_t dl = d + (C::Apart ? 2 * HD : 0);
+#pragma unroll
+                        for (int kk = 0; kk < KT / 16; ++kk) {
+                            mma_ts(dl, p + 8 * kk, vb + kPlaneD + kk * 128, idesc<T>(HD, 1), kk ? 1u : more);
+                            mma_ts(dl, p + KT / 2 + 8 * kk, vb + kk * 128, idesc<T>(HD, 1), 1u);
+                        }
+                    }
+#pragma unroll
+                    for (int kk = 0; kk < KT / 16; ++kk)
+                        mma_ts(d, p + 8 * kk, vb + kk * 128, idesc<T>(HD, 1), kk || (F32 && !C::Apart) ? 1u : more);
+                };
+                auto issue_s = [&](int i) {  // S_i = Q K^T
+                    const uint32_t kb = ringk + ks * kTileD, qb = q0d + (two && i ? C::QTileB >> 4 : 0), d = tm + C::ColS + KT * i;
+                    // channels 16 kk ..: 32 bytes along a row, 64 channels to a half
+                    auto at = [](int kk, int half) { return (uint32_t)((kk >> 2) * (half >> 4) + (kk & 3) * 2); };
+                    if constexpr (F32) {  // the small products first, while the sum is small
+#pragma unroll
+                        for (int kk = 0; kk < HD / 16; ++kk) {
+                            mma_ss(d, qb + at(kk, 128 * 128), kb + kPlaneD + at(kk, KT * 128), idesc<T>(KT, 0), kk != 0);
+                            mma_ss(d, qb + kQPlaneD + at(kk, 128 * 128), kb + at(kk, KT * 128), idesc<T>(KT, 0), 1u);
+                        }
+                    }
+#pragma unroll
+                    for (int kk = 0; kk < HD / 16; ++kk)
+                        mma_ss(d, qb + at(kk, 128 * 128), kb + at(kk, KT * 128), idesc<T>(KT, 0), F32 || kk != 0);
+                };
                 for (int t = 0; t < T2 + 2; ++t) {
                     const int i = t & 1;
                     const bool last = !two || i == 1;  // the tile's last use
-                    const uint32_t sc0 = tm + C::ColS + KT * i;
-                    if (t >= 2) {  // O_i += P V of job t - 2
+                    // The keys of job t are usually there: then its S follows the P V of job t - 2 in one go.
+                    // (Where they wait for that P V's slot, it goes first.)
+                    bool keys = t < T2 && __all_sync(kAll, mbar_test(&full[ks], kph));
+                    if (t >= 2) {
                         ok = mbar_wait_bounded(&full[vs], vph, limit) && mbar_wait_bounded(&p_full[i], i ? pph1 : pph0, limit);
                         ok = __all_sync(kAll, ok && !abort_sh);
                         if (!ok) break;
                         if (i) pph1 ^= 1; else pph0 ^= 1;
                         tc_fence_after();
-                        const uint32_t vb = ringv + vs * kTileD, d = tm + C::ColO + HD * i, more = t >= 4;
                         if (leader) {
-                        if constexpr (F32) {
-                            const uint32_t dl = d + (C::Apart ? 2 * HD : 0);
-#pragma unroll
-                            for (int kk = 0; kk < KT / 16; ++kk) {
-                                mma_ts(dl, sc0 + 8 * kk, vb + kPlaneD + kk * 128, idesc<T>(HD, 1), kk ? 1u : more);
-                                mma_ts(dl, sc0 + KT / 2 + 8 * kk, vb + kk * 128, idesc<T>(HD, 1), 1u);
+                            issue_pv(i, t >= 4);
+                            if (keys) {
+                                issue_s(i);
+                                tc_commit(&s_full[i]);
                             }
-                        }
-#pragma unroll
-                        for (int kk = 0; kk < KT / 16; ++kk)
-                            mma_ts(d, sc0 + 8 * kk, vb + kk * 128, idesc<T>(HD, 1), kk || (F32 && !C::Apart) ? 1u : more);
-                        tc_commit(&o_done[i]);
-                        if (last) tc_commit(&empty[vs]);
+                            tc_commit(&o_done[i]);
+                            if (last) tc_commit(&empty[vs]);
+                            if (last && keys) tc_commit(&empty[ks]);
                         }
                         if (last) step(vs, vph);
+                        if (keys) {
+                            if (last) step(ks, kph);
+                            continue;
+                        }
                     }
-                    if (t < T2) {  // S_i = Q K^T of job t
+                    if (t < T2) {
                         ok = __all_sync(kAll, mbar_wait_bounded(&full[ks], kph, limit));
                         if (!ok) break;
                         tc_fence_after();
-                        const uint32_t kb = ringk + ks * kTileD, qb = q0d + (two && i ? C::QTileB >> 4 : 0);
-                        // channels 16 kk ..: 32 bytes along a row, 64 channels to a half
-                        auto at = [](int kk, int half) { return (uint32_t)((kk >> 2) * (half >> 4) + (kk & 3) * 2); };
                         if (leader) {
-                        if constexpr (F32) {  // the small products first, while the sum is small
-#pragma unroll
-                            for (int kk = 0; kk < HD / 16; ++kk) {
-                                mma_ss(sc0, qb + at(kk, 128 * 128), kb + kPlaneD + at(kk, KT * 128), idesc<T>(KT, 0), kk != 0);
-                                mma_ss(sc0, qb + kQPlaneD + at(kk, 128 * 128), kb + at(kk, KT * 128), idesc<T>(KT, 0), 1u);
-                            }
-                        }
-#pragma unroll
-                        for (int kk = 0; kk < HD / 16; ++kk)
-                            mma_ss(sc0, qb + at(kk, 128 * 128), kb + at(kk, KT * 128), idesc<T>(KT, 0), F32 || kk != 0);
-                        tc_commit(&s_full[i]);
-                        if (last) tc_commit(&empty[ks]);
+                            issue_s(i);
+                            tc_commit(&s_full[i]);
+                            if (last) tc_commit(&empty[ks]);
                         }
                         if (last) step(ks, kph);
                     }
