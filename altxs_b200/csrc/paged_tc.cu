@@ -58,6 +58,7 @@ constexpr int kMostItems = 1184;  // splits of one sequence
 constexpr int kMostSplits = 16;
 constexpr unsigned kAll = 0xffffffffu;
 constexpr float kLazy = 8.0f;
+constexpr int kPolyPairs = 1;  // of every four pairs of 16-bit probabilities, those whose exponentials run on the FMA pipe
 
 template <typename T, int HD>
 struct Tc {
@@ -72,13 +73,15 @@ struct Tc {
     static constexpr int Producers = F32 ? 7 : 3;
     static constexpr int Threads = (kMmaWarp + 1 + Producers) * 32;
     // registers: (8 warps x RegS + the others x RegP) x 32 = Threads x 168 (16 bits) or 128 (fp32)
-    static constexpr int RegS = F32 ? 192 : 208, RegP = F32 ? 64 : 88;
+    static constexpr int RegS = F32 ? 176 : 208, RegP = F32 ? 80 : 88;
     static_assert(256 * RegS + (Threads - 256) * RegP == Threads * (F32 ? 128 : 168), "register split");
     static constexpr int Slots = F32 ? 3 : HD > 64 ? 5 : 11;
     static constexpr int StageB = F32 ? KT * HD * 4 : 0;  // fp32: a tile's raw rows, one stage for keys and one for values
     static constexpr int Ring = Slots > 8 ? 16 : 8;  // key tiles (and items) the producers are ahead of the softmax, at most
     static constexpr int Lag = HD > 64 ? 3 : HD > 32 ? 6 : 8;  // tiles a producer has in flight behind the newest
-    static constexpr int Smem = Rows / 128 * QTileB + Slots * TileB + 2 * StageB + 1024;
+    static constexpr int QB = Rows / 128 * QTileB;
+    static constexpr int MlAt = QB > 32768 ? 32768 : QB + Slots * TileB;  // 256 (m, l): see the softmax warps
+    static constexpr int Smem = QB + Slots * TileB + 2 * StageB + (QB > 32768 ? 0 : 2048) + 1024;
     // Tensor memory of group i: S at KT i, O at 256 + HD i.  fp32 up to 64 channels keeps the small products
     // (hi lo + lo hi) apart at 256 + HD (2 + i): a sum loses least when it meets O's magnitude least often.
     static constexpr bool Apart = F32 && HD <= 64;
@@ -343,6 +346,52 @@ __device__ __forceinline__ uint32_t finite_abs(float x) {
     return b < 0x7f800000u ? b : 0u;
 }
 
+template <int N>
+__device__ __forceinline__ Vec<float, N> ldcg_vec(const float *p) {
+    Vec<float, N> v;
+    if constexpr (N == 4) {
+        const float4 x = __ldcg(reinterpret_cast<const float4 *>(p));
+        v.e[0] = x.x, v.e[1] = x.y, v.e[2] = x.z, v.e[3] = x.w;
+    } else if constexpr (N == 2) {
+        const float2 x = __ldcg(reinterpret_cast<const float2 *>(p));
+        v.e[0] = x.x, v.e[1] = x.y;
+    } else {
+        v.e[0] = __ldcg(p);
+    }
+    return v;
+}
+// two fp32 operations per instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n .reg .b64 a, b, c, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mov.b64 c, {%6, %7};\n"
+        " fma.rn.f32x2 d, a, b, c;\n mov.b64 {%0, %1}, d;\n}\n"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n"
+        " add.rn.f32x2 d, a, b;\n mov.b64 {%0, %1}, d;\n}\n"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+// 2^x for x <= 127 without the special function unit: x = n + f with n the nearest
+// integer (by adding 1.5 2^23, whose sum's low bits are n), 2^f on [-1/2, 1/2] by
+// the polynomial of degree 4 with the least largest relative error (2.6e-6;
+// Remez's exchange), n added to the exponent.  Below -126 it gives 2^-126.
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+    constexpr float kMagic = 12582912.0f;
+    x.x = fmaxf(x.x, -126.0f), x.y = fmaxf(x.y, -126.0f);
+    const float2 r = add2(x, make_float2(kMagic, kMagic)), n = add2(r, make_float2(-kMagic, -kMagic));
+    const float2 f = fma2(n, make_float2(-1.0f, -1.0f), x);
+    float2 p = fma2(f, make_float2(0.009570102207362652f, 0.009570102207362652f), make_float2(0.05591785907745361f, 0.05591785907745361f));
+    p = fma2(p, f, make_float2(0.240247443318367f, 0.240247443318367f));
+    p = fma2(p, f, make_float2(0.6931217908859253f, 0.6931217908859253f));
+    p = fma2(p, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
+    return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(r.x) << 23)),
+                       __int_as_float(__float_as_int(p.y) + (__float_as_int(r.y) << 23)));
+}
+
 // The values of channel `dim` that are not finite, over the positions [lo, hi) that a
 // row at `pos` sees (the tiles that only some rows see hold 0 in their place).
 template <typename T>
@@ -378,7 +427,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
     __shared__ volatile int abort_sh;
     const PagedAttnArgs &a = f.a;
     const uint32_t raw_s = smem_u32(pm_smem_raw);
-    const uint32_t sq = raw_s + ((1024u - (raw_s & 1023u)) & 1023u), ring = sq + C::Rows / 128 * C::QTileB;
+    const uint32_t sq = raw_s + ((1024u - (raw_s & 1023u)) & 1023u), ring = sq + C::QB;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t limit = wait_limit();
     if (tid == 0) {
@@ -637,11 +686,12 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
 #pragma unroll
                     for (int i = 0; i < UW; ++i) {
                         if (pw + i * C::Producers >= Units) break;
+                        float4 x[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float4 x = lds_f4(stage + (pw + i * C::Producers) * 2048 + e * 512);
-                            mf = fmaxf(mf, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
-                        }
+                        for (int e = 0; e < 4; ++e) x[e] = lds_f4(stage + (pw + i * C::Producers) * 2048 + e * 512);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            mf = fmaxf(mf, fmaxf(fmaxf(fabsf(x[e].x), fabsf(x[e].y)), fmaxf(fabsf(x[e].z), fabsf(x[e].w))));
                     }
                     if ((kv && check) || __any_sync(kAll, mf == INFINITY)) {  // the largest finite magnitude; odd values
                         bool odd = false;
@@ -685,13 +735,15 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
 #pragma unroll
                     for (int i = 0; i < UW; ++i) {
                         if (pw + i * C::Producers >= Units) break;
+                        float4 x[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[e] = lds_f4(stage + (pw + i * C::Producers) * 2048 + e * 512);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const int q = e * 32 + lane, r = (pw + i * C::Producers) * UR + q / CR, c4 = q % CR, c = c4 >> 1;
-                            const float4 x = lds_f4(stage + (pw + i * C::Producers) * 2048 + e * 512);
                             uint2 hi, lo;
-                            split2(x.x * scale, x.y * scale, hi.x, lo.x);
-                            split2(x.z * scale, x.w * scale, hi.y, lo.y);
+                            split2(x[e].x * scale, x[e].y * scale, hi.x, lo.x);
+                            split2(x[e].z * scale, x[e].w * scale, hi.y, lo.y);
                             const uint32_t d = dst + (c >> 3) * (KT * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4) + (c4 & 1) * 8;
                             sts8(d, hi);
                             sts8(d + C::PlaneB, lo);
@@ -780,7 +832,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                                 issue_s(i);
                                 tc_commit(&s_full[i]);
                             }
-                            tc_commit(&o_done[i]);
+                            if (t >= T2) tc_commit(&o_done[i]);  // the group's last; before, its next S says as much
                             if (last) tc_commit(&empty[vs]);
                             if (last && keys) tc_commit(&empty[ks]);
                         }
@@ -814,125 +866,120 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
     } else {
         // ---- softmax ----
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::RegS));
-        const int grp = warp >> 2, row = (warp & 3) * 32 + lane;
-        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const int grp = warp >> 2, wq = warp & 3, row = wq * 32 + lane;  // tensor-memory lane `row`
+        const uint32_t lanes = (uint32_t)(wq * 32) << 16;
         const uint32_t ts = tmem + lanes + C::ColS + KT * grp, to = tmem + lanes + C::ColO + HD * grp;
         // a negative scale turns the queries round instead; a scale of 0 stays above it (-inf marks the unseen)
         const float c2 = fmaxf(__fmul_rn(fabsf(a.scale), kLog2e), 1.17549435e-38f);
         // fp32's p carries 2^6 (it is 2^14 at most), so that what it loses below 2^-24 is far from the sum
         constexpr float kBias = F32 ? 6.0f : 0.0f;
-        auto load_o = [](uint32_t at, float *v) {  // 32 columns of an output
-            tc_ld32(at, v);
-            if constexpr (C::Apart) {
-                float u[32];
-                tc_ld32(at + 2 * HD, u);
-#pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = __fadd_rn(v[i], u[i]);
-            }
-        };
         const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
-        uint32_t job = 0, kt = 0, live = 0;
+        unsigned char *qsm = pm_smem_raw + (sq - raw_s);
+        // between an item's last S and the next item's queries their place holds 32 KB of outputs, then 256 (m, l)
+        float *stage = reinterpret_cast<float *>(qsm);
+        float2 *ml = reinterpret_cast<float2 *>(qsm + C::MlAt);
+        uint32_t job = 0, kt = 0, live = 0, done = 0;
         bool ok = true;
         for (int item = blockIdx.x; item < total; item += gridDim.x) {
             const Item it = locate<C>(f, sc, item);
             const int nt = it.t1 - it.t0, p0 = it.q.L - it.q.n;
-            // this thread's row of the block (rows past the end follow the last one and are not stored)
-            const int r_own = it.two ? grp * 128 + row : row;
+            // At most 64 (32) rows are held 2 (4) times, each copy with its share of a tile's columns, its own
+            // (m, l) and O: a thread's chain of exponentials is 2 (4) times shorter.
+            const int rep = it.two ? 1 : it.rows > 64 ? 1 : it.rows > 32 || KT < 128 ? 2 : 4, rrows = it.two ? 256 : 128 / rep;
+            // this thread's row of the block (rows past the end follow the last one and are not stored) and its part
+            const int r_own = it.two ? grp * 128 + row : row & (rrows - 1), part = it.two ? 0 : row / rrows;
             const int r = it.r0 + min(r_own, it.rows - 1), tok = r / f.G, h = it.g * f.G + r - tok * f.G;
             const int pos = p0 + tok;
-            const bool mine = r_own < it.rows;
             float m = -INFINITY, l = 0.0f, cf = c2;  // cf: score to log2 units (fp32: times the tile's and the row's scales)
-            int qe = 0, ve = -100;                    // fp32: exponents of the row's query and of O's values
-            uint32_t njob = 0;  // jobs of this group in this item
+            int qe = 0, ve = -100;                   // fp32: exponents of the row's query and of O's values
+            uint32_t njob = 0;                       // jobs of this group in this item
             if (nt > 0) {
-                const T *qp = static_cast<const T *>(a.q) + (int64_t)(it.q.q0 + tok) * a.ldq + (int64_t)h * HD;
-                const uint32_t d = sq + (it.two ? grp * C::QTileB : 0) + row * 128;
-                if constexpr (F32) {
-                    uint32_t mq = 0;
-#pragma unroll 8
-                    for (int c = 0; c < HD; c += 4) {
-                        const float4 v = __ldg(reinterpret_cast<const float4 *>(qp + c));
-                        mq = max(max(mq, max(finite_abs(v.x), finite_abs(v.y))), max(finite_abs(v.z), finite_abs(v.w)));
-                    }
-                    qe = exp_of(mq);
-                    if (it.two || grp == 0) {
-                        const float sc1 = a.scale < 0.0f ? -pow2(14 - qe) : pow2(14 - qe);
+                // queries: the lanes share rows (16 bytes each); with shared rows each group takes half of a warp's
+                constexpr int NC = HD * (int)sizeof(T) / 16, RPI = 32 / NC;  // pieces of a row, rows per load
+                const int64_t qoff = ((int64_t)(it.q.q0 + tok) * a.ldq + (int64_t)h * HD) * (int)sizeof(T);
+                const uint32_t qd = sq + (it.two ? grp * C::QTileB : 0);
+                // (fp32: both look at all of them, for their exponents)
+                const int e0 = it.two ? 0 : grp * 16, e1 = it.two ? 32 : e0 + 16;
 #pragma unroll 4
-                        for (int c = 0; c < HD / 8; ++c) {
-                            const float4 v0 = __ldg(reinterpret_cast<const float4 *>(qp + 8 * c)),
-                                         v1 = __ldg(reinterpret_cast<const float4 *>(qp + 8 * c + 4));
-                            uint4 hi, lo;
-                            split2(v0.x * sc1, v0.y * sc1, hi.x, lo.x);
-                            split2(v0.z * sc1, v0.w * sc1, hi.y, lo.y);
-                            split2(v1.x * sc1, v1.y * sc1, hi.z, lo.z);
-                            split2(v1.z * sc1, v1.w * sc1, hi.w, lo.w);
-                            const uint32_t dd = d + (c >> 3) * (128 * 128) + (((c & 7) ^ (row & 7)) << 4);
-                            sts16(dd, hi);
-                            sts16(dd + C::QPlaneB, lo);
-                        }
-                    }
-                } else if (it.two || grp == 0) {  // the row's query
+                for (int e = F32 ? 0 : e0; e < (F32 ? 32 : e1); e += RPI) {
+                    const int rl = e + lane / NC, rr = wq * 32 + rl, c = lane % NC;
+                    const int64_t o = __shfl_sync(kAll, qoff, rl);
+                    uint4 v = __ldg(reinterpret_cast<const uint4 *>(static_cast<const char *>(a.q) + o) + c);
+                    if constexpr (F32) {
+                        const float x[4] = {__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w)};
+                        uint32_t mq = max(max(finite_abs(x[0]), finite_abs(x[1])), max(finite_abs(x[2]), finite_abs(x[3])));
 #pragma unroll
-                    for (int c = 0; c < HD / 8; ++c) {
-                        uint4 v = __ldg(reinterpret_cast<const uint4 *>(qp) + c);
+                        for (int d = 1; d < NC; d <<= 1) mq = max(mq, __shfl_xor_sync(kAll, mq, d));
+                        const int ex = exp_of(mq);
+                        const int own = __shfl_sync(kAll, ex, (lane - e) * NC & 31);
+                        if (lane >= e && lane < e + RPI) qe = own;
+                        if (e < e0 || e >= e1) continue;
+                        const float s1 = a.scale < 0.0f ? -pow2(14 - ex) : pow2(14 - ex);
+                        uint2 hi, lo;
+                        split2(x[0] * s1, x[1] * s1, hi.x, lo.x);
+                        split2(x[2] * s1, x[3] * s1, hi.y, lo.y);
+                        const int c8 = c >> 1;
+                        const uint32_t dd = qd + (c8 >> 3) * (128 * 128) + rr * 128 + (((c8 & 7) ^ (rr & 7)) << 4) + (c & 1) * 8;
+                        sts8(dd, hi);
+                        sts8(dd + C::QPlaneB, lo);
+                    } else {
                         v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
-                        sts16(d + (c >> 3) * (128 * 128) + (((c & 7) ^ (row & 7)) << 4), v);
+                        sts16(qd + (c >> 3) * (128 * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), v);
                     }
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&q_full);
-                // positions that all of this warp's rows see: from the first row's and the last row's
-                const int ra = it.r0 + min(it.two ? grp * 128 + (warp & 3) * 32 : (warp & 3) * 32, it.rows - 1);
-                const int rb = it.r0 + min(it.two ? grp * 128 + (warp & 3) * 32 + 31 : (warp & 3) * 32 + 31, it.rows - 1);
+                // positions that all of this warp's rows see: from its first row's and its last row's
+                const int ra = it.r0 + min(r_own - lane, it.rows - 1), rb = it.r0 + min(r_own - lane + 31, it.rows - 1);
                 const int pa = p0 + ra / f.G, pb = p0 + rb / f.G;
-                for (int j = it.two ? 0 : grp; j < nt && ok; j += it.two ? 1 : 2) {
-                    const int kb = it.lo + (it.t0 + j) * KT;
-                    ok = __all_sync(kAll, !abort_sh && mbar_wait_bounded(&s_full[grp], job & 1, limit));
-                    if (!ok) break;
+
+                auto tile = [&](auto rep_c, int j) -> bool {
+                    constexpr int REP = decltype(rep_c)::value, W = KT / REP;  // columns of this thread's share
+                    const int c0 = REP > 1 ? part * W : 0;
+                    const int kb = it.lo + (it.t0 + j) * KT + c0;
+                    if (!__all_sync(kAll, !abort_sh && mbar_wait_bounded(&s_full[grp], job & 1, limit))) return false;
                     tc_fence_after();
-                    float x[KT];
+                    float x[W];
 #pragma unroll
-                    for (int c = 0; c < KT; c += 32) tc_ld32_nowait(ts + c, x + c);
-                    uint32_t km[KT / 16];  // 4 positions to a byte
+                    for (int c = 0; c < W; c += 32) tc_ld32_nowait(ts + c0 + c, x + c);
+                    uint32_t km[W / 16];  // 4 positions to a byte
+                    const uint32_t *kmp = reinterpret_cast<const uint32_t *>(kmask[(kt + j) % C::Ring]) + c0 / 16;
 #pragma unroll
-                    for (int c = 0; c < KT / 16; ++c) km[c] = reinterpret_cast<const uint32_t *>(kmask[(kt + j) % C::Ring])[c];
+                    for (int c = 0; c < W / 16; ++c) km[c] = kmp[c];
                     tc_wait_ld();
 #pragma unroll
-                    for (int c = 0; c < KT; c += 32) tc_tie32(x + c);
+                    for (int c = 0; c < W; c += 32) tc_tie32(x + c);
                     uint32_t have = 0x0f0f0f0fu;
 #pragma unroll
-                    for (int c = 0; c < KT / 16; ++c) have &= km[c];
-                    const bool whole = kb + KT <= pa + 1 && (a.window == 0 || kb > pb - a.window) && have == 0x0f0f0f0fu;
+                    for (int c = 0; c < W / 16; ++c) have &= km[c];
+                    const bool whole = kb + W <= pa + 1 && (a.window == 0 || kb > pb - a.window) && have == 0x0f0f0f0fu;
                     if (!whole) {
                         const int first = a.window > 0 ? max(0, pos - a.window + 1 - kb) : 0, last = pos - kb;
 #pragma unroll
-                        for (int u = 0; u < KT; ++u) {
+                        for (int u = 0; u < W; ++u) {
                             const uint32_t bit = 1u << (8 * (u / 4 % 4) + u % 4);
                             if (u < first || u > last || !(km[u / 16] & bit)) x[u] = -INFINITY;
                         }
                     }
                     float mx = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
-                    for (int u = 0; u < KT; u += 4) {
+                    for (int u = 0; u < W; u += 4) {
                         mx = fmaxf(mx, fmaxf(x[u], x[u + 1]));
                         mx1 = fmaxf(mx1, fmaxf(x[u + 2], x[u + 3]));
                     }
                     mx = fmaxf(mx, mx1);
+                    int vt = 0;  // fp32: exponent of this tile's values
                     if constexpr (F32) {
                         const int ke = kv_exp[(kt + j) % C::Ring][0];
                         cf = fmaxf(__fmul_rn(__fmul_rn(c2, pow2(qe - 14)), pow2(ke - 14)), 1.17549435e-38f);
-                    }
-                    mx = mx == -INFINITY ? mx : __fmul_rn(mx, cf);
-                    const bool grow = mx > __fadd_rn(m, kLazy) || (m == -INFINITY && mx > m);
-                    int vt = 0;  // fp32: exponent of this tile's values
-                    if constexpr (F32) {
                         const uint32_t v = 2 * (kt + j) + 1;  // the values' slot: their exponent comes with them
-                        ok = __all_sync(kAll, mbar_wait_bounded(&full[v % C::Slots], (v / C::Slots) & 1, limit));
-                        if (!ok) break;
+                        if (!__all_sync(kAll, mbar_wait_bounded(&full[v % C::Slots], (v / C::Slots) & 1, limit))) return false;
                         vt = kv_exp[(kt + j) % C::Ring][1];
                         if (njob == 0) ve = vt;
                     }
+                    mx = mx == -INFINITY ? mx : __fmul_rn(mx, cf);
+                    const bool grow = mx > __fadd_rn(m, kLazy) || (m == -INFINITY && mx > m);
                     if (__any_sync(kAll, grow) || (F32 && vt != ve)) {
                         const float mn = grow ? mx : m;
                         float fold = m == -INFINITY ? 0.0f : grow ? ex2(__fsub_rn(m, mn)) : 1.0f;
@@ -942,10 +989,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                             fold = __fmul_rn(fold, pow2(max(ve - vt, -126)));
                             ve = vt;
                         }
-                        if (njob > 0) {  // O of the jobs so far, once the last of them is complete
-                            ok = __all_sync(kAll, mbar_wait_bounded(&o_done[grp], (job - 1) & 1, limit));
-                            if (!ok) break;
-                            tc_fence_after();
+                        if (njob > 0) {  // this job's S came after the products of the jobs before: O is at rest
 #pragma unroll
                             for (int c = 0; c < HD * (C::Apart ? 2 : 1); c += 32) {
                                 const uint32_t at = to + (c < HD ? c : c + HD);
@@ -956,117 +1000,144 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                                 for (int u = 0; u < 32; ++u) w[u] = __float_as_uint(__fmul_rn(v[u], fold));
                                 tc_st32(at, w);
                             }
-                            tc_wait_st();
                         }
                     }
                     const float base = m == -INFINITY ? 0.0f : __fsub_rn(m, kBias);
-                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    const float2 cf2 = make_float2(cf, cf), nb2 = make_float2(-base, -base);
+                    float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-                    for (int c = 0; c < KT; c += 32) {
+                    for (int c = 0; c < W; c += 32) {
                         uint32_t w[16], wl[F32 ? 16 : 1];
 #pragma unroll
                         for (int u = 0; u < 32; u += 2) {
-                            const float e0 = ex2(__fmaf_rn(x[c + u], cf, -base)), e1 = ex2(__fmaf_rn(x[c + u + 1], cf, -base));
-                            sum[u & 2] = __fadd_rn(sum[u & 2], e0);
-                            sum[(u & 2) + 1] = __fadd_rn(sum[(u & 2) + 1], e1);
-                            if constexpr (F32) split2(e0, e1, w[u / 2], wl[u / 2]);
-                            else w[u / 2] = pack2<T>(e0, e1);
+                            const float2 t = fma2(make_float2(x[c + u], x[c + u + 1]), cf2, nb2);
+                            // the special function unit is the bottleneck of the 16-bit types: a part of the
+                            // exponentials runs on the FMA pipe
+                            const float2 e = !F32 && u % 8 >= 8 - 2 * kPolyPairs ? ex2_poly(t) : make_float2(ex2(t.x), ex2(t.y));
+                            sum[u / 2 & 1] = add2(sum[u / 2 & 1], e);
+                            if constexpr (F32) split2(e.x, e.y, w[u / 2], wl[u / 2]);
+                            else w[u / 2] = pack2<T>(e.x, e.y);
                         }
-                        tc_st16(ts + c / 2, w);
-                        if constexpr (F32) tc_st16(ts + KT / 2 + c / 2, wl);
+                        tc_st16(ts + (c0 + c) / 2, w);
+                        if constexpr (F32) tc_st16(ts + KT / 2 + (c0 + c) / 2, wl);
                     }
-                    l = __fadd_rn(l, __fadd_rn(__fadd_rn(sum[0], sum[1]), __fadd_rn(sum[2], sum[3])));
+                    if constexpr (REP > 1) {  // the other copies' columns
+                        const uint32_t z[16] = {};
+#pragma unroll
+                        for (int d = W; d < KT; d += 32) {
+                            const uint32_t at = ts + ((c0 + d) & (KT - 1)) / 2;
+                            tc_st16(at, z);
+                            if constexpr (F32) tc_st16(at + KT / 2, z);
+                        }
+                    }
+                    const float2 s2 = add2(sum[0], sum[1]);
+                    l = __fadd_rn(l, __fadd_rn(s2.x, s2.y));
                     tc_wait_st();
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&p_full[grp]);
                     ++job;
                     ++njob;
-                }
+                    return true;
+                };
+                const int j0 = it.two ? 0 : grp, dj = it.two ? 1 : 2;
+                if (rep == 1)
+                    for (int j = j0; j < nt && ok; j += dj) ok = tile(std::integral_constant<int, 1>{}, j);
+                else if (rep == 2)
+                    for (int j = j0; j < nt && ok; j += dj) ok = tile(std::integral_constant<int, 2>{}, j);
+                else if constexpr (KT == 128)
+                    for (int j = j0; j < nt && ok; j += dj) ok = tile(std::integral_constant<int, 4>{}, j);
                 kt += nt;
-                if (ok && njob > 0) {
-                    ok = __all_sync(kAll, mbar_wait_bounded(&o_done[grp], (job - 1) & 1, limit));
+                if (ok && njob > 0) {  // the group's last products
+                    ok = __all_sync(kAll, mbar_wait_bounded(&o_done[grp], done & 1, limit));
+                    ++done;
                     tc_fence_after();
                 }
             }
             if (!ok) abort_sh = 1;
-            // ---- the item's rows: group 0 joins group 1's when they shared them ----
-            if (!it.two && grp == 1 && ok && nt > 1) {  // in the score columns, which are free
-                uint32_t w[32] = {};
-                w[0] = __float_as_uint(m), w[1] = __float_as_uint(l), w[2] = __float_as_uint(pow2(ve));
-                tc_st32(ts, w);
-                tc_wait_st();
-            }
-            tc_fence_before();
+            // ---- the item's rows: the sets that share a row (its copies, both groups) are joined in order ----
+            const int sets = it.two ? 1 : 2 * rep, set = it.two ? 0 : grp * rep + part;
+            const int slot = set * rrows + r_own;  // 0 .. 255
+            asm volatile("bar.sync 1, 256;" ::: "memory");  // no S is left to read the queries
+            ml[slot] = make_float2(m, l);
             asm volatile("bar.sync 1, 256;" ::: "memory");
-            tc_fence_after();
-            ok = !abort_sh;
-            if (ok && (it.two || grp == 0)) {
-                float f0 = 1.0f, f1 = 0.0f;
-                const bool other = !it.two && nt > 1;  // group 1 had tiles
-                if (other) {
-                    float o1[32];
-                    tc_ld32(ts + KT, o1);
-                    const float m1 = o1[0], M = fmaxf(m, m1);
-                    f0 = m == -INFINITY ? 0.0f : ex2(__fsub_rn(m, M));
-                    f1 = m1 == -INFINITY ? 0.0f : ex2(__fsub_rn(m1, M));
-                    l = __fmaf_rn(o1[1], f1, __fmul_rn(l, f0));
-                    m = M;
-                    if constexpr (F32) f1 = __fmul_rn(__fmul_rn(f1, o1[2]), pow2(-14));
+            float M = m, lt = l;
+            if (sets > 1) {
+                M = -INFINITY, lt = 0.0f;
+                for (int s = 0; s < sets; ++s) M = fmaxf(M, ml[s * rrows + r_own].x);
+                for (int s = 0; s < sets; ++s) {
+                    const float2 v = ml[s * rrows + r_own];
+                    lt = __fmaf_rn(v.y, v.x == -INFINITY ? 0.0f : ex2(__fsub_rn(v.x, M)), lt);
                 }
-                if constexpr (F32) f0 = __fmul_rn(__fmul_rn(f0, pow2(ve)), pow2(-14));
-                bool odd = false;
-                if (nt > 0)
+            }
+            const bool fin = it.nsplit == 1, room = it.slot + it.nsplit <= f.max_slots;
+            float wgt = m == -INFINITY ? 0.0f : ex2(__fsub_rn(m, M));
+            if (m == M) wgt = m == -INFINITY ? 0.0f : 1.0f;
+            if (fin) wgt = __fmul_rn(wgt, M == -INFINITY ? 0.0f : __frcp_rn(lt));
+            if constexpr (F32) wgt = __fmul_rn(__fmul_rn(wgt, pow2(ve)), pow2(-14));
+            bool odd = false;
+            if (nt > 0)
 #pragma unroll
-                    for (int e = 0; e < C::Producers; ++e) odd = odd || odd_sh[live % C::Ring][e] != 0;
-                const bool fin = it.nsplit == 1;
-                const float inv = m == -INFINITY ? 0.0f : __frcp_rn(l), w0 = fin ? __fmul_rn(f0, inv) : f0,
-                            w1 = fin ? __fmul_rn(f1, inv) : f1;
-                const bool room = it.slot + it.nsplit <= f.max_slots;
-                float4 *pp = reinterpret_cast<float4 *>(f.part + (int64_t)(it.slot + it.split) * f.part_rows * (HD + 2));
-                T *yp = static_cast<T *>(a.out) + (int64_t)(it.q.q0 + tok) * a.ldo + (int64_t)h * HD;
+                for (int e = 0; e < C::Producers; ++e) odd = odd || odd_sh[live % C::Ring][e] != 0;
+            const bool whole_ok = !abort_sh;
+            float *pp = f.part + (int64_t)(it.slot + it.split) * f.part_rows * (HD + 2);
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 32) {
+                float v[32];
+                if (njob > 0) {
+                    tc_ld32(to + c, v);
+                    if constexpr (C::Apart) {  // large and small products
+                        float u[32];
+                        tc_ld32(to + 2 * HD + c, u);
 #pragma unroll
-                for (int c = 0; c < HD; c += 32) {
-                    float v[32];
-                    if (nt > 0) {
-                        load_o(to + c, v);
+                        for (int i = 0; i < 32; ++i) v[i] = __fadd_rn(v[i], u[i]);
+                    }
 #pragma unroll
-                        for (int u = 0; u < 32; ++u) v[u] = __fmul_rn(v[u], w0);
-                        if (other) {
-                            float v1[32];
-                            load_o(to + HD + c, v1);
+                    for (int i = 0; i < 32; ++i) v[i] = __fmul_rn(v[i], wgt);
+                } else {
 #pragma unroll
-                            for (int u = 0; u < 32; ++u) v[u] = __fmaf_rn(v1[u], w1, v[u]);
+                    for (int i = 0; i < 32; ++i) v[i] = 0.0f;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i)  // 128-byte rows, swizzled like the tiles
+                    *reinterpret_cast<float4 *>(stage + slot * 32 + ((i ^ (slot & 7)) << 2)) =
+                        make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                for (int i = tid; i < min(rrows, it.rows) * 8; i += 256) {  // row i / 8, channels c + 4 (i % 8) ..
+                    const int ro = i >> 3, q = i & 7;
+                    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    for (int s = 0; s < sets; ++s) {
+                        const int at = s * rrows + ro;
+                        const float4 u = *reinterpret_cast<const float4 *>(stage + at * 32 + ((q ^ (at & 7)) << 2));
+                        y.x = __fadd_rn(y.x, u.x), y.y = __fadd_rn(y.y, u.y), y.z = __fadd_rn(y.z, u.z), y.w = __fadd_rn(y.w, u.w);
+                    }
+                    const int rr = it.r0 + ro, tk = rr / f.G, ch = c + 4 * q;
+                    if (odd) {  // what is not finite replaces the sum that it was kept out of
+                        float *w = reinterpret_cast<float *>(&y);
+                        for (int e = 0; e < 4; ++e) {
+                            const float t = odd_term<T>(a, it.s, it.g, p0 + tk, it.lo + it.t0 * KT, it.lo + it.t1 * KT, ch + e);
+                            if (t != 0.0f) w[e] = t;
                         }
-                    } else {
-#pragma unroll
-                        for (int u = 0; u < 32; ++u) v[u] = 0.0f;
                     }
+                    if (!whole_ok) continue;
                     if (fin) {
-                        if (mine)
-#pragma unroll
-                            for (int u = 0; u < 32; u += 8) store8<T>(yp + c + u, v + u);
+                        T *yp = static_cast<T *>(a.out) + (int64_t)(it.q.q0 + tk) * a.ldo + (int64_t)(it.g * f.G + rr - tk * f.G) * HD + ch;
+                        if constexpr (F32) *reinterpret_cast<float4 *>(yp) = y;
+                        else *reinterpret_cast<uint2 *>(yp) = make_uint2(pack2<T>(y.x, y.y), pack2<T>(y.z, y.w));
                     } else if (room) {
-#pragma unroll
-                        for (int u = 0; u < 32; u += 4)
-                            __stcg(pp + (c + u) / 4 * f.part_rows + r_own, make_float4(v[u], v[u + 1], v[u + 2], v[u + 3]));
+                        __stcg(reinterpret_cast<float4 *>(pp + (int64_t)ro * HD + ch), y);
                     }
                 }
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+            }
+            if (set == 0 && r_own < it.rows && whole_ok) {
                 if (fin) {
-                    if (mine && a.lse)
-                        a.lse[(int64_t)h * a.c.n_tokens + it.q.q0 + tok] = m == -INFINITY ? -INFINITY : __fadd_rn(m, __fsub_rn(log2f(l), kBias));
+                    if (a.lse) a.lse[(int64_t)h * a.c.n_tokens + it.q.q0 + tok] = M == -INFINITY ? -INFINITY : __fadd_rn(M, __fsub_rn(log2f(lt), kBias));
                 } else if (room) {
-                    __stcg(reinterpret_cast<float2 *>(pp + HD / 4 * f.part_rows) + r_own, make_float2(m, l));
-                } else if (tid == 0) {
+                    __stcg(reinterpret_cast<float2 *>(pp + (int64_t)HD * f.part_rows) + r_own, make_float2(M, lt));
+                } else if (r_own == 0) {  // the lengths are above their bounds
                     set_status(a.c.status, ALTXS_ST_BAD_POS);
                 }
-                if (odd && mine)
-                    for (int c = 0; c < HD; ++c) {
-                        const float y = odd_term<T>(a, it.s, it.g, pos, it.lo + it.t0 * KT, it.lo + it.t1 * KT, c);
-                        if (y == 0.0f) continue;
-                        if (fin) yp[c] = from_f<T>(y);
-                        else if (room) __stcg(reinterpret_cast<float *>(pp + c / 4 * f.part_rows + r_own) + c % 4, y);
-                    }
             }
             if (nt > 0) ++live;
             if (it.nsplit > 1) {  // the same barriers on every path
@@ -1074,7 +1145,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                 asm volatile("bar.sync 1, 256;" ::: "memory");
                 if (tid == 0) {
                     last_sh = 0;
-                    if (it.slot + it.nsplit <= f.max_slots) {
+                    if (room) {
                         uint32_t *cnt = f.cnt + it.slot;
                         last_sh = atomicAdd(cnt, 1u) == (uint32_t)it.nsplit - 1;
                         if (last_sh) *cnt = 0;
@@ -1082,47 +1153,36 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                     __threadfence();
                 }
                 asm volatile("bar.sync 1, 256;" ::: "memory");
-                if (last_sh && tid < it.rows) {  // thread = row of the block
+                if (last_sh) {  // join the splits in order: a warp per row
                     const int64_t ps = (int64_t)f.part_rows * (HD + 2);
                     const float *p = f.part + it.slot * ps;
-                    const int rr = it.r0 + tid, tk = rr / f.G, hh = it.g * f.G + rr - tk * f.G;
-                    float M = -INFINITY, lt = 0.0f;
-                    for (int t = 0; t < it.nsplit; ++t)
-                        M = fmaxf(M, __ldcg(reinterpret_cast<const float2 *>(p + t * ps + (int64_t)HD * f.part_rows) + tid).x);
-                    float w[kMostSplits];
-#pragma unroll
-                    for (int t = 0; t < kMostSplits; ++t) {
-                        w[t] = 0.0f;
-                        if (t < it.nsplit) {
-                            const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p + t * ps + (int64_t)HD * f.part_rows) + tid);
-                            w[t] = M == -INFINITY ? 0.0f : ex2(__fsub_rn(ml.x, M));
-                            lt = __fmaf_rn(ml.y, w[t], lt);
-                        }
-                    }
-                    const float inv = M == -INFINITY ? 0.0f : __frcp_rn(lt);
-                    T *yp = static_cast<T *>(a.out) + (int64_t)(it.q.q0 + tk) * a.ldo + (int64_t)hh * HD;
-                    for (int c = 0; c < HD; c += 16) {
-                        float y[16] = {};
+                    for (int ro = warp; ro < it.rows; ro += 8) {
+                        const float2 v = lane < it.nsplit ? __ldcg(reinterpret_cast<const float2 *>(p + lane * ps + (int64_t)HD * f.part_rows) + ro)
+                                                          : make_float2(-INFINITY, 0.0f);
+                        const float Mr = warp_max(v.x), w = v.x == -INFINITY ? 0.0f : ex2(__fsub_rn(v.x, Mr));
+                        float ls = 0.0f, y[HD / 32] = {};
 #pragma unroll
                         for (int t = 0; t < kMostSplits; ++t)
                             if (t < it.nsplit) {
-                                const float4 *pt = reinterpret_cast<const float4 *>(p + t * ps) + (int64_t)(c / 4) * f.part_rows + tid;
+                                const float wt = __shfl_sync(kAll, w, t);
+                                ls = __fmaf_rn(__shfl_sync(kAll, v.y, t), wt, ls);
+                                const Vec<float, HD / 32> u = ldcg_vec<HD / 32>(p + t * ps + (int64_t)ro * HD + lane * (HD / 32));
 #pragma unroll
-                                for (int u = 0; u < 4; ++u) {
-                                    const float4 v = __ldcg(pt + u * f.part_rows);
-                                    y[4 * u] = __fmaf_rn(v.x, w[t], y[4 * u]), y[4 * u + 1] = __fmaf_rn(v.y, w[t], y[4 * u + 1]);
-                                    y[4 * u + 2] = __fmaf_rn(v.z, w[t], y[4 * u + 2]), y[4 * u + 3] = __fmaf_rn(v.w, w[t], y[4 * u + 3]);
-                                }
+                                for (int e = 0; e < HD / 32; ++e) y[e] = __fmaf_rn(u.e[e], wt, y[e]);
                             }
+                        const float inv = Mr == -INFINITY ? 0.0f : __frcp_rn(ls);
+                        const int rr = it.r0 + ro, tk = rr / f.G, hh = it.g * f.G + rr - tk * f.G;
+                        Vec<T, HD / 32> out;
 #pragma unroll
-                        for (int u = 0; u < 16; ++u) y[u] = __fmul_rn(y[u], inv);
-                        store8<T>(yp + c, y);
-                        store8<T>(yp + c + 8, y + 8);
+                        for (int e = 0; e < HD / 32; ++e) out.e[e] = from_f<T>(__fmul_rn(y[e], inv));
+                        *reinterpret_cast<Vec<T, HD / 32> *>(static_cast<T *>(a.out) + (int64_t)(it.q.q0 + tk) * a.ldo +
+                                                             (int64_t)hh * HD + lane * (HD / 32)) = out;
+                        if (a.lse && lane == 0)
+                            a.lse[(int64_t)hh * a.c.n_tokens + it.q.q0 + tk] = Mr == -INFINITY ? -INFINITY : __fadd_rn(Mr, __fsub_rn(log2f(ls), kBias));
                     }
-                    if (a.lse) a.lse[(int64_t)hh * a.c.n_tokens + it.q.q0 + tk] = M == -INFINITY ? -INFINITY : __fadd_rn(M, __fsub_rn(log2f(lt), kBias));
                 }
             }
-            // the next item's queries overwrite this one's, and its first products the outputs
+            // the next item's queries overwrite the staged outputs, and its first products O
             if (tid == 0) stop_sh = abort_sh;
             tc_fence_before();
             asm volatile("bar.sync 1, 256;" ::: "memory");
