@@ -58,7 +58,6 @@ constexpr int kMostItems = 1184;  // splits of one sequence
 constexpr int kMostSplits = 16;
 constexpr unsigned kAll = 0xffffffffu;
 constexpr float kLazy = 8.0f;
-constexpr int kPolyPairs = 1;  // of every four pairs of 16-bit probabilities, those whose exponentials run on the FMA pipe
 
 template <typename T, int HD>
 struct Tc {
@@ -76,9 +75,9 @@ struct Tc {
     static constexpr int RegS = F32 ? 176 : 208, RegP = F32 ? 80 : 88;
     static_assert(256 * RegS + (Threads - 256) * RegP == Threads * (F32 ? 128 : 168), "register split");
     static constexpr int Slots = F32 ? 3 : HD > 64 ? 5 : 11;
+    static constexpr int UnitRows = F32 ? 512 / HD : KT, Units = KT / UnitRows;  // fp32: rows that share an exponent
     static constexpr int StageB = F32 ? KT * HD * 4 : 0;  // fp32: a tile's raw rows, one stage for keys and one for values
     static constexpr int Ring = Slots > 8 ? 16 : 8;  // key tiles (and items) the producers are ahead of the softmax, at most
-    static constexpr int Lag = HD > 64 ? 3 : HD > 32 ? 6 : 8;  // tiles a producer has in flight behind the newest
     static constexpr int QB = Rows / 128 * QTileB;
     static constexpr int MlAt = QB > 32768 ? 32768 : QB + Slots * TileB;  // 256 (m, l): see the softmax warps
     static constexpr int Smem = QB + Slots * TileB + 2 * StageB + (QB > 32768 ? 0 : 2048) + 1024;
@@ -123,6 +122,7 @@ __host__ __device__ inline void split_rule(Shape &w, int nt) {
 struct ManyArgs {
     PagedAttnArgs a;
     int G, min_rows;    // sequences with at least min_rows rows are this kernel's
+    int run;            // positions that lie within a page (16-bit types)
     int64_t max_slots;  // partial slots in the workspace (one per item of a split sequence)
     uint32_t *cnt;      // [max_slots], zero between calls
     float *part;        // [max_slots][part_rows * (HD + 2)]
@@ -153,7 +153,7 @@ struct Item {
     Seq q;
     int s, g, nsplit, split;
     int r0, rows;        // rows of the block
-    int lo, t0, t1, hi;  // positions lo + KT t of key tiles t0 .. t1 of this split; the block sees [lo, hi)
+    int lo, hi, base, t0, t1;  // the block sees [lo, hi); positions base + KT t of key tiles t0 .. t1 of this split
     bool two;            // two row tiles (both groups over every key tile)
     int slot;            // partial slot of the block's split 0
 };
@@ -200,7 +200,8 @@ __device__ __forceinline__ Item locate(const ManyArgs &f, const Scan &sc, int it
     const int p0 = it.q.L - it.q.n, i0 = it.r0 / f.G, i1 = (it.r0 + it.rows - 1) / f.G;
     it.hi = max(0, p0 + i1 + 1);
     it.lo = f.a.window > 0 ? max(0, p0 + i0 - f.a.window + 1) : 0;
-    const int nt = tiles_of(max(0, it.hi - it.lo), C::KT), per = (nt + it.nsplit - 1) / it.nsplit;
+    it.base = it.lo / C::KT * C::KT;  // tiles start at multiples of KT: no run of a page crosses a tile
+    const int nt = tiles_of(max(0, it.hi - it.base), C::KT), per = (nt + it.nsplit - 1) / it.nsplit;
     it.t0 = min(nt, it.split * per);
     it.t1 = min(nt, it.t0 + per);
     return it;
@@ -255,6 +256,13 @@ __device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
         : "r"(smem_u32(bar)), "r"(parity)
         : "memory");
     return ok != 0;
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int w, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+        : "memory");
 }
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
@@ -375,23 +383,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
         : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
 }
-// 2^x for x <= 127 without the special function unit: x = n + f with n the nearest
-// integer (by adding 1.5 2^23, whose sum's low bits are n), 2^f on [-1/2, 1/2] by
-// the polynomial of degree 4 with the least largest relative error (2.6e-6;
-// Remez's exchange), n added to the exponent.  Below -126 it gives 2^-126.
-__device__ __forceinline__ float2 ex2_poly(float2 x) {
-    constexpr float kMagic = 12582912.0f;
-    x.x = fmaxf(x.x, -126.0f), x.y = fmaxf(x.y, -126.0f);
-    const float2 r = add2(x, make_float2(kMagic, kMagic)), n = add2(r, make_float2(-kMagic, -kMagic));
-    const float2 f = fma2(n, make_float2(-1.0f, -1.0f), x);
-    float2 p = fma2(f, make_float2(0.009570102207362652f, 0.009570102207362652f), make_float2(0.05591785907745361f, 0.05591785907745361f));
-    p = fma2(p, f, make_float2(0.240247443318367f, 0.240247443318367f));
-    p = fma2(p, f, make_float2(0.6931217908859253f, 0.6931217908859253f));
-    p = fma2(p, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
-    return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(r.x) << 23)),
-                       __int_as_float(__float_as_int(p.y) + (__float_as_int(r.y) << 23)));
-}
-
 // The values of channel `dim` that are not finite, over the positions [lo, hi) that a
 // row at `pos` sees (the tiles that only some rows see hold 0 in their place).
 template <typename T>
@@ -409,19 +400,20 @@ __device__ __noinline__ float odd_term(const PagedAttnArgs &a, int s, int g, int
 }
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __grid_constant__ ManyArgs f) {
+__global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __grid_constant__ ManyArgs f, const __grid_constant__ CUtensorMap tk,
+                                                                        const __grid_constant__ CUtensorMap tv) {
     using C = Tc<T, HD>;
     constexpr int KT = C::KT;
     constexpr bool F32 = C::F32;
     extern __shared__ unsigned char pm_smem_raw[];
-    __shared__ __align__(8) uint64_t full[C::Slots], empty[C::Slots], s_full[2], p_full[2], o_done[2], q_full, drainb;
+    __shared__ __align__(8) uint64_t full[C::Slots], empty[C::Slots], landed[F32 ? 1 : C::Slots], s_full[2], p_full[2], o_done[2], q_full, drainb;
     __shared__ Scan sc;
-    // by key tile: which positions exist (4 to a byte), and (fp32) the exponents of its keys and of the values so far
+    // by key tile: which positions exist (4 to a byte), and (fp32) the exponents of its units of keys and of values
     __shared__ __align__(16) uint8_t kmask[C::Ring][KT / 4];
-    __shared__ int kv_exp[F32 ? C::Ring : 1][2];
-    __shared__ uint32_t wmax[F32 ? 2 : 1][8];  // (fp32) the producers' maxima, bit 31: a wait gave up
+    __shared__ __align__(16) int8_t kv_exp[F32 ? C::Ring : 1][2][16];
     __shared__ uint32_t tmem_sh;
-    __shared__ uint8_t odd_sh[C::Ring][8];
+    __shared__ __align__(8) uint8_t odd8_sh[F32 ? C::Ring : 1][8];  // by item: values that are not finite were set to 0 (fp32: per warp)
+    __shared__ uint32_t odd_sh[F32 ? 1 : C::Ring];
     __shared__ int2 wsum[kScan / 32];
     __shared__ int last_sh, stop_sh;
     __shared__ volatile int abort_sh;
@@ -432,8 +424,9 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
     const uint32_t limit = wait_limit();
     if (tid == 0) {
         for (int s = 0; s < C::Slots; ++s) {
-            mbar_init(&full[s], C::Producers);
+            mbar_init(&full[s], F32 ? C::Producers : 1);
             mbar_init(&empty[s], 1);
+            if (!F32) mbar_init(&landed[s], 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
@@ -443,6 +436,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
         mbar_init(&q_full, 8);
         mbar_init(&drainb, 1);
         abort_sh = 0;
+        for (int i = 0; i < (F32 ? 1 : C::Ring); ++i) odd_sh[i] = 0;
         fence_mbar_init();
     }
     if (warp == kMmaWarp) {
@@ -485,162 +479,185 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
         auto block_of = [&](int k) { return pshift >= 0 ? k >> pshift : k / P; };
         uint32_t n = 0, kt = 0, live = 0;  // slots, key tiles and items with tiles so far
         bool ok = true;
-        if constexpr (!F32) {
-        constexpr int NC = HD / 8, KPI = 32 / NC;  // 16-byte pieces of a row, rows per warp copy
-        // Warp pw copies the 8-row groups pw, pw + 3, .. of every tile: at most 6 of 16.
-        constexpr int kGroups = (KT / 8 + C::Producers - 1) / C::Producers;
-        uint32_t done = 0;                 // slots published
-        // a published slot needs its values checked when only some rows see them
-        uint32_t check = 0;                // bit (slot n & 31): check before publishing
-        uint32_t odd_of = 0;
-        auto publish = [&](uint32_t m) {   // slot number m has landed (this warp's share)
-            const uint32_t base = ring + (m % C::Slots) * C::TileB;
-            if ((check >> (m & 31)) & 1) {
-                bool odd = false;
-                for (int i = 0; i < kGroups; ++i) {
-                    const int grp = pw + i * C::Producers;
-                    if (grp >= KT / 8) break;
-#pragma unroll
-                    for (int e = 0; e < 8 / KPI; ++e) {
-                        const int r = grp * 8 + e * KPI + lane / NC, c = lane % NC;
-                        const uint32_t d = base + (c >> 3) * (KT * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-                        uint4 v = lds16(d);
-                        uint32_t *w = reinterpret_cast<uint32_t *>(&v);
-                        bool bad = false;
-                        constexpr uint32_t X = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-#pragma unroll
-                        for (int u = 0; u < 4; ++u) {
-                            if ((w[u] & X) == X) w[u] &= 0xffff0000u, bad = true;
-                            if (((w[u] >> 16) & X) == X) w[u] &= 0xffffu, bad = true;
-                        }
-                        if (bad) sts16(d, v), odd = true;
-                    }
+        // The tile whose copies come next: found (and its page numbers on their way) one tile ahead.
+        int item = (int)blockIdx.x - (int)gridDim.x, t = 0;
+        Item it;
+        it.t1 = 0;
+        bool fresh = false, more = true;
+        auto advance = [&]() {  // to the next tile
+            ++t;
+            fresh = false;
+            while (t >= it.t1) {
+                item += gridDim.x;
+                if (item >= total) {
+                    more = false;
+                    return;
                 }
-                check &= ~(1u << (m & 31));
-                if (__any_sync(kAll, odd) && lane == 0) odd_sh[odd_of % C::Ring][pw] = 1;
+                it = locate<C>(f, sc, item);
+                t = it.t0;
+                fresh = true;
             }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&full[m % C::Slots]);
         };
-        for (int item = blockIdx.x; item < total && ok; item += gridDim.x) {
-            const Item it = locate<C>(f, sc, item);
-            if (it.t0 == it.t1) continue;
-            const int p0 = it.q.L - it.q.n, i0 = it.r0 / f.G, i1 = (it.r0 + it.rows - 1) / f.G;
-            const int32_t *table = a.c.page_table + it.s * a.c.table_stride;
-            const char *kbase = static_cast<const char *>(a.kv.k) + (int64_t)it.g * a.kv.head_stride * 2;
-            const char *vbase = static_cast<const char *>(a.kv.v) + (int64_t)it.g * a.kv.head_stride * 2;
-            // the slots still on their way belong to the previous item: publish them under its flag
-            if (check != 0) {
-                asm volatile("cp.async.wait_group 0;" ::: "memory");
-                while (done < n) publish(done++);
-            }
-            odd_of = live++;
-            if (lane == 0) odd_sh[odd_of % C::Ring][pw] = 0;
-            for (int t = it.t0; t < it.t1 && ok; ++t) {
-                const int kb = it.lo + t * KT;
-                // offsets of this warp's rows: lane 8 i' + r holds row r of its i'-th group (two rounds)
-                int64_t off[2];
-                uint32_t seen[2];
+        // Positions [all0, all1) are seen by every row of the block.
+        int all0 = 0, all1 = 0;
+        auto bounds = [&]() {
+            const int p0 = it.q.L - it.q.n;
+            all1 = p0 + it.r0 / f.G + 1;
+            all0 = a.window > 0 ? p0 + (it.r0 + it.rows - 1) / f.G - a.window + 1 : 0;
+        };
+        if constexpr (!F32) {
+            // Runs of `run` positions (the largest power of two up to KT that divides the page size) lie within a
+            // page: one tensor copy per run and 64-channel half.  Runs of no page or outside [lo, hi) take a
+            // page number past the pool, which fills zeros.
+            const int run = f.run, runs = KT / run, mine = runs < 32 ? runs : 32;
+            // A values tile whose rows are not all seen by every row of the block goes to landed[] first, and
+            // warp 10 clears what must not meet a p = 0: rows outside [lo, hi), and values that are not finite
+            // in rows that only some see (the latter reach those in the epilogue).
+            auto mixed = [&]() {
+                const int kb = it.base + t * KT;
+                return kb < max(all0, it.lo) || kb + KT > min(all1, it.hi);
+            };
+            uint32_t lph = 0;  // landed[]'s parities, by slot
+            if (pw == 0) {
+                int page[KT / 32];
+                auto fetch = [&]() {
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int grp = pw + (4 * e + lane / 8) * C::Producers, k = kb + grp * 8 + lane % 8;
-                    const bool want = grp < KT / 8 && k < it.hi;
-                    const int b = want ? block_of(k) : 0, page = want ? __ldg(table + b) : -1;
-                    const bool in = page >= 0 && page < a.kv.n_pages;
-                    if (want && !in) set_status(a.c.status, ALTXS_ST_BAD_POS);
-                    off[e] = in ? ((int64_t)page * a.kv.page_stride + (int64_t)(k - b * P) * a.kv.token_stride) * 2 : -1;
-                    seen[e] = __ballot_sync(kAll, in);
-                }
-                if (lane < kGroups) {  // which rows exist, for the softmax
-                    const int grp = pw + lane * C::Producers;
-                    const uint32_t sb = seen[lane / 4] >> (8 * (lane % 4));
-                    if (grp < KT / 8)
-                        *reinterpret_cast<uint16_t *>(&kmask[kt % C::Ring][2 * grp]) =
-                            (uint16_t)(((sb >> 4) & 15) << 8 | (sb & 15));
-                }
-                ++kt;
-                // every row of the block sees the whole tile?
-                const bool whole = kb + KT <= p0 + i0 + 1 && (a.window == 0 || kb > p0 + i1 - a.window);
-#pragma unroll
-                for (int kv = 0; kv < 2; ++kv, ++n) {
-                    const uint32_t s = n % C::Slots;
-                    if (n >= C::Slots) {
-                        // let what has landed go out before blocking on a slot that waits for it
-                        if (!__all_sync(kAll, mbar_test(&empty[s], ((n / C::Slots) - 1) & 1))) {
-                            asm volatile("cp.async.wait_group 0;" ::: "memory");
-                            while (done < n) publish(done++);
-                            ok = __all_sync(kAll, !abort_sh && mbar_wait_bounded(&empty[s], ((n / C::Slots) - 1) & 1, limit));
-                            if (!ok) break;
-                        }
+                    for (int e = 0; e < KT / 32; ++e) {
+                        const int u = e * 32 + lane, k = it.base + t * KT + u * run;
+                        page[e] = more && u < runs && k < it.hi && k + run > it.lo
+                                      ? __ldg(a.c.page_table + it.s * a.c.table_stride + block_of(k)) : INT32_MIN;
+                        if (e * 32 + 32 >= runs) break;
                     }
-                    const char *src0 = kv ? vbase : kbase;
-                    const uint32_t dst = ring + s * C::TileB;
+                };
+                bool have = false, look = false;
+                uint32_t was_look = 0;  // slots whose last copy went to landed[]
+                int kb = 0, g = 0, pos_in[KT / 32], pg[KT / 32];
+                while (ok) {
+                    advance();
+                    fetch();
+                    if (have) {
+#pragma unroll 1
+                        for (int kv = 0; kv < 2; ++kv, ++n) {
+                            const uint32_t s = n % C::Slots;
+                            if (n >= C::Slots)
+                                ok = __all_sync(kAll, !abort_sh && mbar_wait_bounded(&empty[s], ((n / C::Slots) - 1) & 1, limit));
+                            if (!ok) break;
+                            uint64_t *bar = kv && look ? &landed[s] : &full[s];
+                            if (kv && look) lph ^= 1u << s;
+                            was_look = (was_look & ~(1u << s)) | (kv && look ? 1u << s : 0u);
+                            if (lane == 0) mbar_expect_tx(bar, C::TileB);
+                            __syncwarp();
+                            const CUtensorMap *map = kv ? &tv : &tk;
 #pragma unroll
-                    for (int i = 0; i < kGroups; ++i) {
-                        const int grp = pw + i * C::Producers;
-                        if (grp < KT / 8) {
+                            for (int e = 0; e < KT / 32; ++e) {
+                                if (e * 32 >= runs) break;
+                                if (lane < mine) {
+                                    const uint32_t d = ring + s * C::TileB + (e * 32 + lane) * run * 128;
 #pragma unroll
-                            for (int e = 0; e < 8 / KPI; ++e) {
-                                const int r8 = e * KPI + lane / NC, r = grp * 8 + r8, c = lane % NC;
-                                const int64_t o = __shfl_sync(kAll, off[i / 4], (i % 4) * 8 + r8);
-                                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                                                 dst + (c >> 3) * (KT * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)),
-                                             "l"(src0 + (o < 0 ? 0 : o) + c * 16), "r"(o < 0 ? 0u : 16u)
-                                             : "memory");
+                                    for (int h = 0; h < C::Halves; ++h)
+                                        tma_load_4d(d + h * (KT * 128), map, 64 * h, pos_in[e], g, pg[e], bar);
+                                }
                             }
                         }
                     }
-                    asm volatile("cp.async.commit_group;" ::: "memory");
-                    if (kv && !whole && i1 > i0) check |= 1u << (n & 31);
-                    if (n - done >= C::Lag) {
-                        asm volatile("cp.async.wait_group %0;" ::"n"(C::Lag) : "memory");
-                        publish(done++);
+                    have = more;
+                    if (!more || !ok) break;
+                    if (fresh) bounds();
+                    kb = it.base + t * KT, g = it.g;
+                    look = mixed();
+#pragma unroll
+                    for (int e = 0; e < KT / 32; ++e) {
+                        if (e * 32 >= runs) break;
+                        const int k = kb + (e * 32 + lane) * run;
+                        const bool in = page[e] >= 0 && page[e] < a.kv.n_pages;
+                        if (!in && page[e] != INT32_MIN) set_status(a.c.status, ALTXS_ST_BAD_POS);
+                        pos_in[e] = k - block_of(k) * P;
+                        pg[e] = in ? page[e] : max(a.kv.n_pages, 1);
+                        // which positions exist, for the softmax (what is outside [lo, hi) no row sees)
+                        const uint32_t seen = __ballot_sync(kAll, in);
+                        if (run >= 4) {
+                            if (lane < mine)
+                                for (int i = 0; i < run / 4; ++i) kmask[kt % C::Ring][(e * 32 + lane) * (run / 4) + i] = in ? 15 : 0;
+                        } else if (lane % 4 == 0) {
+                            kmask[kt % C::Ring][e * 8 + lane / 4] = (uint8_t)((seen >> lane) & 15);
+                        }
                     }
+                    __syncwarp();
+                    ++kt;
+                }
+                // every copy has landed before the block can exit
+                for (uint32_t i = n > C::Slots ? n - C::Slots : 0; i < n; ++i) {
+                    const uint32_t s = i % C::Slots;
+                    if ((was_look >> s) & 1) mbar_wait_bounded(&landed[s], ((lph >> s) & 1) ^ 1, kWaitLimit);
+                    else mbar_wait_bounded(&full[s], (i / C::Slots) & 1, kWaitLimit);
+                }
+            } else if (pw == 1) {
+                uint32_t me = 0;
+                while (ok) {
+                    advance();
+                    if (!more) break;
+                    if (fresh) {
+                        bounds();
+                        me = live++ % C::Ring;  // the softmax clears it when the item is done
+                    }
+                    const uint32_t s = (n + 1) % C::Slots;
+                    n += 2;
+                    if (!mixed()) continue;
+                    ok = __all_sync(kAll, !abort_sh && mbar_wait_bounded(&landed[s], (lph >> s) & 1, limit));
+                    if (!ok) break;
+                    lph ^= 1u << s;
+                    const int kb = it.base + t * KT;
+                    bool odd = false;
+                    constexpr int NC = HD / 8;
+                    for (int i = lane; i < KT * NC; i += 32) {
+                        const int r = i / NC, c = i % NC, k = kb + r;
+                        if (k >= max(all0, it.lo) && k < min(all1, it.hi)) continue;
+                        const uint32_t d = ring + s * C::TileB + (c >> 3) * (KT * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                        uint4 v = make_uint4(0, 0, 0, 0);
+                        if (k >= it.lo && k < it.hi) {
+                            v = lds16(d);
+                            uint32_t *w = reinterpret_cast<uint32_t *>(&v);
+                            bool bad = false;
+                            constexpr uint32_t X = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) {
+                                if ((w[u] & X) == X) w[u] &= 0xffff0000u, bad = true;
+                                if (((w[u] >> 16) & X) == X) w[u] &= 0xffffu, bad = true;
+                            }
+                            odd = odd || bad;
+                            if (!bad) continue;
+                        }
+                        sts16(d, v);
+                    }
+                    if (__any_sync(kAll, odd) && lane == 0) odd_sh[me] = 1;
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&full[s]);
                 }
             }
-        }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        while (done < n) publish(done++);
         } else {
-            // fp32: units of 2 KB, 16-byte pieces; warp pw takes units pw, pw + 7, ..  Per tile: copy
-            // the unit rows to the raw stage one tile ahead (each lane its own pieces, so its own
-            // copies are all it waits for), agree on the tile's largest magnitude, write the planes.
-            constexpr int CR = HD / 4, UR = 128 / CR, Units = KT / UR, UW = (Units + C::Producers - 1) / C::Producers;
+            // fp32: units of 2 KB (UR rows), 16-byte pieces; warp pw takes units pw, pw + 7, ..  Per unit: copy
+            // the rows to the raw stage one tile ahead (each lane its own pieces, so its own copies are all it
+            // waits for), find the unit's largest magnitude, write the scaled planes.
+            constexpr int CR = HD / 4, UR = C::UnitRows, Units = C::Units, UW = (Units + C::Producers - 1) / C::Producers;
             static_assert(UW * UR <= 32, "one page look-up per lane");
             const uint32_t raw = ring + C::Slots * C::TileB;
-            int item = (int)blockIdx.x - (int)gridDim.x, t = 0, ve = -100;
-            Item it;
-            it.t1 = 0;
-            // the tile being copied: its row offsets, and for its conversion later
+            const int un0 = pw + lane / UR * C::Producers;  // lane: row lane % UR of this unit
+            const bool mine = lane < UW * UR && un0 < Units;
             int64_t off = -1;
             uint32_t seen = 0;
-            bool whole = true, fresh = false, more = true;
-            auto advance = [&]() {  // to the next tile
-                ++t;
-                fresh = false;
-                while (t >= it.t1) {
-                    item += gridDim.x;
-                    if (item >= total) {
-                        more = false;
-                        return;
-                    }
-                    it = locate<C>(f, sc, item);
-                    t = it.t0;
-                    fresh = true;
-                }
-                const int kb = it.lo + t * KT, p0 = it.q.L - it.q.n, i0 = it.r0 / f.G, i1 = (it.r0 + it.rows - 1) / f.G;
-                // lane: row lane % UR of this warp's unit lane / UR
-                const int un = pw + lane / UR * C::Producers, k = kb + un * UR + lane % UR;
-                const bool want = lane < UW * UR && un < Units && k < it.hi;
-                const int b = want ? block_of(k) : 0;
-                const int page = want ? __ldg(a.c.page_table + it.s * a.c.table_stride + b) : -1;
+            int page = INT32_MIN;
+            auto fetch = [&]() {
+                const int k = it.base + t * KT + un0 * UR + lane % UR;
+                page = more && mine && k >= it.lo && k < it.hi ? __ldg(a.c.page_table + it.s * a.c.table_stride + block_of(k)) : INT32_MIN;
+            };
+            auto resolve = [&]() {
+                const int k = it.base + t * KT + un0 * UR + lane % UR;
                 const bool in = page >= 0 && page < a.kv.n_pages;
-                if (want && !in) set_status(a.c.status, ALTXS_ST_BAD_POS);
-                off = in ? ((int64_t)page * a.kv.page_stride + (int64_t)(k - b * P) * a.kv.token_stride +
+                if (!in && page != INT32_MIN) set_status(a.c.status, ALTXS_ST_BAD_POS);
+                off = in ? ((int64_t)page * a.kv.page_stride + (int64_t)(k - block_of(k) * P) * a.kv.token_stride +
                             (int64_t)it.g * a.kv.head_stride) * 4 : -1;
                 seen = __ballot_sync(kAll, in);
-                whole = (kb + KT <= p0 + i0 + 1 && (a.window == 0 || kb > p0 + i1 - a.window)) || i1 == i0;
             };
             auto copy = [&](int kv) {
                 if (more) {
@@ -661,100 +678,88 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                 }
                 asm volatile("cp.async.commit_group;" ::: "memory");
             };
-            advance();
-            copy(0);
-            copy(1);
-            while (more && ok) {
-                if (fresh) {
-                    ve = -100;  // exponent of the item's values so far
-                    if (lane == 0) odd_sh[live % C::Ring][pw] = 0;
-                    ++live;
-                }
-                const uint32_t me = (live - 1) % C::Ring;
-                const bool check = !whole;
-                {
-                    const int un = pw + lane / UR * C::Producers;
-                    if (lane % 4 == 0 && lane < UW * UR && un < Units)
-                        kmask[kt % C::Ring][(un * UR + lane % UR) / 4] = (uint8_t)((seen >> lane) & 15);
+            bool have = false, look = false;  // a tile is being copied, some of whose values not every row sees
+            uint32_t me = 0;
+            while (ok) {
+                if (have) {
+                    if (fresh) {
+                        bounds();
+                        me = live++ % C::Ring;
+                        if (lane == 0) odd8_sh[me][pw] = 0;
+                    }
+                    const int kb = it.base + t * KT;
+                    look = kb < all0 || kb + KT > all1;
+                    if (lane % 4 == 0 && mine) kmask[kt % C::Ring][(un0 * UR + lane % UR) / 4] = (uint8_t)((seen >> lane) & 15);
                 }
                 advance();
+                fetch();
+                if (!have) {
+                    resolve();
+                    copy(0);
+                    copy(1);
+                    have = more;
+                    if (!more) break;
+                    continue;
+                }
 #pragma unroll
                 for (int kv = 0; kv < 2; ++kv, ++n) {
-                    asm volatile("cp.async.wait_group 1;" ::: "memory");
-                    const uint32_t stage = raw + kv * C::StageB + lane * 16;
-                    float mf = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < UW; ++i) {
-                        if (pw + i * C::Producers >= Units) break;
-                        float4 x[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) x[e] = lds_f4(stage + (pw + i * C::Producers) * 2048 + e * 512);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            mf = fmaxf(mf, fmaxf(fmaxf(fabsf(x[e].x), fabsf(x[e].y)), fmaxf(fabsf(x[e].z), fabsf(x[e].w))));
-                    }
-                    if ((kv && check) || __any_sync(kAll, mf == INFINITY)) {  // the largest finite magnitude; odd values
-                        bool odd = false;
-                        uint32_t mx = 0;
-                        for (int i = 0; i < UW * 4; ++i) {
-                            const int un = pw + i / 4 * C::Producers;
-                            if (un >= Units) break;
-                            const uint32_t at = stage + un * 2048 + i % 4 * 512;
-                            float4 x = lds_f4(at);
-                            float *w = reinterpret_cast<float *>(&x);
-                            bool bad = false;
-#pragma unroll
-                            for (int u = 0; u < 4; ++u) {
-                                mx = max(mx, finite_abs(w[u]));
-                                if (kv && check && !isfinite(w[u])) w[u] = 0.0f, bad = true;
-                            }
-                            if (bad) sts16(at, make_uint4(__float_as_uint(x.x), __float_as_uint(x.y), __float_as_uint(x.z), __float_as_uint(x.w))), odd = true;
-                        }
-                        mf = __uint_as_float(mx);
-                        if (__any_sync(kAll, odd) && lane == 0) odd_sh[me][pw] = 1;
-                    }
                     const uint32_t s = n % C::Slots;
                     if (n >= C::Slots)
                         ok = __all_sync(kAll, !abort_sh && mbar_wait_bounded(&empty[s], ((n / C::Slots) - 1) & 1, limit));
-                    const uint32_t wm = __reduce_max_sync(kAll, __float_as_uint(mf));
-                    if (lane == 0) wmax[n & 1][pw] = wm | (ok ? 0u : 0x80000000u);
-                    asm volatile("bar.sync 2, %0;" ::"n"(C::Producers * 32) : "memory");
-                    uint32_t mx = 0;
+                    if (!ok) break;
+                    asm volatile("cp.async.wait_group 1;" ::: "memory");
+                    const uint32_t stage = raw + kv * C::StageB + lane * 16, dst = ring + s * C::TileB;
+                    float4 x[UW][4];
 #pragma unroll
-                    for (int w = 0; w < C::Producers; ++w) {
-                        const uint32_t o = wmax[n & 1][w];
-                        ok = ok && !(o >> 31);
-                        mx = max(mx, o & 0x7fffffffu);
-                    }
-                    if (!ok) break;  // every producer warp sees the same words
-                    int ex = exp_of(mx);
-                    if (kv) ex = ve = max(ve, ex);
-                    if (pw == 0 && lane == 0) kv_exp[kt % C::Ring][kv] = ex;
-                    const float scale = pow2(14 - ex);
-                    const uint32_t dst = ring + s * C::TileB;
+                    for (int i = 0; i < UW; ++i)
+                        if (pw + i * C::Producers < Units)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) x[i][e] = lds_f4(stage + (pw + i * C::Producers) * 2048 + e * 512);
+                    if (kv == 0) resolve();
+                    copy(kv);  // the next tile's, into the stage just read
 #pragma unroll
                     for (int i = 0; i < UW; ++i) {
-                        if (pw + i * C::Producers >= Units) break;
-                        float4 x[4];
+                        const int un = pw + i * C::Producers;
+                        if (un >= Units) break;
+                        float mf = 0.0f;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) x[e] = lds_f4(stage + (pw + i * C::Producers) * 2048 + e * 512);
+                        for (int e = 0; e < 4; ++e)
+                            mf = fmaxf(mf, fmaxf(fmaxf(fabsf(x[i][e].x), fabsf(x[i][e].y)), fmaxf(fabsf(x[i][e].z), fabsf(x[i][e].w))));
+                        if ((kv && look) || __any_sync(kAll, mf == INFINITY)) {  // the largest finite magnitude; odd values
+                            bool odd = false;
+                            uint32_t mx = 0;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                float *w = reinterpret_cast<float *>(&x[i][e]);
+#pragma unroll
+                                for (int u = 0; u < 4; ++u) {
+                                    mx = max(mx, finite_abs(w[u]));
+                                    if (kv && look && !isfinite(w[u])) w[u] = 0.0f, odd = true;
+                                }
+                            }
+                            mf = __uint_as_float(mx);
+                            if (__any_sync(kAll, odd) && lane == 0) odd8_sh[me][pw] = 1;
+                        }
+                        const int ex = exp_of(__reduce_max_sync(kAll, __float_as_uint(mf)));
+                        if (lane == 0) kv_exp[kt % C::Ring][kv][un] = (int8_t)ex;
+                        const float scale = pow2(14 - ex);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const int q = e * 32 + lane, r = (pw + i * C::Producers) * UR + q / CR, c4 = q % CR, c = c4 >> 1;
+                            const int q = e * 32 + lane, r = un * UR + q / CR, c4 = q % CR, c = c4 >> 1;
                             uint2 hi, lo;
-                            split2(x[e].x * scale, x[e].y * scale, hi.x, lo.x);
-                            split2(x[e].z * scale, x[e].w * scale, hi.y, lo.y);
+                            split2(x[i][e].x * scale, x[i][e].y * scale, hi.x, lo.x);
+                            split2(x[i][e].z * scale, x[i][e].w * scale, hi.y, lo.y);
                             const uint32_t d = dst + (c >> 3) * (KT * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4) + (c4 & 1) * 8;
                             sts8(d, hi);
                             sts8(d + C::PlaneB, lo);
                         }
                     }
-                    copy(kv);  // the next tile's, into the stage just read
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&full[s]);
                 }
                 ++kt;
+                if (!more) break;
             }
             asm volatile("cp.async.wait_group 0;" ::: "memory");
         }
@@ -890,7 +895,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
             const int r_own = it.two ? grp * 128 + row : row & (rrows - 1), part = it.two ? 0 : row / rrows;
             const int r = it.r0 + min(r_own, it.rows - 1), tok = r / f.G, h = it.g * f.G + r - tok * f.G;
             const int pos = p0 + tok;
-            float m = -INFINITY, l = 0.0f, cf = c2;  // cf: score to log2 units (fp32: times the tile's and the row's scales)
+            float m = -INFINITY, l = 0.0f;
             int qe = 0, ve = -100;                   // fp32: exponents of the row's query and of O's values
             uint32_t njob = 0;                       // jobs of this group in this item
             if (nt > 0) {
@@ -937,7 +942,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                 auto tile = [&](auto rep_c, int j) -> bool {
                     constexpr int REP = decltype(rep_c)::value, W = KT / REP;  // columns of this thread's share
                     const int c0 = REP > 1 ? part * W : 0;
-                    const int kb = it.lo + (it.t0 + j) * KT + c0;
+                    const int kb = it.base + (it.t0 + j) * KT + c0;
                     if (!__all_sync(kAll, !abort_sh && mbar_wait_bounded(&s_full[grp], job & 1, limit))) return false;
                     tc_fence_after();
                     float x[W];
@@ -957,30 +962,66 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                     if (!whole) {
                         const int first = a.window > 0 ? max(0, pos - a.window + 1 - kb) : 0, last = pos - kb;
 #pragma unroll
-                        for (int u = 0; u < W; ++u) {
-                            const uint32_t bit = 1u << (8 * (u / 4 % 4) + u % 4);
-                            if (u < first || u > last || !(km[u / 16] & bit)) x[u] = -INFINITY;
+                        for (int c = 0; c < W; c += 32) {  // bit u: column c + u is seen
+                            uint32_t bits = 0;
+#pragma unroll
+                            for (int d = 0; d < 2; ++d) {
+                                const uint32_t k = km[c / 16 + d];
+                                bits |= ((k & 15) | (k >> 4 & 0xf0) | (k >> 8 & 0xf00) | (k >> 12 & 0xf000)) << (16 * d);
+                            }
+                            const int f0 = first - c, l0 = last - c;  // of [0, 31]
+                            bits &= f0 >= 32 ? 0u : f0 <= 0 ? kAll : kAll << f0;
+                            bits &= l0 < 0 ? 0u : l0 >= 31 ? kAll : kAll >> (31 - l0);
+#pragma unroll
+                            for (int u = 0; u < 32; ++u)
+                                if (!(bits & (1u << u))) x[c + u] = -INFINITY;
                         }
                     }
-                    float mx = -INFINITY, mx1 = -INFINITY;
-#pragma unroll
-                    for (int u = 0; u < W; u += 4) {
-                        mx = fmaxf(mx, fmaxf(x[u], x[u + 1]));
-                        mx1 = fmaxf(mx1, fmaxf(x[u + 2], x[u + 3]));
-                    }
-                    mx = fmaxf(mx, mx1);
-                    int vt = 0;  // fp32: exponent of this tile's values
+                    // columns that share a scale, and their factors to log2 units (fp32: times the row's and the unit's)
+                    constexpr int UC = F32 ? C::UnitRows : W, NU = W / UC;
+                    float cf[NU], pf[NU];
+                    int vt = -100;  // fp32: exponent of this tile's values
                     if constexpr (F32) {
-                        const int ke = kv_exp[(kt + j) % C::Ring][0];
-                        cf = fmaxf(__fmul_rn(__fmul_rn(c2, pow2(qe - 14)), pow2(ke - 14)), 1.17549435e-38f);
-                        const uint32_t v = 2 * (kt + j) + 1;  // the values' slot: their exponent comes with them
+                        const float cq = __fmul_rn(c2, pow2(qe - 14));
+                        const int8_t *ke = kv_exp[(kt + j) % C::Ring][0] + c0 / UC, *vx = kv_exp[(kt + j) % C::Ring][1] + c0 / UC;
+#pragma unroll
+                        for (int i = 0; i < NU; ++i) cf[i] = fmaxf(__fmul_rn(cq, pow2(ke[i] - 14)), 1.17549435e-38f);
+                        const uint32_t v = 2 * (kt + j) + 1;  // the values' slot: their exponents come with them
                         if (!__all_sync(kAll, mbar_wait_bounded(&full[v % C::Slots], (v / C::Slots) & 1, limit))) return false;
-                        vt = kv_exp[(kt + j) % C::Ring][1];
+#pragma unroll
+                        for (int i = 0; i < NU; ++i) vt = max(vt, (int)vx[i]);
+                        vt = njob == 0 ? vt : max(ve, vt);
+#pragma unroll
+                        for (int i = 0; i < NU; ++i) pf[i] = pow2(max(vx[i] - vt, -126));
                         if (njob == 0) ve = vt;
+                    } else {
+                        cf[0] = c2;
                     }
-                    mx = mx == -INFINITY ? mx : __fmul_rn(mx, cf);
+                    float mx = -INFINITY;
+                    if constexpr (F32) {
+                        float mu[NU];
+#pragma unroll
+                        for (int i = 0; i < NU; ++i) {
+                            mu[i] = x[i * UC];
+#pragma unroll
+                            for (int u = 1; u < UC; ++u) mu[i] = fmaxf(mu[i], x[i * UC + u]);
+                            mu[i] = mu[i] == -INFINITY ? mu[i] : __fmul_rn(mu[i], cf[i]);
+                        }
+#pragma unroll
+                        for (int i = 0; i < NU; ++i) mx = fmaxf(mx, mu[i]);
+                    } else {
+                        float mu[8];  // short chains: few warps are there to hide their latency
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            mu[i] = x[i];
+#pragma unroll
+                            for (int u = i + 8; u < W; u += 8) mu[i] = fmaxf(mu[i], x[u]);
+                        }
+                        mx = fmaxf(fmaxf(fmaxf(mu[0], mu[1]), fmaxf(mu[2], mu[3])), fmaxf(fmaxf(mu[4], mu[5]), fmaxf(mu[6], mu[7])));
+                        mx = mx == -INFINITY ? mx : __fmul_rn(mx, c2);
+                    }
                     const bool grow = mx > __fadd_rn(m, kLazy) || (m == -INFINITY && mx > m);
-                    if (__any_sync(kAll, grow) || (F32 && vt != ve)) {
+                    if (__any_sync(kAll, grow || (F32 && vt != ve))) {
                         const float mn = grow ? mx : m;
                         float fold = m == -INFINITY ? 0.0f : grow ? ex2(__fsub_rn(m, mn)) : 1.0f;
                         l = __fmul_rn(l, fold);
@@ -1003,19 +1044,18 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                         }
                     }
                     const float base = m == -INFINITY ? 0.0f : __fsub_rn(m, kBias);
-                    const float2 cf2 = make_float2(cf, cf), nb2 = make_float2(-base, -base);
+                    const float2 nb2 = make_float2(-base, -base);
                     float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
                     for (int c = 0; c < W; c += 32) {
                         uint32_t w[16], wl[F32 ? 16 : 1];
 #pragma unroll
                         for (int u = 0; u < 32; u += 2) {
-                            const float2 t = fma2(make_float2(x[c + u], x[c + u + 1]), cf2, nb2);
-                            // the special function unit is the bottleneck of the 16-bit types: a part of the
-                            // exponentials runs on the FMA pipe
-                            const float2 e = !F32 && u % 8 >= 8 - 2 * kPolyPairs ? ex2_poly(t) : make_float2(ex2(t.x), ex2(t.y));
+                            const int un = (c + u) / UC;
+                            const float2 t = fma2(make_float2(x[c + u], x[c + u + 1]), make_float2(cf[un], cf[un]), nb2);
+                            float2 e = make_float2(ex2(t.x), ex2(t.y));
                             sum[u / 2 & 1] = add2(sum[u / 2 & 1], e);
-                            if constexpr (F32) split2(e.x, e.y, w[u / 2], wl[u / 2]);
+                            if constexpr (F32) split2(e.x * pf[un], e.y * pf[un], w[u / 2], wl[u / 2]);
                             else w[u / 2] = pack2<T>(e.x, e.y);
                         }
                         tc_st16(ts + (c0 + c) / 2, w);
@@ -1076,9 +1116,14 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
             if (fin) wgt = __fmul_rn(wgt, M == -INFINITY ? 0.0f : __frcp_rn(lt));
             if constexpr (F32) wgt = __fmul_rn(__fmul_rn(wgt, pow2(ve)), pow2(-14));
             bool odd = false;
-            if (nt > 0)
+            if (nt > 0) {
+                if constexpr (F32) {
 #pragma unroll
-                for (int e = 0; e < C::Producers; ++e) odd = odd || odd_sh[live % C::Ring][e] != 0;
+                    for (int e = 0; e < C::Producers; ++e) odd = odd || odd8_sh[live % C::Ring][e] != 0;
+                } else {
+                    odd = odd_sh[live % C::Ring] != 0;
+                }
+            }
             const bool whole_ok = !abort_sh;
             float *pp = f.part + (int64_t)(it.slot + it.split) * f.part_rows * (HD + 2);
 #pragma unroll 1
@@ -1102,8 +1147,11 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                 for (int i = 0; i < 8; ++i)  // 128-byte rows, swizzled like the tiles
                     *reinterpret_cast<float4 *>(stage + slot * 32 + ((i ^ (slot & 7)) << 2)) =
                         make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-                asm volatile("bar.sync 1, 256;" ::: "memory");
-                for (int i = tid; i < min(rrows, it.rows) * 8; i += 256) {  // row i / 8, channels c + 4 (i % 8) ..
+                // Rows of one set are the warp's own; shared ones meet in the block.
+                if (it.two) __syncwarp();
+                else asm volatile("bar.sync 1, 256;" ::: "memory");
+                const int i1 = it.two ? min(it.rows, (warp + 1) * 32) * 8 : min(rrows, it.rows) * 8;
+                for (int i = it.two ? warp * 256 + lane : tid; i < i1; i += it.two ? 32 : 256) {  // row i / 8, channels c + 4 (i % 8) ..
                     const int ro = i >> 3, q = i & 7;
                     float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     for (int s = 0; s < sets; ++s) {
@@ -1115,7 +1163,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                     if (odd) {  // what is not finite replaces the sum that it was kept out of
                         float *w = reinterpret_cast<float *>(&y);
                         for (int e = 0; e < 4; ++e) {
-                            const float t = odd_term<T>(a, it.s, it.g, p0 + tk, it.lo + it.t0 * KT, it.lo + it.t1 * KT, ch + e);
+                            const float t = odd_term<T>(a, it.s, it.g, p0 + tk, max(it.lo, it.base + it.t0 * KT), it.base + it.t1 * KT, ch + e);
                             if (t != 0.0f) w[e] = t;
                         }
                     }
@@ -1128,7 +1176,8 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                         __stcg(reinterpret_cast<float4 *>(pp + (int64_t)ro * HD + ch), y);
                     }
                 }
-                asm volatile("bar.sync 1, 256;" ::: "memory");
+                if (it.two) __syncwarp();
+                else asm volatile("bar.sync 1, 256;" ::: "memory");
             }
             if (set == 0 && r_own < it.rows && whole_ok) {
                 if (fin) {
@@ -1139,7 +1188,6 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                     set_status(a.c.status, ALTXS_ST_BAD_POS);
                 }
             }
-            if (nt > 0) ++live;
             if (it.nsplit > 1) {  // the same barriers on every path
                 __threadfence();
                 asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -1188,6 +1236,10 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
             asm volatile("bar.sync 1, 256;" ::: "memory");
             tc_fence_after();
             if (stop_sh) break;
+            if (nt > 0) {
+                if (!F32 && tid == 0) odd_sh[live % C::Ring] = 0;
+                ++live;
+            }
         }
         if (abort_sh && tid == 0) set_status(a.c.status, ALTXS_ST_TIMEOUT);
     }
@@ -1199,8 +1251,23 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
     }
 }
 
+// [pages][heads][positions][channels] of a pool as it lies, boxes of `run` positions x 64 channels
+bool pool_map(CUtensorMap *m, const altxs_paged_kv &kv, void *pool, int run) {
+    const auto enc = encoder();
+    if (!enc) return false;
+    const cuuint64_t dims[4] = {(cuuint64_t)kv.head_dim, (cuuint64_t)kv.page_size, (cuuint64_t)kv.n_kv_heads,
+                                (cuuint64_t)std::max(kv.n_pages, 1)};
+    const cuuint64_t strides[3] = {(cuuint64_t)kv.token_stride * 2, (cuuint64_t)kv.head_stride * 2, (cuuint64_t)kv.page_stride * 2};
+    const cuuint32_t box[4] = {64, (cuuint32_t)run, 1, 1}, es[4] = {1, 1, 1, 1};
+    return enc(m, kv.dtype == ALTXS_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, pool, dims, strides,
+               box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int HD>
 int launch(const ManyArgs &f, unsigned grid, cudaStream_t st) {
+    CUtensorMap tk{}, tv{};
+    if (sizeof(T) == 2 && (!pool_map(&tk, f.a.kv, f.a.kv.k, f.run) || !pool_map(&tv, f.a.kv, f.a.kv.v, f.run))) return ALTXS_ECUDA;
     static std::atomic<uint64_t> set{0};  // devices whose shared-memory limit is raised
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return ALTXS_ECUDA;
@@ -1209,7 +1276,7 @@ int launch(const ManyArgs &f, unsigned grid, cudaStream_t st) {
             return ALTXS_ECUDA;
         if (dev < 64) set.fetch_or(1ull << dev);
     }
-    ALTXS_LAUNCH(kKPaged, st, k_paged_many<T, HD><<<grid, Tc<T, HD>::Threads, Tc<T, HD>::Smem, st>>>(f));
+    ALTXS_LAUNCH(kKPaged, st, k_paged_many<T, HD><<<grid, Tc<T, HD>::Threads, Tc<T, HD>::Smem, st>>>(f, tk, tv));
     return ALTXS_OK;
 }
 template <typename T>
@@ -1236,7 +1303,8 @@ ManyPlan paged_many_plan(const altxs_paged_kv &kv, const altxs_chunks &c, int H,
 
 int launch_paged_many(const PagedAttnArgs &a, const ManyPlan &p, int min_rows, uint32_t *cnt, float *part, int sms,
                       cudaStream_t st) {
-    const ManyArgs f{a, a.H / a.kv.n_kv_heads, min_rows, p.slots, cnt, part, p.rows};
+    const int run = std::min(128, a.kv.page_size & -a.kv.page_size);
+    const ManyArgs f{a, a.H / a.kv.n_kv_heads, min_rows, run < 4 ? 1 : run, p.slots, cnt, part, p.rows};
     const unsigned grid = (unsigned)std::min<int64_t>(p.items, sms);
     if (a.kv.dtype == ALTXS_F32) return launch<float>(f, grid, st);
     return a.kv.dtype == ALTXS_BF16 ? launch<__nv_bfloat16>(f, grid, st) : launch<__half>(f, grid, st);
