@@ -354,20 +354,6 @@ __device__ __forceinline__ uint32_t finite_abs(float x) {
     return b < 0x7f800000u ? b : 0u;
 }
 
-template <int N>
-__device__ __forceinline__ Vec<float, N> ldcg_vec(const float *p) {
-    Vec<float, N> v;
-    if constexpr (N == 4) {
-        const float4 x = __ldcg(reinterpret_cast<const float4 *>(p));
-        v.e[0] = x.x, v.e[1] = x.y, v.e[2] = x.z, v.e[3] = x.w;
-    } else if constexpr (N == 2) {
-        const float2 x = __ldcg(reinterpret_cast<const float2 *>(p));
-        v.e[0] = x.x, v.e[1] = x.y;
-    } else {
-        v.e[0] = __ldcg(p);
-    }
-    return v;
-}
 // two fp32 operations per instruction
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     float2 d;
@@ -518,7 +504,10 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                 return kb < max(all0, it.lo) || kb + KT > min(all1, it.hi);
             };
             uint32_t lph = 0;  // landed[]'s parities, by slot
-            if (pw == 0) {
+            if (pw != 1) {  // warp 9 fetches the keys, warp 11 the values: a warp issues one copy in about 100 clocks
+                const int kv = pw >> 1;
+                const CUtensorMap *map = kv ? &tv : &tk;
+                n = kv;
                 int page[KT / 32];
                 auto fetch = [&]() {
 #pragma unroll
@@ -536,35 +525,32 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                     advance();
                     fetch();
                     if (have) {
-#pragma unroll 1
-                        for (int kv = 0; kv < 2; ++kv, ++n) {
-                            const uint32_t s = n % C::Slots;
-                            if (n >= C::Slots)
-                                ok = __all_sync(kAll, !abort_sh && mbar_wait_bounded(&empty[s], ((n / C::Slots) - 1) & 1, limit));
-                            if (!ok) break;
-                            uint64_t *bar = kv && look ? &landed[s] : &full[s];
-                            if (kv && look) lph ^= 1u << s;
-                            was_look = (was_look & ~(1u << s)) | (kv && look ? 1u << s : 0u);
-                            if (lane == 0) mbar_expect_tx(bar, C::TileB);
-                            __syncwarp();
-                            const CUtensorMap *map = kv ? &tv : &tk;
+                        const uint32_t s = n % C::Slots;
+                        if (n >= C::Slots)
+                            ok = __all_sync(kAll, !abort_sh && mbar_wait_bounded(&empty[s], ((n / C::Slots) - 1) & 1, limit));
+                        if (!ok) break;
+                        uint64_t *bar = look ? &landed[s] : &full[s];
+                        if (look) lph ^= 1u << s;
+                        was_look = (was_look & ~(1u << s)) | (look ? 1u << s : 0u);
+                        if (lane == 0) mbar_expect_tx(bar, C::TileB);
+                        __syncwarp();
 #pragma unroll
-                            for (int e = 0; e < KT / 32; ++e) {
-                                if (e * 32 >= runs) break;
-                                if (lane < mine) {
-                                    const uint32_t d = ring + s * C::TileB + (e * 32 + lane) * run * 128;
+                        for (int e = 0; e < KT / 32; ++e) {
+                            if (e * 32 >= runs) break;
+                            if (lane < mine) {
+                                const uint32_t d = ring + s * C::TileB + (e * 32 + lane) * run * 128;
 #pragma unroll
-                                    for (int h = 0; h < C::Halves; ++h)
-                                        tma_load_4d(d + h * (KT * 128), map, 64 * h, pos_in[e], g, pg[e], bar);
-                                }
+                                for (int h = 0; h < C::Halves; ++h)
+                                    tma_load_4d(d + h * (KT * 128), map, 64 * h, pos_in[e], g, pg[e], bar);
                             }
                         }
+                        n += 2;
                     }
                     have = more;
                     if (!more || !ok) break;
                     if (fresh) bounds();
                     kb = it.base + t * KT, g = it.g;
-                    look = mixed();
+                    look = kv && mixed();
 #pragma unroll
                     for (int e = 0; e < KT / 32; ++e) {
                         if (e * 32 >= runs) break;
@@ -575,6 +561,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                         pg[e] = in ? page[e] : max(a.kv.n_pages, 1);
                         // which positions exist, for the softmax (what is outside [lo, hi) no row sees)
                         const uint32_t seen = __ballot_sync(kAll, in);
+                        if (kv) continue;
                         if (run >= 4) {
                             if (lane < mine)
                                 for (int i = 0; i < run / 4; ++i) kmask[kt % C::Ring][(e * 32 + lane) * (run / 4) + i] = in ? 15 : 0;
@@ -586,7 +573,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                     ++kt;
                 }
                 // every copy has landed before the block can exit
-                for (uint32_t i = n > C::Slots ? n - C::Slots : 0; i < n; ++i) {
+                for (int32_t i = (int32_t)n - 2; i >= 0 && i + (int32_t)C::Slots >= (int32_t)n; i -= 2) {
                     const uint32_t s = i % C::Slots;
                     if ((was_look >> s) & 1) mbar_wait_bounded(&landed[s], ((lph >> s) & 1) ^ 1, kWaitLimit);
                     else mbar_wait_bounded(&full[s], (i / C::Slots) & 1, kWaitLimit);
@@ -1201,32 +1188,51 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                     __threadfence();
                 }
                 asm volatile("bar.sync 1, 256;" ::: "memory");
-                if (last_sh) {  // join the splits in order: a warp per row
+                if (last_sh) {  // join the splits in order: their weights by row, then four channels a thread
                     const int64_t ps = (int64_t)f.part_rows * (HD + 2);
                     const float *p = f.part + it.slot * ps;
-                    for (int ro = warp; ro < it.rows; ro += 8) {
-                        const float2 v = lane < it.nsplit ? __ldcg(reinterpret_cast<const float2 *>(p + lane * ps + (int64_t)HD * f.part_rows) + ro)
-                                                          : make_float2(-INFINITY, 0.0f);
-                        const float Mr = warp_max(v.x), w = v.x == -INFINITY ? 0.0f : ex2(__fsub_rn(v.x, Mr));
-                        float ls = 0.0f, y[HD / 32] = {};
-#pragma unroll
-                        for (int t = 0; t < kMostSplits; ++t)
-                            if (t < it.nsplit) {
-                                const float wt = __shfl_sync(kAll, w, t);
-                                ls = __fmaf_rn(__shfl_sync(kAll, v.y, t), wt, ls);
-                                const Vec<float, HD / 32> u = ldcg_vec<HD / 32>(p + t * ps + (int64_t)ro * HD + lane * (HD / 32));
-#pragma unroll
-                                for (int e = 0; e < HD / 32; ++e) y[e] = __fmaf_rn(u.e[e], wt, y[e]);
-                            }
+                    const int n4 = (it.nsplit + 3) & ~3;
+                    float *wt = stage;  // [n4][256]
+                    if (tid < it.rows) {
+                        const float *q = p + (int64_t)HD * f.part_rows + 2 * tid;
+                        float Mr = -INFINITY, ls = 0.0f;
+#pragma unroll 4
+                        for (int t = 0; t < it.nsplit; ++t) Mr = fmaxf(Mr, __ldcg(q + t * ps));
+#pragma unroll 4
+                        for (int t = 0; t < it.nsplit; ++t) {
+                            const float2 v = __ldcg(reinterpret_cast<const float2 *>(q + t * ps));
+                            const float w = v.x == -INFINITY ? 0.0f : ex2(__fsub_rn(v.x, Mr));
+                            ls = __fmaf_rn(v.y, w, ls);
+                            wt[t * 256 + tid] = w;
+                        }
                         const float inv = Mr == -INFINITY ? 0.0f : __frcp_rn(ls);
-                        const int rr = it.r0 + ro, tk = rr / f.G, hh = it.g * f.G + rr - tk * f.G;
-                        Vec<T, HD / 32> out;
+                        for (int t = 0; t < n4; ++t) wt[t * 256 + tid] = t < it.nsplit ? __fmul_rn(wt[t * 256 + tid], inv) : 0.0f;
+                        const int rr = it.r0 + tid, tk = rr / f.G;
+                        if (a.lse)
+                            a.lse[(int64_t)(it.g * f.G + rr - tk * f.G) * a.c.n_tokens + it.q.q0 + tk] =
+                                Mr == -INFINITY ? -INFINITY : __fadd_rn(Mr, __fsub_rn(log2f(ls), kBias));
+                    }
+                    asm volatile("bar.sync 1, 256;" ::: "memory");
+#pragma unroll 2
+                    for (int i = tid; i < it.rows * (HD / 4); i += 256) {
+                        const int ro = i / (HD / 4), c = i % (HD / 4) * 4;
+                        const float *q = p + (int64_t)ro * HD + c;
+                        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        for (int t = 0; t < n4; t += 4) {
+                            float4 u[4];
 #pragma unroll
-                        for (int e = 0; e < HD / 32; ++e) out.e[e] = from_f<T>(__fmul_rn(y[e], inv));
-                        *reinterpret_cast<Vec<T, HD / 32> *>(static_cast<T *>(a.out) + (int64_t)(it.q.q0 + tk) * a.ldo +
-                                                             (int64_t)hh * HD + lane * (HD / 32)) = out;
-                        if (a.lse && lane == 0)
-                            a.lse[(int64_t)hh * a.c.n_tokens + it.q.q0 + tk] = Mr == -INFINITY ? -INFINITY : __fadd_rn(Mr, __fsub_rn(log2f(ls), kBias));
+                            for (int d = 0; d < 4; ++d) u[d] = __ldcg(reinterpret_cast<const float4 *>(q + min(t + d, it.nsplit - 1) * ps));
+#pragma unroll
+                            for (int d = 0; d < 4; ++d) {
+                                const float w = wt[(t + d) * 256 + ro];
+                                y.x = __fmaf_rn(u[d].x, w, y.x), y.y = __fmaf_rn(u[d].y, w, y.y);
+                                y.z = __fmaf_rn(u[d].z, w, y.z), y.w = __fmaf_rn(u[d].w, w, y.w);
+                            }
+                        }
+                        const int rr = it.r0 + ro, tk = rr / f.G;
+                        T *yp = static_cast<T *>(a.out) + (int64_t)(it.q.q0 + tk) * a.ldo + (int64_t)(it.g * f.G + rr - tk * f.G) * HD + c;
+                        if constexpr (F32) *reinterpret_cast<float4 *>(yp) = y;
+                        else *reinterpret_cast<uint2 *>(yp) = make_uint2(pack2<T>(y.x, y.y), pack2<T>(y.z, y.w));
                     }
                 }
             }
