@@ -649,7 +649,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
             auto copy = [&](int kv) {
                 if (more) {
                     const char *src0 = static_cast<const char *>(kv ? a.kv.v : a.kv.k);
-#pragma unroll
+#pragma unroll 1
                     for (int i = 0; i < UW; ++i) {
                         const int un = pw + i * C::Producers;
                         if (un >= Units) break;
@@ -688,7 +688,8 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                     if (!more) break;
                     continue;
                 }
-#pragma unroll
+                // (Loops are left rolled: with everything unrolled the block's roles miss the instruction cache.)
+#pragma unroll 1
                 for (int kv = 0; kv < 2; ++kv, ++n) {
                     const uint32_t s = n % C::Slots;
                     if (n >= C::Slots)
@@ -696,28 +697,21 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                     if (!ok) break;
                     asm volatile("cp.async.wait_group 1;" ::: "memory");
                     const uint32_t stage = raw + kv * C::StageB + lane * 16, dst = ring + s * C::TileB;
-                    float4 x[UW][4];
+#pragma unroll 1
+                    for (int un = pw; un < Units; un += C::Producers) {
+                        float4 x[4];
 #pragma unroll
-                    for (int i = 0; i < UW; ++i)
-                        if (pw + i * C::Producers < Units)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) x[i][e] = lds_f4(stage + (pw + i * C::Producers) * 2048 + e * 512);
-                    if (kv == 0) resolve();
-                    copy(kv);  // the next tile's, into the stage just read
-#pragma unroll
-                    for (int i = 0; i < UW; ++i) {
-                        const int un = pw + i * C::Producers;
-                        if (un >= Units) break;
+                        for (int e = 0; e < 4; ++e) x[e] = lds_f4(stage + un * 2048 + e * 512);
                         float mf = 0.0f;
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            mf = fmaxf(mf, fmaxf(fmaxf(fabsf(x[i][e].x), fabsf(x[i][e].y)), fmaxf(fabsf(x[i][e].z), fabsf(x[i][e].w))));
+                            mf = fmaxf(mf, fmaxf(fmaxf(fabsf(x[e].x), fabsf(x[e].y)), fmaxf(fabsf(x[e].z), fabsf(x[e].w))));
                         if ((kv && look) || __any_sync(kAll, mf == INFINITY)) {  // the largest finite magnitude; odd values
                             bool odd = false;
                             uint32_t mx = 0;
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
-                                float *w = reinterpret_cast<float *>(&x[i][e]);
+                                float *w = reinterpret_cast<float *>(&x[e]);
 #pragma unroll
                                 for (int u = 0; u < 4; ++u) {
                                     mx = max(mx, finite_abs(w[u]));
@@ -734,13 +728,15 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                         for (int e = 0; e < 4; ++e) {
                             const int q = e * 32 + lane, r = un * UR + q / CR, c4 = q % CR, c = c4 >> 1;
                             uint2 hi, lo;
-                            split2(x[i][e].x * scale, x[i][e].y * scale, hi.x, lo.x);
-                            split2(x[i][e].z * scale, x[i][e].w * scale, hi.y, lo.y);
+                            split2(x[e].x * scale, x[e].y * scale, hi.x, lo.x);
+                            split2(x[e].z * scale, x[e].w * scale, hi.y, lo.y);
                             const uint32_t d = dst + (c >> 3) * (KT * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4) + (c4 & 1) * 8;
                             sts8(d, hi);
                             sts8(d + C::PlaneB, lo);
                         }
                     }
+                    if (kv == 0) resolve();
+                    copy(kv);  // the next tile's, into the stage just read
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&full[s]);
