@@ -33,46 +33,57 @@ constexpr int kWarps = 4;
 constexpr int kSlots = 3;
 constexpr int kChunkBytes = 8192;  // keys and values of one chunk
 constexpr int kMaxRows = 16;
-constexpr int kSplitCap = 64;    // splits of a sequence at most
-constexpr int kSplitUnit = 256;  // keys
+constexpr int kSplitUnit = 512;  // keys of a split at least
+constexpr int kSplitItems = 296;  // items of a sequence at most, about: two blocks on each of 148 SMs
 constexpr unsigned kAll = 0xffffffffu;
 
-__host__ __device__ inline int split_keys(int keys) {
-    const int u = kSplitUnit * kSplitCap;
-    return kSplitUnit * (keys > u ? (keys + u - 1) / u : 1);
+// Keys of a split of a sequence that shows `keys` of them to `width` (head, row group) pairs: a long one by
+// itself fills the card once.  (An item costs some microseconds besides its keys' time: 100000 keys x 8 heads
+// in 98 splits of 1024 took 286 us next to two like it, in 37 of 2752 XXX us.)
+__host__ __device__ inline int split_keys(int keys, int width) {
+    const int most = width < kSplitItems ? kSplitItems / width : 1;
+    const int each = (keys + most - 1) / most;
+    return each > kSplitUnit ? (each + 63) / 64 * 64 : kSplitUnit;
 }
-__host__ __device__ inline int split_count(int keys) {
-    const int k = split_keys(keys);
+__host__ __device__ inline int split_count(int keys, int width) {
+    const int k = split_keys(keys, width);
     return keys > k ? (keys + k - 1) / k : 1;
 }
 
 struct FewArgs {
     PagedAttnArgs a;
-    int G;
+    int G, min_rows, max_rows;  // sequences with rows in this range are the kernel's
+    int group;                  // rows of an item at most
     int64_t max_items;  // partial slots in the workspace
-    uint32_t *cnt;      // [n_seqs * Hkv], zero between calls
+    uint32_t *cnt;      // [n_seqs * Hkv * groups], zero between calls
+    int groups;         // row groups of a sequence at most
     float *part;        // [max_items][rows][HD + 2]
     int part_rows;
 };
 
-// Items of the sequences before each group of `per` sequences.
+// Items of the sequences before each run of `per` sequences.
 struct ItemScan {
     int before[kWarps * 32 + 1];
     int per;
 };
 
+// items of a split: a (key/value head, row group) each
+__device__ __forceinline__ int few_width(const FewArgs &f, const Seq &q) {
+    return f.a.kv.n_kv_heads * ((q.n * f.G + f.group - 1) / f.group);
+}
 __device__ __forceinline__ int few_splits(const FewArgs &f, const Seq &q) {
-    if (q.n <= 0 || q.n * f.G > kMaxRows) return 0;
-    return split_count(max(0, q.L - first_seen(q.n, q.L, f.a.window)));
+    if (q.n <= 0 || q.n * f.G < f.min_rows || q.n * f.G > f.max_rows) return 0;
+    return split_count(max(0, q.L - first_seen(q.n, q.L, f.a.window)), few_width(f, q));
 }
 
 __device__ __forceinline__ void scan_items(const FewArgs &f, ItemScan &sc) {
     const int n = f.a.c.n_seqs, per = (n + kWarps * 32 - 1) / (kWarps * 32);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int sum = 0;
-    for (int s = tid * per; s < min(n, (tid + 1) * per); ++s)
-        sum += few_splits(f, blockIdx.x == 0 ? load_seq_report(f.a.c, s) : load_seq(f.a.c, s));
-    sum *= f.a.kv.n_kv_heads;
+    for (int s = tid * per; s < min(n, (tid + 1) * per); ++s) {
+        const Seq q = blockIdx.x == 0 ? load_seq_report(f.a.c, s) : load_seq(f.a.c, s);
+        sum += few_splits(f, q) * few_width(f, q);
+    }
     int inc = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -86,6 +97,31 @@ __device__ __forceinline__ void scan_items(const FewArgs &f, ItemScan &sc) {
     sc.before[tid + 1] = inc;
     if (tid == 0) sc.before[0] = 0, sc.per = per;
     __syncthreads();
+}
+
+// item -> sequence, split, head (heads fastest: they share the rows' DRAM pages), row group
+struct Where {
+    Seq q;
+    int s, split, g, grp, width;  // width: items from one split to the next
+};
+__device__ __forceinline__ Where locate(const FewArgs &f, const ItemScan &sc, int item) {
+    int lo = 0, hi = kWarps * 32;
+    while (hi - lo > 1) {
+        const int m = (lo + hi) >> 1;
+        if (sc.before[m] <= item) lo = m; else hi = m;
+    }
+    Where w;
+    w.s = lo * sc.per;
+    int local = item - sc.before[lo];
+    w.q = load_seq(f.a.c, w.s);
+    for (int n; w.s < f.a.c.n_seqs - 1 && local >= (n = few_splits(f, w.q) * few_width(f, w.q)); w.q = load_seq(f.a.c, ++w.s))
+        local -= n;
+    w.width = few_width(f, w.q);
+    w.split = local / w.width;
+    const int x = local - w.split * w.width;
+    w.grp = x / f.a.kv.n_kv_heads;
+    w.g = x - w.grp * f.a.kv.n_kv_heads;
+    return w;
 }
 
 __device__ __forceinline__ uint32_t f2u(float x) { return __float_as_uint(x); }
@@ -114,6 +150,11 @@ __device__ __forceinline__ void lds128(uint32_t addr, uint32_t *r) {
     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 
+__device__ __forceinline__ float4 ldg_stream(const float *p) {  // read once
+    float4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
+    return v;
+}
 template <typename T>
 __device__ __forceinline__ void mma16(float *d, const uint32_t *a, uint32_t b0, uint32_t b1) {
     if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value)
@@ -122,17 +163,6 @@ __device__ __forceinline__ void mma16(float *d, const uint32_t *a, uint32_t b0, 
     else
         asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma_tf32(float *d, const uint32_t *a, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// x = hi + lo + O(2^-22 x), both read by the tensor cores to 11 significant bits:
-// hi is x rounded half up there, lo the exact rest rounded by the same addition.
-// (An infinity becomes NaN: inf - inf.)
-__device__ __forceinline__ void split_tf32(uint32_t x, uint32_t &hi, uint32_t &lo) {
-    hi = (x + 0x1000u) & 0xffffe000u;
-    lo = f2u(__fsub_rn(__uint_as_float(x), __uint_as_float(hi))) + 0x1000u;
 }
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -151,14 +181,125 @@ struct Few {
     static constexpr int CK = kChunkBytes / (2 * RB);         // positions of a chunk
     static constexpr int NC = RB / 16;                        // 16-byte pieces of a row
     static constexpr int NK = CK / 8, NO = HD / 8;            // score and output column tiles
-    static constexpr bool F32 = ES == 4;
-    static constexpr int QS = F32 ? HD / 8 : HD / 16;         // k steps of Q K^T
     // piece c of position k in shared memory: conflict-free for the reads below
     static __device__ __forceinline__ uint32_t at(int k, int c) {
-        const int sw = F32 ? (k & 6) ^ ((k & 1) << 2) : NC >= 8 ? k & 7 : (k >> 1) & 3;
+        const int sw = NC >= 8 ? k & 7 : (k >> 1) & 3;
         return k * RB + ((c ^ sw) << 4);
     }
 };
+
+// The keys that only some of a sequence's rows see: positions of [k0, k1) outside [all0, all1).
+struct OddKeys {
+    int k0, k1, all0, all1;
+};
+
+// The end of an item: `sets` partial rows (m, l in ml, o in rows, [set][stride][HD], shared memory) are joined
+// in order; a sequence of one split is finished, else the rows go to the workspace and the block that brings
+// the last split joins them.  odd: values that are not finite were kept out of o; they are added to the rows
+// that see them.
+template <typename T, int HD>
+__device__ __forceinline__ void finish_item(const FewArgs &f, int item, const Where &w0, int nsplit, int R, int sets, int stride,
+                                            float *rows, const float *ml, int *last_sh, const OddKeys *odd) {
+    const PagedAttnArgs &a = f.a;
+    const Seq &q = w0.q;
+    const int G = f.G, s = w0.s, g = w0.g, r0 = w0.grp * f.group;  // row r of the item is row r0 + r of the sequence
+    for (int i = threadIdx.x; i < R * (HD / 4); i += kWarps * 32) {
+        const int r = i / (HD / 4), c = (i % (HD / 4)) * 4;
+        float M = -INFINITY, lt = 0.0f, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int w = 0; w < sets; ++w) M = fmaxf(M, ml[2 * (w * stride + r)]);
+#pragma unroll 4
+        for (int w = 0; w < sets; ++w) {
+            const float2 v = *reinterpret_cast<const float2 *>(ml + 2 * (w * stride + r));
+            const float sc2 = M == -INFINITY ? 0.0f : ex2(__fsub_rn(v.x, M));
+            const float4 x = *reinterpret_cast<const float4 *>(rows + (w * stride + r) * HD + c);
+            lt = __fmaf_rn(v.y, sc2, lt);
+            y[0] = __fmaf_rn(x.x, sc2, y[0]), y[1] = __fmaf_rn(x.y, sc2, y[1]);
+            y[2] = __fmaf_rn(x.z, sc2, y[2]), y[3] = __fmaf_rn(x.w, sc2, y[3]);
+        }
+        if (odd) {
+            const int pos = q.L - q.n + (r0 + r) / G;
+            for (int k = odd->k0; k < odd->k1; ++k) {
+                if (k >= odd->all0 && k < odd->all1) continue;
+                if (k > pos || (a.window > 0 && k <= pos - a.window)) continue;
+                const int b = k / a.kv.page_size, page = __ldg(a.c.page_table + s * a.c.table_stride + b);
+                if (page < 0 || page >= a.kv.n_pages) continue;
+                const T *v = static_cast<const T *>(a.kv.v) + (int64_t)page * a.kv.page_stride +
+                             (int64_t)(k - b * a.kv.page_size) * a.kv.token_stride + (int64_t)g * a.kv.head_stride + c;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (!isfinite(to_f(v[e]))) y[e] = __fadd_rn(y[e], to_f(v[e]));
+            }
+        }
+        if (nsplit == 1) {
+            const int tok = q.q0 + (r0 + r) / G, h = g * G + (r0 + r) % G;
+            const float inv = M == -INFINITY ? 0.0f : __frcp_rn(lt);
+            Vec<T, 4> out;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) out.e[e] = from_f<T>(__fmul_rn(y[e], inv));
+            *reinterpret_cast<Vec<T, 4> *>(static_cast<T *>(a.out) + (int64_t)tok * a.ldo + (int64_t)h * HD + c) = out;
+            if (a.lse && c == 0)
+                a.lse[(int64_t)h * a.c.n_tokens + tok] = M == -INFINITY ? -INFINITY : __fadd_rn(M, log2f(lt));
+        } else if (item < f.max_items) {
+            float *p = f.part + ((int64_t)item * f.part_rows + r) * (HD + 4);
+            __stcg(reinterpret_cast<float4 *>(p + c), make_float4(y[0], y[1], y[2], y[3]));
+            if (c == 0) __stcg(reinterpret_cast<float2 *>(p + HD), make_float2(M, lt));
+        } else if (i == 0) {  // the lengths' sum is above its bound
+            set_status(a.c.status, ALTXS_ST_BAD_POS);
+        }
+    }
+    if (nsplit == 1) return;
+    __syncthreads();
+    const int64_t first = item - (int64_t)w0.split * w0.width;  // the rows' split 0
+    if (threadIdx.x == 0) {
+        __threadfence();  // the block's rows are ordered before its arrival
+        uint32_t *cnt = f.cnt + ((int64_t)s * a.kv.n_kv_heads + g) * f.groups + w0.grp;
+        const bool last = atomicAdd(cnt, 1u) == (uint32_t)nsplit - 1;
+        if (last) *cnt = 0;
+        __threadfence();
+        *last_sh = last;
+    }
+    __syncthreads();
+    if (!*last_sh || first + (int64_t)(nsplit - 1) * w0.width >= f.max_items) return;
+    // all (m, l) first, then the rows' weights, in shared memory
+    float *ms = rows;                                                  // [nsplit][R], then [R] 1 / sum
+    float2 *in = reinterpret_cast<float2 *>(rows + ((nsplit + 1) * R + 1 & ~1));  // [nsplit][R]
+    const float *p0 = f.part + first * f.part_rows * (HD + 4);
+    const int64_t ps = (int64_t)w0.width * f.part_rows * (HD + 4);
+    for (int i = threadIdx.x; i < nsplit * R; i += kWarps * 32)
+        in[i] = __ldcg(reinterpret_cast<const float2 *>(p0 + i / R * ps + i % R * (HD + 4) + HD));
+    __syncthreads();
+    for (int r = threadIdx.x; r < R; r += kWarps * 32) {
+        float M = -INFINITY, lt = 0.0f;
+        for (int t = 0; t < nsplit; ++t) M = fmaxf(M, in[t * R + r].x);
+        for (int t = 0; t < nsplit; ++t) {
+            const float2 x = in[t * R + r];
+            const float w = M == -INFINITY ? 0.0f : ex2(__fsub_rn(x.x, M));
+            ms[t * R + r] = w;
+            lt = __fmaf_rn(x.y, w, lt);
+        }
+        ms[nsplit * R + r] = M == -INFINITY ? 0.0f : __frcp_rn(lt);
+        if (a.lse)
+            a.lse[(int64_t)(g * G + (r0 + r) % G) * a.c.n_tokens + q.q0 + (r0 + r) / G] =
+                M == -INFINITY ? -INFINITY : __fadd_rn(M, log2f(lt));
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < R * (HD / 4); i += kWarps * 32) {
+        const int r = i / (HD / 4), c = (i % (HD / 4)) * 4;
+        float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+        for (int t = 0; t < nsplit; ++t) {
+            const float4 x = __ldcg(reinterpret_cast<const float4 *>(p0 + t * ps + r * (HD + 4) + c));
+            const float w = ms[t * R + r];
+            y[0] = __fmaf_rn(x.x, w, y[0]), y[1] = __fmaf_rn(x.y, w, y[1]);
+            y[2] = __fmaf_rn(x.z, w, y[2]), y[3] = __fmaf_rn(x.w, w, y[3]);
+        }
+        const float inv = ms[nsplit * R + r];
+        Vec<T, 4> out;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out.e[e] = from_f<T>(__fmul_rn(y[e], inv));
+        *reinterpret_cast<Vec<T, 4> *>(static_cast<T *>(a.out) + (int64_t)(q.q0 + (r0 + r) / G) * a.ldo + (int64_t)(g * G + (r0 + r) % G) * HD + c) = out;
+    }
+}
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(kWarps * 32, 2) k_paged_few(const __grid_constant__ FewArgs f) {
@@ -179,18 +320,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_paged_few(const __grid_const
     const int total = sc.before[kWarps * 32];
 
     for (int item = blockIdx.x; item < total; item += gridDim.x) {
-        // item -> sequence, split, head (heads fastest: they share the rows' DRAM pages)
-        int lo = 0, hi = kWarps * 32;
-        while (hi - lo > 1) {
-            const int m = (lo + hi) >> 1;
-            if (sc.before[m] <= item) lo = m; else hi = m;
-        }
-        int s = lo * sc.per, local = item - sc.before[lo];
-        Seq q = load_seq(a.c, s);
-        for (int w; s < a.c.n_seqs - 1 && local >= (w = few_splits(f, q) * Hkv); q = load_seq(a.c, ++s)) local -= w;
-        const int g = local % Hkv, split = local / Hkv;
+        const Where at = locate(f, sc, item);
+        const Seq q = at.q;
+        const int s = at.s, g = at.g, split = at.split;
         const int R = q.n * G, kfirst = first_seen(q.n, q.L, a.window), keys = max(0, q.L - kfirst);
-        const int nsplit = split_count(keys), slen = split_keys(keys);
+        const int nsplit = split_count(keys, at.width), slen = split_keys(keys, at.width);
         const int k0 = kfirst + split * slen, k1 = min(q.L, k0 + slen);
         const int nchunk = k1 > k0 ? (k1 - k0 + CK - 1) / CK : 0;
         const int p0 = q.L - q.n;  // position of the first new token
@@ -247,29 +381,17 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_paged_few(const __grid_const
             fetch_pages(next);
         }
         // Q fragments: rows quad, quad + 8 (row r = token r / G, head r % G of the group)
-        uint32_t qa[F::QS][F::F32 ? 8 : 4];
+        uint32_t qa[HD / 16][4];
         int rpos[2];
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
             const int r = quad + 8 * hh, i = r / G, h = g * G + r - i * G;
             rpos[hh] = r < R ? p0 + i : -1;
             const T *qp = static_cast<const T *>(a.q) + (int64_t)(q.q0 + i) * a.ldq + (int64_t)h * HD;
-            if constexpr (F::F32) {
 #pragma unroll
-                for (int kk = 0; kk < HD / 16; ++kk) {  // channels 16 kk + 4 j ..: two k steps of (j, j + 4)
-                    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (r < R) x = *reinterpret_cast<const float4 *>(qp + 16 * kk + 4 * j);
-                    split_tf32(f2u(x.x), qa[2 * kk][hh], qa[2 * kk][4 + hh]);
-                    split_tf32(f2u(x.y), qa[2 * kk][2 + hh], qa[2 * kk][6 + hh]);
-                    split_tf32(f2u(x.z), qa[2 * kk + 1][hh], qa[2 * kk + 1][4 + hh]);
-                    split_tf32(f2u(x.w), qa[2 * kk + 1][2 + hh], qa[2 * kk + 1][6 + hh]);
-                }
-            } else {
-#pragma unroll
-                for (int kk = 0; kk < HD / 16; ++kk) {
-                    qa[kk][hh] = r < R ? *reinterpret_cast<const uint32_t *>(qp + 16 * kk + 2 * j) : 0u;
-                    qa[kk][2 + hh] = r < R ? *reinterpret_cast<const uint32_t *>(qp + 16 * kk + 8 + 2 * j) : 0u;
-                }
+            for (int kk = 0; kk < HD / 16; ++kk) {
+                qa[kk][hh] = r < R ? *reinterpret_cast<const uint32_t *>(qp + 16 * kk + 2 * j) : 0u;
+                qa[kk][2 + hh] = r < R ? *reinterpret_cast<const uint32_t *>(qp + 16 * kk + 8 + 2 * j) : 0u;
             }
         }
         float o[NO][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
@@ -291,33 +413,15 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_paged_few(const __grid_const
             float sacc[NK][4];
 #pragma unroll
             for (int t = 0; t < NK; ++t) sacc[t][0] = sacc[t][1] = sacc[t][2] = sacc[t][3] = 0.0f;
-            if constexpr (F::F32) {
 #pragma unroll
-                for (int t = 0; t < NK; ++t)
+            for (int t = 0; t < NK; t += 2)
 #pragma unroll
-                    for (int kk = 0; kk < HD / 16; ++kk) {
-                        uint32_t x[4], hi[4], lo[4];
-                        lds128(kt + F::at(8 * t + quad, 4 * kk + j), x);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) split_tf32(x[e], hi[e], lo[e]);
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            mma_tf32(sacc[t], qa[2 * kk + e] + 4, hi[2 * e], hi[2 * e + 1]);
-                            mma_tf32(sacc[t], qa[2 * kk + e], lo[2 * e], lo[2 * e + 1]);
-                            mma_tf32(sacc[t], qa[2 * kk + e], hi[2 * e], hi[2 * e + 1]);
-                        }
-                    }
-            } else {
-#pragma unroll
-                for (int t = 0; t < NK; t += 2)
-#pragma unroll
-                    for (int kk = 0; kk < HD / 16; ++kk) {
-                        uint32_t b[4];
-                        ldsm4<0>(kt + F::at(8 * t + (lane & 7) + ((lane >> 4) << 3), 2 * kk + ((lane >> 3) & 1)), b);
-                        mma16<T>(sacc[t], qa[kk], b[0], b[1]);
-                        mma16<T>(sacc[t + 1], qa[kk], b[2], b[3]);
-                    }
-            }
+                for (int kk = 0; kk < HD / 16; ++kk) {
+                    uint32_t b[4];
+                    ldsm4<0>(kt + F::at(8 * t + (lane & 7) + ((lane >> 4) << 3), 2 * kk + ((lane >> 3) & 1)), b);
+                    mma16<T>(sacc[t], qa[kk], b[0], b[1]);
+                    mma16<T>(sacc[t + 1], qa[kk], b[2], b[3]);
+                }
             // scale, mask, running maximum
             const int kc = k0 + ci * CK;
             const bool whole = kc >= all0 && kc + CK <= min(all1, k1) &&
@@ -337,6 +441,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_paged_few(const __grid_const
             float sum[2] = {0.0f, 0.0f};
 #pragma unroll
             for (int hh = 0; hh < 2; ++hh) {
+                if (hh == 1 && R <= 8) break;  // rows 8 .. are empty
                 mx[hh] = fmaxf(mx[hh], __shfl_xor_sync(kAll, mx[hh], 1));
                 mx[hh] = fmaxf(mx[hh], __shfl_xor_sync(kAll, mx[hh], 2));
                 const float base = mx[hh] == -INFINITY ? 0.0f : mx[hh];  // nothing seen yet: every p is 2^-inf = 0
@@ -354,6 +459,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_paged_few(const __grid_const
             for (int t = 0; t < NK; ++t)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
+                    if (e >= 2 && R <= 8) break;  // (their p is whatever the scores are: finite, and not stored)
                     sacc[t][e] = ex2(__fsub_rn(sacc[t][e], mx[e >> 1]));
                     sum[e >> 1] = __fadd_rn(sum[e >> 1], sacc[t][e]);
                 }
@@ -371,13 +477,9 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_paged_few(const __grid_const
                     bool bad = false;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        if constexpr (F::F32) {
-                            if ((w[e] & 0x7f800000u) == 0x7f800000u) w[e] = 0, bad = true;
-                        } else {
-                            constexpr uint32_t X = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-                            if ((w[e] & X) == X) w[e] &= 0xffff0000u, bad = true;
-                            if (((w[e] >> 16) & X) == X) w[e] &= 0xffffu, bad = true;
-                        }
+                        constexpr uint32_t X = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+                        if ((w[e] & X) == X) w[e] &= 0xffff0000u, bad = true;
+                        if (((w[e] >> 16) & X) == X) w[e] &= 0xffffu, bad = true;
                     }
                     if (bad) {
                         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(d), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
@@ -388,43 +490,16 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_paged_few(const __grid_const
                 __syncwarp();
             }
             // O += P V
-            if constexpr (F::F32) {
 #pragma unroll
-                for (int t = 0; t < NK; ++t) {
-                    // k index j is position 8 t + 2 j, j + 4 is 8 t + 2 j + 1 (how the scores lie)
-                    uint32_t ph[4], pl[4];
-                    split_tf32(f2u(sacc[t][0]), ph[0], pl[0]);
-                    split_tf32(f2u(sacc[t][2]), ph[1], pl[1]);
-                    split_tf32(f2u(sacc[t][1]), ph[2], pl[2]);
-                    split_tf32(f2u(sacc[t][3]), ph[3], pl[3]);
+            for (int t = 0; t < NK; t += 2) {
+                const uint32_t pa[4] = {pack2<T>(sacc[t][0], sacc[t][1]), pack2<T>(sacc[t][2], sacc[t][3]),
+                                        pack2<T>(sacc[t + 1][0], sacc[t + 1][1]), pack2<T>(sacc[t + 1][2], sacc[t + 1][3])};
 #pragma unroll
-                    for (int b = 0; b < HD / 32; ++b) {  // column quad of tile 4 b + e is channel 32 b + 4 quad + e
-                        uint32_t x[4], y[4];
-                        lds128(vt + F::at(8 * t + 2 * j, 8 * b + quad), x);
-                        lds128(vt + F::at(8 * t + 2 * j + 1, 8 * b + quad), y);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            uint32_t xh, xl, yh, yl;
-                            split_tf32(x[e], xh, xl);
-                            split_tf32(y[e], yh, yl);
-                            mma_tf32(o[4 * b + e], pl, xh, yh);
-                            mma_tf32(o[4 * b + e], ph, xl, yl);
-                            mma_tf32(o[4 * b + e], ph, xh, yh);
-                        }
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int t = 0; t < NK; t += 2) {
-                    const uint32_t pa[4] = {pack2<T>(sacc[t][0], sacc[t][1]), pack2<T>(sacc[t][2], sacc[t][3]),
-                                            pack2<T>(sacc[t + 1][0], sacc[t + 1][1]), pack2<T>(sacc[t + 1][2], sacc[t + 1][3])};
-#pragma unroll
-                    for (int n = 0; n < NO; n += 2) {
-                        uint32_t b[4];
-                        ldsm4<1>(vt + F::at(8 * t + (lane & 15), n + (lane >> 4)), b);
-                        mma16<T>(o[n], pa, b[0], b[1]);
-                        mma16<T>(o[n + 1], pa, b[2], b[3]);
-                    }
+                for (int n = 0; n < NO; n += 2) {
+                    uint32_t b[4];
+                    ldsm4<1>(vt + F::at(8 * t + (lane & 15), n + (lane >> 4)), b);
+                    mma16<T>(o[n], pa, b[0], b[1]);
+                    mma16<T>(o[n + 1], pa, b[2], b[3]);
                 }
             }
             slot = slot == kSlots - 1 ? 0 : slot + 1;
@@ -432,6 +507,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_paged_few(const __grid_const
         cp_wait<0>();
         __syncthreads();  // every warp is done with its slots: they take the warps' rows [warp][row][HD]
         float *rows = reinterpret_cast<float *>(few_smem);
+        const OddKeys odd{k0, k1, all0, all1};
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
             l[hh] = __fadd_rn(l[hh], __shfl_xor_sync(kAll, l[hh], 1));
@@ -440,117 +516,139 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_paged_few(const __grid_const
             if (r >= R) continue;
             if (j == 0) ml_sh[warp][r][0] = m[hh], ml_sh[warp][r][1] = l[hh];
             float *y = rows + (warp * kMaxRows + r) * HD;
-            if constexpr (F::F32) {
 #pragma unroll
-                for (int b = 0; b < HD / 32; ++b)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)  // channels 32 b + 8 j + 4 e ..
-                        *reinterpret_cast<float4 *>(y + 32 * b + 8 * j + 4 * e) =
-                            make_float4(o[4 * b][2 * hh + e], o[4 * b + 1][2 * hh + e], o[4 * b + 2][2 * hh + e], o[4 * b + 3][2 * hh + e]);
-            } else {
-#pragma unroll
-                for (int t = 0; t < NO; ++t)
-                    *reinterpret_cast<float2 *>(y + 8 * t + 2 * j) = make_float2(o[t][2 * hh], o[t][2 * hh + 1]);
-            }
+            for (int t = 0; t < NO; ++t)
+                *reinterpret_cast<float2 *>(y + 8 * t + 2 * j) = make_float2(o[t][2 * hh], o[t][2 * hh + 1]);
         }
         __syncthreads();
-        // join the four warps in order; one thread per (row, four channels)
-        const int64_t pbase = (int64_t)(item - split * Hkv - g) * f.part_rows;  // first split's rows; Hkv items a split
-        for (int i = threadIdx.x; i < R * (HD / 4); i += kWarps * 32) {
-            const int r = i / (HD / 4), c = (i % (HD / 4)) * 4;
-            float M = -INFINITY, lt = 0.0f, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) M = fmaxf(M, ml_sh[w][r][0]);
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float sc2 = M == -INFINITY ? 0.0f : ex2(__fsub_rn(ml_sh[w][r][0], M));
-                const float4 x = *reinterpret_cast<const float4 *>(rows + (w * kMaxRows + r) * HD + c);
-                lt = __fmaf_rn(ml_sh[w][r][1], sc2, lt);
-                y[0] = __fmaf_rn(x.x, sc2, y[0]), y[1] = __fmaf_rn(x.y, sc2, y[1]);
-                y[2] = __fmaf_rn(x.z, sc2, y[2]), y[3] = __fmaf_rn(x.w, sc2, y[3]);
-            }
-            if (odd_sh) {  // values that are not finite, from the positions that only some rows see
-                const int pos = p0 + r / G;
-                for (int k = k0; k < k1; ++k) {
-                    if (k >= all0 && k < all1) continue;
-                    if (k > pos || (a.window > 0 && k <= pos - a.window)) continue;
-                    const int b = block_of(k), page = __ldg(table + b);
-                    if (page < 0 || page >= a.kv.n_pages) continue;
-                    const T *v = reinterpret_cast<const T *>(vb) + (int64_t)page * a.kv.page_stride +
-                                 (int64_t)(k - b * P) * a.kv.token_stride + c;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (!isfinite(to_f(v[e]))) y[e] = __fadd_rn(y[e], to_f(v[e]));
-                }
-            }
-            if (nsplit == 1) {
-                const int tok = q.q0 + r / G, h = g * G + r % G;
-                const float inv = M == -INFINITY ? 0.0f : __frcp_rn(lt);
-                Vec<T, 4> out;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) out.e[e] = from_f<T>(__fmul_rn(y[e], inv));
-                *reinterpret_cast<Vec<T, 4> *>(static_cast<T *>(a.out) + (int64_t)tok * a.ldo + (int64_t)h * HD + c) = out;
-                if (a.lse && c == 0)
-                    a.lse[(int64_t)h * a.c.n_tokens + tok] = M == -INFINITY ? -INFINITY : __fadd_rn(M, log2f(lt));
-            } else if (item < f.max_items) {
-                float *p = f.part + ((int64_t)item * f.part_rows + r) * (HD + 4);
-                __stcg(reinterpret_cast<float4 *>(p + c), make_float4(y[0], y[1], y[2], y[3]));
-                if (c == 0) __stcg(reinterpret_cast<float2 *>(p + HD), make_float2(M, lt));
-            } else if (i == 0) {  // the lengths' sum is above its bound
-                set_status(a.c.status, ALTXS_ST_BAD_POS);
-            }
-        }
-        if (nsplit > 1) {
-            __threadfence();
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                uint32_t *cnt = f.cnt + (int64_t)s * Hkv + g;
-                const bool last = atomicAdd(cnt, 1u) == (uint32_t)nsplit - 1;
-                if (last) *cnt = 0;
-                __threadfence();
-                last_sh = last;
-            }
-            __syncthreads();
-            if (last_sh && item - (int64_t)split * Hkv + (int64_t)(nsplit - 1) * Hkv < f.max_items) {
-                // join the splits in order; the rows' maxima and sums first, in shared memory
-                float *ms = rows;  // [nsplit][R] weights, then [R] 1 / sum
-                const float *p0s = f.part + pbase * (HD + 4) + (int64_t)g * f.part_rows * (HD + 4);
-                const int64_t ps = (int64_t)Hkv * f.part_rows * (HD + 4);  // one split to the next
-                for (int r = threadIdx.x; r < R; r += kWarps * 32) {
-                    float M = -INFINITY, lt = 0.0f;
-                    for (int t = 0; t < nsplit; ++t) M = fmaxf(M, __ldcg(p0s + t * ps + r * (HD + 4) + HD));
-                    for (int t = 0; t < nsplit; ++t) {
-                        const float2 x = __ldcg(reinterpret_cast<const float2 *>(p0s + t * ps + r * (HD + 4) + HD));
-                        const float w = M == -INFINITY ? 0.0f : ex2(__fsub_rn(x.x, M));
-                        ms[t * R + r] = w;
-                        lt = __fmaf_rn(x.y, w, lt);
-                    }
-                    ms[nsplit * R + r] = M == -INFINITY ? 0.0f : __frcp_rn(lt);
-                    if (a.lse)
-                        a.lse[(int64_t)(g * G + r % G) * a.c.n_tokens + q.q0 + r / G] =
-                            M == -INFINITY ? -INFINITY : __fadd_rn(M, log2f(lt));
-                }
-                __syncthreads();
-                for (int i = threadIdx.x; i < R * (HD / 4); i += kWarps * 32) {
-                    const int r = i / (HD / 4), c = (i % (HD / 4)) * 4;
-                    float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 8
-                    for (int t = 0; t < nsplit; ++t) {
-                        const float4 x = __ldcg(reinterpret_cast<const float4 *>(p0s + t * ps + r * (HD + 4) + c));
-                        const float w = ms[t * R + r];
-                        y[0] = __fmaf_rn(x.x, w, y[0]), y[1] = __fmaf_rn(x.y, w, y[1]);
-                        y[2] = __fmaf_rn(x.z, w, y[2]), y[3] = __fmaf_rn(x.w, w, y[3]);
-                    }
-                    const float inv = ms[nsplit * R + r];
-                    Vec<T, 4> out;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) out.e[e] = from_f<T>(__fmul_rn(y[e], inv));
-                    *reinterpret_cast<Vec<T, 4> *>(static_cast<T *>(a.out) + (int64_t)(q.q0 + r / G) * a.ldo +
-                                                   (int64_t)(g * G + r % G) * HD + c) = out;
-                }
-            }
-        }
+        finish_item<T, HD>(f, item, at, nsplit, R, kWarps, kMaxRows, rows, &ml_sh[0][0][0], &last_sh,
+                           odd_sh ? &odd : nullptr);
         __syncthreads();  // before the slots and the shared words are used again
+    }
+}
+
+// fp32 and at most four rows (a few query heads of one token): 2 flops a byte and row, so plain fp32
+// arithmetic keeps up with HBM and the 16-row MMA tile (three tf32 products, a dozen instructions per pair
+// of values to split them) does not.  HD / 8 lanes share a position, each with eight channels of its key and
+// value straight from global memory (two 16-byte loads each, the row contiguous over the lanes); a warp
+// has 8 KB in flight and 16 warps an SM.  Every group of lanes keeps its own (m, l, o) over its
+// positions, joined at the end.
+constexpr int kVecRows = 8;
+template <int HD, int R>
+__global__ void __launch_bounds__(kWarps * 32, R == 1 ? 5 : R < 8 ? 3 : 2) k_paged_vec(const __grid_constant__ FewArgs f) {
+    constexpr int LPK = HD / 8, KS = 32 / LPK, U = 4, B = U * KS, Sets = kWarps * KS;  // lanes a position, positions a step
+    __shared__ ItemScan sc;
+    static_assert(HD * Sets >= 3 * kSplitItems + 1, "what the join of the splits keeps fits");
+    __shared__ __align__(16) float rows[Sets * R * HD];
+    __shared__ __align__(8) float ml[Sets * R * 2];
+    __shared__ int last_sh;
+    const PagedAttnArgs &a = f.a;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kg = lane / LPK, li = lane % LPK;
+    const int G = f.G, P = a.kv.page_size, pshift = (P & (P - 1)) == 0 ? 31 - __clz(P) : -1;
+    const float c2 = __fmul_rn(a.scale, kLog2e);
+    scan_items(f, sc);
+    const int total = sc.before[kWarps * 32];
+    for (int item = blockIdx.x; item < total; item += gridDim.x) {
+        const Where at = locate(f, sc, item);
+        const Seq q = at.q;
+        const int s = at.s, g = at.g, split = at.split;
+        const int r0 = at.grp * f.group, n = min(f.group, q.n * G - r0), kfirst = first_seen(q.n, q.L, a.window), keys = max(0, q.L - kfirst);
+        const int nsplit = split_count(keys, at.width), slen = split_keys(keys, at.width);
+        const int k0 = kfirst + split * slen, k1 = min(q.L, k0 + slen), p0 = q.L - q.n;
+        const float *kb = static_cast<const float *>(a.kv.k) + (int64_t)g * a.kv.head_stride + 4 * li;
+        const float *vb = static_cast<const float *>(a.kv.v) + (int64_t)g * a.kv.head_stride + 4 * li;
+        const int32_t *table = a.c.page_table + s * a.c.table_stride;
+        float qr[R][8], o[R][8], m[R], l[R];
+        int pos[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int i = (r0 + r) / G;
+            pos[r] = r < n ? p0 + i : -1;
+            m[r] = -INFINITY, l[r] = 0.0f;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+            if (r < n) {
+                const float *qp = static_cast<const float *>(a.q) + (int64_t)(q.q0 + i) * a.ldq + (int64_t)(g * G + r0 + r - i * G) * HD + 4 * li;
+                x = __ldg(reinterpret_cast<const float4 *>(qp)), y = __ldg(reinterpret_cast<const float4 *>(qp + HD / 2));
+            }
+            const float t[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) qr[r][e] = __fmul_rn(t[e], c2), o[r][e] = 0.0f;
+        }
+        auto block_of = [&](int k) { return pshift >= 0 ? k >> pshift : k / P; };
+        int page[U];
+        auto fetch = [&](int kb0) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int k = kb0 + u * KS + kg;
+                page[u] = k < k1 ? __ldg(table + block_of(k)) : INT32_MIN;
+            }
+        };
+        fetch(k0 + warp * B);
+        for (int kc = k0 + warp * B; kc < k1; kc += kWarps * B) {
+            float kr[U][8], vr[U][8];
+            bool in[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int k = kc + u * KS + kg;
+                in[u] = page[u] >= 0 && page[u] < a.kv.n_pages;
+                if (!in[u] && page[u] != INT32_MIN) set_status(a.c.status, ALTXS_ST_BAD_POS);
+                const int64_t off = (int64_t)page[u] * a.kv.page_stride + (int64_t)(k - block_of(k) * P) * a.kv.token_stride;
+                float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x, z = x, w = x;
+                if (in[u]) {
+                    x = ldg_stream(kb + off), y = ldg_stream(kb + off + HD / 2);
+                    z = ldg_stream(vb + off), w = ldg_stream(vb + off + HD / 2);
+                }
+                kr[u][0] = x.x, kr[u][1] = x.y, kr[u][2] = x.z, kr[u][3] = x.w, kr[u][4] = y.x, kr[u][5] = y.y, kr[u][6] = y.z, kr[u][7] = y.w;
+                vr[u][0] = z.x, vr[u][1] = z.y, vr[u][2] = z.z, vr[u][3] = z.w, vr[u][4] = w.x, vr[u][5] = w.y, vr[u][6] = w.z, vr[u][7] = w.w;
+            }
+            fetch(kc + kWarps * B);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float sco[U], mx = m[r];
+                bool see[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    float d = __fmul_rn(qr[r][0], kr[u][0]);
+#pragma unroll
+                    for (int e = 1; e < 8; ++e) d = __fmaf_rn(qr[r][e], kr[u][e], d);
+                    sco[u] = d;
+                }
+#pragma unroll
+                for (int w = 1; w < LPK; w <<= 1)
+#pragma unroll
+                    for (int u = 0; u < U; ++u) sco[u] = __fadd_rn(sco[u], __shfl_xor_sync(kAll, sco[u], w));
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int k = kc + u * KS + kg;
+                    see[u] = in[u] && k <= pos[r] && (a.window == 0 || k > pos[r] - a.window);
+                    if (see[u]) mx = fmaxf(mx, sco[u]);
+                }
+                const float fold = mx == -INFINITY ? 0.0f : ex2(__fsub_rn(m[r], mx)), base = mx == -INFINITY ? 0.0f : mx;
+                m[r] = mx;
+                l[r] = __fmul_rn(l[r], fold);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[r][e] = __fmul_rn(o[r][e], fold);
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (see[u]) {
+                        const float p = ex2(__fsub_rn(sco[u], base));
+                        l[r] = __fadd_rn(l[r], p);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) o[r][e] = __fmaf_rn(p, vr[u][e], o[r][e]);
+                    }
+            }
+        }
+        const int set = warp * KS + kg;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float *y = rows + (set * R + r) * HD + 4 * li;
+            *reinterpret_cast<float4 *>(y) = make_float4(o[r][0], o[r][1], o[r][2], o[r][3]);
+            *reinterpret_cast<float4 *>(y + HD / 2) = make_float4(o[r][4], o[r][5], o[r][6], o[r][7]);
+            if (li == 0) ml[2 * (set * R + r)] = m[r], ml[2 * (set * R + r) + 1] = l[r];
+        }
+        __syncthreads();
+        finish_item<float, HD>(f, item, at, nsplit, n, Sets, R, rows, ml, &last_sh, nullptr);
+        __syncthreads();  // before the shared rows are used again
     }
 }
 
@@ -560,6 +658,7 @@ constexpr int64_t kCounters = 65536;  // more than these are cleared by the call
 
 struct Plan {
     bool few, many;       // which kernels the host's bounds allow work for
+    int group, groups;    // few: rows of an item, items of a (split, head) at most
     int64_t items;        // few: bound on the items
     int part_rows;
     ManyPlan mp;
@@ -572,19 +671,22 @@ Plan plan_of(const altxs_paged_kv &kv, const altxs_chunks &c, int H, int window)
     if (n == 0 || c.max_new == 0) return p;
     const bool same = c.n_tokens == n * c.max_new;  // every sequence has max_new tokens
     p.many = (int64_t)c.max_new * G > kMaxRows;
-    p.few = G <= kMaxRows && (!p.many || !same);
+    const int64_t least = same ? (int64_t)c.max_new * G : G, most = (int64_t)c.max_new * G;  // rows of a sequence
+    p.few = least <= kMaxRows;
+    p.group = kv.dtype == ALTXS_F32 ? kVecRows : kMaxRows;
+    p.groups = (int)((std::min<int64_t>(kMaxRows, most) + p.group - 1) / p.group);
     const int64_t keys = window > 0 ? std::min<int64_t>(c.max_kv, (int64_t)window + c.max_new - 1) : c.max_kv;
     int64_t total = n * keys, part = 0;
     if (c.total_kv > 0) total = std::min(total, c.total_kv);
-    const bool split = split_count((int)keys) > 1;
-    p.items = (split ? total / kSplitUnit + n : n) * kv.n_kv_heads;
-    p.part_rows = (int)std::min<int64_t>(kMaxRows, (int64_t)c.max_new * G);
+    const bool split = keys > kSplitUnit;
+    p.items = (split ? total / kSplitUnit + n : n) * kv.n_kv_heads * std::max(p.groups, 1);
+    p.part_rows = (int)std::min<int64_t>(p.group, most);
     if (p.few && split) part = p.items * p.part_rows * (kv.head_dim + 4) * 4;
     if (p.many) {
         p.mp = paged_many_plan(kv, c, H, window);
         part = std::max(part, p.mp.slots * p.mp.slot_bytes);
     }
-    p.few_cnt = align_up(4 * std::max(kCounters, n * kv.n_kv_heads), 256);
+    p.few_cnt = align_up(4 * std::max(kCounters, n * kv.n_kv_heads * std::max(p.groups, 1)), 256);
     p.many_cnt = align_up(4 * std::max(kCounters, p.mp.slots), 256);
     if (part > 0) p.bytes = p.few_cnt + p.many_cnt + part;
     return p;
@@ -611,21 +713,31 @@ int launch(const PagedAttnArgs &a, const Plan &p, cudaStream_t st) {
             cudaMemsetAsync(ws, 0, p.few_cnt + p.many_cnt, st) != cudaSuccess)
             return ALTXS_ECUDA;
     }
+    const FewArgs f{a, a.H / a.kv.n_kv_heads, 1, kMaxRows, p.group, p.bytes > 0 ? p.items : 0, few_cnt, p.groups, part, p.part_rows};
+    const int64_t sms = sm_count();
     if (p.few) {
-        constexpr int smem = kWarps * kSlots * kChunkBytes;
-        static std::atomic<uint64_t> set{0};  // devices whose shared-memory limit is raised
-        int dev = 0;
-        if (cudaGetDevice(&dev) != cudaSuccess) return ALTXS_ECUDA;
-        if (dev >= 64 || !((set.load() >> dev) & 1)) {
-            if (cudaFuncSetAttribute(k_paged_few<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-                return ALTXS_ECUDA;
-            if (dev < 64) set.fetch_or(1ull << dev);
+        if constexpr (std::is_same<T, float>::value) {
+            const int64_t most = (int64_t)a.c.max_new * f.G;  // rows
+            const unsigned grid = (unsigned)std::min<int64_t>(p.items, (most == 1 ? 5 : most <= 4 ? 3 : 2) * sms);
+            if (most == 1) ALTXS_LAUNCH(kKPaged, st, k_paged_vec<HD, 1><<<grid, kWarps * 32, 0, st>>>(f));
+            else if (most == 2) ALTXS_LAUNCH(kKPaged, st, k_paged_vec<HD, 2><<<grid, kWarps * 32, 0, st>>>(f));
+            else if (most <= 4) ALTXS_LAUNCH(kKPaged, st, k_paged_vec<HD, 4><<<grid, kWarps * 32, 0, st>>>(f));
+            else ALTXS_LAUNCH(kKPaged, st, k_paged_vec<HD, 8><<<grid, kWarps * 32, 0, st>>>(f));
+        } else {
+            constexpr int smem = kWarps * kSlots * kChunkBytes;
+            static std::atomic<uint64_t> set{0};  // devices whose shared-memory limit is raised
+            int dev = 0;
+            if (cudaGetDevice(&dev) != cudaSuccess) return ALTXS_ECUDA;
+            if (dev >= 64 || !((set.load() >> dev) & 1)) {
+                if (cudaFuncSetAttribute(k_paged_few<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+                    return ALTXS_ECUDA;
+                if (dev < 64) set.fetch_or(1ull << dev);
+            }
+            const unsigned grid = (unsigned)std::min<int64_t>(p.items, 2 * sms);
+            ALTXS_LAUNCH(kKPaged, st, k_paged_few<T, HD><<<grid, kWarps * 32, smem, st>>>(f));
         }
-        const FewArgs f{a, a.H / a.kv.n_kv_heads, p.bytes > 0 ? p.items : 0, few_cnt, part, p.part_rows};
-        const unsigned grid = (unsigned)std::min<int64_t>(p.items, 2 * sm_count());
-        ALTXS_LAUNCH(kKPaged, st, k_paged_few<T, HD><<<grid, kWarps * 32, smem, st>>>(f));
     }
-    if (p.many) return launch_paged_many(a, p.mp, kMaxRows + 1, many_cnt, part, sm_count(), st);
+    if (p.many) return launch_paged_many(a, p.mp, kMaxRows + 1, many_cnt, part, (int)sms, st);
     return ALTXS_OK;
 }
 template <typename T>
