@@ -61,10 +61,12 @@ struct FewArgs {
     int part_rows;
 };
 
-// Items of the sequences before each run of `per` sequences.
+// Items of the sequences before each run of `per` sequences; the sequences themselves while they fit.
+constexpr int kScan = 128;
 struct ItemScan {
-    int before[kWarps * 32 + 1];
+    int before[kScan + 1];
     int per;
+    Seq seq[kScan];
 };
 
 // items of a split: a (key/value head, row group) each
@@ -77,25 +79,29 @@ __device__ __forceinline__ int few_splits(const FewArgs &f, const Seq &q) {
 }
 
 __device__ __forceinline__ void scan_items(const FewArgs &f, ItemScan &sc) {
-    const int n = f.a.c.n_seqs, per = (n + kWarps * 32 - 1) / (kWarps * 32);
+    __shared__ int wsum[kScan / 32];
+    const int n = f.a.c.n_seqs, per = (n + kScan - 1) / kScan;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    int sum = 0;
-    for (int s = tid * per; s < min(n, (tid + 1) * per); ++s) {
-        const Seq q = blockIdx.x == 0 ? load_seq_report(f.a.c, s) : load_seq(f.a.c, s);
-        sum += few_splits(f, q) * few_width(f, q);
-    }
-    int inc = sum;
+    int inc = 0;
+    if (tid < kScan) {
+        for (int s = tid * per; s < min(n, (tid + 1) * per); ++s) {
+            const Seq q = blockIdx.x == 0 ? load_seq_report(f.a.c, s) : load_seq(f.a.c, s);
+            inc += few_splits(f, q) * few_width(f, q);
+            if (per == 1) sc.seq[s] = q;
+        }
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(kAll, inc, o);
-        if (lane >= o) inc += v;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(kAll, inc, o);
+            if (lane >= o) inc += v;
+        }
+        if (lane == 31) wsum[warp] = inc;
     }
-    __shared__ int wsum[kWarps];
-    if (lane == 31) wsum[warp] = inc;
     __syncthreads();
-    for (int w = 0; w < warp; ++w) inc += wsum[w];
-    sc.before[tid + 1] = inc;
-    if (tid == 0) sc.before[0] = 0, sc.per = per;
+    if (tid < kScan) {
+        for (int w = 0; w < warp; ++w) inc += wsum[w];
+        sc.before[tid + 1] = inc;
+        if (tid == 0) sc.before[0] = 0, sc.per = per;
+    }
     __syncthreads();
 }
 
@@ -105,7 +111,7 @@ struct Where {
     int s, split, g, grp, width;  // width: items from one split to the next
 };
 __device__ __forceinline__ Where locate(const FewArgs &f, const ItemScan &sc, int item) {
-    int lo = 0, hi = kWarps * 32;
+    int lo = 0, hi = kScan;
     while (hi - lo > 1) {
         const int m = (lo + hi) >> 1;
         if (sc.before[m] <= item) lo = m; else hi = m;
@@ -113,8 +119,8 @@ __device__ __forceinline__ Where locate(const FewArgs &f, const ItemScan &sc, in
     Where w;
     w.s = lo * sc.per;
     int local = item - sc.before[lo];
-    w.q = load_seq(f.a.c, w.s);
-    for (int n; w.s < f.a.c.n_seqs - 1 && local >= (n = few_splits(f, w.q) * few_width(f, w.q)); w.q = load_seq(f.a.c, ++w.s))
+    w.q = sc.per == 1 ? sc.seq[lo] : load_seq(f.a.c, w.s);
+    for (int n; sc.per > 1 && w.s < f.a.c.n_seqs - 1 && local >= (n = few_splits(f, w.q) * few_width(f, w.q)); w.q = load_seq(f.a.c, ++w.s))
         local -= n;
     w.width = few_width(f, w.q);
     w.split = local / w.width;
@@ -203,7 +209,7 @@ __device__ __forceinline__ void finish_item(const FewArgs &f, int item, const Wh
     const PagedAttnArgs &a = f.a;
     const Seq &q = w0.q;
     const int G = f.G, s = w0.s, g = w0.g, r0 = w0.grp * f.group;  // row r of the item is row r0 + r of the sequence
-    for (int i = threadIdx.x; i < R * (HD / 4); i += kWarps * 32) {
+    for (int i = threadIdx.x; i < R * (HD / 4); i += blockDim.x) {
         const int r = i / (HD / 4), c = (i % (HD / 4)) * 4;
         float M = -INFINITY, lt = 0.0f, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         for (int w = 0; w < sets; ++w) M = fmaxf(M, ml[2 * (w * stride + r)]);
@@ -265,10 +271,10 @@ __device__ __forceinline__ void finish_item(const FewArgs &f, int item, const Wh
     float2 *in = reinterpret_cast<float2 *>(rows + ((nsplit + 1) * R + 1 & ~1));  // [nsplit][R]
     const float *p0 = f.part + first * f.part_rows * (HD + 4);
     const int64_t ps = (int64_t)w0.width * f.part_rows * (HD + 4);
-    for (int i = threadIdx.x; i < nsplit * R; i += kWarps * 32)
+    for (int i = threadIdx.x; i < nsplit * R; i += blockDim.x)
         in[i] = __ldcg(reinterpret_cast<const float2 *>(p0 + i / R * ps + i % R * (HD + 4) + HD));
     __syncthreads();
-    for (int r = threadIdx.x; r < R; r += kWarps * 32) {
+    for (int r = threadIdx.x; r < R; r += blockDim.x) {
         float M = -INFINITY, lt = 0.0f;
         for (int t = 0; t < nsplit; ++t) M = fmaxf(M, in[t * R + r].x);
         for (int t = 0; t < nsplit; ++t) {
@@ -283,7 +289,7 @@ __device__ __forceinline__ void finish_item(const FewArgs &f, int item, const Wh
                 M == -INFINITY ? -INFINITY : __fadd_rn(M, log2f(lt));
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < R * (HD / 4); i += kWarps * 32) {
+    for (int i = threadIdx.x; i < R * (HD / 4); i += blockDim.x) {
         const int r = i / (HD / 4), c = (i % (HD / 4)) * 4;
         float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 8
@@ -317,7 +323,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_paged_few(const __grid_const
     const float c2 = __fmul_rn(a.scale, kLog2e);
     const uint32_t ring = smem_u32(few_smem) + warp * kSlots * kChunkBytes;
     scan_items(f, sc);
-    const int total = sc.before[kWarps * 32];
+    const int total = sc.before[kScan];
 
     for (int item = blockIdx.x; item < total; item += gridDim.x) {
         const Where at = locate(f, sc, item);
@@ -527,19 +533,20 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_paged_few(const __grid_const
     }
 }
 
-// fp32 and at most four rows (a few query heads of one token): 2 flops a byte and row, so plain fp32
-// arithmetic keeps up with HBM and the 16-row MMA tile (three tf32 products, a dozen instructions per pair
-// of values to split them) does not.  HD / 8 lanes share a position, each with eight channels of its key and
-// value straight from global memory (two 16-byte loads each, the row contiguous over the lanes); a warp
-// has 8 KB in flight and 16 warps an SM.  Every group of lanes keeps its own (m, l, o) over its
-// positions, joined at the end.
-constexpr int kVecRows = 8;
+// fp32: half a flop a byte and row, so plain fp32 arithmetic keeps up with HBM for a few rows.  HD / 8 lanes
+// share a position, each with eight channels of its key and value straight from global memory (two 16-byte
+// loads each, the row contiguous over the lanes); a warp has 8 KB in flight, 16 warps an SM.  Every group of
+// lanes keeps its own (m, l, o) over its positions, joined at the end.  More than eight rows are two items that
+// read the same keys.  (As 16-row MMA tiles of three tf32 products, with a dozen instructions to split each pair
+// of values, 256 streams took 471 us where this takes XXX.)
+constexpr int kVecRows = 8, kVecWarps = 8;
 template <int HD, int R>
-__global__ void __launch_bounds__(kWarps * 32, R == 1 ? 5 : R < 8 ? 3 : 2) k_paged_vec(const __grid_constant__ FewArgs f) {
-    constexpr int LPK = HD / 8, KS = 32 / LPK, U = 4, B = U * KS, Sets = kWarps * KS;  // lanes a position, positions a step
+__global__ void __launch_bounds__(kVecWarps * 32, R == 1 ? 4 : R < 4 ? 2 : 1) k_paged_vec(const __grid_constant__ FewArgs f) {
+    constexpr int LPK = HD / 8, KS = 32 / LPK, U = 2, B = U * KS, Sets = kVecWarps;  // lanes a position, positions a step
     __shared__ ItemScan sc;
-    static_assert(HD * Sets >= 3 * kSplitItems + 1, "what the join of the splits keeps fits");
-    __shared__ __align__(16) float rows[Sets * R * HD];
+    // (the join of the splits keeps three words for each of them there)
+    constexpr int Words = Sets * HD > 3 * kSplitItems + 4 ? Sets * HD : 3 * kSplitItems + 4;
+    __shared__ __align__(16) float rows[Words * R];
     __shared__ __align__(8) float ml[Sets * R * 2];
     __shared__ int last_sh;
     const PagedAttnArgs &a = f.a;
@@ -547,7 +554,7 @@ __global__ void __launch_bounds__(kWarps * 32, R == 1 ? 5 : R < 8 ? 3 : 2) k_pag
     const int G = f.G, P = a.kv.page_size, pshift = (P & (P - 1)) == 0 ? 31 - __clz(P) : -1;
     const float c2 = __fmul_rn(a.scale, kLog2e);
     scan_items(f, sc);
-    const int total = sc.before[kWarps * 32];
+    const int total = sc.before[kScan];
     for (int item = blockIdx.x; item < total; item += gridDim.x) {
         const Where at = locate(f, sc, item);
         const Seq q = at.q;
@@ -584,7 +591,7 @@ __global__ void __launch_bounds__(kWarps * 32, R == 1 ? 5 : R < 8 ? 3 : 2) k_pag
             }
         };
         fetch(k0 + warp * B);
-        for (int kc = k0 + warp * B; kc < k1; kc += kWarps * B) {
+        for (int kc = k0 + warp * B; kc < k1; kc += kVecWarps * B) {
             float kr[U][8], vr[U][8];
             bool in[U];
 #pragma unroll
@@ -601,7 +608,7 @@ __global__ void __launch_bounds__(kWarps * 32, R == 1 ? 5 : R < 8 ? 3 : 2) k_pag
                 kr[u][0] = x.x, kr[u][1] = x.y, kr[u][2] = x.z, kr[u][3] = x.w, kr[u][4] = y.x, kr[u][5] = y.y, kr[u][6] = y.z, kr[u][7] = y.w;
                 vr[u][0] = z.x, vr[u][1] = z.y, vr[u][2] = z.z, vr[u][3] = z.w, vr[u][4] = w.x, vr[u][5] = w.y, vr[u][6] = w.z, vr[u][7] = w.w;
             }
-            fetch(kc + kWarps * B);
+            fetch(kc + kVecWarps * B);
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 float sco[U], mx = m[r];
@@ -638,14 +645,27 @@ __global__ void __launch_bounds__(kWarps * 32, R == 1 ? 5 : R < 8 ? 3 : 2) k_pag
                     }
             }
         }
-        const int set = warp * KS + kg;
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            float *y = rows + (set * R + r) * HD + 4 * li;
-            *reinterpret_cast<float4 *>(y) = make_float4(o[r][0], o[r][1], o[r][2], o[r][3]);
-            *reinterpret_cast<float4 *>(y + HD / 2) = make_float4(o[r][4], o[r][5], o[r][6], o[r][7]);
-            if (li == 0) ml[2 * (set * R + r)] = m[r], ml[2 * (set * R + r) + 1] = l[r];
-        }
+        for (int w = LPK; w < 32; w <<= 1)  // the warp's groups of lanes, in a fixed tree
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const float m1 = __shfl_xor_sync(kAll, m[r], w), l1 = __shfl_xor_sync(kAll, l[r], w), M = fmaxf(m[r], m1);
+                const float f0 = m[r] == -INFINITY ? 0.0f : ex2(__fsub_rn(m[r], M)), f1 = m1 == -INFINITY ? 0.0f : ex2(__fsub_rn(m1, M));
+                // the two sides add the same two products, so they agree
+                l[r] = __fadd_rn(__fmul_rn(l[r], f0), __fmul_rn(l1, f1));
+                m[r] = M;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    o[r][e] = __fadd_rn(__fmul_rn(o[r][e], f0), __fmul_rn(__shfl_xor_sync(kAll, o[r][e], w), f1));
+            }
+        if (kg == 0)
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float *y = rows + (warp * R + r) * HD + 4 * li;
+                *reinterpret_cast<float4 *>(y) = make_float4(o[r][0], o[r][1], o[r][2], o[r][3]);
+                *reinterpret_cast<float4 *>(y + HD / 2) = make_float4(o[r][4], o[r][5], o[r][6], o[r][7]);
+                if (li == 0) ml[2 * (warp * R + r)] = m[r], ml[2 * (warp * R + r) + 1] = l[r];
+            }
         __syncthreads();
         finish_item<float, HD>(f, item, at, nsplit, n, Sets, R, rows, ml, &last_sh, nullptr);
         __syncthreads();  // before the shared rows are used again
@@ -718,11 +738,11 @@ int launch(const PagedAttnArgs &a, const Plan &p, cudaStream_t st) {
     if (p.few) {
         if constexpr (std::is_same<T, float>::value) {
             const int64_t most = (int64_t)a.c.max_new * f.G;  // rows
-            const unsigned grid = (unsigned)std::min<int64_t>(p.items, (most == 1 ? 5 : most <= 4 ? 3 : 2) * sms);
-            if (most == 1) ALTXS_LAUNCH(kKPaged, st, k_paged_vec<HD, 1><<<grid, kWarps * 32, 0, st>>>(f));
-            else if (most == 2) ALTXS_LAUNCH(kKPaged, st, k_paged_vec<HD, 2><<<grid, kWarps * 32, 0, st>>>(f));
-            else if (most <= 4) ALTXS_LAUNCH(kKPaged, st, k_paged_vec<HD, 4><<<grid, kWarps * 32, 0, st>>>(f));
-            else ALTXS_LAUNCH(kKPaged, st, k_paged_vec<HD, 8><<<grid, kWarps * 32, 0, st>>>(f));
+            const unsigned grid = (unsigned)std::min<int64_t>(p.items, (most == 1 ? 4 : most <= 2 ? 2 : 1) * sms);
+            if (most == 1) ALTXS_LAUNCH(kKPaged, st, k_paged_vec<HD, 1><<<grid, kVecWarps * 32, 0, st>>>(f));
+            else if (most == 2) ALTXS_LAUNCH(kKPaged, st, k_paged_vec<HD, 2><<<grid, kVecWarps * 32, 0, st>>>(f));
+            else if (most <= 4) ALTXS_LAUNCH(kKPaged, st, k_paged_vec<HD, 4><<<grid, kVecWarps * 32, 0, st>>>(f));
+            else ALTXS_LAUNCH(kKPaged, st, k_paged_vec<HD, 8><<<grid, kVecWarps * 32, 0, st>>>(f));
         } else {
             constexpr int smem = kWarps * kSlots * kChunkBytes;
             static std::atomic<uint64_t> set{0};  // devices whose shared-memory limit is raised

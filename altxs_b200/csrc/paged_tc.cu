@@ -149,6 +149,12 @@ struct Scan {
     int4 seq[kCached];
 };
 
+// The k-th item of a block: rounds alternate their direction, so that the longest items of a round do not
+// all meet those of the next.
+__device__ __forceinline__ int item_of(int k) {
+    return k * (int)gridDim.x + (int)(k & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+}
+
 struct Item {
     Seq q;
     int s, g, nsplit, split;
@@ -466,7 +472,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
         uint32_t n = 0, kt = 0, live = 0;  // slots, key tiles and items with tiles so far
         bool ok = true;
         // The tile whose copies come next: found (and its page numbers on their way) one tile ahead.
-        int item = (int)blockIdx.x - (int)gridDim.x, t = 0;
+        int round = 0, t = 0;
         Item it;
         it.t1 = 0;
         bool fresh = false, more = true;
@@ -474,7 +480,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
             ++t;
             fresh = false;
             while (t >= it.t1) {
-                item += gridDim.x;
+                const int item = item_of(round++);
                 if (item >= total) {
                     more = false;
                     return;
@@ -765,7 +771,9 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
             constexpr uint32_t kTileD = C::TileB >> 4, kPlaneD = C::PlaneB >> 4, kQPlaneD = C::QPlaneB >> 4;
             const uint32_t ringk = desc_lo(ring, 16), ringv = desc_lo(ring, KT * 128), q0d = desc_lo(sq, 16);
             bool ok = true;
-            for (int item = blockIdx.x; item < total && ok; item += gridDim.x) {
+            for (int round = 0; ok; ++round) {
+                const int item = item_of(round);
+                if (item >= total) break;
                 const Item it = locate<C>(f, sc, item);
                 const int nt = __shfl_sync(kAll, it.t1 - it.t0, 0);
                 const bool two = __shfl_sync(kAll, (int)it.two, 0) != 0;
@@ -868,7 +876,9 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
         float2 *ml = reinterpret_cast<float2 *>(qsm + C::MlAt);
         uint32_t job = 0, kt = 0, live = 0, done = 0;
         bool ok = true;
-        for (int item = blockIdx.x; item < total; item += gridDim.x) {
+        for (int round = 0;; ++round) {
+            const int item = item_of(round);
+            if (item >= total) break;
             const Item it = locate<C>(f, sc, item);
             const int nt = it.t1 - it.t0, p0 = it.q.L - it.q.n;
             // At most 64 (32) rows are held 2 (4) times, each copy with its share of a tile's columns, its own

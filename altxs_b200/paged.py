@@ -30,9 +30,13 @@ import numpy as np
 import torch
 
 from . import _lib
-from .engine import _stream_handle
 
 _DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+
+def _stream_handle(device: torch.device) -> int:
+    """The current stream of a device as the driver's handle (a torch Stream object costs 2 us a call)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def rope_table(positions: int, dims: int, base: float = 1e4, *, scaling: str | None = None, factor: float = 1.0,
@@ -123,7 +127,7 @@ def _rope(x: torch.Tensor, rotary: Rotary, pos: torch.Tensor, out: torch.Tensor 
     n, h, d = x.shape
     p = _positions(pos, n, rotary.device)
     if out is None:
-        out = torch.empty((n, h, d), dtype=x.dtype, device=x.device)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
         ldy = h * d
     else:
         ldy = _heads(out, "out", x.dtype, rotary.device)
@@ -232,7 +236,7 @@ class PagedKV:
         if q is not None:
             ldq, H = _heads(q, "q", self.dtype, self.device), q.shape[1]
             if q_out is None:
-                q_out = torch.empty((n, H, self.head_dim), dtype=self.dtype, device=self.device)
+                q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
             ldqo = _heads(q_out, "q_out", self.dtype, self.device)
             if q.shape != (n, H, self.head_dim) or q_out.shape != q.shape:
                 raise ValueError("q and q_out must be [tokens][heads][head_dim]")
@@ -254,7 +258,7 @@ class PagedKV:
         if d != self.head_dim or H % self.kv_heads:
             raise ValueError("q must be [tokens][heads][head_dim] with heads a multiple of kv_heads")
         if out is None:
-            out = torch.empty((n, H, d), dtype=self.dtype, device=self.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
             ldo = H * d
         else:
             ldo = _heads(out, "out", self.dtype, self.device)
