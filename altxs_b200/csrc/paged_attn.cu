@@ -707,8 +707,8 @@ Plan plan_of(const altxs_paged_kv &kv, const altxs_chunks &c, int H, int window)
         part = std::max(part, p.mp.slots * p.mp.slot_bytes);
     }
     p.few_cnt = align_up(4 * std::max(kCounters, n * kv.n_kv_heads * std::max(p.groups, 1)), 256);
-    p.many_cnt = align_up(4 * std::max(kCounters, p.mp.slots), 256);
-    if (part > 0) p.bytes = p.few_cnt + p.many_cnt + part;
+    p.many_cnt = align_up(4 * std::max(kCounters, p.mp.slots + 1), 256);  // its first word: the item tickets
+    if (part > 0 || p.many) p.bytes = p.few_cnt + p.many_cnt + part;
     return p;
 }
 

@@ -53,9 +53,10 @@ namespace {
 
 constexpr int kMmaWarp = 8;
 constexpr int kScan = 64;        // sequences are counted in this many groups
-constexpr int kCached = 48;       // up to this many sequences' shares are kept in shared memory
+constexpr int kCached = 40;       // up to this many sequences' shares are kept in shared memory
 constexpr int kMostItems = 1184;  // splits of one sequence
 constexpr int kMostSplits = 16;
+constexpr int kNext = 4;           // items announced to a block's roles ahead
 constexpr unsigned kAll = 0xffffffffu;
 constexpr float kLazy = 8.0f;
 
@@ -69,8 +70,9 @@ struct Tc {
     static constexpr int PlaneB = Halves * KT * 128;         // HD 32 leaves half of each 128-byte row unused
     static constexpr int TileB = Planes * PlaneB;
     static constexpr int QPlaneB = Halves * 128 * 128, QTileB = Planes * QPlaneB;  // 128 rows
-    static constexpr int Producers = F32 ? 7 : 3;
-    static constexpr int Threads = (kMmaWarp + 1 + Producers) * 32;
+    static constexpr int Loaders = F32 ? 7 : 3;  // warps from 9 on
+    static constexpr int Converters = 6;         // fp32: of them, warps 10 to 15
+    static constexpr int Threads = (kMmaWarp + 1 + Loaders) * 32;
     // registers: (8 warps x RegS + the others x RegP) x 32 = Threads x 168 (16 bits) or 128 (fp32)
     static constexpr int RegS = F32 ? 176 : 208, RegP = F32 ? 80 : 88;
     static_assert(256 * RegS + (Threads - 256) * RegP == Threads * (F32 ? 128 : 168), "register split");
@@ -122,9 +124,10 @@ __host__ __device__ inline void split_rule(Shape &w, int nt) {
 struct ManyArgs {
     PagedAttnArgs a;
     int G, min_rows;    // sequences with at least min_rows rows are this kernel's
-    int run;            // positions that lie within a page (16-bit types)
+    int run;            // positions that lie within a page
     int64_t max_slots;  // partial slots in the workspace (one per item of a split sequence)
     uint32_t *cnt;      // [max_slots], zero between calls
+    uint32_t *ticket;   // items handed out beyond the first of each block, zero between calls
     float *part;        // [max_slots][part_rows * (HD + 2)]
     int part_rows;
 };
@@ -148,12 +151,6 @@ struct Scan {
     // up to kCached sequences: each one's rows (q0, n, L) and its share (whole << 5 | nsplit)
     int4 seq[kCached];
 };
-
-// The k-th item of a block: rounds alternate their direction, so that the longest items of a round do not
-// all meet those of the next.
-__device__ __forceinline__ int item_of(int k) {
-    return k * (int)gridDim.x + (int)(k & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-}
 
 struct Item {
     Seq q;
@@ -398,7 +395,8 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
     constexpr int KT = C::KT;
     constexpr bool F32 = C::F32;
     extern __shared__ unsigned char pm_smem_raw[];
-    __shared__ __align__(8) uint64_t full[C::Slots], empty[C::Slots], landed[F32 ? 1 : C::Slots], s_full[2], p_full[2], o_done[2], q_full, drainb;
+    __shared__ __align__(8) uint64_t full[C::Slots], empty[C::Slots], landed[F32 ? 1 : C::Slots], s_full[2], p_full[2], o_done[2], q_full, drainb,
+        raw_full[2], raw_empty[2], next_full[kNext], next_empty[kNext];
     __shared__ Scan sc;
     // by key tile: which positions exist (4 to a byte), and (fp32) the exponents of its units of keys and of values
     __shared__ __align__(16) uint8_t kmask[C::Ring][KT / 4];
@@ -407,7 +405,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
     __shared__ __align__(8) uint8_t odd8_sh[F32 ? C::Ring : 1][8];  // by item: values that are not finite were set to 0 (fp32: per warp)
     __shared__ uint32_t odd_sh[F32 ? 1 : C::Ring];
     __shared__ int2 wsum[kScan / 32];
-    __shared__ int last_sh, stop_sh;
+    __shared__ int last_sh, item_sh, next_sh[kNext];
     __shared__ volatile int abort_sh;
     const PagedAttnArgs &a = f.a;
     const uint32_t raw_s = smem_u32(pm_smem_raw);
@@ -416,7 +414,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
     const uint32_t limit = wait_limit();
     if (tid == 0) {
         for (int s = 0; s < C::Slots; ++s) {
-            mbar_init(&full[s], F32 ? C::Producers : 1);
+            mbar_init(&full[s], F32 ? C::Converters : 1);
             mbar_init(&empty[s], 1);
             if (!F32) mbar_init(&landed[s], 1);
         }
@@ -424,6 +422,14 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 4);
             mbar_init(&o_done[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&raw_full[i], 1);
+            mbar_init(&raw_empty[i], C::Converters);
+        }
+        for (int i = 0; i < kNext; ++i) {
+            mbar_init(&next_full[i], 1);
+            mbar_init(&next_empty[i], C::Loaders + 1);  // the other loaders, the MMA warp, softmax warp 0
         }
         mbar_init(&q_full, 8);
         mbar_init(&drainb, 1);
@@ -462,6 +468,17 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
     tc_fence_after();
     const uint32_t tmem = tmem_sh;
     const int total = sc.before[kScan];
+    // Items go to whoever is free (they differ in length several times over): warp 9 draws a ticket per item and
+    // announces it; a warp's r-th item, total or more when there is none.
+    auto announced = [&](int r) {
+        uint64_t *bar = &next_full[r % kNext];
+        const bool got = __all_sync(kAll, mbar_wait_bounded(bar, (r / kNext) & 1, limit));
+        const int item = got ? next_sh[r % kNext] : INT32_MAX;
+        __syncwarp();
+        if (got && lane == 0) mbar_arrive(&next_empty[r % kNext]);
+        if (!got) abort_sh = 1;
+        return item;
+    };
 
     if (warp > kMmaWarp) {
         // ---- producers ----
@@ -472,7 +489,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
         uint32_t n = 0, kt = 0, live = 0;  // slots, key tiles and items with tiles so far
         bool ok = true;
         // The tile whose copies come next: found (and its page numbers on their way) one tile ahead.
-        int round = 0, t = 0;
+        int round = 0, t = 0, drawn = blockIdx.x;
         Item it;
         it.t1 = 0;
         bool fresh = false, more = true;
@@ -480,7 +497,23 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
             ++t;
             fresh = false;
             while (t >= it.t1) {
-                const int item = item_of(round++);
+                int item;
+                if (pw == 0) {
+                    item = __shfl_sync(kAll, drawn, 0);  // drawn an item ago
+                    const int slot = round % kNext;
+                    if (round >= kNext && !__all_sync(kAll, mbar_wait_bounded(&next_empty[slot], (round / kNext - 1) & 1, limit))) {
+                        ok = more = false;
+                        return;
+                    }
+                    if (lane == 0) {
+                        next_sh[slot] = item;
+                        mbar_arrive(&next_full[slot]);
+                        if (item < total) drawn = (int)gridDim.x + (int)atomicAdd(f.ticket, 1u);
+                    }
+                    ++round;
+                } else {
+                    item = announced(round++);
+                }
                 if (item >= total) {
                     more = false;
                     return;
@@ -629,130 +662,159 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                 }
             }
         } else {
-            // fp32: units of 2 KB (UR rows), 16-byte pieces; warp pw takes units pw, pw + 7, ..  Per unit: copy
-            // the rows to the raw stage one tile ahead (each lane its own pieces, so its own copies are all it
-            // waits for), find the unit's largest magnitude, write the scaled planes.
-            constexpr int CR = HD / 4, UR = C::UnitRows, Units = C::Units, UW = (Units + C::Producers - 1) / C::Producers;
-            static_assert(UW * UR <= 32, "one page look-up per lane");
+            const int run = f.run, runs = KT / run, issue = runs < 32 ? runs : 32;
             const uint32_t raw = ring + C::Slots * C::TileB;
-            const int un0 = pw + lane / UR * C::Producers;  // lane: row lane % UR of this unit
-            const bool mine = lane < UW * UR && un0 < Units;
-            int64_t off = -1;
-            uint32_t seen = 0;
-            int page = INT32_MIN;
-            auto fetch = [&]() {
-                const int k = it.base + t * KT + un0 * UR + lane % UR;
-                page = more && mine && k >= it.lo && k < it.hi ? __ldg(a.c.page_table + it.s * a.c.table_stride + block_of(k)) : INT32_MIN;
-            };
-            auto resolve = [&]() {
-                const int k = it.base + t * KT + un0 * UR + lane % UR;
-                const bool in = page >= 0 && page < a.kv.n_pages;
-                if (!in && page != INT32_MIN) set_status(a.c.status, ALTXS_ST_BAD_POS);
-                off = in ? ((int64_t)page * a.kv.page_stride + (int64_t)(k - block_of(k) * P) * a.kv.token_stride +
-                            (int64_t)it.g * a.kv.head_stride) * 4 : -1;
-                seen = __ballot_sync(kAll, in);
-            };
-            auto copy = [&](int kv) {
-                if (more) {
-                    const char *src0 = static_cast<const char *>(kv ? a.kv.v : a.kv.k);
-#pragma unroll 1
-                    for (int i = 0; i < UW; ++i) {
-                        const int un = pw + i * C::Producers;
-                        if (un >= Units) break;
+            if (pw == 0) {  // warp 9: a tile's raw rows, keys to one stage and values to the other, run by run
+                int page[KT / 32];
+                auto fetch = [&]() {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int q = e * 32 + lane;  // piece of the unit: row q / CR, channels 4 (q % CR) ..
-                            const int64_t o = __shfl_sync(kAll, off, i * UR + q / CR);
-                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(raw + kv * C::StageB + un * 2048 + q * 16),
-                                         "l"(src0 + (o < 0 ? 0 : o) + q % CR * 16), "r"(o < 0 ? 0u : 16u)
-                                         : "memory");
+                    for (int e = 0; e < KT / 32; ++e) {
+                        const int u = e * 32 + lane, k = it.base + t * KT + u * run;
+                        page[e] = more && u < runs && k < it.hi && k + run > it.lo
+                                      ? __ldg(a.c.page_table + it.s * a.c.table_stride + block_of(k)) : INT32_MIN;
+                        if (e * 32 + 32 >= runs) break;
+                    }
+                };
+                bool have = false;
+                int g = 0, pos_in[KT / 32], pg[KT / 32];
+                uint32_t sent[2] = {0, 0};
+                while (ok) {
+                    advance();
+                    fetch();
+                    if (have) {
+#pragma unroll
+                        for (int kv = 0; kv < 2; ++kv) {
+                            if (ok && sent[kv] > 0)
+                                ok = __all_sync(kAll, !abort_sh && mbar_wait_bounded(&raw_empty[kv], (sent[kv] - 1) & 1, limit));
+                            if (!ok) continue;
+                            ++sent[kv];
+                            if (lane == 0) mbar_expect_tx(&raw_full[kv], C::StageB);
+                            __syncwarp();
+                            const CUtensorMap *map = kv ? &tv : &tk;
+#pragma unroll
+                            for (int e = 0; e < KT / 32; ++e) {
+                                if (e * 32 >= runs) break;
+                                if (lane < issue)
+                                    tma_load_4d(raw + kv * C::StageB + (e * 32 + lane) * run * HD * 4, map, 0, pos_in[e], g, pg[e], &raw_full[kv]);
+                            }
+                                                    }
+                        if (!ok) break;
+                    }
+                    have = more;
+                    if (!more) break;
+                    const int kb = it.base + t * KT;
+                    g = it.g;
+#pragma unroll
+                    for (int e = 0; e < KT / 32; ++e) {
+                        if (e * 32 >= runs) break;
+                        const int k = kb + (e * 32 + lane) * run;
+                        const bool in = page[e] >= 0 && page[e] < a.kv.n_pages;
+                        if (!in && page[e] != INT32_MIN) set_status(a.c.status, ALTXS_ST_BAD_POS);
+                        pos_in[e] = k - block_of(k) * P;
+                        pg[e] = in ? page[e] : max(a.kv.n_pages, 1);
+                        const uint32_t seen = __ballot_sync(kAll, in);
+                        if (run >= 4) {
+                            if (lane < issue)
+                                for (int i = 0; i < run / 4; ++i) kmask[kt % C::Ring][(e * 32 + lane) * (run / 4) + i] = in ? 15 : 0;
+                        } else if (lane % 4 == 0) {
+                            kmask[kt % C::Ring][e * 8 + lane / 4] = (uint8_t)((seen >> lane) & 15);
                         }
                     }
+                    __syncwarp();
+                    ++kt;
                 }
-                asm volatile("cp.async.commit_group;" ::: "memory");
-            };
-            bool have = false, look = false;  // a tile is being copied, some of whose values not every row sees
-            uint32_t me = 0;
-            while (ok) {
-                if (have) {
+                // every copy has landed before the block can exit
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv)
+                    if (sent[kv] > 0) mbar_wait_bounded(&raw_full[kv], (sent[kv] - 1) & 1, kWaitLimit);
+            } else {
+                // Units of 2 KB (UR rows), 16-byte pieces; warp cw takes units cw, cw + 6, ..: find the unit's
+                // largest magnitude, write the scaled planes.  (Loops are left rolled: with everything
+                // unrolled the block's roles miss the instruction cache.)
+                constexpr int CR = HD / 4, UR = C::UnitRows, Units = C::Units;
+                const int cw = pw - 1;
+                uint32_t me = 0;
+                while (ok) {
+                    advance();
+                    if (!more) break;
                     if (fresh) {
                         bounds();
                         me = live++ % C::Ring;
-                        if (lane == 0) odd8_sh[me][pw] = 0;
+                        if (lane == 0) odd8_sh[me][cw] = 0;
                     }
                     const int kb = it.base + t * KT;
-                    look = kb < all0 || kb + KT > all1;
-                    if (lane % 4 == 0 && mine) kmask[kt % C::Ring][(un0 * UR + lane % UR) / 4] = (uint8_t)((seen >> lane) & 15);
-                }
-                advance();
-                fetch();
-                if (!have) {
-                    resolve();
-                    copy(0);
-                    copy(1);
-                    have = more;
-                    if (!more) break;
-                    continue;
-                }
-                // (Loops are left rolled: with everything unrolled the block's roles miss the instruction cache.)
+                    const bool look = kb < all0 || kb + KT > all1, edge = kb < it.lo || kb + KT > it.hi;
 #pragma unroll 1
-                for (int kv = 0; kv < 2; ++kv, ++n) {
-                    const uint32_t s = n % C::Slots;
-                    if (n >= C::Slots)
-                        ok = __all_sync(kAll, !abort_sh && mbar_wait_bounded(&empty[s], ((n / C::Slots) - 1) & 1, limit));
-                    if (!ok) break;
-                    asm volatile("cp.async.wait_group 1;" ::: "memory");
-                    const uint32_t stage = raw + kv * C::StageB + lane * 16, dst = ring + s * C::TileB;
+                    for (int kv = 0; kv < 2; ++kv, ++n) {
+                        const uint32_t s = n % C::Slots;
+                        ok = mbar_wait_bounded(&raw_full[kv], kt & 1, limit);
+                        if (n >= C::Slots) ok = ok && mbar_wait_bounded(&empty[s], ((n / C::Slots) - 1) & 1, limit);
+                        ok = __all_sync(kAll, ok && !abort_sh);
+                        if (!ok) break;
+                        const uint32_t stage = raw + kv * C::StageB + lane * 16, dst = ring + s * C::TileB;
 #pragma unroll 1
-                    for (int un = pw; un < Units; un += C::Producers) {
-                        float4 x[4];
+                        for (int un = cw; un < Units; un += C::Converters) {
+                            float4 x[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) x[e] = lds_f4(stage + un * 2048 + e * 512);
-                        float mf = 0.0f;
+                            for (int e = 0; e < 4; ++e) x[e] = lds_f4(stage + un * 2048 + e * 512);
+                            if (edge) {  // rows outside [lo, hi): whatever the page holds there
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            mf = fmaxf(mf, fmaxf(fmaxf(fabsf(x[e].x), fabsf(x[e].y)), fmaxf(fabsf(x[e].z), fabsf(x[e].w))));
-                        if ((kv && look) || __any_sync(kAll, mf == INFINITY)) {  // the largest finite magnitude; odd values
-                            bool odd = false;
-                            uint32_t mx = 0;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                float *w = reinterpret_cast<float *>(&x[e]);
-#pragma unroll
-                                for (int u = 0; u < 4; ++u) {
-                                    mx = max(mx, finite_abs(w[u]));
-                                    if (kv && look && !isfinite(w[u])) w[u] = 0.0f, odd = true;
+                                for (int e = 0; e < 4; ++e) {
+                                    const int k = kb + un * UR + (e * 32 + lane) / CR;
+                                    if (k < it.lo || k >= it.hi) x[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                                 }
                             }
-                            mf = __uint_as_float(mx);
-                            if (__any_sync(kAll, odd) && lane == 0) odd8_sh[me][pw] = 1;
-                        }
-                        const int ex = exp_of(__reduce_max_sync(kAll, __float_as_uint(mf)));
-                        if (lane == 0) kv_exp[kt % C::Ring][kv][un] = (int8_t)ex;
-                        const float scale = pow2(14 - ex);
+                            float mf = 0.0f;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int q = e * 32 + lane, r = un * UR + q / CR, c4 = q % CR, c = c4 >> 1;
-                            uint2 hi, lo;
-                            split2(x[e].x * scale, x[e].y * scale, hi.x, lo.x);
-                            split2(x[e].z * scale, x[e].w * scale, hi.y, lo.y);
-                            const uint32_t d = dst + (c >> 3) * (KT * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4) + (c4 & 1) * 8;
-                            sts8(d, hi);
-                            sts8(d + C::PlaneB, lo);
+                            for (int e = 0; e < 4; ++e)
+                                mf = fmaxf(mf, fmaxf(fmaxf(fabsf(x[e].x), fabsf(x[e].y)), fmaxf(fabsf(x[e].z), fabsf(x[e].w))));
+                            uint32_t mx = __reduce_max_sync(kAll, __float_as_uint(mf));
+                            if ((kv && look) || mx == 0x7f800000u) {  // the largest finite magnitude; odd values
+                                bool odd = false;
+                                mx = 0;
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    float *w = reinterpret_cast<float *>(&x[e]);
+#pragma unroll
+                                    for (int u = 0; u < 4; ++u) {
+                                        mx = max(mx, finite_abs(w[u]));
+                                        if (kv && look && !isfinite(w[u])) w[u] = 0.0f, odd = true;
+                                    }
+                                }
+                                mx = __reduce_max_sync(kAll, mx);
+                                if (__any_sync(kAll, odd) && lane == 0) odd8_sh[me][cw] = 1;
+                            }
+                            const int ex = exp_of(mx);
+                            if (lane == 0) kv_exp[kt % C::Ring][kv][un] = (int8_t)ex;
+                            const float scale = pow2(14 - ex);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const int q = e * 32 + lane, r = un * UR + q / CR, c4 = q % CR, c = c4 >> 1;
+                                uint2 hi, lo;
+                                split2(x[e].x * scale, x[e].y * scale, hi.x, lo.x);
+                                split2(x[e].z * scale, x[e].w * scale, hi.y, lo.y);
+                                const uint32_t d = dst + (c >> 3) * (KT * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4) + (c4 & 1) * 8;
+                                sts8(d, hi);
+                                sts8(d + C::PlaneB, lo);
+                            }
+                        }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) {
+                            mbar_arrive(&raw_empty[kv]);
+                            mbar_arrive(&full[s]);
                         }
                     }
-                    if (kv == 0) resolve();
-                    copy(kv);  // the next tile's, into the stage just read
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&full[s]);
+                    ++kt;
                 }
-                ++kt;
-                if (!more) break;
             }
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
         }
         if (!ok) abort_sh = 1;
+        if (pw == 0 && lane == 0) {
+            // every block draws one ticket past the end (after a wait that gave up, here): the last of them resets the count
+            while (drawn < total) drawn = (int)gridDim.x + (int)atomicAdd(f.ticket, 1u);
+            if (blockIdx.x < total && drawn - (int)gridDim.x == total - 1) *f.ticket = 0;
+        }
     } else if (warp == kMmaWarp) {
         // ---- MMA issuer ----
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::RegP));
@@ -772,7 +834,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
             const uint32_t ringk = desc_lo(ring, 16), ringv = desc_lo(ring, KT * 128), q0d = desc_lo(sq, 16);
             bool ok = true;
             for (int round = 0; ok; ++round) {
-                const int item = item_of(round);
+                const int item = announced(round);
                 if (item >= total) break;
                 const Item it = locate<C>(f, sc, item);
                 const int nt = __shfl_sync(kAll, it.t1 - it.t0, 0);
@@ -876,8 +938,19 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
         float2 *ml = reinterpret_cast<float2 *>(qsm + C::MlAt);
         uint32_t job = 0, kt = 0, live = 0, done = 0;
         bool ok = true;
-        for (int round = 0;; ++round) {
-            const int item = item_of(round);
+        // the item is warp 0's to ask for: the groups meet at barriers, so all of them end at the same one
+        int round = 0;
+        auto ask = [&]() {
+            if (warp == 0) {
+                const int next = announced(round);
+                if (lane == 0) item_sh = abort_sh ? INT32_MAX : next;
+            }
+            ++round;
+        };
+        ask();
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        for (;;) {
+            const int item = item_sh;
             if (item >= total) break;
             const Item it = locate<C>(f, sc, item);
             const int nt = it.t1 - it.t0, p0 = it.q.L - it.q.n;
@@ -898,29 +971,44 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                 const uint32_t qd = sq + (it.two ? grp * C::QTileB : 0);
                 // (fp32: both look at all of them, for their exponents)
                 const int e0 = it.two ? 0 : grp * 16, e1 = it.two ? 32 : e0 + 16;
-#pragma unroll 4
-                for (int e = F32 ? 0 : e0; e < (F32 ? 32 : e1); e += RPI) {
-                    const int rl = e + lane / NC, rr = wq * 32 + rl, c = lane % NC;
-                    const int64_t o = __shfl_sync(kAll, qoff, rl);
-                    uint4 v = __ldg(reinterpret_cast<const uint4 *>(static_cast<const char *>(a.q) + o) + c);
-                    if constexpr (F32) {
-                        const float x[4] = {__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w)};
-                        uint32_t mq = max(max(finite_abs(x[0]), finite_abs(x[1])), max(finite_abs(x[2]), finite_abs(x[3])));
+                auto query = [&](int e) {  // rows e ..
+                    const int64_t o = __shfl_sync(kAll, qoff, e + lane / NC);
+                    return __ldg(reinterpret_cast<const uint4 *>(static_cast<const char *>(a.q) + o) + lane % NC);
+                };
+                if constexpr (F32) {
+                    constexpr int B = 8;  // loads in flight
+#pragma unroll 1
+                    for (int eb = 0; eb < 32; eb += B * RPI) {
+                        uint4 v[B];
 #pragma unroll
-                        for (int d = 1; d < NC; d <<= 1) mq = max(mq, __shfl_xor_sync(kAll, mq, d));
-                        const int ex = exp_of(mq);
-                        const int own = __shfl_sync(kAll, ex, (lane - e) * NC & 31);
-                        if (lane >= e && lane < e + RPI) qe = own;
-                        if (e < e0 || e >= e1) continue;
-                        const float s1 = a.scale < 0.0f ? -pow2(14 - ex) : pow2(14 - ex);
-                        uint2 hi, lo;
-                        split2(x[0] * s1, x[1] * s1, hi.x, lo.x);
-                        split2(x[2] * s1, x[3] * s1, hi.y, lo.y);
-                        const int c8 = c >> 1;
-                        const uint32_t dd = qd + (c8 >> 3) * (128 * 128) + rr * 128 + (((c8 & 7) ^ (rr & 7)) << 4) + (c & 1) * 8;
-                        sts8(dd, hi);
-                        sts8(dd + C::QPlaneB, lo);
-                    } else {
+                        for (int i = 0; i < B; ++i) v[i] = query(min(eb + i * RPI, 32 - RPI));
+#pragma unroll
+                        for (int i = 0; i < B; ++i) {
+                            const int e = eb + i * RPI, rr = wq * 32 + e + lane / NC, c = lane % NC;
+                            const float x[4] = {__uint_as_float(v[i].x), __uint_as_float(v[i].y), __uint_as_float(v[i].z), __uint_as_float(v[i].w)};
+                            uint32_t mq = max(max(finite_abs(x[0]), finite_abs(x[1])), max(finite_abs(x[2]), finite_abs(x[3])));
+#pragma unroll
+                            for (int d = 1; d < NC; d <<= 1) mq = max(mq, __shfl_xor_sync(kAll, mq, d));
+                            const int ex = exp_of(mq);
+                            const int own = __shfl_sync(kAll, ex, (lane - e) * NC & 31);
+                            if (lane >= e && lane < e + RPI) qe = own;
+                            if (e >= e0 && e < e1) {
+                                const float s1 = a.scale < 0.0f ? -pow2(14 - ex) : pow2(14 - ex);
+                                uint2 hi, lo;
+                                split2(x[0] * s1, x[1] * s1, hi.x, lo.x);
+                                split2(x[2] * s1, x[3] * s1, hi.y, lo.y);
+                                const int c8 = c >> 1;
+                                const uint32_t dd = qd + (c8 >> 3) * (128 * 128) + rr * 128 + (((c8 & 7) ^ (rr & 7)) << 4) + (c & 1) * 8;
+                                sts8(dd, hi);
+                                sts8(dd + C::QPlaneB, lo);
+                            }
+                        }
+                    }
+                } else {
+#pragma unroll 4
+                    for (int e = e0; e < e1; e += RPI) {
+                        const int rr = wq * 32 + e + lane / NC, c = lane % NC;
+                        uint4 v = query(e);
                         v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
                         sts16(qd + (c >> 3) * (128 * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4), v);
                     }
@@ -1112,7 +1200,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
             if (nt > 0) {
                 if constexpr (F32) {
 #pragma unroll
-                    for (int e = 0; e < C::Producers; ++e) odd = odd || odd8_sh[live % C::Ring][e] != 0;
+                    for (int e = 0; e < C::Converters; ++e) odd = odd || odd8_sh[live % C::Ring][e] != 0;
                 } else {
                     odd = odd_sh[live % C::Ring] != 0;
                 }
@@ -1182,9 +1270,9 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                 }
             }
             if (it.nsplit > 1) {  // the same barriers on every path
-                __threadfence();
                 asm volatile("bar.sync 1, 256;" ::: "memory");
                 if (tid == 0) {
+                    __threadfence();  // the block's rows are ordered before its arrival
                     last_sh = 0;
                     if (room) {
                         uint32_t *cnt = f.cnt + it.slot;
@@ -1243,11 +1331,10 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                 }
             }
             // the next item's queries overwrite the staged outputs, and its first products O
-            if (tid == 0) stop_sh = abort_sh;
+            ask();
             tc_fence_before();
             asm volatile("bar.sync 1, 256;" ::: "memory");
             tc_fence_after();
-            if (stop_sh) break;
             if (nt > 0) {
                 if (!F32 && tid == 0) odd_sh[live % C::Ring] = 0;
                 ++live;
@@ -1263,23 +1350,25 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
     }
 }
 
-// [pages][heads][positions][channels] of a pool as it lies, boxes of `run` positions x 64 channels
+// [pages][heads][positions][channels] of a pool as it lies, boxes of `run` positions x 64 channels (fp32: all)
 bool pool_map(CUtensorMap *m, const altxs_paged_kv &kv, void *pool, int run) {
     const auto enc = encoder();
     if (!enc) return false;
     const cuuint64_t dims[4] = {(cuuint64_t)kv.head_dim, (cuuint64_t)kv.page_size, (cuuint64_t)kv.n_kv_heads,
                                 (cuuint64_t)std::max(kv.n_pages, 1)};
-    const cuuint64_t strides[3] = {(cuuint64_t)kv.token_stride * 2, (cuuint64_t)kv.head_stride * 2, (cuuint64_t)kv.page_stride * 2};
-    const cuuint32_t box[4] = {64, (cuuint32_t)run, 1, 1}, es[4] = {1, 1, 1, 1};
-    return enc(m, kv.dtype == ALTXS_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, pool, dims, strides,
-               box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    const bool f32 = kv.dtype == ALTXS_F32;
+    const cuuint64_t b = f32 ? 4 : 2;
+    const cuuint64_t strides[3] = {(cuuint64_t)kv.token_stride * b, (cuuint64_t)kv.head_stride * b, (cuuint64_t)kv.page_stride * b};
+    const cuuint32_t box[4] = {f32 ? (cuuint32_t)kv.head_dim : 64, (cuuint32_t)run, 1, 1}, es[4] = {1, 1, 1, 1};
+    return enc(m, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : kv.dtype == ALTXS_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+               4, pool, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, f32 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <typename T, int HD>
 int launch(const ManyArgs &f, unsigned grid, cudaStream_t st) {
     CUtensorMap tk{}, tv{};
-    if (sizeof(T) == 2 && (!pool_map(&tk, f.a.kv, f.a.kv.k, f.run) || !pool_map(&tv, f.a.kv, f.a.kv.v, f.run))) return ALTXS_ECUDA;
+    if ((!pool_map(&tk, f.a.kv, f.a.kv.k, f.run) || !pool_map(&tv, f.a.kv, f.a.kv.v, f.run))) return ALTXS_ECUDA;
     static std::atomic<uint64_t> set{0};  // devices whose shared-memory limit is raised
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return ALTXS_ECUDA;
@@ -1315,8 +1404,8 @@ ManyPlan paged_many_plan(const altxs_paged_kv &kv, const altxs_chunks &c, int H,
 
 int launch_paged_many(const PagedAttnArgs &a, const ManyPlan &p, int min_rows, uint32_t *cnt, float *part, int sms,
                       cudaStream_t st) {
-    const int run = std::min(128, a.kv.page_size & -a.kv.page_size);
-    const ManyArgs f{a, a.H / a.kv.n_kv_heads, min_rows, run < 4 ? 1 : run, p.slots, cnt, part, p.rows};
+    const int run = std::min(tile_keys(a.kv.dtype, a.kv.head_dim), a.kv.page_size & -a.kv.page_size);
+    const ManyArgs f{a, a.H / a.kv.n_kv_heads, min_rows, run < 4 ? 1 : run, p.slots, cnt + 1, cnt, part, p.rows};
     const unsigned grid = (unsigned)std::min<int64_t>(p.items, sms);
     if (a.kv.dtype == ALTXS_F32) return launch<float>(f, grid, st);
     return a.kv.dtype == ALTXS_BF16 ? launch<__nv_bfloat16>(f, grid, st) : launch<__half>(f, grid, st);
