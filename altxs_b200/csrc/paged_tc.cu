@@ -1005,7 +1005,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                         }
                     }
                 } else {
-#pragma unroll 4
+#pragma unroll 8
                     for (int e = e0; e < e1; e += RPI) {
                         const int rr = wq * 32 + e + lane / NC, c = lane % NC;
                         uint4 v = query(e);
@@ -1207,6 +1207,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
             }
             const bool whole_ok = !abort_sh;
             float *pp = f.part + (int64_t)(it.slot + it.split) * f.part_rows * (HD + 2);
+            const int64_t ooff = (int64_t)(it.q.q0 + tok) * a.ldo + (int64_t)h * HD;
 #pragma unroll 1
             for (int c = 0; c < HD; c += 32) {
                 float v[32];
@@ -1228,33 +1229,46 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                 for (int i = 0; i < 8; ++i)  // 128-byte rows, swizzled like the tiles
                     *reinterpret_cast<float4 *>(stage + slot * 32 + ((i ^ (slot & 7)) << 2)) =
                         make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-                // Rows of one set are the warp's own; shared ones meet in the block.
+                // Rows of one set are the warp's own; shared ones meet in the block.  Then four lanes a row, eight
+                // channels each.
                 if (it.two) __syncwarp();
                 else asm volatile("bar.sync 1, 256;" ::: "memory");
-                const int i1 = it.two ? min(it.rows, (warp + 1) * 32) * 8 : min(rrows, it.rows) * 8;
-                for (int i = it.two ? warp * 256 + lane : tid; i < i1; i += it.two ? 32 : 256) {  // row i / 8, channels c + 4 (i % 8) ..
-                    const int ro = i >> 3, q = i & 7;
-                    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                const int rend = it.two ? min(it.rows, (warp + 1) * 32) : min(rrows, it.rows), step = it.two ? 8 : 64;
+#pragma unroll 1
+                for (int rq = it.two ? warp * 32 : warp * 8; rq < rend; rq += step) {
+                    const int ro = rq + (lane >> 2), q = (lane & 3) * 2, ch = c + 4 * q;
+                    float y[8] = {};
+#pragma unroll 1
                     for (int s = 0; s < sets; ++s) {
                         const int at = s * rrows + ro;
-                        const float4 u = *reinterpret_cast<const float4 *>(stage + at * 32 + ((q ^ (at & 7)) << 2));
-                        y.x = __fadd_rn(y.x, u.x), y.y = __fadd_rn(y.y, u.y), y.z = __fadd_rn(y.z, u.z), y.w = __fadd_rn(y.w, u.w);
-                    }
-                    const int rr = it.r0 + ro, tk = rr / f.G, ch = c + 4 * q;
-                    if (odd) {  // what is not finite replaces the sum that it was kept out of
-                        float *w = reinterpret_cast<float *>(&y);
-                        for (int e = 0; e < 4; ++e) {
-                            const float t = odd_term<T>(a, it.s, it.g, p0 + tk, max(it.lo, it.base + it.t0 * KT), it.base + it.t1 * KT, ch + e);
-                            if (t != 0.0f) w[e] = t;
+#pragma unroll
+                        for (int d = 0; d < 2; ++d) {
+                            const float4 u = *reinterpret_cast<const float4 *>(stage + (at & 255) * 32 + (((q + d) ^ (at & 7)) << 2));
+                            y[4 * d] = __fadd_rn(y[4 * d], u.x), y[4 * d + 1] = __fadd_rn(y[4 * d + 1], u.y);
+                            y[4 * d + 2] = __fadd_rn(y[4 * d + 2], u.z), y[4 * d + 3] = __fadd_rn(y[4 * d + 3], u.w);
                         }
                     }
-                    if (!whole_ok) continue;
+                    // the row's output: this warp's lanes hold its rows' places, else it is worked out again
+                    int64_t o = __shfl_sync(kAll, ooff, ro & 31);
+                    if (!it.two) {
+                        const int rr = it.r0 + ro, tk = rr / f.G;
+                        o = (int64_t)(it.q.q0 + tk) * a.ldo + (int64_t)(it.g * f.G + rr - tk * f.G) * HD;
+                    }
+                    if (ro >= rend || !whole_ok) continue;
+                    if (odd) {  // what is not finite replaces the sum that it was kept out of
+#pragma unroll 1
+                        for (int e = 0; e < 8; ++e) {
+                            const float t = odd_term<T>(a, it.s, it.g, p0 + (it.r0 + ro) / f.G, max(it.lo, it.base + it.t0 * KT), it.base + it.t1 * KT, ch + e);
+#pragma unroll
+                            for (int d = 0; d < 8; ++d)
+                                if (d == e && t != 0.0f) y[d] = t;
+                        }
+                    }
                     if (fin) {
-                        T *yp = static_cast<T *>(a.out) + (int64_t)(it.q.q0 + tk) * a.ldo + (int64_t)(it.g * f.G + rr - tk * f.G) * HD + ch;
-                        if constexpr (F32) *reinterpret_cast<float4 *>(yp) = y;
-                        else *reinterpret_cast<uint2 *>(yp) = make_uint2(pack2<T>(y.x, y.y), pack2<T>(y.z, y.w));
+                        store8<T>(static_cast<T *>(a.out) + o + ch, y);
                     } else if (room) {
-                        __stcg(reinterpret_cast<float4 *>(pp + (int64_t)ro * HD + ch), y);
+                        __stcg(reinterpret_cast<float4 *>(pp + (int64_t)ro * HD + ch), make_float4(y[0], y[1], y[2], y[3]));
+                        __stcg(reinterpret_cast<float4 *>(pp + (int64_t)ro * HD + ch + 4), make_float4(y[4], y[5], y[6], y[7]));
                     }
                 }
                 if (it.two) __syncwarp();
