@@ -81,7 +81,8 @@ def _raise_status(word: torch.Tensor, what: str) -> None:
     v = int(word.item())
     if v:
         word.zero_()
-        raise RuntimeError(f"{what}: device status {v:#x} (position, page or length out of range)")
+        why = "a device wait gave up" if v & _lib.ST_TIMEOUT else "position, page or length out of range"
+        raise RuntimeError(f"{what}: device status {v:#x} ({why})")
 
 
 class Rotary:
@@ -280,8 +281,12 @@ class PagedKV:
         return (out, lse) if return_lse else out
 
     def check_status(self) -> None:
-        """Waits; raises if a call met a position, page or length out of range."""
-        _raise_status(self.status, "paged cache")
+        """Waits; raises if a call met a position, page or length out of range, or gave up waiting."""
+        try:
+            _raise_status(self.status, "paged cache")
+        except RuntimeError:
+            self._ws.clear()  # a call that gave up may leave its counters counting: later calls start from zeroed ones
+            raise
 
 
 class PageAllocator:
