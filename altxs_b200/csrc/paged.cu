@@ -338,10 +338,14 @@ int check_kv(const altxs_paged_kv &kv) {
     if (kv.page_stride < 0 || kv.token_stride < kv.head_dim || kv.head_stride < kv.head_dim) return ALTXS_EINVAL;
     return ALTXS_OK;
 }
+constexpr int kMaxLength = 1 << 30;  // positions of a sequence: their sums with windows and tiles stay in 32 bits
+// a window that covers every position is none
+int window_of(const altxs_chunks &c, int window) { return window >= c.max_kv ? 0 : window; }
 int check_chunks(const altxs_paged_kv &kv, const altxs_chunks &c) {
     if (c.n_seqs < 0 || c.n_tokens < 0 || c.max_new < 0 || c.max_kv < 0 || c.table_stride < 0 || c.total_kv < 0)
         return ALTXS_EINVAL;
-    return c.table_stride * kv.page_size < c.max_kv ? ALTXS_EINVAL : ALTXS_OK;
+    if (c.table_stride * kv.page_size < c.max_kv) return ALTXS_EINVAL;
+    return c.max_kv > kMaxLength || c.max_new > kMaxLength ? ALTXS_ENOTSUP : ALTXS_OK;
 }
 
 }  // namespace
@@ -410,7 +414,7 @@ int64_t altxs_paged_attention_workspace_bytes(const altxs_paged_kv *kv, const al
                                               int window) {
     if (!kv || !c || check_kv(*kv) || check_chunks(*kv, *c) || n_heads < 1 || n_heads % kv->n_kv_heads || window < 0)
         return -1;
-    return paged_attention_ws(*kv, *c, n_heads, window);
+    return paged_attention_ws(*kv, *c, n_heads, window_of(*c, window));
 }
 
 int altxs_paged_attention(const altxs_paged_kv *kv, const altxs_chunks *c, int n_heads, float scale, int window,
@@ -424,6 +428,7 @@ int altxs_paged_attention(const altxs_paged_kv *kv, const altxs_chunks *c, int n
     if (ldq < width || ldo < width || ldq % u || ldo % u || !aligned16(q) || !aligned16(out)) return ALTXS_EINVAL;
     if (c->n_seqs == 0 || c->n_tokens == 0) return ALTXS_OK;
     if (!q || !out || !kv->k || !kv->v || !c->q_start || !c->kv_len || !c->page_table) return ALTXS_EINVAL;
+    window = window_of(*c, window);
     const int64_t need = paged_attention_ws(*kv, *c, n_heads, window);
     if (workspace_bytes < need || (need > 0 && !workspace) || !aligned16(workspace)) return ALTXS_ENOSPC;
     return launch_paged_attention(PagedAttnArgs{*kv, *c, n_heads, window, scale, q, ldq, out, ldo, lse, workspace,

@@ -244,7 +244,7 @@ __device__ __forceinline__ void finish_item(const FewArgs &f, int item, const Wh
             for (int e = 0; e < 4; ++e) out.e[e] = from_f<T>(__fmul_rn(y[e], inv));
             *reinterpret_cast<Vec<T, 4> *>(static_cast<T *>(a.out) + (int64_t)tok * a.ldo + (int64_t)h * HD + c) = out;
             if (a.lse && c == 0)
-                a.lse[(int64_t)h * a.c.n_tokens + tok] = M == -INFINITY ? -INFINITY : __fadd_rn(M, log2f(lt));
+                a.lse[(int64_t)h * a.c.n_tokens + tok] = lt == 0.0f ? -INFINITY : __fadd_rn(M, log2f(lt));
         } else if (item < f.max_items) {
             float *p = f.part + ((int64_t)item * f.part_rows + r) * (HD + 4);
             __stcg(reinterpret_cast<float4 *>(p + c), make_float4(y[0], y[1], y[2], y[3]));
@@ -286,7 +286,7 @@ __device__ __forceinline__ void finish_item(const FewArgs &f, int item, const Wh
         ms[nsplit * R + r] = M == -INFINITY ? 0.0f : __frcp_rn(lt);
         if (a.lse)
             a.lse[(int64_t)(g * G + (r0 + r) % G) * a.c.n_tokens + q.q0 + (r0 + r) / G] =
-                M == -INFINITY ? -INFINITY : __fadd_rn(M, log2f(lt));
+                lt == 0.0f ? -INFINITY : __fadd_rn(M, log2f(lt));
     }
     __syncthreads();
     for (int i = threadIdx.x; i < R * (HD / 4); i += blockDim.x) {
@@ -688,10 +688,11 @@ Plan plan_of(const altxs_paged_kv &kv, const altxs_chunks &c, int H, int window)
     Plan p{};
     const int G = H / kv.n_kv_heads;
     const int64_t n = c.n_seqs;
-    if (n == 0 || c.max_new == 0) return p;
-    const bool same = c.n_tokens == n * c.max_new;  // every sequence has max_new tokens
-    p.many = (int64_t)c.max_new * G > kMaxRows;
-    const int64_t least = same ? (int64_t)c.max_new * G : G, most = (int64_t)c.max_new * G;  // rows of a sequence
+    if (n == 0) return p;
+    const int64_t max_new = std::max(c.max_new, 1);  // (sequences above a bound of 0 are the kernels' to report)
+    const bool same = c.n_tokens == n * max_new;     // every sequence has max_new tokens
+    p.many = max_new * G > kMaxRows;
+    const int64_t least = same ? max_new * G : G, most = max_new * G;  // rows of a sequence
     p.few = least <= kMaxRows;
     p.group = kv.dtype == ALTXS_F32 ? kVecRows : kMaxRows;
     p.groups = (int)((std::min<int64_t>(kMaxRows, most) + p.group - 1) / p.group);

@@ -53,7 +53,7 @@ namespace {
 
 constexpr int kMmaWarp = 8;
 constexpr int kScan = 64;        // sequences are counted in this many groups
-constexpr int kCached = 40;       // up to this many sequences' shares are kept in shared memory
+constexpr int kCached = 32;       // up to this many sequences' shares are kept in shared memory
 constexpr int kMostItems = 1184;  // splits of one sequence
 constexpr int kMostSplits = 16;
 constexpr int kNext = 4;           // items announced to a block's roles ahead
@@ -79,7 +79,9 @@ struct Tc {
     static constexpr int Slots = F32 ? 3 : HD > 64 ? 5 : 11;
     static constexpr int UnitRows = F32 ? 512 / HD : KT, Units = KT / UnitRows;  // fp32: rows that share an exponent
     static constexpr int StageB = F32 ? KT * HD * 4 : 0;  // fp32: a tile's raw rows, one stage for keys and one for values
-    static constexpr int Ring = Slots > 8 ? 16 : 8;  // key tiles (and items) the producers are ahead of the softmax, at most
+    // Key tiles (and items) the producers are ahead of the softmax, at most.  fp32: while the oldest tile's values
+    // keep their slot, the next tile is in the slots, one more in the stages and the masks of the one after it known.
+    static constexpr int Ring = F32 ? 4 : Slots > 8 ? 16 : 8;
     static constexpr int QB = Rows / 128 * QTileB;
     static constexpr int MlAt = QB > 32768 ? 32768 : QB + Slots * TileB;  // 256 (m, l): see the softmax warps
     static constexpr int Smem = QB + Slots * TileB + 2 * StageB + (QB > 32768 ? 0 : 2048) + 1024;
@@ -323,6 +325,17 @@ __device__ __forceinline__ void tc_ld32_nowait(uint32_t taddr, float *f) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r[i]);
 }
+__device__ __forceinline__ void tc_ld16(uint32_t taddr, float *f) {
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr) : "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(r[i]);
+}
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_tie32(float *f) {
 #pragma unroll
@@ -349,12 +362,18 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t 
     hi = *reinterpret_cast<const uint32_t *>(&h);
     lo = *reinterpret_cast<const uint32_t *>(&l);
 }
-// Exponent e of the largest finite magnitude (its bits), within +-100: 2^(14 - e) scales it to 2^14 ..
-__device__ __forceinline__ int exp_of(uint32_t bits) { return min(max((int)(bits >> 23) - 127, -100), 100); }
+// Exponent e of the largest finite magnitude (its bits), -100 at least: 2^(14 - e) scales it to 2^14 ..
+__device__ __forceinline__ int exp_of(uint32_t bits) { return max((int)(bits >> 23) - 127, -100); }
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((127 + e) << 23); }
 __device__ __forceinline__ uint32_t finite_abs(float x) {
     const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
     return b < 0x7f800000u ? b : 0u;
+}
+
+// Exponents travel as the bytes of fp32's exponent field: keys' of 2^(e - 14), values' of 2^(e - kVal).
+constexpr int kVal = 12;
+__device__ __forceinline__ float pow2_byte(uint32_t word, int i) {  // of byte i
+    return __uint_as_float((i == 0 ? word << 23 : i == 1 ? word << 15 : i == 2 ? word << 7 : word >> 1) & 0x7f800000u);
 }
 
 // two fp32 operations per instruction
@@ -369,6 +388,13 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     float2 d;
     asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n"
         " add.rn.f32x2 d, a, b;\n mov.b64 {%0, %1}, d;\n}\n"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n"
+        " mul.rn.f32x2 d, a, b;\n mov.b64 {%0, %1}, d;\n}\n"
         : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
 }
@@ -398,9 +424,11 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
     __shared__ __align__(8) uint64_t full[C::Slots], empty[C::Slots], landed[F32 ? 1 : C::Slots], s_full[2], p_full[2], o_done[2], q_full, drainb,
         raw_full[2], raw_empty[2], next_full[kNext], next_empty[kNext];
     __shared__ Scan sc;
-    // by key tile: which positions exist (4 to a byte), and (fp32) the exponents of its units of keys and of values
+    // by key tile: which positions exist (4 to a byte), and (fp32) the exponents of its positions' keys and values.
+    // Two tiles of those do: a tile's are written once the values' slot of the tile two before is free.
     __shared__ __align__(16) uint8_t kmask[C::Ring][KT / 4];
-    __shared__ __align__(16) int8_t kv_exp[F32 ? C::Ring : 1][2][16];
+    __shared__ __align__(16) uint8_t kv_exp[F32 ? 2 : 1][2][F32 ? KT : 16];
+    static_assert(!F32 || C::Slots <= 3, "exponents of two tiles");
     __shared__ uint32_t tmem_sh;
     __shared__ __align__(8) uint8_t odd8_sh[F32 ? C::Ring : 1][8];  // by item: values that are not finite were set to 0 (fp32: per warp)
     __shared__ uint32_t odd_sh[F32 ? 1 : C::Ring];
@@ -697,7 +725,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                                 if (lane < issue)
                                     tma_load_4d(raw + kv * C::StageB + (e * 32 + lane) * run * HD * 4, map, 0, pos_in[e], g, pg[e], &raw_full[kv]);
                             }
-                                                    }
+                        }
                         if (!ok) break;
                     }
                     have = more;
@@ -729,8 +757,10 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                     if (sent[kv] > 0) mbar_wait_bounded(&raw_full[kv], (sent[kv] - 1) & 1, kWaitLimit);
             } else {
                 // Units of 2 KB (UR rows), 16-byte pieces; warp cw takes units cw, cw + 6, ..: find the unit's
-                // largest magnitude, write the scaled planes.  (Loops are left rolled: with everything
-                // unrolled the block's roles miss the instruction cache.)
+                // largest magnitude, write the scaled planes.  Where some rows of the block do not see the whole
+                // tile, every position has its own exponent: what a row does not see must not set the scale of
+                // what it sees.  (Loops are left rolled: with everything unrolled the block's roles miss the
+                // instruction cache.)
                 constexpr int CR = HD / 4, UR = C::UnitRows, Units = C::Units;
                 const int cw = pw - 1;
                 uint32_t me = 0;
@@ -769,30 +799,42 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                             for (int e = 0; e < 4; ++e)
                                 mf = fmaxf(mf, fmaxf(fmaxf(fabsf(x[e].x), fabsf(x[e].y)), fmaxf(fabsf(x[e].z), fabsf(x[e].w))));
                             uint32_t mx = __reduce_max_sync(kAll, __float_as_uint(mf));
-                            if ((kv && look) || mx == 0x7f800000u) {  // the largest finite magnitude; odd values
+                            uint8_t *exps = kv_exp[kt & 1][kv] + un * UR;
+                            const int bias = 127 - (kv ? kVal : 14);
+                            float scale[4];
+                            if (look || mx == 0x7f800000u) {  // finite magnitudes alone; odd values; by row
                                 bool odd = false;
-                                mx = 0;
+                                uint32_t me4[4] = {};
 #pragma unroll
                                 for (int e = 0; e < 4; ++e) {
                                     float *w = reinterpret_cast<float *>(&x[e]);
 #pragma unroll
                                     for (int u = 0; u < 4; ++u) {
-                                        mx = max(mx, finite_abs(w[u]));
+                                        me4[e] = max(me4[e], finite_abs(w[u]));
                                         if (kv && look && !isfinite(w[u])) w[u] = 0.0f, odd = true;
                                     }
                                 }
-                                mx = __reduce_max_sync(kAll, mx);
+                                if (!look) me4[0] = me4[1] = me4[2] = me4[3] = __reduce_max_sync(kAll, max(max(me4[0], me4[1]), max(me4[2], me4[3])));
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+#pragma unroll
+                                    for (int d = 1; d < CR; d <<= 1) me4[e] = max(me4[e], __shfl_xor_sync(kAll, me4[e], d));
+                                    const int ex = exp_of(me4[e]);
+                                    scale[e] = pow2(14 - ex);
+                                    if (lane % CR == 0) exps[(e * 32 + lane) / CR] = (uint8_t)(ex + bias);
+                                }
                                 if (__any_sync(kAll, odd) && lane == 0) odd8_sh[me][cw] = 1;
+                            } else {
+                                const int ex = exp_of(mx);
+                                scale[0] = scale[1] = scale[2] = scale[3] = pow2(14 - ex);
+                                if (lane < UR) exps[lane] = (uint8_t)(ex + bias);
                             }
-                            const int ex = exp_of(mx);
-                            if (lane == 0) kv_exp[kt % C::Ring][kv][un] = (int8_t)ex;
-                            const float scale = pow2(14 - ex);
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
                                 const int q = e * 32 + lane, r = un * UR + q / CR, c4 = q % CR, c = c4 >> 1;
                                 uint2 hi, lo;
-                                split2(x[e].x * scale, x[e].y * scale, hi.x, lo.x);
-                                split2(x[e].z * scale, x[e].w * scale, hi.y, lo.y);
+                                split2(x[e].x * scale[e], x[e].y * scale[e], hi.x, lo.x);
+                                split2(x[e].z * scale[e], x[e].w * scale[e], hi.y, lo.y);
                                 const uint32_t d = dst + (c >> 3) * (KT * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4) + (c4 & 1) * 8;
                                 sts8(d, hi);
                                 sts8(d + C::PlaneB, lo);
@@ -1018,7 +1060,9 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                 if (lane == 0) mbar_arrive(&q_full);
                 // positions that all of this warp's rows see: from its first row's and its last row's
                 const int ra = it.r0 + min(r_own - lane, it.rows - 1), rb = it.r0 + min(r_own - lane + 31, it.rows - 1);
-                const int pa = p0 + ra / f.G, pb = p0 + rb / f.G;
+                int pa = p0 + ra / f.G, pb = p0 + rb / f.G;
+                // fp32: from the block's, whose other tiles have an exponent for every position
+                if (F32) pa = p0 + it.r0 / f.G, pb = p0 + (it.r0 + it.rows - 1) / f.G;
 
                 auto tile = [&](auto rep_c, int j) -> bool {
                     constexpr int REP = decltype(rep_c)::value, W = KT / REP;  // columns of this thread's share
@@ -1026,22 +1070,72 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                     const int kb = it.base + (it.t0 + j) * KT + c0;
                     if (!__all_sync(kAll, !abort_sh && mbar_wait_bounded(&s_full[grp], job & 1, limit))) return false;
                     tc_fence_after();
-                    float x[W];
-#pragma unroll
-                    for (int c = 0; c < W; c += 32) tc_ld32_nowait(ts + c0 + c, x + c);
-                    uint32_t km[W / 16];  // 4 positions to a byte
-                    const uint32_t *kmp = reinterpret_cast<const uint32_t *>(kmask[(kt + j) % C::Ring]) + c0 / 16;
-#pragma unroll
-                    for (int c = 0; c < W / 16; ++c) km[c] = kmp[c];
-                    tc_wait_ld();
-#pragma unroll
-                    for (int c = 0; c < W; c += 32) tc_tie32(x + c);
+                    // positions that exist, 4 to a byte; what all the warp's rows see
+                    const uint32_t *km = reinterpret_cast<const uint32_t *>(kmask[(kt + j) % C::Ring]) + c0 / 16;
                     uint32_t have = 0x0f0f0f0fu;
 #pragma unroll
                     for (int c = 0; c < W / 16; ++c) have &= km[c];
-                    const bool whole = kb + W <= pa + 1 && (a.window == 0 || kb > pb - a.window) && have == 0x0f0f0f0fu;
-                    if (!whole) {
-                        const int first = a.window > 0 ? max(0, pos - a.window + 1 - kb) : 0, last = pos - kb;
+                    const int ka = F32 ? kb - c0 : kb, kw = F32 ? KT : W;  // fp32: the whole tile
+                    const bool whole = ka + kw <= pa + 1 && (a.window == 0 || ka > pb - a.window) && have == 0x0f0f0f0fu;
+                    const uint8_t *ke = kv_exp[F32 ? (kt + j) & 1 : 0][0] + (F32 ? c0 : 0), *vx = kv_exp[F32 ? (kt + j) & 1 : 0][1] + (F32 ? c0 : 0);
+                    const float cq = F32 ? __fmul_rn(c2, pow2(qe - 14)) : c2;
+                    uint32_t top = 0;  // fp32: byte of the largest exponent of the values that the row sees
+                    if constexpr (F32) {
+                        const uint32_t v = 2 * (kt + j) + 1;  // the values' slot: their exponents come with them
+                        if (!__all_sync(kAll, mbar_wait_bounded(&full[v % C::Slots], (v / C::Slots) & 1, limit))) return false;
+                    }
+                    const int first = a.window > 0 ? max(0, pos - a.window + 1 - kb) : 0, last = pos - kb;
+                    if (F32 && !whole) {
+                        // Scaled, every position by its own, and masked where they lie, 16 columns at a time: such
+                        // tiles are few, and unrolled over the registers this came from beyond the instruction
+                        // cache each time (encoder windows 98 us where this takes 89).
+#pragma unroll 1
+                        for (int c = 0; c < W; c += 16) {
+                            float y[16];
+                            tc_ld16(ts + c0 + c, y);
+                            const uint32_t k = km[c / 16];
+                            uint32_t see = (k & 15) | (k >> 4 & 0xf0) | (k >> 8 & 0xf00) | (k >> 12 & 0xf000);
+                            const int f0 = first - c, l0 = last - c;  // of [0, 15]
+                            see &= f0 >= 16 ? 0u : f0 <= 0 ? kAll : kAll << f0;
+                            see &= l0 < 0 ? 0u : l0 >= 15 ? kAll : kAll >> (31 - l0);
+#pragma unroll
+                            for (int u = 0; u < 16; u += 4) {
+                                const uint32_t kx = *reinterpret_cast<const uint32_t *>(ke + c + u);
+#pragma unroll
+                                for (int d = 0; d < 4; ++d) y[u + d] = __fmul_rn(y[u + d], __fmul_rn(cq, pow2_byte(kx, d)));
+                                const uint32_t vw = *reinterpret_cast<const uint32_t *>(vx + c + u) &
+                                                    (((see >> u & 15) * 0x00204081u & 0x01010101u) * 255u);
+                                top = __vmaxu2(top, __vmaxu2(vw & 0x00ff00ffu, vw >> 8 & 0x00ff00ffu));
+                            }
+                            uint32_t w[16];
+#pragma unroll
+                            for (int u = 0; u < 16; ++u) w[u] = see & (1u << u) ? __float_as_uint(y[u]) : 0xff800000u;
+                            tc_st16(ts + c0 + c, w);
+                        }
+                        tc_wait_st();
+                        top = max(top & 0xffffu, top >> 16);
+                    }
+                    float x[W];
+#pragma unroll
+                    for (int c = 0; c < W; c += 32) tc_ld32_nowait(ts + c0 + c, x + c);
+                    // columns that share a scale, and their factors to log2 units (fp32: times the row's and the unit's)
+                    constexpr int UC = F32 ? C::UnitRows : W, NU = W / UC;
+                    float cf[NU];
+#pragma unroll
+                    for (int i = 0; i < NU; ++i) cf[i] = !F32 ? c2 : whole ? fmaxf(__fmul_rn(cq, pow2_byte(ke[i * UC], 0)), 1.17549435e-38f) : 1.0f;
+                    int vt = -100;  // fp32: the values' exponent
+                    if constexpr (F32) {
+                        if (whole)
+#pragma unroll
+                            for (int i = 0; i < NU; ++i) top = max(top, (uint32_t)vx[i * UC]);
+                        vt = max(vt, (int)top - (127 - kVal));
+                        vt = njob == 0 ? vt : max(ve, vt);
+                        if (njob == 0) ve = vt;
+                    }
+                    tc_wait_ld();
+#pragma unroll
+                    for (int c = 0; c < W; c += 32) tc_tie32(x + c);
+                    if (!F32 && !whole) {
 #pragma unroll
                         for (int c = 0; c < W; c += 32) {  // bit u: column c + u is seen
                             uint32_t bits = 0;
@@ -1057,26 +1151,6 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                             for (int u = 0; u < 32; ++u)
                                 if (!(bits & (1u << u))) x[c + u] = -INFINITY;
                         }
-                    }
-                    // columns that share a scale, and their factors to log2 units (fp32: times the row's and the unit's)
-                    constexpr int UC = F32 ? C::UnitRows : W, NU = W / UC;
-                    float cf[NU], pf[NU];
-                    int vt = -100;  // fp32: exponent of this tile's values
-                    if constexpr (F32) {
-                        const float cq = __fmul_rn(c2, pow2(qe - 14));
-                        const int8_t *ke = kv_exp[(kt + j) % C::Ring][0] + c0 / UC, *vx = kv_exp[(kt + j) % C::Ring][1] + c0 / UC;
-#pragma unroll
-                        for (int i = 0; i < NU; ++i) cf[i] = fmaxf(__fmul_rn(cq, pow2(ke[i] - 14)), 1.17549435e-38f);
-                        const uint32_t v = 2 * (kt + j) + 1;  // the values' slot: their exponents come with them
-                        if (!__all_sync(kAll, mbar_wait_bounded(&full[v % C::Slots], (v / C::Slots) & 1, limit))) return false;
-#pragma unroll
-                        for (int i = 0; i < NU; ++i) vt = max(vt, (int)vx[i]);
-                        vt = njob == 0 ? vt : max(ve, vt);
-#pragma unroll
-                        for (int i = 0; i < NU; ++i) pf[i] = pow2(max(vx[i] - vt, -126));
-                        if (njob == 0) ve = vt;
-                    } else {
-                        cf[0] = c2;
                     }
                     float mx = -INFINITY;
                     if constexpr (F32) {
@@ -1126,18 +1200,24 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                     }
                     const float base = m == -INFINITY ? 0.0f : __fsub_rn(m, kBias);
                     const float2 nb2 = make_float2(-base, -base);
+                    const float rs = F32 ? pow2(kVal - vt) : 1.0f;  // fp32: p in the units of its row's values
                     float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
                     for (int c = 0; c < W; c += 32) {
-                        uint32_t w[16], wl[F32 ? 16 : 1];
+                        uint32_t w[16], wl[F32 ? 16 : 1], vw = 0;
 #pragma unroll
                         for (int u = 0; u < 32; u += 2) {
                             const int un = (c + u) / UC;
                             const float2 t = fma2(make_float2(x[c + u], x[c + u + 1]), make_float2(cf[un], cf[un]), nb2);
                             float2 e = make_float2(ex2(t.x), ex2(t.y));
                             sum[u / 2 & 1] = add2(sum[u / 2 & 1], e);
-                            if constexpr (F32) split2(e.x * pf[un], e.y * pf[un], w[u / 2], wl[u / 2]);
-                            else w[u / 2] = pack2<T>(e.x, e.y);
+                            if constexpr (F32) {
+                                if (u % 4 == 0) vw = *reinterpret_cast<const uint32_t *>(vx + c + u);
+                                e = mul2(mul2(e, make_float2(rs, rs)), make_float2(pow2_byte(vw, u % 4), pow2_byte(vw, u % 4 + 1)));
+                                split2(e.x, e.y, w[u / 2], wl[u / 2]);
+                            } else {
+                                w[u / 2] = pack2<T>(e.x, e.y);
+                            }
                         }
                         tc_st16(ts + (c0 + c) / 2, w);
                         if constexpr (F32) tc_st16(ts + KT / 2 + (c0 + c) / 2, wl);
@@ -1276,7 +1356,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
             }
             if (set == 0 && r_own < it.rows && whole_ok) {
                 if (fin) {
-                    if (a.lse) a.lse[(int64_t)h * a.c.n_tokens + it.q.q0 + tok] = M == -INFINITY ? -INFINITY : __fadd_rn(M, __fsub_rn(log2f(lt), kBias));
+                    if (a.lse) a.lse[(int64_t)h * a.c.n_tokens + it.q.q0 + tok] = lt == 0.0f ? -INFINITY : __fadd_rn(M, __fsub_rn(log2f(lt), kBias));
                 } else if (room) {
                     __stcg(reinterpret_cast<float2 *>(pp + (int64_t)HD * f.part_rows) + r_own, make_float2(M, lt));
                 } else if (r_own == 0) {  // the lengths are above their bounds
@@ -1318,7 +1398,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                         const int rr = it.r0 + tid, tk = rr / f.G;
                         if (a.lse)
                             a.lse[(int64_t)(it.g * f.G + rr - tk * f.G) * a.c.n_tokens + it.q.q0 + tk] =
-                                Mr == -INFINITY ? -INFINITY : __fadd_rn(Mr, __fsub_rn(log2f(ls), kBias));
+                                ls == 0.0f ? -INFINITY : __fadd_rn(Mr, __fsub_rn(log2f(ls), kBias));
                     }
                     asm volatile("bar.sync 1, 256;" ::: "memory");
 #pragma unroll 2
@@ -1372,7 +1452,9 @@ bool pool_map(CUtensorMap *m, const altxs_paged_kv &kv, void *pool, int run) {
                                 (cuuint64_t)std::max(kv.n_pages, 1)};
     const bool f32 = kv.dtype == ALTXS_F32;
     const cuuint64_t b = f32 ? 4 : 2;
-    const cuuint64_t strides[3] = {(cuuint64_t)kv.token_stride * b, (cuuint64_t)kv.head_stride * b, (cuuint64_t)kv.page_stride * b};
+    // the stride over a single page is never taken: any valid one will do
+    const cuuint64_t strides[3] = {(cuuint64_t)kv.token_stride * b, (cuuint64_t)kv.head_stride * b,
+                                   kv.n_pages > 1 ? (cuuint64_t)kv.page_stride * b : 16};
     const cuuint32_t box[4] = {f32 ? (cuuint32_t)kv.head_dim : 64, (cuuint32_t)run, 1, 1}, es[4] = {1, 1, 1, 1};
     return enc(m, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : kv.dtype == ALTXS_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                4, pool, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, f32 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,

@@ -542,7 +542,8 @@ typedef struct altxs_paged_kv {
  * q_start[s+1] of the token arrays; they are the last of its kv_len[s]
  * positions (kv_len counts them).  Entry b of its page-table row holds
  * positions b*page_size ..; entries of blocks that no new token sees are not
- * read.  max_new and max_kv bound the device lengths on the host side; a
+ * read.  max_new and max_kv (each at most 2^30, else ALTXS_ENOTSUP) bound the
+ * device lengths on the host side; a
  * sequence outside its bounds (or with rows outside [0, n_tokens)) sets
  * ALTXS_ST_BAD_POS and is left out. */
 typedef struct altxs_chunks {

@@ -552,3 +552,97 @@ def test_short_workspace_is_refused():
     rc = L.altxs_paged_attention(b.cache._ref, b.chunks._ref, 4, ctypes.c_float(0.1), 0, q.data_ptr(), 256, q.data_ptr(), 256,
                                  None, None, need - 1, None)
     assert rc == _lib.ALTXS_ENOSPC
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_attention_ignores_huge_values_that_its_mask_hides(dtype, hd):
+    """Finite values near the type's end in keys and values that only some rows see (later tokens
+    of the chunk, keys before the later rows' windows) leave the other rows as they are."""
+    big = torch.finfo(DT[dtype]).max
+    for n, G in ((1, 2), (4, 2), (64, 2), (150, 2)):
+        L, w = 400, 180
+        b = Batch(dtype, hd, 2, 16, [n], [L], seed=21)
+        q = (2.0 * _rand(_gen(22), n, 2 * G, hd)).to(DT[dtype])
+        want, _ = b.ref(q, hd ** -0.5, w)
+        first, half = L - n - w + 1, n // 2  # row i sees [first + i, L - n + i]
+        for p0, p1 in ((0, first + half), (L - n + half + 1, L)):
+            page, slot = b.slots(0, max(p0, 0), p1)
+            b.cache.k[page, slot], b.cache.v[page, slot] = big, -big
+        out = b.cache.attend(b.chunks, q, window=w)
+        vmax = b.V[0].abs().max().item()
+        assert (out[half].double() - want[half]).abs().max().item() <= ATT_TOL[dtype] * vmax
+        b.cache.check_status()
+
+
+@pytest.mark.parametrize("n", [1, 4, 64])
+def test_attention_scales_of_keys_and_values(n):
+    """fp32 keys 2^40 below and queries 2^40 above 1, values near the type's end: as if none were scaled."""
+    b = Batch("f32", 64, 2, 16, [n], [300], seed=23)
+    q = 2.0 * _rand(_gen(24), n, 4, 64)
+    want, wl = b.ref(q, 0.125, 0)
+    b.cache.k.mul_(2.0 ** -40)
+    b.cache.v.mul_(2.0 ** 120)
+    out, lse = b.cache.attend(b.chunks, q * 2.0 ** 40, return_lse=True)
+    vmax = b.V[0].abs().max().item()
+    assert (out.double() * 2.0 ** -120 - want).abs().max().item() <= ATT_TOL["f32"] * vmax
+    assert (lse.double() - wl).abs().max().item() <= LSE_TOL
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [1, 4, 64, 300])
+def test_attention_of_a_nan_query(dtype, n):
+    """A query of NaN makes its own row NaN, output and sum, and no other."""
+    b = Batch(dtype, 64, 2, 16, [n], [4000], seed=25)
+    q = (2.0 * _rand(_gen(26), n, 4, 64)).to(DT[dtype])
+    want, wl = b.cache.attend(b.chunks, q, return_lse=True)
+    q[n // 2, 1] = float("nan")
+    out, lse = b.cache.attend(b.chunks, q, return_lse=True)
+    assert torch.isnan(out[n // 2, 1]).all() and torch.isnan(lse[1, n // 2])
+    out[n // 2, 1], lse[1, n // 2] = want[n // 2, 1], wl[1, n // 2]
+    assert torch.equal(out, want) and torch.equal(lse, wl)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_attention_windows_beyond_the_cache_see_everything(dtype):
+    news, kvs = [1, 20, 8, 300], [700, 500, 3, 1300]
+    b = Batch(dtype, 64, 2, 16, news, kvs, seed=27)
+    q = _rand(_gen(28), sum(news), 4, 64).to(DT[dtype])
+    want = b.cache.attend(b.chunks, q)
+    for w in (1300, 2000, 2 ** 31 - 1):
+        assert torch.equal(b.cache.attend(b.chunks, q, window=w), want)
+    b.cache.check_status()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attention_of_a_pool_of_one_page(dtype):
+    """The stride over a single page is never taken, whatever it is."""
+    b = Batch(dtype, 64, 2, 64, [40], [50], seed=29, spare=0)
+    q = _rand(_gen(30), 40, 4, 64).to(DT[dtype])
+    want = b.cache.attend(b.chunks, q)
+    k, v = (torch.as_strided(x, x.shape, (0, *x.stride()[1:])) for x in (b.cache.k, b.cache.v))
+    assert torch.equal(paged.PagedKV(k, v).attend(b.chunks, q), want)
+
+
+@pytest.mark.parametrize("heads", [2, 40])
+def test_sequences_above_a_bound_of_no_new_tokens_are_reported(heads):
+    b = Batch("bf16", 64, 1, 16, [3], [50], seed=31)
+    q = _rand(_gen(32), 3, heads, 64).bfloat16()
+    b.cache.attend(b.make_chunks(max_new=0), q)
+    with pytest.raises(RuntimeError):
+        b.cache.check_status()
+
+
+def test_lengths_beyond_the_limits_are_refused():
+    """max_kv and max_new above 2^30 (the pools' pages would cover them): no kernel runs."""
+    k, v = (torch.empty((1, 1 << 16, 1, 32), dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    cache = paged.PagedKV(k, v)
+    table = torch.zeros(1, 1 << 15, dtype=torch.int32, device=DEV)
+    one = torch.tensor([0, 1], dtype=torch.int32, device=DEV)
+    q = torch.zeros((1, 1, 32), dtype=torch.bfloat16, device=DEV)
+    for max_new, max_kv in ((1, 2 ** 30 + 1), (2 ** 30 + 1, 64)):
+        c = paged.Chunks(one, one[1:], table, max_new=max_new, max_kv=max_kv)
+        with pytest.raises(RuntimeError):
+            cache.attend(c, q)
+        with pytest.raises(RuntimeError):
+            cache.append(c, q, q)
