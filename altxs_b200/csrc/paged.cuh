@@ -72,7 +72,7 @@ struct PagedAttnArgs {
     int64_t ws_bytes;
 };
 int64_t paged_attention_ws(const altxs_paged_kv &kv, const altxs_chunks &c, int H, int window);
-// The tensor-core kernel for many rows (16-bit types): bounds on its items and
+// The tensor-core kernel for many rows: bounds on its items and
 // partial slots from the host's bounds on the lengths.
 struct ManyPlan {
     int64_t items, slots, slot_bytes;

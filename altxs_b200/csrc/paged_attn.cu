@@ -1,24 +1,32 @@
-// Attention of a few new tokens over a paged key/value cache: the rows of one
-// key/value head (its query heads times the sequence's new tokens) fit one
-// 16-row MMA tile.
+// Attention of a few new tokens over a paged key/value cache: at most 16 rows
+// (the query heads of one key/value head times the sequence's new tokens), and
+// the launch of all paged attention (paged_tc.cu has the kernel for more rows).
 //
-// Every cached key and value is read once and serves at most 16 rows, so HBM
-// bounds it (8 flops a byte at 16 rows in 16 bits against the card's 260).  A
-// sequence's visible keys are cut into splits (split_keys: a function of their
-// number alone, so a row's bits do not depend on the batch); an item is one
-// split of one key/value head, taken by a block of four warps.  Each warp
+// o = sum_j p_j v_j / sum_j p_j with p_j = 2^(x_j - m), x = scale log2(e) q . k:
+// one pass over the keys with the running maximum m and sum.  Every cached key
+// and value is read once and serves at most 16 rows, so HBM bounds it (8 flops
+// a byte at 16 rows in 16 bits against the card's 260).
+//
+// A sequence's visible keys are cut into splits (split_keys: a function of the
+// sequence's own lengths, so a row's bits do not depend on the batch); an item
+// is one split of one key/value head.  A split's rows go to the workspace as
+// (m, l, o); the block that finishes the last split of a (sequence, head) joins
+// them in split order.
+//
+// 16-bit types (k_paged_few): a block of four warps per item.  Each warp
 // streams 8 KB chunks (keys and values of CK positions) through its own three
-// slots with 16-byte asynchronous copies, gathering rows through the page
-// table (a page may end anywhere in a chunk; rows past the end are filled with
+// slots with 16-byte asynchronous copies, gathering rows through the page table
+// (a page may end anywhere in a chunk; rows past the end are filled with
 // zeros), two chunks in flight while one is computed; there is no block-wide
 // barrier until the four warps' partial rows meet.  Per chunk a warp forms
-// S = Q K^T, the online softmax and O += P V as 16-row mma.sync fragments: the
-// 16-bit types in m16n8k16 with fp32 sums, fp32 as three tf32 products of
-// hi/lo halves (22 significant bits).  The tcgen05 tile would be at least 128
-// rows for at most 16 real ones and is not what bounds this kernel.
-//
-// A split's rows go to the workspace as (m, l, o); the block that finishes the
-// last split of a (sequence, head) joins them in split order.
+// S = Q K^T, the online softmax and O += P V as m16n8k16 fragments with fp32
+// sums, p rounded once to the type.  The tcgen05 tile is 128 rows for at most
+// 16 real ones.  More rows in groups of 16 read the keys again and lose to it:
+// 256 streams of up to 2048 keys, 20 rows a head, took 251 us against 137.
+// Measured: three contexts of 60000 to 100000 keys, 32 heads over 8, hd 128 in
+// bf16: 1.12 GB in 205 us (5.5 TB/s).
+// fp32 (k_paged_vec, below): 256 streams of up to 2048 keys, 8 heads of 64:
+// 1.10 GB in 190 us (5.8 TB/s); one stream of 2049 keys 13 us.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -39,7 +47,7 @@ constexpr unsigned kAll = 0xffffffffu;
 
 // Keys of a split of a sequence that shows `keys` of them to `width` (head, row group) pairs: a long one by
 // itself fills the card once.  (An item costs some microseconds besides its keys' time: 100000 keys x 8 heads
-// in 98 splits of 1024 took 286 us next to two like it, in 37 of 2752 XXX us.)
+// in 98 splits of 1024 took 286 us next to two like it, in 37 of 2752 205 us.)
 __host__ __device__ inline int split_keys(int keys, int width) {
     const int most = width < kSplitItems ? kSplitItems / width : 1;
     const int each = (keys + most - 1) / most;
@@ -535,10 +543,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_paged_few(const __grid_const
 
 // fp32: half a flop a byte and row, so plain fp32 arithmetic keeps up with HBM for a few rows.  HD / 8 lanes
 // share a position, each with eight channels of its key and value straight from global memory (two 16-byte
-// loads each, the row contiguous over the lanes); a warp has 8 KB in flight, 16 warps an SM.  Every group of
-// lanes keeps its own (m, l, o) over its positions, joined at the end.  More than eight rows are two items that
-// read the same keys.  (As 16-row MMA tiles of three tf32 products, with a dozen instructions to split each pair
-// of values, 256 streams took 471 us where this takes XXX.)
+// loads each, the row contiguous over the lanes); at one row a head a warp has 4 KB in flight and an SM 32 warps.
+// Every group of lanes keeps its own (m, l, o) over its positions, joined at the end.  More than eight rows are two
+// items that read the same keys.  (As 16-row MMA tiles of three tf32 products, with a dozen instructions to split
+// each pair of values, 256 streams took 471 us where this takes 190.  Four warps a block: 185 us, but one stream
+// 15.4 us where eight take 13.)
 constexpr int kVecRows = 8, kVecWarps = 8;
 template <int HD, int R>
 __global__ void __launch_bounds__(kVecWarps * 32, R == 1 ? 4 : R < 4 ? 2 : 1) k_paged_vec(const __grid_constant__ FewArgs f) {

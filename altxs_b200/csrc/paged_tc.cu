@@ -9,30 +9,45 @@
 //   warp 8          issues the MMAs: S = Q K^T into a group's tensor-memory
 //                   score columns, then (P written over S) O += P V, P read
 //                   from tensor memory, V as it lies (MN-major);
-//   the rest        gather key and value rows through the page table into a
-//                   ring of tiles, rows that no position of the block needs
-//                   filled with zeros.
+//   the rest        fetch key and value rows through the page table into a
+//                   ring of tiles by tensor copies, one for each run of
+//                   positions within a page (16 bits: and 64-channel half);
+//                   runs that no row of the block needs are filled with zeros.
 // With more than 128 rows each group owns 128 of them and every key tile
 // serves both; with at most 128 the two groups share the rows and take even
-// and odd key tiles, and group 0 joins both outputs at the end.  Either way
-// the MMA warp alternates between the groups, so one group's softmax runs
-// under the other's MMAs.
+// and odd key tiles, and both outputs are joined at the end.  Either way the
+// MMA warp alternates between the groups, so one group's softmax runs under
+// the other's MMAs.  At most 64 (32) rows are held 2 (4) times, each copy with
+// its share of a tile's columns.
 //
 // Softmax: x = s scale log2(e) in fp32, p = 2^(x - m), the sum from the
 // unrounded p.  m follows the running maximum only when that grows by more
 // than 2^8: until then p <= 256 is as exact, and O (fp32, in tensor memory) is
 // not touched.
 //
-// 16-bit types: the tiles are the cache's own rows (16-byte asynchronous
-// copies), p is rounded once to the type.
+// 16-bit types: the tiles are the cache's own rows, p is rounded once to the
+// type.  Warp 9 fetches keys, warp 11 values, warp 10 clears what must not meet
+// a p = 0 in tiles that not every row sees whole.
 // fp32: every operand is a pair of fp16 planes, hi = fp16(v 2^a) and lo =
-// fp16(v 2^a - hi), a power of two per query row, per key tile and (running)
-// for the values that puts the largest magnitude at 2^14: hi + lo keeps 22
-// significant bits of everything within 2^-18 of that magnitude, and 2^-40 of
-// it below.  A product is hi hi + hi lo + lo hi with fp32 sums.  Three fp16
-// products instead of six with bf16 planes or three at half the rate with
-// tf32; the producer warps hold a tile's rows in registers, agree on its
-// exponent and write the planes.
+// fp16(v 2^a - hi), the power of two chosen per query row and per 2 KB of keys
+// and of values (per position in tiles that not every row sees whole) so that
+// the largest magnitude is at 2^14: hi + lo keeps 22 significant bits of
+// everything within 2^-18 of that magnitude, and 2^-40 of it below.  p carries
+// the values' powers, O their running largest per row.  A product is
+// hi hi + hi lo + lo hi with fp32 sums: three fp16 products instead of six with
+// bf16 planes or three at half the rate with tf32.  Warp 9 fetches raw rows to
+// a stage each for keys and values, warps 10 to 15 write the planes.
+//
+// Bounds: at full tiles the softmax group's own chain (wait for S and the P V
+// before it, load and maximum, exponentials, store: about 4000 clocks for two
+// jobs of 128 x 128 x 128, of which the MMAs are 2050); otherwise an item's
+// start and end (its code is cold: 6000 to 8000 clocks for the queries, 13000
+// to 16000 for the outputs).  Items are drawn by ticket, longest first.
+// Measured: 4096 new tokens over 20000 positions, 16 heads over 8, hd 128 in
+// fp16: 632 us (953 TFLOP/s); nine ragged sequences of up to 1999 new tokens,
+// 16 heads over 4, bf16: 219 us (605 TFLOP/s); 5 new tokens of 48 streams in
+// windows of 1024, 16-token pages, fp16: 35 us; 64 new tokens of 16 streams
+// over windows of 2048, 8 heads of 64, fp32: 89 us.
 //
 // Splits of a block go to the workspace as (m, l, O); the item that arrives
 // last joins them in split order.  Tiles, blocks and splits are functions of
@@ -248,10 +263,6 @@ constexpr uint32_t idesc(int n, int bmn) {  // kind::f16 (bf16, or fp16: fp32's 
     const uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     return (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)bmn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
-// Matrix descriptors of 128-byte-swizzled tiles: the upper word is the same for
-// all of them (8-row groups every 1024 bytes), the lower one holds the address
-// and, for MN-major tiles, the distance of 64-channel halves; offsets are added
-// in units of 16 bytes.
 // whether a phase is complete, without waiting (mbar_try_wait may sleep for a while first)
 __device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
     uint32_t ok;
@@ -274,6 +285,10 @@ __device__ __forceinline__ bool elect_one() {
     asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
     return p != 0;
 }
+// Matrix descriptors of 128-byte-swizzled tiles: the upper word is the same for
+// all of them (8-row groups every 1024 bytes), the lower one holds the address
+// and, for MN-major tiles, the distance of 64-channel halves; offsets are added
+// in units of 16 bytes.
 __device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo) { return (saddr >> 4) | (lbo >> 4) << 16; }
 constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
 __device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t accumulate) {
