@@ -86,6 +86,9 @@ __device__ __forceinline__ int few_splits(const FewArgs &f, const Seq &q) {
     return split_count(max(0, q.L - first_seen(q.n, q.L, f.a.window)), few_width(f, q));
 }
 
+// The kernel for many rows may start as this one's blocks leave (they share no sequence).
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 __device__ __forceinline__ void scan_items(const FewArgs &f, ItemScan &sc) {
     __shared__ int wsum[kScan / 32];
     const int n = f.a.c.n_seqs, per = (n + kScan - 1) / kScan;
@@ -330,6 +333,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_paged_few(const __grid_const
     const int pshift = (P & (P - 1)) == 0 ? 31 - __clz(P) : -1;
     const float c2 = __fmul_rn(a.scale, kLog2e);
     const uint32_t ring = smem_u32(few_smem) + warp * kSlots * kChunkBytes;
+    launch_dependents();
     scan_items(f, sc);
     const int total = sc.before[kScan];
 
@@ -562,6 +566,7 @@ __global__ void __launch_bounds__(kVecWarps * 32, R == 1 ? 4 : R < 4 ? 2 : 1) k_
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kg = lane / LPK, li = lane % LPK;
     const int G = f.G, P = a.kv.page_size, pshift = (P & (P - 1)) == 0 ? 31 - __clz(P) : -1;
     const float c2 = __fmul_rn(a.scale, kLog2e);
+    launch_dependents();
     scan_items(f, sc);
     const int total = sc.before[kScan];
     for (int item = blockIdx.x; item < total; item += gridDim.x) {
@@ -691,7 +696,7 @@ struct Plan {
     int64_t items;        // few: bound on the items
     int part_rows;
     ManyPlan mp;
-    int64_t few_cnt, many_cnt, bytes;  // counters' bytes (both lists), then the partial rows, shared
+    int64_t few_cnt, many_cnt, few_part, bytes;  // both lists of counters, then both kernels' partial rows
 };
 Plan plan_of(const altxs_paged_kv &kv, const altxs_chunks &c, int H, int window) {
     Plan p{};
@@ -706,16 +711,14 @@ Plan plan_of(const altxs_paged_kv &kv, const altxs_chunks &c, int H, int window)
     p.group = kv.dtype == ALTXS_F32 ? kVecRows : kMaxRows;
     p.groups = (int)((std::min<int64_t>(kMaxRows, most) + p.group - 1) / p.group);
     const int64_t keys = window > 0 ? std::min<int64_t>(c.max_kv, (int64_t)window + c.max_new - 1) : c.max_kv;
-    int64_t total = n * keys, part = 0;
+    int64_t total = n * keys;
     if (c.total_kv > 0) total = std::min(total, c.total_kv);
     const bool split = keys > kSplitUnit;
     p.items = (split ? total / kSplitUnit + n : n) * kv.n_kv_heads * std::max(p.groups, 1);
     p.part_rows = (int)std::min<int64_t>(p.group, most);
-    if (p.few && split) part = p.items * p.part_rows * (kv.head_dim + 4) * 4;
-    if (p.many) {
-        p.mp = paged_many_plan(kv, c, H, window);
-        part = std::max(part, p.mp.slots * p.mp.slot_bytes);
-    }
+    if (p.few && split) p.few_part = align_up(p.items * p.part_rows * (kv.head_dim + 4) * 4, 256);
+    if (p.many) p.mp = paged_many_plan(kv, c, H, window);
+    const int64_t part = p.few_part + p.mp.slots * p.mp.slot_bytes;
     p.few_cnt = align_up(4 * std::max(kCounters, n * kv.n_kv_heads * std::max(p.groups, 1)), 256);
     p.many_cnt = align_up(4 * std::max(kCounters, p.mp.slots + 1), 256);  // its first word: the item tickets
     if (part > 0 || p.many) p.bytes = p.few_cnt + p.many_cnt + part;
@@ -734,11 +737,12 @@ template <typename T, int HD>
 int launch(const PagedAttnArgs &a, const Plan &p, cudaStream_t st) {
     unsigned char *ws = static_cast<unsigned char *>(a.ws);
     uint32_t *few_cnt = nullptr, *many_cnt = nullptr;
-    float *part = nullptr;
+    float *part = nullptr, *many_part = nullptr;
     if (p.bytes > 0) {
         few_cnt = reinterpret_cast<uint32_t *>(ws);
         many_cnt = reinterpret_cast<uint32_t *>(ws + p.few_cnt);
         part = reinterpret_cast<float *>(ws + p.few_cnt + p.many_cnt);
+        many_part = reinterpret_cast<float *>(ws + p.few_cnt + p.many_cnt + p.few_part);
         if ((p.few_cnt > 4 * kCounters || p.many_cnt > 4 * kCounters) &&
             cudaMemsetAsync(ws, 0, p.few_cnt + p.many_cnt, st) != cudaSuccess)
             return ALTXS_ECUDA;
@@ -767,7 +771,7 @@ int launch(const PagedAttnArgs &a, const Plan &p, cudaStream_t st) {
             ALTXS_LAUNCH(kKPaged, st, k_paged_few<T, HD><<<grid, kWarps * 32, smem, st>>>(f));
         }
     }
-    if (p.many) return launch_paged_many(a, p.mp, kMaxRows + 1, many_cnt, part, (int)sms, st);
+    if (p.many) return launch_paged_many(a, p.mp, kMaxRows + 1, many_cnt, many_part, (int)sms, p.few, st);
     return ALTXS_OK;
 }
 template <typename T>
