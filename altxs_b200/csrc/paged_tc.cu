@@ -45,7 +45,7 @@
 // to 16000 for the outputs).  Items are drawn by ticket, longest first.
 // Measured: 4096 new tokens over 20000 positions, 16 heads over 8, hd 128 in
 // fp16: 632 us (953 TFLOP/s); nine ragged sequences of up to 1999 new tokens,
-// 16 heads over 4, bf16: 219 us (605 TFLOP/s); 5 new tokens of 48 streams in
+// 16 heads over 4, bf16: 206 us (641 TFLOP/s); 5 new tokens of 48 streams in
 // windows of 1024, 16-token pages, fp16: 35 us; 64 new tokens of 16 streams
 // over windows of 2048, 8 heads of 64, fp32: 89 us.
 //
