@@ -26,8 +26,9 @@
 // not touched.
 //
 // 16-bit types: the tiles are the cache's own rows, p is rounded once to the
-// type.  Warp 9 fetches keys, warp 11 values, warp 10 clears what must not meet
-// a p = 0 in tiles that not every row sees whole.
+// type.  Warps 9 and 11 fetch every other tile, warp 10 draws and announces the
+// items and clears what must not meet a p = 0 in tiles that not every row sees
+// whole.
 // fp32: every operand is a pair of fp16 planes, hi = fp16(v 2^a) and lo =
 // fp16(v 2^a - hi), the power of two chosen per query row and per 2 KB of keys
 // and of values (per position in tiles that not every row sees whole) so that
@@ -36,18 +37,22 @@
 // the values' powers, O their running largest per row.  A product is
 // hi hi + hi lo + lo hi with fp32 sums: three fp16 products instead of six with
 // bf16 planes or three at half the rate with tf32.  Warp 9 fetches raw rows to
-// a stage each for keys and values, warps 10 to 15 write the planes.
+// a stage each for keys and values (and announces the items), warps 10 to 15
+// write the planes.
 //
 // Bounds: at full tiles the softmax group's own chain (wait for S and the P V
 // before it, load and maximum, exponentials, store: about 4000 clocks for two
 // jobs of 128 x 128 x 128, of which the MMAs are 2050); otherwise an item's
-// start and end (its code is cold: 6000 to 8000 clocks for the queries, 13000
-// to 16000 for the outputs).  Items are drawn by ticket, longest first.
+// start and end (mostly cold code; with 64 channels about 4000 clocks to find
+// the first item, 2000 for the queries, 1500 for the last products and 7000 for
+// the outputs).  Items are drawn by ticket, longest first, one ahead: two or
+// three ahead the long piece took 743 us.  (Found by every role for itself
+// instead of by one ahead of all: 5 tokens of 48 streams 35 us.)
 // Measured: 4096 new tokens over 20000 positions, 16 heads over 8, hd 128 in
 // fp16: 632 us (953 TFLOP/s); nine ragged sequences of up to 1999 new tokens,
 // 16 heads over 4, bf16: 206 us (641 TFLOP/s); 5 new tokens of 48 streams in
-// windows of 1024, 16-token pages, fp16: 35 us; 64 new tokens of 16 streams
-// over windows of 2048, 8 heads of 64, fp32: 89 us.
+// windows of 1024, 16-token pages, fp16: 32 us; 64 new tokens of 16 streams
+// over windows of 2048, 8 heads of 64, fp32: 88 us.
 //
 // Splits of a block go to the workspace as (m, l, O); the item that arrives
 // last joins them in split order.  Tiles, blocks and splits are functions of
@@ -68,7 +73,6 @@ namespace {
 
 constexpr int kMmaWarp = 8;
 constexpr int kScan = 64;        // sequences are counted in this many groups
-constexpr int kCached = 32;       // up to this many sequences' shares are kept in shared memory
 constexpr int kMostItems = 1184;  // splits of one sequence
 constexpr int kMostSplits = 16;
 constexpr int kNext = 4;           // items announced to a block's roles ahead
@@ -165,8 +169,7 @@ __device__ __forceinline__ Shape shape_of(const ManyArgs &f, const Seq &q) {
 struct Scan {
     int before[kScan + 1], slots[kScan + 1];  // items, and partial slots, before each group of sequences
     int per;
-    // up to kCached sequences: each one's rows (q0, n, L) and its share (whole << 5 | nsplit)
-    int4 seq[kCached];
+    uint32_t share[kScan];  // groups of one sequence: whole << 5 | nsplit of its shape
 };
 
 struct Item {
@@ -190,12 +193,10 @@ __device__ __forceinline__ Item locate(const ManyArgs &f, const Scan &sc, int it
     it.s = lo * sc.per;
     int local = item - sc.before[lo], slot = sc.slots[lo];
     Shape w;
-    if (f.a.c.n_seqs <= kCached) {
-        const int4 v = sc.seq[lo];
-        it.q = Seq{v.x, v.y, v.z};
-        w.whole = v.w >> 5, w.nsplit = v.w & 31;
+    it.q = load_seq(f.a.c, it.s);
+    if (sc.per == 1) {
+        w.whole = sc.share[lo] >> 5, w.nsplit = sc.share[lo] & 31;
     } else {
-        it.q = load_seq(f.a.c, it.s);
         w = shape_of<C>(f, it.q);
         for (int n; it.s < f.a.c.n_seqs - 1 && local >= (n = w.items()); w = shape_of<C>(f, it.q)) {
             local -= n;
@@ -437,7 +438,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
     constexpr bool F32 = C::F32;
     extern __shared__ unsigned char pm_smem_raw[];
     __shared__ __align__(8) uint64_t full[C::Slots], empty[C::Slots], landed[F32 ? 1 : C::Slots], s_full[2], p_full[2], o_done[2], q_full, drainb,
-        raw_full[2], raw_empty[2], next_full[kNext], next_empty[kNext];
+        raw_full[2], raw_empty[2], next_full[kNext], next_empty[kNext], want;
     __shared__ Scan sc;
     // by key tile: which positions exist (4 to a byte), and (fp32) the exponents of its positions' keys and values.
     // Two tiles of those do: a tile's are written once the values' slot of the tile two before is free.
@@ -448,7 +449,8 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
     __shared__ __align__(8) uint8_t odd8_sh[F32 ? C::Ring : 1][8];  // by item: values that are not finite were set to 0 (fp32: per warp)
     __shared__ uint32_t odd_sh[F32 ? 1 : C::Ring];
     __shared__ int2 wsum[kScan / 32];
-    __shared__ int last_sh, item_sh, next_sh[kNext];
+    __shared__ int last_sh, item_sh;
+    __shared__ __align__(16) Item next_sh[kNext];
     __shared__ volatile int abort_sh;
     const PagedAttnArgs &a = f.a;
     const uint32_t raw_s = smem_u32(pm_smem_raw);
@@ -476,6 +478,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
         }
         mbar_init(&q_full, 8);
         mbar_init(&drainb, 1);
+        mbar_init(&want, 1);
         abort_sh = 0;
         for (int i = 0; i < (F32 ? 1 : C::Ring); ++i) odd_sh[i] = 0;
         fence_mbar_init();
@@ -493,7 +496,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
             const Shape w = shape_of<C>(f, q);
             sum += w.items();
             if (w.nsplit > 1) cut += w.items() - w.whole;
-            if (n <= kCached) sc.seq[s] = make_int4(q.q0, q.n, q.L, w.whole << 5 | w.nsplit);
+            if (per == 1) sc.share[s] = w.whole << 5 | w.nsplit;
         }
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -511,16 +514,15 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
     tc_fence_after();
     const uint32_t tmem = tmem_sh;
     const int total = sc.before[kScan];
-    // Items go to whoever is free (they differ in length several times over): warp 9 draws a ticket per item and
-    // announces it; a warp's r-th item, total or more when there is none.
-    auto announced = [&](int r) {
-        uint64_t *bar = &next_full[r % kNext];
-        const bool got = __all_sync(kAll, mbar_wait_bounded(bar, (r / kNext) & 1, limit));
-        const int item = got ? next_sh[r % kNext] : INT32_MAX;
+    // Items go to whoever is free (they differ in length several times over): one warp (the one with the least to do)
+    // draws a ticket per item, finds what it is and announces it, an item ahead; s = -1: there is none.
+    constexpr int kAnnouncer = F32 ? 0 : 1;  // of the producers
+    auto announced = [&](int r, Item &it) {  // a warp's r-th item
+        const bool got = __all_sync(kAll, mbar_wait_bounded(&next_full[r % kNext], (r / kNext) & 1, limit));
+        if (got) it = next_sh[r % kNext];
+        else it.s = -1, abort_sh = 1;
         __syncwarp();
         if (got && lane == 0) mbar_arrive(&next_empty[r % kNext]);
-        if (!got) abort_sh = 1;
-        return item;
     };
 
     if (warp > kMmaWarp) {
@@ -532,39 +534,53 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
         uint32_t n = 0, kt = 0, live = 0;  // slots, key tiles and items with tiles so far
         bool ok = true;
         // The tile whose copies come next: found (and its page numbers on their way) one tile ahead.
-        int round = 0, t = 0, drawn = blockIdx.x;
+        int round = 0, t = 0, drawn = blockIdx.x, told = 0;  // items taken, tile, last item drawn, items announced
         Item it;
         it.t1 = 0;
-        bool fresh = false, more = true;
-        auto advance = [&]() {  // to the next tile
-            ++t;
-            fresh = false;
-            while (t >= it.t1) {
-                int item;
-                if (pw == 0) {
-                    item = __shfl_sync(kAll, drawn, 0);  // drawn an item ago
-                    const int slot = round % kNext;
-                    if (round >= kNext && !__all_sync(kAll, mbar_wait_bounded(&next_empty[slot], (round / kNext - 1) & 1, limit))) {
-                        ok = more = false;
-                        return;
-                    }
-                    if (lane == 0) {
-                        next_sh[slot] = item;
-                        mbar_arrive(&next_full[slot]);
-                        if (item < total) drawn = (int)gridDim.x + (int)atomicAdd(f.ticket, 1u);
-                    }
-                    ++round;
-                } else {
-                    item = announced(round++);
-                }
-                if (item >= total) {
-                    more = false;
-                    return;
-                }
-                it = locate<C>(f, sc, item);
-                t = it.t0;
-                fresh = true;
+        bool fresh = false, more = true, none = false;
+        auto announce = [&]() {
+            // not before the loads have come to the item ahead of it: an item drawn early is one that a free block misses
+            if (!F32 && told > 0 && !__all_sync(kAll, !abort_sh && mbar_wait_bounded(&want, (told - 1) & 1, limit))) {
+                ok = more = false;
+                return;
             }
+            if (told > 0 && lane == 0) drawn = (int)gridDim.x + (int)atomicAdd(f.ticket, 1u);
+            const int item = __shfl_sync(kAll, drawn, 0), slot = told % kNext;
+            if (told >= kNext && !__all_sync(kAll, mbar_wait_bounded(&next_empty[slot], (told / kNext - 1) & 1, limit))) {
+                ok = more = false;
+                return;
+            }
+            Item next;
+            next.s = -1;
+            if (item < total) next = locate<C>(f, sc, item);
+            if (lane == 0) {
+                next_sh[slot] = next;
+                mbar_arrive(&next_full[slot]);
+            }
+            __syncwarp();
+            ++told;
+        };
+        // To the next tile, or past one item that has none: a warp issues the copies it holds back before it goes on to
+        // another item, whose announcement may wait for the softmax to take an item that waits for those copies.
+        auto advance = [&]() {
+            ++t;
+            fresh = none = false;
+            if (t < it.t1) return;
+            if (pw == kAnnouncer) {
+                if (told == round) announce();
+                if (!ok) return;
+                it = next_sh[round++ % kNext];
+            } else {
+                announced(round++, it);
+                if (pw == 0 && lane == 0) mbar_arrive(&want);
+            }
+            if (it.s < 0) {
+                more = false;
+                return;
+            }
+            t = it.t0;
+            fresh = true;
+            none = t >= it.t1;
         };
         // Positions [all0, all1) are seen by every row of the block.
         int all0 = 0, all1 = 0;
@@ -586,53 +602,67 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                 return kb < max(all0, it.lo) || kb + KT > min(all1, it.hi);
             };
             uint32_t lph = 0;  // landed[]'s parities, by slot
-            if (pw != 1) {  // warp 9 fetches the keys, warp 11 the values: a warp issues one copy in about 100 clocks
-                const int kv = pw >> 1;
-                const CUtensorMap *map = kv ? &tv : &tk;
-                n = kv;
+            if (pw != 1) {
+                // Warp 9 fetches the even tiles, warp 11 the odd ones: a warp issues one copy in about 100 clocks, and
+                // finding a tile's pages takes as long as eight of them.  (With all keys to one and all values to the
+                // other it was no faster or slower.)
+                const uint32_t odd = pw >> 1;
+                uint32_t issued = 0, was_look = 0;  // copies up to this warp's last; slots whose last copy went to landed[]
                 int page[KT / 32];
                 auto fetch = [&]() {
 #pragma unroll
                     for (int e = 0; e < KT / 32; ++e) {
                         const int u = e * 32 + lane, k = it.base + t * KT + u * run;
-                        page[e] = more && u < runs && k < it.hi && k + run > it.lo
+                        page[e] = more && !none && u < runs && k < it.hi && k + run > it.lo
                                       ? __ldg(a.c.page_table + it.s * a.c.table_stride + block_of(k)) : INT32_MIN;
                         if (e * 32 + 32 >= runs) break;
                     }
                 };
                 bool have = false, look = false;
-                uint32_t was_look = 0;  // slots whose last copy went to landed[]
-                int kb = 0, g = 0, pos_in[KT / 32], pg[KT / 32];
+                uint32_t cur = 0;  // the tile whose copies come next
+                int g = 0, pos_in[KT / 32], pg[KT / 32];
                 while (ok) {
-                    advance();
+                    uint32_t at = 0;
+                    bool mix = false;
+                    do {  // on to this warp's next tile
+                        advance();
+                        if (!more || none) break;
+                        if (fresh) bounds();
+                        at = kt++;
+                        mix = mixed();
+                        const uint32_t bit = 1u << (2 * at + 1) % C::Slots;
+                        if (mix) lph ^= bit;
+                        was_look = (was_look & ~bit) | (mix ? bit : 0u);
+                    } while ((at & 1) != odd);
                     fetch();
                     if (have) {
-                        const uint32_t s = n % C::Slots;
-                        if (n >= C::Slots)
-                            ok = __all_sync(kAll, !abort_sh && mbar_wait_bounded(&empty[s], ((n / C::Slots) - 1) & 1, limit));
-                        if (!ok) break;
-                        uint64_t *bar = look ? &landed[s] : &full[s];
-                        if (look) lph ^= 1u << s;
-                        was_look = (was_look & ~(1u << s)) | (look ? 1u << s : 0u);
-                        if (lane == 0) mbar_expect_tx(bar, C::TileB);
-                        __syncwarp();
 #pragma unroll
-                        for (int e = 0; e < KT / 32; ++e) {
-                            if (e * 32 >= runs) break;
-                            if (lane < mine) {
-                                const uint32_t d = ring + s * C::TileB + (e * 32 + lane) * run * 128;
+                        for (int kv = 0; kv < 2; ++kv) {
+                            const uint32_t n = 2 * cur + kv, s = n % C::Slots;
+                            if (n >= C::Slots)
+                                ok = ok && __all_sync(kAll, !abort_sh && mbar_wait_bounded(&empty[s], ((n / C::Slots) - 1) & 1, limit));
+                            if (!ok) continue;
+                            uint64_t *bar = kv && look ? &landed[s] : &full[s];
+                            if (lane == 0) mbar_expect_tx(bar, C::TileB);
+                            __syncwarp();
 #pragma unroll
-                                for (int h = 0; h < C::Halves; ++h)
-                                    tma_load_4d(d + h * (KT * 128), map, 64 * h, pos_in[e], g, pg[e], bar);
+                            for (int e = 0; e < KT / 32; ++e) {
+                                if (e * 32 >= runs) break;
+                                if (lane < mine) {
+                                    const uint32_t d = ring + s * C::TileB + (e * 32 + lane) * run * 128;
+#pragma unroll
+                                    for (int h = 0; h < C::Halves; ++h)
+                                        tma_load_4d(d + h * (KT * 128), kv ? &tv : &tk, 64 * h, pos_in[e], g, pg[e], bar);
+                                }
                             }
+                            issued = n + 1;
                         }
-                        n += 2;
                     }
-                    have = more;
+                    have = more && !none;
                     if (!more || !ok) break;
-                    if (fresh) bounds();
-                    kb = it.base + t * KT, g = it.g;
-                    look = kv && mixed();
+                    if (none) continue;
+                    const int kb = it.base + t * KT;
+                    cur = at, look = mix, g = it.g;
 #pragma unroll
                     for (int e = 0; e < KT / 32; ++e) {
                         if (e * 32 >= runs) break;
@@ -643,21 +673,21 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                         pg[e] = in ? page[e] : max(a.kv.n_pages, 1);
                         // which positions exist, for the softmax (what is outside [lo, hi) no row sees)
                         const uint32_t seen = __ballot_sync(kAll, in);
-                        if (kv) continue;
                         if (run >= 4) {
                             if (lane < mine)
-                                for (int i = 0; i < run / 4; ++i) kmask[kt % C::Ring][(e * 32 + lane) * (run / 4) + i] = in ? 15 : 0;
+                                for (int i = 0; i < run / 4; ++i) kmask[cur % C::Ring][(e * 32 + lane) * (run / 4) + i] = in ? 15 : 0;
                         } else if (lane % 4 == 0) {
-                            kmask[kt % C::Ring][e * 8 + lane / 4] = (uint8_t)((seen >> lane) & 15);
+                            kmask[cur % C::Ring][e * 8 + lane / 4] = (uint8_t)((seen >> lane) & 15);
                         }
                     }
                     __syncwarp();
-                    ++kt;
                 }
-                // every copy has landed before the block can exit
-                for (int32_t i = (int32_t)n - 2; i >= 0 && i + (int32_t)C::Slots >= (int32_t)n; i -= 2) {
+                // every copy of this warp has landed before the block can exit: those that are the last in their slots
+                const uint32_t end = ok ? 2 * kt : issued;
+                for (uint32_t i = end > C::Slots ? end - C::Slots : 0; i < issued; ++i) {
                     const uint32_t s = i % C::Slots;
-                    if ((was_look >> s) & 1) mbar_wait_bounded(&landed[s], ((lph >> s) & 1) ^ 1, kWaitLimit);
+                    if ((i >> 1 & 1) != odd) continue;
+                    if ((i & 1) && ((was_look >> s) & 1)) mbar_wait_bounded(&landed[s], ((lph >> s) & 1) ^ 1, kWaitLimit);
                     else mbar_wait_bounded(&full[s], (i / C::Slots) & 1, kWaitLimit);
                 }
             } else if (pw == 1) {
@@ -665,6 +695,8 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                 while (ok) {
                     advance();
                     if (!more) break;
+                    if (fresh && told == round) announce();
+                    if (none || !ok) continue;
                     if (fresh) {
                         bounds();
                         me = live++ % C::Ring;  // the softmax clears it when the item is done
@@ -713,7 +745,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
 #pragma unroll
                     for (int e = 0; e < KT / 32; ++e) {
                         const int u = e * 32 + lane, k = it.base + t * KT + u * run;
-                        page[e] = more && u < runs && k < it.hi && k + run > it.lo
+                        page[e] = more && !none && u < runs && k < it.hi && k + run > it.lo
                                       ? __ldg(a.c.page_table + it.s * a.c.table_stride + block_of(k)) : INT32_MIN;
                         if (e * 32 + 32 >= runs) break;
                     }
@@ -743,10 +775,12 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                         }
                         if (!ok) break;
                     }
-                    have = more;
+                    have = more && !none;
                     if (!more) break;
+                    if (none) continue;
                     const int kb = it.base + t * KT;
                     g = it.g;
+                    const bool ahead = fresh && told == round;
 #pragma unroll
                     for (int e = 0; e < KT / 32; ++e) {
                         if (e * 32 >= runs) break;
@@ -765,6 +799,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                     }
                     __syncwarp();
                     ++kt;
+                    if (ahead) announce();
                 }
                 // every copy has landed before the block can exit
 #pragma unroll
@@ -782,6 +817,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                 while (ok) {
                     advance();
                     if (!more) break;
+                    if (none) continue;
                     if (fresh) {
                         bounds();
                         me = live++ % C::Ring;
@@ -867,8 +903,8 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
             }
         }
         if (!ok) abort_sh = 1;
-        if (pw == 0 && lane == 0) {
-            // every block draws one ticket past the end (after a wait that gave up, here): the last of them resets the count
+        if (pw == kAnnouncer && lane == 0) {
+            // every block draws until it is past the end (after a wait that gave up, here): the last of them resets the count
             while (drawn < total) drawn = (int)gridDim.x + (int)atomicAdd(f.ticket, 1u);
             if (blockIdx.x < total && drawn - (int)gridDim.x == total - 1) *f.ticket = 0;
         }
@@ -891,9 +927,9 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
             const uint32_t ringk = desc_lo(ring, 16), ringv = desc_lo(ring, KT * 128), q0d = desc_lo(sq, 16);
             bool ok = true;
             for (int round = 0; ok; ++round) {
-                const int item = announced(round);
-                if (item >= total) break;
-                const Item it = locate<C>(f, sc, item);
+                Item it;
+                announced(round, it);
+                if (__shfl_sync(kAll, it.s, 0) < 0) break;
                 const int nt = __shfl_sync(kAll, it.t1 - it.t0, 0);
                 const bool two = __shfl_sync(kAll, (int)it.two, 0) != 0;
                 if (nt == 0) continue;
@@ -999,17 +1035,19 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
         int round = 0;
         auto ask = [&]() {
             if (warp == 0) {
-                const int next = announced(round);
-                if (lane == 0) item_sh = abort_sh ? INT32_MAX : next;
+                if (round > 0 && lane == 0) mbar_arrive(&next_empty[(round - 1) % kNext]);  // all warps have read it
+                const bool got = __all_sync(kAll, mbar_wait_bounded(&next_full[round % kNext], (round / kNext) & 1, limit));
+                if (!got) abort_sh = 1;
+                if (lane == 0) item_sh = got && !abort_sh;
             }
             ++round;
         };
         ask();
         asm volatile("bar.sync 1, 256;" ::: "memory");
         for (;;) {
-            const int item = item_sh;
-            if (item >= total) break;
-            const Item it = locate<C>(f, sc, item);
+            if (!item_sh) break;
+            const Item it = next_sh[(round - 1) % kNext];
+            if (it.s < 0) break;
             const int nt = it.t1 - it.t0, p0 = it.q.L - it.q.n;
             // At most 64 (32) rows are held 2 (4) times, each copy with its share of a tile's columns, its own
             // (m, l) and O: a thread's chain of exponentials is 2 (4) times shorter.

@@ -646,3 +646,22 @@ def test_lengths_beyond_the_limits_are_refused():
             cache.attend(c, q)
         with pytest.raises(RuntimeError):
             cache.append(c, q, q)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attention_of_many_rows_that_see_nothing(dtype):
+    """Far more new tokens than positions: thousands of blocks of rows without a key between a few that have some."""
+    n, L = 40000, 300
+    b = Batch(dtype, 32, 4, 16, [n], [L], seed=35)
+    q = torch.zeros(n, 16, 32, dtype=DT[dtype], device=DEV)
+    q[n - L:] = (2.0 * _rand(_gen(36), L, 16, 32)).to(DT[dtype])
+    out, lse = b.cache.attend(b.chunks, q, return_lse=True)
+    b.cache.check_status()
+    assert not out[:n - L].any() and torch.isneginf(lse[:, :n - L]).all()
+    c = paged.Chunks(torch.tensor([0, L], dtype=torch.int32, device=DEV), b.kv_len, b.tab, max_new=L, max_kv=L)
+    tail, tl = b.cache.attend(c, q[n - L:], return_lse=True)
+    want, wl = Batch(dtype, 32, 4, 16, [L], [L], seed=35).ref(q[n - L:], 32 ** -0.5, 0)
+    vmax = b.V[0].abs().max().item()
+    for o, l1 in ((out[n - L:], lse[:, n - L:]), (tail, tl)):
+        assert (o.double() - want).abs().max().item() <= ATT_TOL[dtype] * vmax
+        assert (l1.double() - wl).abs().max().item() <= LSE_TOL
