@@ -51,7 +51,7 @@
 // Measured: 4096 new tokens over 20000 positions, 16 heads over 8, hd 128 in
 // fp16: 632 us (953 TFLOP/s); nine ragged sequences of up to 1999 new tokens,
 // 16 heads over 4, bf16: 206 us (641 TFLOP/s); 5 new tokens of 48 streams in
-// windows of 1024, 16-token pages, fp16: 32 us; 64 new tokens of 16 streams
+// windows of 1024, 16-token pages, fp16: 31 us; 64 new tokens of 16 streams
 // over windows of 2048, 8 heads of 64, fp32: 88 us.
 //
 // Splits of a block go to the workspace as (m, l, O); the item that arrives
@@ -560,8 +560,8 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
             __syncwarp();
             ++told;
         };
-        // To the next tile, or past one item that has none: a warp issues the copies it holds back before it goes on to
-        // another item, whose announcement may wait for the softmax to take an item that waits for those copies.
+        // To the next tile, or past one item that has none: a warp issues the copies it holds back before it goes past
+        // more items, whose announcements may wait for the softmax to take one that waits for those copies.
         auto advance = [&]() {
             ++t;
             fresh = none = false;
@@ -623,8 +623,10 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                 int g = 0, pos_in[KT / 32], pg[KT / 32];
                 while (ok) {
                     uint32_t at = 0;
-                    bool mix = false;
-                    do {  // on to this warp's next tile
+                    bool mix = false, flush = false;
+                    do {  // on to this warp's next tile; not to an item that is not announced before what is held back is issued
+                        flush = have && t + 1 >= it.t1 && !__all_sync(kAll, mbar_test(&next_full[round % kNext], (round / kNext) & 1));
+                        if (flush) break;
                         advance();
                         if (!more || none) break;
                         if (fresh) bounds();
@@ -634,7 +636,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                         if (mix) lph ^= bit;
                         was_look = (was_look & ~bit) | (mix ? bit : 0u);
                     } while ((at & 1) != odd);
-                    fetch();
+                    if (!flush) fetch();
                     if (have) {
 #pragma unroll
                         for (int kv = 0; kv < 2; ++kv) {
@@ -658,9 +660,9 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                             issued = n + 1;
                         }
                     }
-                    have = more && !none;
+                    have = more && !none && !flush;
                     if (!more || !ok) break;
-                    if (none) continue;
+                    if (none || flush) continue;
                     const int kb = it.base + t * KT;
                     cur = at, look = mix, g = it.g;
 #pragma unroll
@@ -695,45 +697,47 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                 while (ok) {
                     advance();
                     if (!more) break;
-                    if (fresh && told == round) announce();
-                    if (none || !ok) continue;
+                    if (none) continue;
+                    const bool ahead = fresh && told == round;  // the next item, once the first tile is on its way
                     if (fresh) {
                         bounds();
                         me = live++ % C::Ring;  // the softmax clears it when the item is done
                     }
                     const uint32_t s = (n + 1) % C::Slots;
                     n += 2;
-                    if (!mixed()) continue;
-                    ok = __all_sync(kAll, !abort_sh && mbar_wait_bounded(&landed[s], (lph >> s) & 1, limit));
-                    if (!ok) break;
-                    lph ^= 1u << s;
-                    const int kb = it.base + t * KT;
-                    bool odd = false;
-                    constexpr int NC = HD / 8;
-                    for (int i = lane; i < KT * NC; i += 32) {
-                        const int r = i / NC, c = i % NC, k = kb + r;
-                        if (k >= max(all0, it.lo) && k < min(all1, it.hi)) continue;
-                        const uint32_t d = ring + s * C::TileB + (c >> 3) * (KT * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-                        uint4 v = make_uint4(0, 0, 0, 0);
-                        if (k >= it.lo && k < it.hi) {
-                            v = lds16(d);
-                            uint32_t *w = reinterpret_cast<uint32_t *>(&v);
-                            bool bad = false;
-                            constexpr uint32_t X = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+                    if (mixed()) {
+                        ok = __all_sync(kAll, !abort_sh && mbar_wait_bounded(&landed[s], (lph >> s) & 1, limit));
+                        if (!ok) break;
+                        lph ^= 1u << s;
+                        const int kb = it.base + t * KT;
+                        bool odd = false;
+                        constexpr int NC = HD / 8;
+                        for (int i = lane; i < KT * NC; i += 32) {
+                            const int r = i / NC, c = i % NC, k = kb + r;
+                            if (k >= max(all0, it.lo) && k < min(all1, it.hi)) continue;
+                            const uint32_t d = ring + s * C::TileB + (c >> 3) * (KT * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                            uint4 v = make_uint4(0, 0, 0, 0);
+                            if (k >= it.lo && k < it.hi) {
+                                v = lds16(d);
+                                uint32_t *w = reinterpret_cast<uint32_t *>(&v);
+                                bool bad = false;
+                                constexpr uint32_t X = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
 #pragma unroll
-                            for (int u = 0; u < 4; ++u) {
-                                if ((w[u] & X) == X) w[u] &= 0xffff0000u, bad = true;
-                                if (((w[u] >> 16) & X) == X) w[u] &= 0xffffu, bad = true;
+                                for (int u = 0; u < 4; ++u) {
+                                    if ((w[u] & X) == X) w[u] &= 0xffff0000u, bad = true;
+                                    if (((w[u] >> 16) & X) == X) w[u] &= 0xffffu, bad = true;
+                                }
+                                odd = odd || bad;
+                                if (!bad) continue;
                             }
-                            odd = odd || bad;
-                            if (!bad) continue;
+                            sts16(d, v);
                         }
-                        sts16(d, v);
+                        if (__any_sync(kAll, odd) && lane == 0) odd_sh[me] = 1;
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&full[s]);
                     }
-                    if (__any_sync(kAll, odd) && lane == 0) odd_sh[me] = 1;
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&full[s]);
+                    if (ahead) announce();
                 }
             }
         } else {
@@ -1371,7 +1375,7 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                 for (int rq = it.two ? warp * 32 : warp * 8; rq < rend; rq += step) {
                     const int ro = rq + (lane >> 2), q = (lane & 3) * 2, ch = c + 4 * q;
                     float y[8] = {};
-#pragma unroll 1
+#pragma unroll 2
                     for (int s = 0; s < sets; ++s) {
                         const int at = s * rrows + ro;
 #pragma unroll

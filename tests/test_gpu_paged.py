@@ -665,3 +665,13 @@ def test_attention_of_many_rows_that_see_nothing(dtype):
     for o, l1 in ((out[n - L:], lse[:, n - L:]), (tail, tl)):
         assert (o.double() - want).abs().max().item() <= ATT_TOL[dtype] * vmax
         assert (l1.double() - wl).abs().max().item() <= LSE_TOL
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("kv", [20, 150])
+def test_attention_of_many_short_sequences(dtype, kv):
+    """Hundreds of chunks of one or two key tiles each: several in a row for every block."""
+    n = 450
+    b = Batch(dtype, 64, 2, 16, [20 - (s % 3) for s in range(n)], [kv + (s % 7) for s in range(n)], seed=37)
+    q = (2.0 * _rand(_gen(38), sum(b.news), 4, 64)).to(DT[dtype])
+    _check(b, q)
