@@ -704,10 +704,11 @@ Plan plan_of(const altxs_paged_kv &kv, const altxs_chunks &c, int H, int window)
     const int64_t n = c.n_seqs;
     if (n == 0) return p;
     const int64_t max_new = std::max(c.max_new, 1);  // (sequences above a bound of 0 are the kernels' to report)
-    const bool same = c.n_tokens == n * max_new;     // every sequence has max_new tokens
-    p.many = max_new * G > kMaxRows;
-    const int64_t least = same ? max_new * G : G, most = max_new * G;  // rows of a sequence
-    p.few = least <= kMaxRows;
+    // The lengths are the device's: n_tokens = n max_new does not say that every sequence has max_new (rows may belong
+    // to none), so the kernel for few rows is left out only where a single token has too many of them.
+    const int64_t most = max_new * G;  // rows of a sequence
+    p.many = most > kMaxRows;
+    p.few = G <= kMaxRows;
     p.group = kv.dtype == ALTXS_F32 ? kVecRows : kMaxRows;
     p.groups = (int)((std::min<int64_t>(kMaxRows, most) + p.group - 1) / p.group);
     const int64_t keys = window > 0 ? std::min<int64_t>(c.max_kv, (int64_t)window + c.max_new - 1) : c.max_kv;

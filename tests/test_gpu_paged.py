@@ -675,3 +675,23 @@ def test_attention_of_many_short_sequences(dtype, kv):
     b = Batch(dtype, 64, 2, 16, [20 - (s % 3) for s in range(n)], [kv + (s % 7) for s in range(n)], seed=37)
     q = (2.0 * _rand(_gen(38), sum(b.news), 4, 64)).to(DT[dtype])
     _check(b, q)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("G", [1, 4, 16])
+def test_attention_of_a_padded_token_buffer(dtype, G):
+    """A buffer of n_seqs x max_new rows of which the sequences own fewer: every sequence is computed, short ones
+    included, and the rows of no sequence stay as they are."""
+    news, kvs, pad = [32, 1, 1, 0, 2, 32], [300, 70, 5, 9, 900, 600], 6 * 32
+    b = Batch(dtype, 64, 2, 16, news, kvs, seed=41)
+    q = (2.0 * _rand(_gen(42), pad, 2 * G, 64)).to(DT[dtype])
+    T = sum(news)
+    out = torch.full_like(q, 7.0)
+    b.cache.attend(b.chunks, q, out=out)
+    _, lse = b.cache.attend(b.chunks, q, return_lse=True)
+    want, wl = b.ref(q, 0.125, 0)
+    vmax = max(v.abs().max().item() for v in b.V if v.numel())
+    assert (out[:T].double() - want[:T]).abs().max().item() <= ATT_TOL[dtype] * vmax
+    assert (lse[:, :T].double() - wl[:, :T]).abs().max().item() <= LSE_TOL
+    assert (out[T:] == 7.0).all()
+    b.cache.check_status()

@@ -137,3 +137,14 @@ def test_rope_table_rules():
             paged.rope_table(4, 16, device="cpu", **kw)
     with pytest.raises(ValueError):
         paged.rope_table(4, 15, device="cpu")
+
+
+@pytest.mark.parametrize("dtype", [_lib.F32, _lib.BF16, _lib.F16])
+def test_workspace_covers_short_sequences_of_a_padded_buffer(dtype):
+    """A token buffer of n_seqs x max_new rows may hold rows of no sequence, so it says nothing about the
+    lengths: the plan for it holds what a buffer of one row less needs."""
+    L = _lib.lib()
+    size = lambda ch: L.altxs_paged_attention_workspace_bytes(C.byref(_kv(dtype=dtype)), C.byref(ch), 4, 0)  # noqa: E731
+    for new in (16, 32):
+        c = [_ch(n_seqs=4, n_tokens=4 * new - d, max_new=new, max_kv=100000, table_stride=10000) for d in (1, 0)]
+        assert size(c[1]) >= size(c[0]) > 0
