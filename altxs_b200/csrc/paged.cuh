@@ -79,9 +79,8 @@ struct ManyPlan {
     int rows;  // rows of a slot
 };
 ManyPlan paged_many_plan(const altxs_paged_kv &kv, const altxs_chunks &c, int H, int window);
-// beside: a kernel of the same call over other sequences is just ahead in the stream and need not have ended
 int launch_paged_many(const PagedAttnArgs &a, const ManyPlan &p, int min_rows, uint32_t *cnt, float *part, int sms,
-                      bool beside, cudaStream_t stream);
+                      cudaStream_t stream);
 int set_wait_limit_paged(uint32_t limit);
 int launch_paged_attention(const PagedAttnArgs &a, cudaStream_t stream);
 

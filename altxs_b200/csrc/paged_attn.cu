@@ -86,8 +86,11 @@ __device__ __forceinline__ int few_splits(const FewArgs &f, const Seq &q) {
     return split_count(max(0, q.L - first_seen(q.n, q.L, f.a.window)), few_width(f, q));
 }
 
-// The kernel for many rows may start as this one's blocks leave (they share no sequence).
-__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// The kernel for many rows, where the call has one, is just ahead in the stream and need not have ended (they share no
+// sequence): this one ends after it.
+__device__ __forceinline__ void end_after_many() {
+    if (blockIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+}
 
 __device__ __forceinline__ void scan_items(const FewArgs &f, ItemScan &sc) {
     __shared__ int wsum[kScan / 32];
@@ -333,7 +336,6 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_paged_few(const __grid_const
     const int pshift = (P & (P - 1)) == 0 ? 31 - __clz(P) : -1;
     const float c2 = __fmul_rn(a.scale, kLog2e);
     const uint32_t ring = smem_u32(few_smem) + warp * kSlots * kChunkBytes;
-    launch_dependents();
     scan_items(f, sc);
     const int total = sc.before[kScan];
 
@@ -543,6 +545,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_paged_few(const __grid_const
                            odd_sh ? &odd : nullptr);
         __syncthreads();  // before the slots and the shared words are used again
     }
+    end_after_many();
 }
 
 // fp32: half a flop a byte and row, so plain fp32 arithmetic keeps up with HBM for a few rows.  HD / 8 lanes
@@ -566,7 +569,6 @@ __global__ void __launch_bounds__(kVecWarps * 32, R == 1 ? 4 : R < 4 ? 2 : 1) k_
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kg = lane / LPK, li = lane % LPK;
     const int G = f.G, P = a.kv.page_size, pshift = (P & (P - 1)) == 0 ? 31 - __clz(P) : -1;
     const float c2 = __fmul_rn(a.scale, kLog2e);
-    launch_dependents();
     scan_items(f, sc);
     const int total = sc.before[kScan];
     for (int item = blockIdx.x; item < total; item += gridDim.x) {
@@ -684,6 +686,7 @@ __global__ void __launch_bounds__(kVecWarps * 32, R == 1 ? 4 : R < 4 ? 2 : 1) k_
         finish_item<float, HD>(f, item, at, nsplit, n, Sets, R, rows, ml, &last_sh, nullptr);
         __syncthreads();  // before the shared rows are used again
     }
+    end_after_many();
 }
 
 // Workspace: arrival counters (zero between calls: a call's last arrivals reset
@@ -734,6 +737,23 @@ int sm_count() {
     return sms[dev] > 0 ? sms[dev] : 148;
 }
 
+// beside: the kernel for many rows is just ahead in the stream and need not have ended
+int launch_few(void (*k)(FewArgs), const FewArgs &f, unsigned grid, int threads, int smem, bool beside, cudaStream_t st) {
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = threads;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = &early;
+    cfg.numAttrs = beside ? 1 : 0;
+    if (beside) cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
+    ALTXS_LAUNCH(kKPaged, st, cudaLaunchKernelEx(&cfg, k, f));
+    return ALTXS_OK;
+}
+
 template <typename T, int HD>
 int launch(const PagedAttnArgs &a, const Plan &p, cudaStream_t st) {
     unsigned char *ws = static_cast<unsigned char *>(a.ws);
@@ -750,30 +770,27 @@ int launch(const PagedAttnArgs &a, const Plan &p, cudaStream_t st) {
     }
     const FewArgs f{a, a.H / a.kv.n_kv_heads, 1, kMaxRows, p.group, p.bytes > 0 ? p.items : 0, few_cnt, p.groups, part, p.part_rows};
     const int64_t sms = sm_count();
-    if (p.few) {
-        if constexpr (std::is_same<T, float>::value) {
-            const int64_t most = (int64_t)a.c.max_new * f.G;  // rows
-            const unsigned grid = (unsigned)std::min<int64_t>(p.items, (most == 1 ? 4 : most <= 2 ? 2 : 1) * sms);
-            if (most == 1) ALTXS_LAUNCH(kKPaged, st, k_paged_vec<HD, 1><<<grid, kVecWarps * 32, 0, st>>>(f));
-            else if (most == 2) ALTXS_LAUNCH(kKPaged, st, k_paged_vec<HD, 2><<<grid, kVecWarps * 32, 0, st>>>(f));
-            else if (most <= 4) ALTXS_LAUNCH(kKPaged, st, k_paged_vec<HD, 4><<<grid, kVecWarps * 32, 0, st>>>(f));
-            else ALTXS_LAUNCH(kKPaged, st, k_paged_vec<HD, 8><<<grid, kVecWarps * 32, 0, st>>>(f));
-        } else {
-            constexpr int smem = kWarps * kSlots * kChunkBytes;
-            static std::atomic<uint64_t> set{0};  // devices whose shared-memory limit is raised
-            int dev = 0;
-            if (cudaGetDevice(&dev) != cudaSuccess) return ALTXS_ECUDA;
-            if (dev >= 64 || !((set.load() >> dev) & 1)) {
-                if (cudaFuncSetAttribute(k_paged_few<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-                    return ALTXS_ECUDA;
-                if (dev < 64) set.fetch_or(1ull << dev);
-            }
-            const unsigned grid = (unsigned)std::min<int64_t>(p.items, 2 * sms);
-            ALTXS_LAUNCH(kKPaged, st, k_paged_few<T, HD><<<grid, kWarps * 32, smem, st>>>(f));
+    if (p.many)
+        if (const int rc = launch_paged_many(a, p.mp, kMaxRows + 1, many_cnt, many_part, (int)sms, st)) return rc;
+    if (!p.few) return ALTXS_OK;
+    if constexpr (std::is_same<T, float>::value) {
+        const int64_t most = (int64_t)a.c.max_new * f.G;  // rows
+        const unsigned grid = (unsigned)std::min<int64_t>(p.items, (most == 1 ? 4 : most <= 2 ? 2 : 1) * sms);
+        constexpr int n = kVecWarps * 32;
+        return most == 1 ? launch_few(k_paged_vec<HD, 1>, f, grid, n, 0, p.many, st) : most == 2 ? launch_few(k_paged_vec<HD, 2>, f, grid, n, 0, p.many, st)
+               : most <= 4 ? launch_few(k_paged_vec<HD, 4>, f, grid, n, 0, p.many, st) : launch_few(k_paged_vec<HD, 8>, f, grid, n, 0, p.many, st);
+    } else {
+        constexpr int smem = kWarps * kSlots * kChunkBytes;
+        static std::atomic<uint64_t> set{0};  // devices whose shared-memory limit is raised
+        int dev = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess) return ALTXS_ECUDA;
+        if (dev >= 64 || !((set.load() >> dev) & 1)) {
+            if (cudaFuncSetAttribute(k_paged_few<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+                return ALTXS_ECUDA;
+            if (dev < 64) set.fetch_or(1ull << dev);
         }
+        return launch_few(k_paged_few<T, HD>, f, (unsigned)std::min<int64_t>(p.items, 2 * sms), kWarps * 32, smem, p.many, st);
     }
-    if (p.many) return launch_paged_many(a, p.mp, kMaxRows + 1, many_cnt, many_part, (int)sms, p.few, st);
-    return ALTXS_OK;
 }
 template <typename T>
 int launch(const PagedAttnArgs &a, const Plan &p, cudaStream_t st) {

@@ -457,6 +457,8 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
     const uint32_t sq = raw_s + ((1024u - (raw_s & 1023u)) & 1023u), ring = sq + C::QB;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t limit = wait_limit();
+    // the kernel for few rows (it shares no sequence with this one) may start as these blocks leave
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (tid == 0) {
         for (int s = 0; s < C::Slots; ++s) {
             mbar_init(&full[s], F32 ? C::Converters : 1);
@@ -1499,8 +1501,6 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }
-    // the kernel that this one may run beside has ended before this one does
-    asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // [pages][heads][positions][channels] of a pool as it lies, boxes of `run` positions x 64 channels (fp32: all)
@@ -1521,7 +1521,7 @@ bool pool_map(CUtensorMap *m, const altxs_paged_kv &kv, void *pool, int run) {
 }
 
 template <typename T, int HD>
-int launch(const ManyArgs &f, unsigned grid, bool beside, cudaStream_t st) {
+int launch(const ManyArgs &f, unsigned grid, cudaStream_t st) {
     CUtensorMap tk{}, tv{};
     if ((!pool_map(&tk, f.a.kv, f.a.kv.k, f.run) || !pool_map(&tv, f.a.kv, f.a.kv.v, f.run))) return ALTXS_ECUDA;
     static std::atomic<uint64_t> set{0};  // devices whose shared-memory limit is raised
@@ -1532,23 +1532,13 @@ int launch(const ManyArgs &f, unsigned grid, bool beside, cudaStream_t st) {
             return ALTXS_ECUDA;
         if (dev < 64) set.fetch_or(1ull << dev);
     }
-    cudaLaunchAttribute early{};
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = Tc<T, HD>::Threads;
-    cfg.dynamicSmemBytes = Tc<T, HD>::Smem;
-    cfg.stream = st;
-    cfg.attrs = &early;
-    cfg.numAttrs = beside ? 1 : 0;
-    ALTXS_LAUNCH(kKPaged, st, cudaLaunchKernelEx(&cfg, k_paged_many<T, HD>, f, tk, tv));
+    ALTXS_LAUNCH(kKPaged, st, k_paged_many<T, HD><<<grid, Tc<T, HD>::Threads, Tc<T, HD>::Smem, st>>>(f, tk, tv));
     return ALTXS_OK;
 }
 template <typename T>
-int launch(const ManyArgs &f, unsigned grid, bool beside, cudaStream_t st) {
+int launch(const ManyArgs &f, unsigned grid, cudaStream_t st) {
     const int hd = f.a.kv.head_dim;
-    return hd == 32 ? launch<T, 32>(f, grid, beside, st) : hd == 64 ? launch<T, 64>(f, grid, beside, st) : launch<T, 128>(f, grid, beside, st);
+    return hd == 32 ? launch<T, 32>(f, grid, st) : hd == 64 ? launch<T, 64>(f, grid, st) : launch<T, 128>(f, grid, st);
 }
 
 }  // namespace
@@ -1568,12 +1558,12 @@ ManyPlan paged_many_plan(const altxs_paged_kv &kv, const altxs_chunks &c, int H,
 }
 
 int launch_paged_many(const PagedAttnArgs &a, const ManyPlan &p, int min_rows, uint32_t *cnt, float *part, int sms,
-                      bool beside, cudaStream_t st) {
+                      cudaStream_t st) {
     const int run = std::min(tile_keys(a.kv.dtype, a.kv.head_dim), a.kv.page_size & -a.kv.page_size);
     const ManyArgs f{a, a.H / a.kv.n_kv_heads, min_rows, run < 4 ? 1 : run, p.slots, cnt + 1, cnt, part, p.rows};
     const unsigned grid = (unsigned)std::min<int64_t>(p.items, sms);
-    if (a.kv.dtype == ALTXS_F32) return launch<float>(f, grid, beside, st);
-    return a.kv.dtype == ALTXS_BF16 ? launch<__nv_bfloat16>(f, grid, beside, st) : launch<__half>(f, grid, beside, st);
+    if (a.kv.dtype == ALTXS_F32) return launch<float>(f, grid, st);
+    return a.kv.dtype == ALTXS_BF16 ? launch<__nv_bfloat16>(f, grid, st) : launch<__half>(f, grid, st);
 }
 
 int set_wait_limit_paged(uint32_t limit) {
