@@ -485,13 +485,15 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_paged_few(const __grid_const
                 }
             l[0] = __fadd_rn(l[0], sum[0]);
             l[1] = __fadd_rn(l[1], sum[1]);
-            // Some rows do not see some of these values: one that is not finite must not meet
-            // their p = 0.  It becomes 0 here and is added to the rows that see it at the end.
+            // Some rows do not see some of these values: one of those that is not finite must not
+            // meet their p = 0.  It becomes 0 here and is added to the rows that see it at the end.
             if (!whole && q.n > 1) {
                 bool odd = false;
 #pragma unroll
                 for (int i = 0; i < CK * NC / 32; ++i) {
                     const uint32_t d = vt + (i * 32 + lane) * 16;
+                    const int k = kc + (i * 32 + lane) / NC;
+                    if (k >= all0 && k < all1) continue;  // every row sees it
                     uint32_t w[4];
                     lds128(d, w);
                     bool bad = false;

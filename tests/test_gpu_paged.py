@@ -695,3 +695,30 @@ def test_attention_of_a_padded_token_buffer(dtype, G):
     assert (lse[:, :T].double() - wl[:, :T]).abs().max().item() <= LSE_TOL
     assert (out[T:] == 7.0).all()
     b.cache.check_status()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("n", [2, 4, 7, 8])
+def test_attention_keeps_what_every_row_sees(dtype, hd, n):
+    """A NaN and an infinity among the values that all rows see, next to positions that only some see, reach
+    every row; one in the last token's value reaches the last row alone."""
+    L = 300
+    b = Batch(dtype, hd, 2, 16, [n], [L], seed=43)
+    q = (0.1 * _rand(_gen(44), n, 4, hd)).to(DT[dtype])  # even weights: none of them is 0
+    for window in (0, 150):
+        want, _ = b.ref(q, hd ** -0.5, window)
+        first = L - window if window else 0  # what the last row, so every row, sees begins here
+        for p, c, x in ((L - n - 1, 3, float("nan")), (L - n, 5, float("inf")), (first + 1, 7, -float("inf")),
+                        (L - 1, 9, float("inf"))):
+            page, slot = b.slots(0, p, p + 1)
+            b.cache.v[page, slot, :, c] = x
+        out = b.cache.attend(b.chunks, q, window=window).double()
+        assert torch.isnan(out[:, :, 3]).all()
+        assert (out[:, :, 5] == math.inf).all() and (out[:, :, 7] == -math.inf).all()
+        assert torch.isfinite(out[:-1, :, 9]).all() and (out[-1, :, 9] == math.inf).all()
+        rest = [c for c in range(hd) if c not in (3, 5, 7, 9)]
+        vmax = b.V[0].abs().max().item()
+        assert (out - want)[:, :, rest].abs().max().item() <= ATT_TOL[dtype] * vmax
+        b.fill(0, 0, L)
+    b.cache.check_status()
