@@ -335,6 +335,9 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_paged_few(const __grid_const
     const int Hkv = a.kv.n_kv_heads, G = f.G, P = a.kv.page_size;
     const int pshift = (P & (P - 1)) == 0 ? 31 - __clz(P) : -1;
     const float c2 = __fmul_rn(a.scale, kLog2e);
+    // fp16 ends at 2^-24: p carries 2^14 (and is at most that), so that what a dominant key leaves to each of many
+    // others is not rounded to 0 while the row's sum has it
+    constexpr float kBias = std::is_same<T, __half>::value ? 14.0f : 0.0f, unbias = std::is_same<T, __half>::value ? 1.0f / 16384.0f : 1.0f;
     const uint32_t ring = smem_u32(few_smem) + warp * kSlots * kChunkBytes;
     scan_items(f, sc);
     const int total = sc.before[kScan];
@@ -467,7 +470,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_paged_few(const __grid_const
                 const float base = mx[hh] == -INFINITY ? 0.0f : mx[hh];  // nothing seen yet: every p is 2^-inf = 0
                 const float fold = ex2(__fsub_rn(m[hh], base));
                 m[hh] = mx[hh];
-                mx[hh] = base;
+                mx[hh] = __fsub_rn(base, kBias);
                 l[hh] = __fmul_rn(l[hh], fold);
 #pragma unroll
                 for (int t = 0; t < NO; ++t) {
@@ -536,11 +539,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_paged_few(const __grid_const
             l[hh] = __fadd_rn(l[hh], __shfl_xor_sync(kAll, l[hh], 2));
             const int r = quad + 8 * hh;
             if (r >= R) continue;
-            if (j == 0) ml_sh[warp][r][0] = m[hh], ml_sh[warp][r][1] = l[hh];
+            if (j == 0) ml_sh[warp][r][0] = m[hh], ml_sh[warp][r][1] = __fmul_rn(l[hh], unbias);
             float *y = rows + (warp * kMaxRows + r) * HD;
 #pragma unroll
             for (int t = 0; t < NO; ++t)
-                *reinterpret_cast<float2 *>(y + 8 * t + 2 * j) = make_float2(o[t][2 * hh], o[t][2 * hh + 1]);
+                *reinterpret_cast<float2 *>(y + 8 * t + 2 * j) = make_float2(__fmul_rn(o[t][2 * hh], unbias), __fmul_rn(o[t][2 * hh + 1], unbias));
         }
         __syncthreads();
         finish_item<T, HD>(f, item, at, nsplit, R, kWarps, kMaxRows, rows, &ml_sh[0][0][0], &last_sh,

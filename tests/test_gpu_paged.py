@@ -722,3 +722,23 @@ def test_attention_keeps_what_every_row_sees(dtype, hd, n):
         assert (out - want)[:, :, rest].abs().max().item() <= ATT_TOL[dtype] * vmax
         b.fill(0, 0, L)
     b.cache.check_status()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("n,G", [(1, 2), (4, 4), (20, 1), (20, 16)])
+def test_attention_of_a_long_context_behind_one_key(dtype, n, G):
+    """One key takes all but 2^-25.5 of each of 60000 others: those weigh 0.13 % together.  Relative error of their
+    part: p rounded once (2^-11, and 2^-10.5 where fp16 has left its normal range; 2^-8 for bf16), the result once."""
+    L = 60000
+    b = Batch(dtype, 64, 1, 64, [n], [L], seed=45)
+    b.K[0].zero_()
+    b.V[0].fill_(1.0)
+    b.K[0][0, 0, 0], b.V[0][0] = 1131 / 256 if dtype == "f16" else 4.40625, 0.0
+    b.fill(0, 0, L)
+    q = torch.zeros(n, G, 64, device=DEV).to(DT[dtype])
+    q[:, :, 0] = 4.0
+    want, wl = b.ref(q, 1.0, 0)
+    out, lse = b.cache.attend(b.chunks, q, scale=1.0, return_lse=True)
+    assert 1e-3 < want.min().item() and want.max().item() < 2e-3
+    assert ((out.double() - want) / want).abs().max().item() <= {"f16": 2.0 ** -9, "bf16": 2.0 ** -7}[dtype]
+    assert (lse.double() - wl).abs().max().item() <= LSE_TOL
