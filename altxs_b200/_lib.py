@@ -17,6 +17,7 @@ ALTXS_EINVAL, ALTXS_ENOSPC, ALTXS_ENOTSUP, ALTXS_ECUDA, ALTXS_ENOMEM = -22, -28,
 ST_OVERFLOW, ST_BAD_SYMBOL, ST_BAD_TOTAL, ST_NONFINITE, ST_TIMEOUT, ST_BAD_POS = 1, 2, 4, 8, 16, 32
 CDF_FIXED, CDF_REF = 0, 1
 F32, BF16, F16 = 0, 1, 2
+PAGED_COUNTER_BYTES = 524288
 STEP_LOGITS, STEP_ENCODE, STEP_DECODE = 0, 1, 2
 
 EXPORTS = (

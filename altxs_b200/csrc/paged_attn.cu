@@ -696,7 +696,8 @@ __global__ void __launch_bounds__(kVecWarps * 32, R == 1 ? 4 : R < 4 ? 2 : 1) k_
 
 // Workspace: arrival counters (zero between calls: a call's last arrivals reset
 // them), then partial rows.
-constexpr int64_t kCounters = 65536;  // more than these are cleared by the call that needs them
+constexpr int64_t kCounters = 65536;  // more than these of a kind are cleared by the call that needs them
+static_assert(2 * 4 * kCounters == ALTXS_PAGED_COUNTER_BYTES, "what the caller zeroes");
 
 struct Plan {
     bool few, many;       // which kernels the host's bounds allow work for

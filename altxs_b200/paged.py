@@ -150,6 +150,13 @@ def rope_backward(dy: torch.Tensor, rotary: Rotary, pos: torch.Tensor, out: torc
     return _rope(dy, rotary, pos, out, 1)
 
 
+def _workspace(need: int, device: torch.device) -> torch.Tensor:
+    """A new workspace of the attention: its counters are zero, the rest needs no value."""
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=device)
+    ws[:_lib.PAGED_COUNTER_BYTES].zero_()
+    return ws
+
+
 class Chunks:
     """The new tokens of a batch of sequences (``altxs_chunks``).
 
@@ -273,7 +280,7 @@ class PagedKV:
         if ws is None or ws.numel() < need:
             if need < 0:
                 _lib.check(_lib.ALTXS_EINVAL, "altxs_paged_attention_workspace_bytes")
-            ws = self._ws[st] = torch.zeros(max(need, 16), dtype=torch.uint8, device=self.device)
+            ws = self._ws[st] = _workspace(need, self.device)
         rc = L.altxs_paged_attention(self._ref, cref, H, self.head_dim ** -0.5 if scale is None else scale, window,
                                      q.data_ptr(), ldq, out.data_ptr(), ldo, lse.data_ptr() if return_lse else None,
                                      ws.data_ptr(), ws.numel(), st)

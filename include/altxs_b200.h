@@ -574,11 +574,13 @@ int altxs_paged_append(const altxs_paged_kv *kv, const altxs_chunks *c, const al
  * lse: optional device [n_heads][n_tokens], log2 of each row's sum of
  * 2^(scale * log2(e) * q . K) (-inf for a row that sees nothing).  Positions on
  * a page out of range (ALTXS_ST_BAD_POS) count as unseen.  A row's result does
- * not depend on the other sequences of the call.  The workspace (16-byte
- * aligned) must be zeroed before its first use; a call leaves it ready for the
+ * not depend on the other sequences of the call.  The first
+ * ALTXS_PAGED_COUNTER_BYTES of the workspace (16-byte aligned; all of it where it
+ * is smaller) must be zero before its first use; a call leaves it ready for the
  * next one on the same stream, of any shape it is large enough for (after
- * ALTXS_ST_TIMEOUT, zero it again).  Results are finite where the inputs a row
+ * ALTXS_ST_TIMEOUT, zero them again).  Results are finite where the inputs a row
  * sees are: NaN and infinities that its mask hides do not reach it. */
+#define ALTXS_PAGED_COUNTER_BYTES 524288
 int64_t altxs_paged_attention_workspace_bytes(const altxs_paged_kv *kv, const altxs_chunks *c, int n_heads,
                                               int window);
 int altxs_paged_attention(const altxs_paged_kv *kv, const altxs_chunks *c, int n_heads, float scale, int window,

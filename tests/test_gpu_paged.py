@@ -742,3 +742,25 @@ def test_attention_of_a_long_context_behind_one_key(dtype, n, G):
     assert 1e-3 < want.min().item() and want.max().item() < 2e-3
     assert ((out.double() - want) / want).abs().max().item() <= {"f16": 2.0 ** -9, "bf16": 2.0 ** -7}[dtype]
     assert (lse.double() - wl).abs().max().item() <= LSE_TOL
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attention_needs_zeros_in_its_counters_alone(dtype):
+    """The rest of a workspace may hold anything: splits of few and of many rows, and more counters than the
+    caller zeroes."""
+    b = Batch(dtype, 64, 4, 64, [1, 40], [4000, 6000], seed=47)
+    n = _lib.PAGED_COUNTER_BYTES // 32 + 1  # sequences, on the same pages, of four heads: counters beyond the bound
+    one = Batch(dtype, 64, 4, 64, [1], [513], seed=48)
+    many = paged.Chunks(torch.arange(n + 1, dtype=torch.int32, device=DEV), one.kv_len.repeat(n), one.tab.repeat(n, 1),
+                        max_new=1, max_kv=513)
+    for cache, chunks, rows in ((b.cache, b.chunks, 41), (one.cache, many, n)):
+        q = (2.0 * _rand(_gen(49), rows, 8, 64)).to(DT[dtype])
+        want = cache.attend(chunks, q)
+        (ws,) = cache._ws.values()
+        assert ws.numel() > _lib.PAGED_COUNTER_BYTES
+        ws.fill_(0xff)
+        ws[:_lib.PAGED_COUNTER_BYTES].zero_()
+        for _ in range(2):
+            assert torch.equal(cache.attend(chunks, q), want)
+        assert torch.isfinite(want).all()
+        cache.check_status()

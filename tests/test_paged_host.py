@@ -148,3 +148,9 @@ def test_workspace_covers_short_sequences_of_a_padded_buffer(dtype):
     for new in (16, 32):
         c = [_ch(n_seqs=4, n_tokens=4 * new - d, max_new=new, max_kv=100000, table_stride=10000) for d in (1, 0)]
         assert size(c[1]) >= size(c[0]) > 0
+
+
+def test_a_new_workspace_has_zero_counters():
+    for need in (0, 1000, _lib.PAGED_COUNTER_BYTES + 4096):
+        ws = paged._workspace(need, torch.device("cpu"))
+        assert ws.numel() == max(need, 16) and not ws[:_lib.PAGED_COUNTER_BYTES].any()
