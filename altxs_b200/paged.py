@@ -227,6 +227,16 @@ class PagedKV:
         c.struct.status = self.status.data_ptr()
         return c._ref
 
+    def _workspace_for(self, need: int, stream: int) -> torch.Tensor:
+        """One workspace per stream.  A call that is captured has its own, from the graph's memory and cleared in
+        the graph: it lives as long as the graph does, and no other call, captured or not, meets its counters."""
+        if torch.cuda.is_current_stream_capturing():
+            return _workspace(need, self.device)
+        ws = self._ws.get(stream)
+        if ws is None or ws.numel() < need:
+            ws = self._ws[stream] = _workspace(need, self.device)
+        return ws
+
     def append(self, chunks: Chunks, k: torch.Tensor, v: torch.Tensor, *, rotary: Rotary | None = None,
                q: torch.Tensor | None = None, positions: torch.Tensor | None = None,
                q_out: torch.Tensor | None = None) -> torch.Tensor | None:
@@ -276,14 +286,12 @@ class PagedKV:
         L = _lib.lib()
         cref, st = self._chunks(chunks, n), _stream_handle(self.device)
         need = L.altxs_paged_attention_workspace_bytes(self._ref, cref, H, window)
-        ws = self._ws.get(st)
-        if ws is None or ws.numel() < need:
-            if need < 0:
-                _lib.check(_lib.ALTXS_EINVAL, "altxs_paged_attention_workspace_bytes")
-            ws = self._ws[st] = _workspace(need, self.device)
+        if need < 0:
+            _lib.check(_lib.ALTXS_EINVAL, "altxs_paged_attention_workspace_bytes")
+        ws = self._workspace_for(need, st) if need else None
         rc = L.altxs_paged_attention(self._ref, cref, H, self.head_dim ** -0.5 if scale is None else scale, window,
                                      q.data_ptr(), ldq, out.data_ptr(), ldo, lse.data_ptr() if return_lse else None,
-                                     ws.data_ptr(), ws.numel(), st)
+                                     ws.data_ptr() if need else None, ws.numel() if need else 0, st)
         _lib.check(rc, "altxs_paged_attention")
         return (out, lse) if return_lse else out
 

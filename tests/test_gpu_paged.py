@@ -764,3 +764,40 @@ def test_attention_needs_zeros_in_its_counters_alone(dtype):
             assert torch.equal(cache.attend(chunks, q), want)
         assert torch.isfinite(want).all()
         cache.check_status()
+
+
+def test_graphs_keep_their_workspaces():
+    """Two graphs from one stream whose first call is the first's capture; then larger calls on that stream, other
+    tensors in what memory is free, and replays in both orders and on another stream."""
+    b = Batch("bf16", 64, 2, 16, [1, 40, 1], [3000, 5000, 90], seed=51)
+    q = [(2.0 * _rand(_gen(52 + i), 42, 4, 64)).bfloat16() for i in range(2)]
+    want = [b.cache.attend(b.chunks, x) for x in q]
+    big = Batch("bf16", 64, 2, 16, [1] * 8 + [300], [9000] * 9, seed=53)
+    bq = _rand(_gen(54), 308, 4, 64).bfloat16()
+    bw = big.cache.attend(big.chunks, bq)
+    cache = paged.PagedKV(b.cache.k, b.cache.v)
+    s, other = torch.cuda.Stream(), torch.cuda.Stream()
+    graphs, outs = [], [torch.zeros_like(x) for x in want]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        for x, o in zip(q, outs):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=s):
+                cache.attend(b.chunks, x, out=o)
+            graphs.append(g)
+        assert torch.equal(cache.attend(b.chunks, q[0]), want[0])  # before any replay
+        far = paged.PagedKV(big.cache.k, big.cache.v)
+        far._ws = cache._ws  # (the same stream's)
+        assert torch.equal(far.attend(big.chunks, bq), bw)
+        junk = [torch.full((1 << 20,), 0xff, dtype=torch.uint8, device=DEV) for _ in range(32)]
+        s.synchronize()
+    for order in ((1, 0), (0, 1), (1, 1), (0, 0)):
+        for i in order:
+            outs[i].zero_()
+            torch.cuda.synchronize()
+            with torch.cuda.stream(other):
+                graphs[i].replay()
+            torch.cuda.synchronize()
+            assert torch.equal(outs[i], want[i])
+    assert all((j == 0xff).all() for j in junk)
+    cache.check_status()

@@ -154,3 +154,21 @@ def test_a_new_workspace_has_zero_counters():
     for need in (0, 1000, _lib.PAGED_COUNTER_BYTES + 4096):
         ws = paged._workspace(need, torch.device("cpu"))
         assert ws.numel() == max(need, 16) and not ws[:_lib.PAGED_COUNTER_BYTES].any()
+
+
+def test_a_captured_call_has_a_workspace_of_its_own(monkeypatch):
+    """What a graph holds is neither kept for other calls nor replaced by them: a larger call, or a cache whose
+    status raised, must not give away memory that a graph still writes."""
+    cache = object.__new__(paged.PagedKV)
+    cache.device, cache._ws = torch.device("cpu"), {}
+    capturing = False
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing)
+    eager = cache._workspace_for(1000, 7)
+    assert cache._workspace_for(900, 7) is eager and cache._workspace_for(900, 8) is not eager
+    capturing = True
+    first, second = cache._workspace_for(900, 7), cache._workspace_for(900, 7)
+    assert first is not second and first is not eager and not first.any() and cache._ws[7] is eager
+    assert cache._workspace_for(900, 9) is not None and 9 not in cache._ws
+    capturing = False
+    bigger = cache._workspace_for(5000, 7)
+    assert cache._ws[7] is bigger and bigger.numel() >= 5000
