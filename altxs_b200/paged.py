@@ -31,6 +31,7 @@ import torch
 
 from . import _lib
 
+_GROWTH = 64 << 20  # bytes that a workspace grows by at most beyond what a call needs
 _DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
 
@@ -233,8 +234,9 @@ class PagedKV:
         if torch.cuda.is_current_stream_capturing():
             return _workspace(need, self.device)
         ws = self._ws.get(stream)
-        if ws is None or ws.numel() < need:
-            ws = self._ws[stream] = _workspace(need, self.device)
+        if ws is None or ws.numel() < need:  # with room for the next steps of growing streams
+            more = 0 if ws is None else ws.numel() + min(ws.numel() // 2, _GROWTH)
+            ws = self._ws[stream] = _workspace(max(need, more), self.device)
         return ws
 
     def append(self, chunks: Chunks, k: torch.Tensor, v: torch.Tensor, *, rotary: Rotary | None = None,

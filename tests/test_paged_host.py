@@ -172,3 +172,21 @@ def test_a_captured_call_has_a_workspace_of_its_own(monkeypatch):
     capturing = False
     bigger = cache._workspace_for(5000, 7)
     assert cache._ws[7] is bigger and bigger.numel() >= 5000
+
+
+def test_workspaces_of_growing_streams_are_not_replaced_at_every_step(monkeypatch):
+    """256 streams of eight heads of 64, a token at a time from 600 positions on, sized by their total as the allocator
+    gives it: the need grows at most steps, the workspace seldom."""
+    cache = object.__new__(paged.PagedKV)
+    cache.device, cache._ws = torch.device("cpu"), {}
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    needs, sizes = [], []
+    for step in range(0, 2000, 16):
+        ch = _ch(n_seqs=256, n_tokens=256, max_kv=600 + step, table_stride=1000, total_kv=256 * (600 + step))
+        needs.append(_lib.lib().altxs_paged_attention_workspace_bytes(C.byref(_kv(n_kv_heads=8)), C.byref(ch), 8, 0))
+        sizes.append(cache._workspace_for(needs[-1], 0).numel())
+        assert sizes[-1] >= needs[-1] > 0
+    assert len(set(needs)) > 50 and len(set(sizes)) <= 5 and sizes[-1] <= 1.5 * needs[-1]
+    huge = max(needs[-1] * 100, 1 << 30)
+    cache._ws[0] = torch.empty(0, dtype=torch.uint8).new_empty(huge)
+    assert cache._workspace_for(huge + 1, 0).numel() <= huge + (64 << 20)
