@@ -342,7 +342,11 @@ class PageAllocator:
 
     def trim(self, seq: int, window: int) -> int:
         """Takes back the pages that no later token of a ``window``-wide attention
-        sees; returns how many."""
+        sees (``window`` 0 sees everything); returns how many."""
+        if window < 0:
+            raise ValueError("window must be >= 0")
+        if window == 0:
+            return 0
         first = max(0, int(self.len[seq]) + 1 - window) // self.page_size  # block of the next token's first position
         n = 0
         for b in range(first):

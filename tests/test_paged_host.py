@@ -190,3 +190,14 @@ def test_workspaces_of_growing_streams_are_not_replaced_at_every_step(monkeypatc
     huge = max(needs[-1] * 100, 1 << 30)
     cache._ws[0] = torch.empty(0, dtype=torch.uint8).new_empty(huge)
     assert cache._workspace_for(huge + 1, 0).numel() <= huge + (64 << 20)
+
+
+def test_trim_of_a_window_that_sees_everything():
+    """Window 0 sees everything, as in attend: nothing comes back; a negative one is refused."""
+    a = paged.PageAllocator(1, 6, 4, 20, "cpu")
+    a.extend([17])
+    before = a.table.copy()
+    assert a.trim(0, 0) == 0 and (a.table == before).all() and len(a.free) == 1
+    with pytest.raises(ValueError, match="window"):
+        a.trim(0, -1)
+    assert (a.table == before).all() and a.trim(0, 1) == 4
