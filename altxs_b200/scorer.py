@@ -13,7 +13,8 @@ the stream lengths.
 
 The linears run on the library's mixed-bit kernels, keys and values are rotated
 and stored by ``PagedKV.append`` and read by ``PagedKV.attend`` in fp32.
-Adapters are not applied; models with motifs are refused.
+Adapters are not applied; models with motifs, or whose context is rebuilt at every
+segment (``context_mode="reset"``), are refused.
 """
 
 from __future__ import annotations
@@ -41,6 +42,8 @@ class PagedScorer:
         if (cfg.smear_gate_enabled or cfg.xsa_last_n or cfg.sparse_attn_gate_enabled or cfg.asym_logit_rescale
                 or cfg.num_loops or cfg.parallel_start_layer):
             raise ValueError("PagedScorer runs plain models only (no motifs)")
+        if cfg.context_mode != "sliding":
+            raise ValueError(f"PagedScorer scores with a sliding window, not context_mode={cfg.context_mode!r}")
         if chunk < 1 or max_len < 1 or n_streams < 1:
             raise ValueError("chunk, max_len and n_streams must be positive")
         self.dm, self.cfg, self.n, self.chunk, self.window = dm, cfg, int(n_streams), int(chunk), int(cfg.ctx)

@@ -201,3 +201,21 @@ def test_trim_of_a_window_that_sees_everything():
     with pytest.raises(ValueError, match="window"):
         a.trim(0, -1)
     assert (a.table == before).all() and a.trim(0, 1) == 4
+
+
+def _plain_cfg(**kw):
+    from altxs_b200.config import ModelConfig
+
+    d = dict(vocab_size=512, num_layers=3, model_dim=128, num_heads=4, num_kv_heads=2, mlp_mult=4.0, rope_dims=16,
+             block_size=48, online_retrain_every=64, seed=11, retrain_mode="none")
+    return ModelConfig(**{**d, **kw})
+
+
+def test_the_scorer_refuses_reset_contexts():
+    """It scores with a sliding window: a model whose context is rebuilt at every segment costs other bits."""
+    from types import SimpleNamespace
+
+    from altxs_b200.scorer import PagedScorer
+
+    with pytest.raises(ValueError, match="context_mode"):
+        PagedScorer(SimpleNamespace(cfg=_plain_cfg(context_mode="reset")), 1, 64)
