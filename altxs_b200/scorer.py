@@ -44,6 +44,8 @@ class PagedScorer:
             raise ValueError("PagedScorer runs plain models only (no motifs)")
         if cfg.context_mode != "sliding":
             raise ValueError(f"PagedScorer scores with a sliding window, not context_mode={cfg.context_mode!r}")
+        if cfg.head_dim not in (32, 64, 128):
+            raise ValueError(f"the paged cache has heads of 32, 64 or 128 channels, not {cfg.head_dim}")
         if chunk < 1 or max_len < 1 or n_streams < 1:
             raise ValueError("chunk, max_len and n_streams must be positive")
         self.dm, self.cfg, self.n, self.chunk, self.window = dm, cfg, int(n_streams), int(chunk), int(cfg.ctx)

@@ -219,3 +219,15 @@ def test_the_scorer_refuses_reset_contexts():
 
     with pytest.raises(ValueError, match="context_mode"):
         PagedScorer(SimpleNamespace(cfg=_plain_cfg(context_mode="reset")), 1, 64)
+
+
+def test_the_scorer_refuses_head_sizes_without_a_kernel():
+    """At construction, not in the first append after pages were granted."""
+    from types import SimpleNamespace
+
+    from altxs_b200.scorer import PagedScorer
+
+    cfg = _plain_cfg(model_dim=192)  # heads of 48
+    cfg.validate()
+    with pytest.raises(ValueError, match="head"):
+        PagedScorer(SimpleNamespace(cfg=cfg), 1, 64)
