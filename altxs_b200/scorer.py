@@ -58,12 +58,16 @@ class PagedScorer:
         self.caches = [PagedKV.empty(n_pages, page_size, cfg.num_kv_heads, cfg.head_dim, device=dm.device)
                        for _ in range(cfg.num_layers)]
         emb = dm.q["emb"]
-        self.emb = torch.empty((emb.rows, emb.cols), dtype=torch.float32, device=dm.device)
-        if dm.full_params:
-            self.emb.copy_(dm.params[dm.layout.emb:dm.layout.emb + self.emb.numel()].view_as(self.emb))
+        if dm.full_params:  # the arena's own: an update between calls changes it
+            self.emb = dm.arena("emb").view(emb.rows, emb.cols)
         else:
+            self.emb = torch.empty((emb.rows, emb.cols), dtype=torch.float32, device=dm.device)
             _lib.check(_lib.lib().altxs_dequant(C.byref(emb), self.emb.data_ptr(), emb.cols, _stream_handle(dm.device)),
                        "altxs_dequant")
+        layers, d = cfg.num_layers, cfg.model_dim
+        shapes = {"q_gain": (layers, cfg.num_heads), "attn_scale": (layers, d), "mlp_scale": (layers, d),
+                  "resid_mix": (layers, 2, d), "ln_scale": (layers,), "skip_weights": (-1, d), "skip_gates": (-1, d)}
+        self.small = {k: dm.small[k].view(shape) for k, shape in shapes.items()}  # (an arena's are flat)
         self._ws = torch.empty(0, dtype=torch.uint8, device=dm.device)
 
     def _linear(self, name: str, row0: int, rows: int, x: torch.Tensor) -> torch.Tensor:
@@ -80,7 +84,7 @@ class PagedScorer:
     def advance(self, new: Sequence[np.ndarray]) -> torch.Tensor:
         """Consumes ``new[s]`` (any number of symbols, also none) of every stream and
         returns the logits after each: ``[sum of lengths][vocab]``, stream by stream."""
-        cfg, sm, dev = self.cfg, self.dm.small, self.dm.device
+        cfg, sm, dev = self.cfg, self.small, self.dm.device
         lens = [len(a) for a in new]
         tokens = torch.from_numpy(np.concatenate([np.asarray(a, dtype=np.int64) for a in new])).to(dev)
         if tokens.numel() and (int(tokens.min()) < 0 or int(tokens.max()) >= cfg.vocab_size):

@@ -95,3 +95,25 @@ def test_refusals():
     motif = _cfg(xsa_last_n=1)
     with pytest.raises(ValueError, match="plain"):
         PagedScorer(DeviceModel(C.synth_weights(motif, seed=1), DEV), 1, 64)
+
+
+@pytest.mark.parametrize("tensor_cores", [True, False])
+def test_arena_models_score_with_their_live_parameters(tensor_cores):
+    """A model whose parameters lie in one arena scores like the oracle; after an update (the embedding's rows in
+    another order: symbol i is the old symbol perm[i], on both sides), input rows and head are the new ones."""
+    cfg = _cfg()
+    w = C.synth_weights(cfg, seed=8)
+    dm = DeviceModel(w, DEV, tensor_cores=tensor_cores, full_params=True)
+    T = 60
+    data = zipf_markov(T, cfg.vocab_size, np.arange(1) + 9)
+    sc = PagedScorer(dm, 1, 200, chunk=64, page_size=16)
+    got = sc.advance([data[0]]).cpu().numpy()
+    assert np.abs(got - _oracle_logits(w, data[0])).max() < TOL
+    perm = np.random.default_rng(5).permutation(cfg.vocab_size)
+    emb = dm.arena("emb").view(cfg.vocab_size, cfg.model_dim)
+    emb.copy_(emb.clone()[torch.from_numpy(perm).to(DEV)])
+    dm.refresh()
+    new = np.argsort(perm)[data[0]]  # the new names of the same symbols
+    for s in (sc, PagedScorer(dm, 1, 200, chunk=64, page_size=16)):
+        s.pages.release(0)
+        assert np.abs(s.advance([new]).cpu().numpy() - got[:, perm]).max() < 1e-5
