@@ -40,6 +40,10 @@ def _stream_handle(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
+# the index of the current device: kernels launch there, whatever device their arguments are on
+_current_device = torch._C._cuda_getDevice
+
+
 def rope_table(positions: int, dims: int, base: float = 1e4, *, scaling: str | None = None, factor: float = 1.0,
                trained: int | None = None, device: torch.device | str = "cuda") -> tuple[torch.Tensor, torch.Tensor]:
     """cos/sin ``[positions][dims/2]`` (fp32, rounded once from 64 bits).
@@ -123,6 +127,9 @@ def _positions(pos: torch.Tensor, n: int, device: torch.device) -> int:
 
 
 def _rope(x: torch.Tensor, rotary: Rotary, pos: torch.Tensor, out: torch.Tensor | None, backward: int) -> torch.Tensor:
+    if _current_device() != rotary.device.index:
+        with torch.cuda.device(rotary.device):
+            return _rope(x, rotary, pos, out, backward)
     if x.dtype not in _DTYPES:
         raise ValueError(f"unsupported dtype {x.dtype}")
     ldx = _heads(x, "x", x.dtype, rotary.device)
@@ -245,6 +252,9 @@ class PagedKV:
         """Writes the new tokens' keys (rotated) and values to their pages; returns
         the rotated queries when ``q`` is given.  ``positions``: rotary positions
         where they are not the cache's own."""
+        if _current_device() != self.device.index:
+            with torch.cuda.device(self.device):
+                return self.append(chunks, k, v, rotary=rotary, q=q, positions=positions, q_out=q_out)
         ldk, ldv = _heads(k, "k", self.dtype, self.device), _heads(v, "v", self.dtype, self.device)
         n = k.shape[0]
         if k.shape != v.shape or k.shape[1:] != (self.kv_heads, self.head_dim):
@@ -273,6 +283,9 @@ class PagedKV:
         """Attention of the new tokens over the cache: ``[tokens][heads][head_dim]``, and
         with ``return_lse`` each row's log2 sum ``[heads][tokens]`` (fp32).
         ``scale`` defaults to ``head_dim ** -0.5``; ``window`` 0 sees everything."""
+        if _current_device() != self.device.index:
+            with torch.cuda.device(self.device):
+                return self.attend(chunks, q, scale=scale, window=window, out=out, return_lse=return_lse)
         ldq = _heads(q, "q", self.dtype, self.device)
         n, H, d = q.shape
         if d != self.head_dim or H % self.kv_heads:

@@ -500,7 +500,9 @@ int altxs_split_params(const altxs_model_desc *desc, const float *params, const 
  * softmax and the rotation are fp32 and rounded once at the end.  Data errors
  * never fault: a position or a page out of range sets ALTXS_ST_BAD_POS in the
  * caller's status word (a device word, NULL = not wanted), the access is
- * skipped, and what depends on it is said at each call. */
+ * skipped, and what depends on it is said at each call.  As everywhere here, the
+ * device that all pointers belong to must be the current one (altxs_b200.paged
+ * makes it so). */
 #define ALTXS_F32 0
 #define ALTXS_BF16 1
 #define ALTXS_F16 2

@@ -231,3 +231,31 @@ def test_the_scorer_refuses_head_sizes_without_a_kernel():
     cfg.validate()
     with pytest.raises(ValueError, match="head"):
         PagedScorer(SimpleNamespace(cfg=cfg), 1, 64)
+
+
+@pytest.mark.parametrize("current,entered", [(0, [1]), (1, [])])
+def test_calls_run_on_the_tensors_device(monkeypatch, current, entered):
+    """Kernels launch on the current device: where the tensors' is another one, it is made current for the call."""
+    dev, seen = torch.device("cuda", 1), []
+
+    class On:
+        def __init__(self, d):
+            seen.append(d.index)
+
+        def __enter__(self):
+            monkeypatch.setattr(paged, "_current_device", lambda: 1)
+
+        def __exit__(self, *a):
+            monkeypatch.setattr(paged, "_current_device", lambda: current)
+
+    monkeypatch.setattr(torch.cuda, "device", On)
+    monkeypatch.setattr(paged, "_current_device", lambda: current)
+    cache, rot, x = object.__new__(paged.PagedKV), object.__new__(paged.Rotary), torch.zeros(1, 2, 64)
+    cache.device = rot.device = dev
+    cache.dtype = torch.float32
+    for call in (lambda: cache.attend(None, x), lambda: cache.append(None, x, x), lambda: paged.rope(x, rot, None),
+                 lambda: paged.rope_backward(x, rot, None)):
+        seen.clear()
+        with pytest.raises(ValueError, match="cuda:1"):  # x is not there: the call got as far as its checks
+            call()
+        assert seen == entered
