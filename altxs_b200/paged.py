@@ -15,7 +15,8 @@ it has cached (causal, optionally a sliding window): the role of the
 reference's static cache and its encoder's multi-symbol windows
 (``StaticACEngine``, altxs ``src/xsa_ttt/incremental.py:203-1218``,
 ``run_window`` ``:1268-1290``).  All tensors of a call share one type (fp32,
-bf16 or fp16); work is enqueued on the current stream.  Errors of the arguments
+bf16 or fp16); work is enqueued on the current stream.  No call records a
+gradient (inputs that require one raise; ``rope_backward`` is ``rope``'s).  Errors of the arguments
 raise; errors of the device data (a position beyond the tables, a page out of
 range, lengths beyond their bounds) set bits that ``check_status`` raises on.
 """
@@ -120,6 +121,13 @@ def _heads(x: torch.Tensor, what: str, dtype: torch.dtype, device: torch.device)
     return st[0] if n > 1 else max(st[0], h * d)
 
 
+def _no_history(what: str) -> None:
+    """For an input that a gradient is asked for: raises, since what these calls return has no history."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{what} records no gradient: detach its inputs or call it under torch.no_grad() "
+                           "(rope_backward is rope's gradient)")
+
+
 def _positions(pos: torch.Tensor, n: int, device: torch.device) -> int:
     if pos.dtype != torch.int64 or pos.shape != (n,) or pos.device != device or not pos.is_contiguous():
         raise ValueError(f"positions must be a contiguous int64 [{n}] tensor on {device}")
@@ -132,6 +140,8 @@ def _rope(x: torch.Tensor, rotary: Rotary, pos: torch.Tensor, out: torch.Tensor 
             return _rope(x, rotary, pos, out, backward)
     if x.dtype not in _DTYPES:
         raise ValueError(f"unsupported dtype {x.dtype}")
+    if x.requires_grad:
+        _no_history("rope")
     ldx = _heads(x, "x", x.dtype, rotary.device)
     n, h, d = x.shape
     p = _positions(pos, n, rotary.device)
@@ -255,6 +265,8 @@ class PagedKV:
         if _current_device() != self.device.index:
             with torch.cuda.device(self.device):
                 return self.append(chunks, k, v, rotary=rotary, q=q, positions=positions, q_out=q_out)
+        if k.requires_grad or v.requires_grad or (q is not None and q.requires_grad):
+            _no_history("append")
         ldk, ldv = _heads(k, "k", self.dtype, self.device), _heads(v, "v", self.dtype, self.device)
         n = k.shape[0]
         if k.shape != v.shape or k.shape[1:] != (self.kv_heads, self.head_dim):
@@ -286,6 +298,8 @@ class PagedKV:
         if _current_device() != self.device.index:
             with torch.cuda.device(self.device):
                 return self.attend(chunks, q, scale=scale, window=window, out=out, return_lse=return_lse)
+        if q.requires_grad:
+            _no_history("attend")
         ldq = _heads(q, "q", self.dtype, self.device)
         n, H, d = q.shape
         if d != self.head_dim or H % self.kv_heads:

@@ -801,3 +801,20 @@ def test_graphs_keep_their_workspaces():
             assert torch.equal(outs[i], want[i])
     assert all((j == 0xff).all() for j in junk)
     cache.check_status()
+
+
+def test_inputs_with_a_history_are_refused():
+    """No call records a gradient: rather than lose one in silence it raises, unless gradients are off."""
+    b = Batch("f32", 64, 2, 16, [1], [40], seed=55)
+    q, kv = _rand(_gen(56), 1, 4, 64), _rand(_gen(57), 1, 2, 64)
+    rot, pos = paged.Rotary(*_table(64, 16)), torch.tensor([39], device=DEV)
+    g = lambda x: x.clone().requires_grad_()  # noqa: E731
+    for call in (lambda f: paged.rope(f(q), rot, pos), lambda f: paged.rope_backward(f(q), rot, pos),
+                 lambda f: b.cache.append(b.chunks, f(kv), kv), lambda f: b.cache.append(b.chunks, kv, f(kv)),
+                 lambda f: b.cache.append(b.chunks, kv, kv, q=f(q)), lambda f: b.cache.attend(b.chunks, f(q))):
+        with pytest.raises(RuntimeError, match="gradient"):
+            call(g)
+        with torch.no_grad():
+            call(g)
+        call(torch.clone)
+    b.cache.check_status()
