@@ -216,7 +216,8 @@ __device__ __forceinline__ void place_token(const AppendArgs &a, const int32_t *
             off = page * a.kv.page_stride + (int64_t)(p % a.kv.page_size) * a.kv.token_stride;
     }
     if (!a.pos) rp = bad ? -1 : p;
-    if (a.r.dims && (rp < 0 || rp >= a.r.positions)) rp = -1, off = -1;
+    if (!a.r.dims) rp = 0;  // nothing to look up
+    else if (rp < 0 || rp >= a.r.positions) rp = -1, off = -1;
     if (off < 0) set_status(a.c.status, ALTXS_ST_BAD_POS);
 }
 

@@ -818,3 +818,19 @@ def test_inputs_with_a_history_are_refused():
             call(g)
         call(torch.clone)
     b.cache.check_status()
+
+
+@pytest.mark.parametrize("given", [False, True])
+def test_append_without_rotation_copies_every_query(given):
+    """Whatever a token's position, its cache's or a given one: queries of sequences are copied, rows of no sequence
+    are left."""
+    b = Batch("f32", 32, 1, 16, [5], [2], seed=59)  # cache positions -3 .. 1
+    k, v, q = _rand(_gen(1), 7, 1, 32), _rand(_gen(2), 7, 1, 32), _rand(_gen(3), 7, 2, 32)
+    pos = torch.tensor([-3, -2, -1, 0, -2, -2, 7], device=DEV) if given else None
+    out = torch.full_like(q, 7.0)
+    b.cache.append(b.chunks, k, v, q=q, q_out=out, positions=pos)
+    assert torch.equal(out[:5], q[:5]) and (out[5:] == 7.0).all()
+    page, slot = b.slots(0, 0, 2)
+    assert torch.equal(b.cache.k[page, slot], k[3:5]) and torch.equal(b.cache.v[page, slot], v[3:5])
+    with pytest.raises(RuntimeError, match="status 0x20"):  # three of them have no place
+        b.cache.check_status()
