@@ -118,7 +118,7 @@ def _heads(x: torch.Tensor, what: str, dtype: torch.dtype, device: torch.device)
     n, h, d = x.shape
     if (d > 1 and st[2] != 1) or (h > 1 and st[1] != d):
         raise ValueError(f"{what}: the heads of a token must lie side by side")
-    return st[0] if n > 1 else max(st[0], h * d)
+    return st[0] if n > 1 else h * d  # the stride over one token is never taken
 
 
 def _no_history(what: str) -> None:

@@ -259,3 +259,13 @@ def test_calls_run_on_the_tensors_device(monkeypatch, current, entered):
         with pytest.raises(ValueError, match="cuda:1"):  # x is not there: the call got as far as its checks
             call()
         assert seen == entered
+
+
+def test_the_stride_over_a_single_token_does_not_count():
+    """It is never taken: a row of an odd-sized buffer is as good as any."""
+    dev = torch.device("cpu")
+    wide = torch.zeros(3, 4 * 64 + 5)
+    x = wide[:, :256].unflatten(1, (4, 64))[1:2]
+    assert x.stride(0) == 261 and paged._heads(x, "q", torch.float32, dev) == 256
+    assert paged._heads(wide[:, :256].unflatten(1, (4, 64)), "q", torch.float32, dev) == 261
+    assert paged._heads(x[:0], "q", torch.float32, dev) == 256
