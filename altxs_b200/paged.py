@@ -196,6 +196,8 @@ class Chunks:
             raise ValueError("q_start, kv_len and the rows of page_table must be contiguous")
         if page_table.shape[0] > 1 and page_table.stride(0) < page_table.shape[1]:
             raise ValueError("the rows of page_table must not overlap")
+        if not (0 <= max_new < 1 << 31 and 0 <= max_kv < 1 << 31 and 0 <= total_kv < 1 << 63):
+            raise ValueError("max_new, max_kv and total_kv must be counts (of 31, 31 and 63 bits)")
         self.q_start, self.kv_len, self.page_table = q_start, kv_len, page_table
         self.device, self.max_kv = q_start.device, int(max_kv)
         self.struct = _lib.Chunks(q_start=q_start.data_ptr(), kv_len=kv_len.data_ptr(),
@@ -312,6 +314,7 @@ class PagedKV:
             if out.shape != q.shape:
                 raise ValueError("out must have q's shape")
         lse = torch.empty((H, n), dtype=torch.float32, device=self.device) if return_lse else None
+        window = max(-1, min(window, (1 << 31) - 1))  # (beyond 32 bits it would arrive as another)
         L = _lib.lib()
         cref, st = self._chunks(chunks, n), _stream_handle(self.device)
         need = L.altxs_paged_attention_workspace_bytes(self._ref, cref, H, window)

@@ -834,3 +834,14 @@ def test_append_without_rotation_copies_every_query(given):
     assert torch.equal(b.cache.k[page, slot], k[3:5]) and torch.equal(b.cache.v[page, slot], v[3:5])
     with pytest.raises(RuntimeError, match="status 0x20"):  # three of them have no place
         b.cache.check_status()
+
+
+def test_windows_beyond_32_bits_see_everything():
+    b = Batch("bf16", 64, 2, 16, [1, 20], [70, 50], seed=61)
+    q = _rand(_gen(62), 21, 4, 64).bfloat16()
+    want = b.cache.attend(b.chunks, q)
+    for w in (2 ** 31, 2 ** 32 + 5, 2 ** 63 - 1):
+        assert torch.equal(b.cache.attend(b.chunks, q, window=w), want)
+    with pytest.raises(RuntimeError):
+        b.cache.attend(b.chunks, q, window=-2 ** 32 + 5)
+    b.cache.check_status()

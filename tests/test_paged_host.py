@@ -269,3 +269,15 @@ def test_the_stride_over_a_single_token_does_not_count():
     assert x.stride(0) == 261 and paged._heads(x, "q", torch.float32, dev) == 256
     assert paged._heads(wide[:, :256].unflatten(1, (4, 64)), "q", torch.float32, dev) == 261
     assert paged._heads(x[:0], "q", torch.float32, dev) == 256
+
+
+def test_bounds_that_do_not_fit_are_refused():
+    """Instead of reaching the library modulo 2^32."""
+    z, one = torch.zeros(2, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    table = torch.zeros(1, 4, dtype=torch.int32)
+    for kw in (dict(max_new=2 ** 32 + 1, max_kv=4), dict(max_new=1, max_kv=2 ** 32 + 4), dict(max_new=2 ** 31, max_kv=4),
+               dict(max_new=-1, max_kv=4), dict(max_new=1, max_kv=-1), dict(max_new=1, max_kv=4, total_kv=-1)):
+        with pytest.raises(ValueError, match="max_new"):
+            paged.Chunks(z, one, table, **kw)
+    c = paged.Chunks(z, one, table, max_new=2 ** 31 - 1, max_kv=2 ** 31 - 1)
+    assert c.struct.max_new == c.struct.max_kv == 2 ** 31 - 1
