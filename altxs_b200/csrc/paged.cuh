@@ -79,8 +79,8 @@ struct ManyPlan {
     int rows;  // rows of a slot
 };
 ManyPlan paged_many_plan(const altxs_paged_kv &kv, const altxs_chunks &c, int H, int window);
-int launch_paged_many(const PagedAttnArgs &a, const ManyPlan &p, int min_rows, uint32_t *cnt, float *part, int sms,
-                      cudaStream_t stream);
+int launch_paged_many(const PagedAttnArgs &a, const ManyPlan &p, int min_rows, uint32_t *spoilt, uint32_t *cnt,
+                      float *part, int sms, cudaStream_t stream);
 int set_wait_limit_paged(uint32_t limit);
 int launch_paged_attention(const PagedAttnArgs &a, cudaStream_t stream);
 

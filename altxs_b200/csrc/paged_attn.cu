@@ -694,8 +694,9 @@ __global__ void __launch_bounds__(kVecWarps * 32, R == 1 ? 4 : R < 4 ? 2 : 1) k_
     end_after_many();
 }
 
-// Workspace: arrival counters (zero between calls: a call's last arrivals reset
-// them), then partial rows.
+// Workspace: a word that a call which gave up sets, arrival counters (zero between calls: a call's last arrivals
+// reset them), then partial rows.
+constexpr int64_t kHead = 4;  // words ahead of the counters
 constexpr int64_t kCounters = 65536;  // more than these of a kind are cleared by the call that needs them
 static_assert(2 * 4 * kCounters == ALTXS_PAGED_COUNTER_BYTES, "what the caller zeroes");
 
@@ -729,7 +730,7 @@ Plan plan_of(const altxs_paged_kv &kv, const altxs_chunks &c, int H, int window)
     if (p.few && split) p.few_part = align_up(p.items * p.part_rows * (kv.head_dim + 4) * 4, 256);
     if (p.many) p.mp = paged_many_plan(kv, c, H, window);
     const int64_t part = p.few_part + p.mp.slots * p.mp.slot_bytes;
-    p.few_cnt = align_up(4 * std::max(kCounters, n * kv.n_kv_heads * std::max(p.groups, 1)), 256);
+    p.few_cnt = align_up(4 * std::max(kCounters, kHead + n * kv.n_kv_heads * std::max(p.groups, 1)), 256);
     p.many_cnt = align_up(4 * std::max(kCounters, p.mp.slots + 1), 256);  // its first word: the item tickets
     if (part > 0 || p.many) p.bytes = p.few_cnt + p.many_cnt + part;
     return p;
@@ -763,10 +764,11 @@ int launch_few(void (*k)(FewArgs), const FewArgs &f, unsigned grid, int threads,
 template <typename T, int HD>
 int launch(const PagedAttnArgs &a, const Plan &p, cudaStream_t st) {
     unsigned char *ws = static_cast<unsigned char *>(a.ws);
-    uint32_t *few_cnt = nullptr, *many_cnt = nullptr;
+    uint32_t *spoilt = nullptr, *few_cnt = nullptr, *many_cnt = nullptr;
     float *part = nullptr, *many_part = nullptr;
     if (p.bytes > 0) {
-        few_cnt = reinterpret_cast<uint32_t *>(ws);
+        spoilt = reinterpret_cast<uint32_t *>(ws);
+        few_cnt = spoilt + kHead;
         many_cnt = reinterpret_cast<uint32_t *>(ws + p.few_cnt);
         part = reinterpret_cast<float *>(ws + p.few_cnt + p.many_cnt);
         many_part = reinterpret_cast<float *>(ws + p.few_cnt + p.many_cnt + p.few_part);
@@ -777,7 +779,7 @@ int launch(const PagedAttnArgs &a, const Plan &p, cudaStream_t st) {
     const FewArgs f{a, a.H / a.kv.n_kv_heads, 1, kMaxRows, p.group, p.bytes > 0 ? p.items : 0, few_cnt, p.groups, part, p.part_rows};
     const int64_t sms = sm_count();
     if (p.many)
-        if (const int rc = launch_paged_many(a, p.mp, kMaxRows + 1, many_cnt, many_part, (int)sms, st)) return rc;
+        if (const int rc = launch_paged_many(a, p.mp, kMaxRows + 1, spoilt, many_cnt, many_part, (int)sms, st)) return rc;
     if (!p.few) return ALTXS_OK;
     if constexpr (std::is_same<T, float>::value) {
         const int64_t most = (int64_t)a.c.max_new * f.G;  // rows

@@ -146,6 +146,7 @@ struct ManyArgs {
     int G, min_rows;    // sequences with at least min_rows rows are this kernel's
     int run;            // positions that lie within a page
     int64_t max_slots;  // partial slots in the workspace (one per item of a split sequence)
+    uint32_t *spoilt;   // set by a call that gave up: its counters may still be counting
     uint32_t *cnt;      // [max_slots], zero between calls
     uint32_t *ticket;   // items handed out beyond the first of each block, zero between calls
     float *part;        // [max_slots][part_rows * (HD + 2)]
@@ -1493,7 +1494,10 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
                 ++live;
             }
         }
-        if (abort_sh && tid == 0) set_status(a.c.status, ALTXS_ST_TIMEOUT);
+        if (tid == 0) {  // in a workspace left by a call that gave up, splits may have been joined early
+            if (abort_sh) *f.spoilt = 1;
+            if (abort_sh || (blockIdx.x == 0 && __ldcg(f.spoilt) != 0)) set_status(a.c.status, ALTXS_ST_TIMEOUT);
+        }
     }
     tc_fence_before();
     __syncthreads();
@@ -1557,10 +1561,10 @@ ManyPlan paged_many_plan(const altxs_paged_kv &kv, const altxs_chunks &c, int H,
     return p;
 }
 
-int launch_paged_many(const PagedAttnArgs &a, const ManyPlan &p, int min_rows, uint32_t *cnt, float *part, int sms,
-                      cudaStream_t st) {
+int launch_paged_many(const PagedAttnArgs &a, const ManyPlan &p, int min_rows, uint32_t *spoilt, uint32_t *cnt,
+                      float *part, int sms, cudaStream_t st) {
     const int run = std::min(tile_keys(a.kv.dtype, a.kv.head_dim), a.kv.page_size & -a.kv.page_size);
-    const ManyArgs f{a, a.H / a.kv.n_kv_heads, min_rows, run < 4 ? 1 : run, p.slots, cnt + 1, cnt, part, p.rows};
+    const ManyArgs f{a, a.H / a.kv.n_kv_heads, min_rows, run < 4 ? 1 : run, p.slots, spoilt, cnt + 1, cnt, part, p.rows};
     const unsigned grid = (unsigned)std::min<int64_t>(p.items, sms);
     if (a.kv.dtype == ALTXS_F32) return launch<float>(f, grid, st);
     return a.kv.dtype == ALTXS_BF16 ? launch<__nv_bfloat16>(f, grid, st) : launch<__half>(f, grid, st);

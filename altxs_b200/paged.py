@@ -25,6 +25,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import weakref
 from typing import Sequence
 
 import numpy as np
@@ -32,6 +33,8 @@ import torch
 
 from . import _lib
 
+# the workspaces of the caches that are alive, by device and stream
+_shared: weakref.WeakValueDictionary[tuple[torch.device, int], torch.Tensor] = weakref.WeakValueDictionary()
 _GROWTH = 64 << 20  # bytes that a workspace grows by at most beyond what a call needs
 _DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
@@ -248,14 +251,18 @@ class PagedKV:
         return c._ref
 
     def _workspace_for(self, need: int, stream: int) -> torch.Tensor:
-        """One workspace per stream.  A call that is captured has its own, from the graph's memory and cleared in
+        """One workspace per stream, shared by the caches whose calls follow one another there and freed with the
+        last of them (a call that gives up spoils it for all of them: each then reports that).  A call that is captured has its own, from the graph's memory and cleared in
         the graph: it lives as long as the graph does, and no other call, captured or not, meets its counters."""
         if torch.cuda.is_current_stream_capturing():
             return _workspace(need, self.device)
         ws = self._ws.get(stream)
-        if ws is None or ws.numel() < need:  # with room for the next steps of growing streams
-            more = 0 if ws is None else ws.numel() + min(ws.numel() // 2, _GROWTH)
-            ws = self._ws[stream] = _workspace(max(need, more), self.device)
+        if ws is None or ws.numel() < need:
+            ws = _shared.get((self.device, stream))
+            if ws is None or ws.numel() < need:  # with room for the next steps of growing streams
+                more = 0 if ws is None else ws.numel() + min(ws.numel() // 2, _GROWTH)
+                ws = _shared[self.device, stream] = _workspace(max(need, more), self.device)
+            self._ws[stream] = ws
         return ws
 
     def append(self, chunks: Chunks, k: torch.Tensor, v: torch.Tensor, *, rotary: Rotary | None = None,
@@ -332,7 +339,16 @@ class PagedKV:
         try:
             _raise_status(self.status, "paged cache")
         except RuntimeError:
-            self._ws.clear()  # a call that gave up may leave its counters counting: later calls start from zeroed ones
+            # A call that gave up may leave its counters counting: later calls start from zeroed ones, on this
+            # stream in the same workspace, elsewhere in another.
+            here = _stream_handle(self.device) if self._ws else 0
+            for stream, ws in list(self._ws.items()):
+                if stream == here:
+                    ws[:_lib.PAGED_COUNTER_BYTES].zero_()
+                else:
+                    del self._ws[stream]
+                    if _shared.get((self.device, stream)) is ws:
+                        del _shared[self.device, stream]
             raise
 
 

@@ -39,3 +39,38 @@ def test_waits_give_up_report_and_recover(dtype):
     for _ in range(2):
         assert torch.equal(cache.attend(chunks, q), want)
     cache.check_status()
+
+
+def test_a_spoilt_workspace_is_reported_by_every_cache_that_shares_it():
+    """A call that gave up may leave counters counting: until they are zeroed, calls of other caches in the same
+    workspace report it too."""
+    L = _lib.lib()
+    g = torch.Generator(device=DEV)
+    g.manual_seed(2)
+    caches = [paged.PagedKV.empty(150, 16, 2, 64, torch.bfloat16) for _ in range(2)]
+    for c in caches:
+        c.k.copy_(torch.randn(c.k.shape, generator=g, device=DEV))
+        c.v.copy_(torch.randn(c.v.shape, generator=g, device=DEV))
+    alloc = paged.PageAllocator(1, 150, 16, 2400, DEV)
+    alloc.extend([2300])
+    chunks = alloc.extend([40])
+    q = torch.randn(40, 4, 64, generator=g, device=DEV).bfloat16()
+    want = [c.attend(chunks, q) for c in caches]
+    assert [*caches[0]._ws.values()][0] is [*caches[1]._ws.values()][0]
+    for c in caches:
+        c.check_status()
+    try:
+        assert L.altxs_set_wait_limit(0) == 0
+        caches[0].attend(chunks, q)
+        torch.cuda.synchronize()
+    finally:
+        assert L.altxs_set_wait_limit(L.altxs_default_wait_limit()) == 0
+    caches[1].attend(chunks, q)
+    for c in caches:
+        with pytest.raises(RuntimeError, match="status 0x10"):
+            c.check_status()
+    for _ in range(2):
+        for c, w in zip(caches, want):
+            assert torch.equal(c.attend(chunks, q), w)
+    for c in caches:
+        c.check_status()

@@ -281,3 +281,25 @@ def test_bounds_that_do_not_fit_are_refused():
             paged.Chunks(z, one, table, **kw)
     c = paged.Chunks(z, one, table, max_new=2 ** 31 - 1, max_kv=2 ** 31 - 1)
     assert c.struct.max_new == c.struct.max_kv == 2 ** 31 - 1
+
+
+def test_caches_of_one_stream_share_a_workspace(monkeypatch):
+    """Not those of different streams or devices; it goes with the last cache that has used it."""
+    import gc
+
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(paged, "_shared", type(paged._shared)())
+
+    def cache():
+        c = object.__new__(paged.PagedKV)
+        c.device, c._ws = torch.device("cpu"), {}
+        return c
+
+    a, b = cache(), cache()
+    ws = a._workspace_for(1000, 7)
+    assert b._workspace_for(900, 7) is ws and b._workspace_for(900, 8) is not ws
+    bigger = b._workspace_for(3000, 7)
+    assert bigger.numel() >= 3000 and a._workspace_for(1000, 7) is ws and a._workspace_for(2500, 7) is bigger
+    del ws, bigger, a, b
+    gc.collect()
+    assert len(paged._shared) == 0
