@@ -74,6 +74,7 @@ namespace {
 constexpr int kMmaWarp = 8;
 constexpr int kScan = 64;        // sequences are counted in this many groups
 constexpr int kMostItems = 1184;  // splits of one sequence
+constexpr int kSms = 148;
 constexpr int kMostSplits = 16;
 constexpr int kNext = 4;           // items announced to a block's roles ahead
 constexpr unsigned kAll = 0xffffffffu;
@@ -125,7 +126,6 @@ __host__ __device__ inline int tiles_of(int keys, int kt) { return (keys + kt - 
 // tiles to a split (a split costs about 4.5 tiles' time, a whole item 1.5) and
 // only for a twentieth or more of the sequence's time.
 __host__ __device__ inline void split_rule(Shape &w, int nt) {
-    constexpr int kSms = 148;
     const int waves = w.pairs / kSms, rest = w.pairs - waves * kSms, most = nt / 8;
     w.whole = w.pairs;
     w.nsplit = 1;
@@ -139,6 +139,15 @@ __host__ __device__ inline void split_rule(Shape &w, int nt) {
         if (ns <= most && rest * ns <= kMostItems && c < cost) cost = c, w.nsplit = ns;
     }
     if (w.nsplit > 1) w.whole = waves * kSms;
+}
+
+// Waves that the cut pairs of a sequence of nt tiles take at most: the least tiles for which the rule chooses 2, 3, ..
+// waves for any number of pairs (less one, for sums that round otherwise on the device).
+inline int most_waves(int64_t nt) {
+    constexpr int from[] = {16, 26, 60, 110, 180, 275, 401, 565};
+    int w = 0;
+    while (w < 8 && nt >= from[w]) ++w;
+    return w;
 }
 
 struct ManyArgs {
@@ -1553,10 +1562,17 @@ ManyPlan paged_many_plan(const altxs_paged_kv &kv, const altxs_chunks &c, int H,
     const int rows = block_rows(kv.dtype, kv.head_dim);
     const int64_t blocks = (int64_t)c.n_tokens * G / rows + c.n_seqs;
     const int64_t keys = window > 0 ? std::min<int64_t>(c.max_kv, (int64_t)window + rows) : c.max_kv;
-    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kMostSplits, tiles_of((int)keys, tile_keys(kv.dtype, kv.head_dim)) / 8));
+    const int kt = tile_keys(kv.dtype, kv.head_dim);
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(kMostSplits, tiles_of((int)keys, kt) / 8));
     p.items = blocks * kv.n_kv_heads * most;
     p.rows = (int64_t)c.max_new * G <= 128 ? 128 : rows;
-    if (most > 1) p.slots = std::min<int64_t>(p.items, (int64_t)c.n_seqs * kMostItems);
+    if (most > 1) {  // one per item of the last, partly filled wave of a sequence that is cut
+        const int64_t nt = tiles_of((int)keys, kt), pairs = ((int64_t)std::max(c.max_new, 1) * G + rows - 1) / rows * kv.n_kv_heads;
+        const int64_t each = std::min<int64_t>({(int64_t)most_waves(nt) * kSms, std::min<int64_t>(pairs, kSms - 1) * most, kMostItems});
+        // a sequence is cut from 16 tiles on
+        const int64_t seqs = c.total_kv > 0 ? std::min<int64_t>(c.n_seqs, c.total_kv / (15 * kt)) : c.n_seqs;
+        p.slots = std::min(p.items, seqs * each);
+    }
     p.slot_bytes = (int64_t)p.rows * (kv.head_dim + 2) * 4;
     return p;
 }

@@ -303,3 +303,40 @@ def test_caches_of_one_stream_share_a_workspace(monkeypatch):
     del ws, bigger, a, b
     gc.collect()
     assert len(paged._shared) == 0
+
+
+def _cut_items(pairs, nt):
+    """Items of a sequence's last, partly filled wave over 148 SMs that are splits: the cheapest number of splits of at
+    least 8 tiles, where a split costs 4.5 tiles' time besides its own and a whole item 1.5, and a twentieth is gained."""
+    f = np.float32
+    waves, rest = divmod(pairs, 148)
+    cost, best = (f(nt) + f(1.5)) * (f(1) - f(0.05) * f(waves + 1)), 1
+    for ns in range(2, min(16, nt // 8) + 1):
+        c = f(-(-rest * ns // 148)) * (f(nt) * f(1 / ns) + f(4.5))
+        if rest * ns <= 1184 and c < cost * f(1 - 1e-6):
+            cost, best = c, ns
+    return rest * best if best > 1 else 0
+
+
+def test_workspace_holds_every_split_and_not_much_more():
+    """bf16, 32 heads over 8 of 128 channels (64 tokens to a block of 256 rows)."""
+    L = _lib.lib()
+    kv = _kv(dtype=_lib.BF16, head_dim=128, n_kv_heads=8, page_size=128, token_stride=1024, head_stride=128,
+             page_stride=1 << 17)
+
+    def slots(n, new, max_kv, total=0):
+        ch = _ch(n_seqs=n, n_tokens=n * new, max_new=new, max_kv=max_kv, table_stride=max_kv // 128 + 1, total_kv=total)
+        ws = L.altxs_paged_attention_workspace_bytes(C.byref(kv), C.byref(ch), 32, 0)
+        few = ((total or n * max_kv) // 512 + n) * 8 * 16 * 132 * 4
+        return ws, (ws - _lib.PAGED_COUNTER_BYTES - few) // (256 * 130 * 4)
+
+    for nt in (16, 26, 27, 40, 60, 61, 100, 111, 181, 276, 402, 566, 1300):
+        for blocks in list(range(1, 20)) + [37, 55, 74]:
+            got = slots(1, 64 * blocks, 128 * nt)[1]
+            assert got >= max(_cut_items(8 * b, k) for b in range(1, blocks + 1) for k in {nt, nt - 1, (nt + 15) // 2, 16})
+    cache = 2 * 8 * 128 * 2  # bytes of a position
+    for n, new, max_kv, most in ((8, 2048, 4096, 400 << 20), (64, 4096, 8192, 2 * 64 * 8192 * cache),
+                                 (256, 1024, 4096, 3 * 256 * 4096 * cache)):
+        assert slots(n, new, max_kv)[0] <= most
+    # sequences of fewer than 16 tiles are not split: a known total bounds the number of those that are
+    assert slots(64, 4096, 8192, 10 * 15 * 128)[1] <= 10 * 3 * 148
