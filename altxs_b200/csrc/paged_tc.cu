@@ -22,8 +22,8 @@
 //
 // Softmax: x = s scale log2(e) in fp32, p = 2^(x - m), the sum from the
 // unrounded p.  m follows the running maximum only when that grows by more
-// than 2^8 (fp16: 2^4, for its range): until then p <= 256 is as exact, and O
-// (fp32, in tensor memory) is not touched.
+// than 2^8: until then p <= 256 is as exact, and O (fp32, in tensor memory) is
+// not touched.
 //
 // 16-bit types: the tiles are the cache's own rows, p is rounded once to the
 // type.  Warps 9 and 11 fetch every other tile, warp 10 draws and announces the
@@ -78,6 +78,7 @@ constexpr int kSms = 148;
 constexpr int kMostSplits = 16;
 constexpr int kNext = 4;           // items announced to a block's roles ahead
 constexpr unsigned kAll = 0xffffffffu;
+constexpr float kLazy = 8.0f;
 
 template <typename T, int HD>
 struct Tc {
@@ -1037,9 +1038,11 @@ __global__ void __launch_bounds__(Tc<T, HD>::Threads, 1) k_paged_many(const __gr
         const uint32_t ts = tmem + lanes + C::ColS + KT * grp, to = tmem + lanes + C::ColO + HD * grp;
         // a negative scale turns the queries round instead; a scale of 0 stays above it (-inf marks the unseen)
         const float c2 = fmaxf(__fmul_rn(fabsf(a.scale), kLog2e), 1.17549435e-38f);
-        // fp16 ends at 2^-24.  p carries a power of two (with the lag of m it is 2^15 at most), so that what it loses
-        // there is far from the sum: of 100000 keys behind a dominant one, each at 2^-25 of it, nothing may be left out.
-        constexpr float kBias = F32 ? 6.0f : Half ? 11.0f : 0.0f, kLazy = Half ? 4.0f : 8.0f;
+        // fp16 ends at 2^-24.  p carries a power of two (with the lag of m it is 2^15 at most, fp32's with its values'
+        // powers 2^14), so that what it loses there is far from the sum: at 2^-32 of the maximum a key, a million
+        // keys lose half an fp16 rounding.  (A lag of 2^4 and 2^11 for fp16: long piece 653 us against 648, ragged
+        // prompts 278 against 273.)
+        constexpr float kBias = F32 ? 6.0f : Half ? 7.0f : 0.0f;
         const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
         unsigned char *qsm = pm_smem_raw + (sq - raw_s);
         // between an item's last S and the next item's queries their place holds 32 KB of outputs, then 256 (m, l)
