@@ -17,6 +17,7 @@
 // fp16 rotated and appended in 219 us (1.28 GB, 5.9 TB/s); one token of 64
 // streams in 3.9 us (a launch and two dependent rounds of loads).
 #include <algorithm>
+#include <cmath>
 
 #include "paged.cuh"
 #include "prof.cuh"
@@ -429,7 +430,7 @@ int altxs_paged_attention(const altxs_paged_kv *kv, const altxs_chunks *c, int n
     if (!kv || !c) return ALTXS_EINVAL;
     if (const int rc = check_kv(*kv)) return rc;
     if (const int rc = check_chunks(*kv, *c)) return rc;
-    if (n_heads < 1 || n_heads % kv->n_kv_heads || window < 0) return ALTXS_EINVAL;
+    if (n_heads < 1 || n_heads % kv->n_kv_heads || window < 0 || !std::isfinite(scale)) return ALTXS_EINVAL;
     const int64_t width = (int64_t)n_heads * kv->head_dim, u = 16 / es_of(kv->dtype);
     if (ldq < width || ldo < width || ldq % u || ldo % u || !aligned16(q) || !aligned16(out)) return ALTXS_EINVAL;
     if (c->n_seqs == 0 || c->n_tokens == 0) return ALTXS_OK;

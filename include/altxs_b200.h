@@ -572,7 +572,9 @@ int altxs_paged_append(const altxs_paged_kv *kv, const altxs_chunks *c, const al
 /* out[i][h] = sum_j softmax_j(scale * q[i][h] . K_j) V_j over the cached
  * positions j of token i's sequence with j <= pos(i) and, with window > 0,
  * j > pos(i) - window; query head h reads key/value head h / (n_heads /
- * n_kv_heads).  A token that sees nothing (negative position) gets zeros.
+ * n_kv_heads).  scale must be finite.  A token that sees nothing (negative
+ * position) gets zeros; rows of no sequence, or of one that is left out, are not
+ * written.
  * lse: optional device [n_heads][n_tokens], log2 of each row's sum of
  * 2^(scale * log2(e) * q . K) (-inf for a row that sees nothing).  Positions on
  * a page out of range (ALTXS_ST_BAD_POS) count as unseen.  A row's result does

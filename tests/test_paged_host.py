@@ -340,3 +340,13 @@ def test_workspace_holds_every_split_and_not_much_more():
         assert slots(n, new, max_kv)[0] <= most
     # sequences of fewer than 16 tiles are not split: a known total bounds the number of those that are
     assert slots(64, 4096, 8192, 10 * 15 * 128)[1] <= 10 * 3 * 148
+
+
+@pytest.mark.parametrize("scale", [math.nan, math.inf, -math.inf])
+def test_attention_refuses_a_scale_that_is_not_finite(scale):
+    """One of NaN gave every key the same weight where a sequence has many rows, and NaN where it has few."""
+    rc = _lib.lib().altxs_paged_attention(C.byref(_kv()), C.byref(_ch()), 4, scale, 0, 4096, 256, 4096, 256, None, 0, 0, None)
+    assert rc == _lib.ALTXS_EINVAL
+    rc = _lib.lib().altxs_paged_attention(C.byref(_kv()), C.byref(_ch(n_tokens=0)), 4, scale, 0, 4096, 256, 4096, 256, None, 0,
+                                          0, None)
+    assert rc == _lib.ALTXS_EINVAL
