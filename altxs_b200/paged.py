@@ -109,7 +109,7 @@ class Rotary:
         self._ref = C.byref(self.struct)
 
     def check_status(self) -> None:
-        """Waits; raises if a position of ``rope`` was outside the tables."""
+        """Waits for the current stream; raises if a position of ``rope`` was outside the tables."""
         _raise_status(self.status, "rope")
 
 
@@ -303,7 +303,8 @@ class PagedKV:
                out: torch.Tensor | None = None, return_lse: bool = False):
         """Attention of the new tokens over the cache: ``[tokens][heads][head_dim]``, and
         with ``return_lse`` each row's log2 sum ``[heads][tokens]`` (fp32).
-        ``scale`` defaults to ``head_dim ** -0.5``; ``window`` 0 sees everything."""
+        ``scale`` defaults to ``head_dim ** -0.5``; ``window`` 0 sees everything.  Rows of no
+        sequence are not written."""
         if _current_device() != self.device.index:
             with torch.cuda.device(self.device):
                 return self.attend(chunks, q, scale=scale, window=window, out=out, return_lse=return_lse)
@@ -335,7 +336,8 @@ class PagedKV:
         return (out, lse) if return_lse else out
 
     def check_status(self) -> None:
-        """Waits; raises if a call met a position, page or length out of range, or gave up waiting."""
+        """Waits for the current stream (the calls' own, or one that follows it); raises if a call met a position,
+        page or length out of range, or gave up waiting."""
         try:
             _raise_status(self.status, "paged cache")
         except RuntimeError:

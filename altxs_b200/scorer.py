@@ -82,8 +82,10 @@ class PagedScorer:
         return y
 
     def advance(self, new: Sequence[np.ndarray]) -> torch.Tensor:
-        """Consumes ``new[s]`` (any number of symbols, also none) of every stream and
-        returns the logits after each: ``[sum of lengths][vocab]``, stream by stream."""
+        """Consumes ``new[s]`` (also none) of every stream and returns the logits after
+        each: ``[sum of lengths][vocab]``, stream by stream.  The default ``n_pages``
+        hold ``chunk`` symbols of every stream at a time; more may raise "out of pages"
+        (nothing is consumed then)."""
         cfg, sm, dev = self.cfg, self.small, self.dm.device
         lens = [len(a) for a in new]
         tokens = torch.from_numpy(np.concatenate([np.asarray(a, dtype=np.int64) for a in new])).to(dev)

@@ -496,8 +496,10 @@ int altxs_split_params(const altxs_model_desc *desc, const float *params, const 
  * src/xsa_ttt/incremental.py:203-1218, run_window :1268-1290; GPT.static_extend,
  * model.py:1617-1781).
  *
- * Types: activations and cache share one type, fp32, bf16 or fp16; sums, the
- * softmax and the rotation are fp32 and rounded once at the end.  Data errors
+ * Types: activations and cache share one type, fp32, bf16 or fp16.  Sums, the
+ * softmax's maximum and sum and the rotation are fp32, outputs rounded once at
+ * the end; in the 16-bit types the probabilities are rounded to the type for
+ * their product with the values.  Data errors
  * never fault: a position or a page out of range sets ALTXS_ST_BAD_POS in the
  * caller's status word (a device word, NULL = not wanted), the access is
  * skipped, and what depends on it is said at each call.  As everywhere here, the
@@ -585,7 +587,8 @@ int altxs_paged_append(const altxs_paged_kv *kv, const altxs_chunks *c, const al
  * ALTXS_ST_TIMEOUT zero them again: until then every call that may split its rows
  * among blocks of the tensor-core kernel sets ALTXS_ST_TIMEOUT too, so caches
  * whose calls follow one another on a stream can share a workspace.  Results are finite where the inputs a row
- * sees are: NaN and infinities that its mask hides do not reach it. */
+ * sees are: NaN and infinities that its mask hides do not reach it; one that it
+ * sees leaves its output infinite or NaN. */
 #define ALTXS_PAGED_COUNTER_BYTES 524288
 int64_t altxs_paged_attention_workspace_bytes(const altxs_paged_kv *kv, const altxs_chunks *c, int n_heads,
                                               int window);
