@@ -217,7 +217,9 @@ class PagedKV:
     ``transpose(1, 2)``).  ``PagedKV.empty`` allocates them."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor):
-        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.stride() != v.stride():
+        # a stride over one element is never taken: whatever it is, it stands for the channels of a head
+        strides = [[s if m > 1 else x.shape[-1] for m, s in zip(x.shape, x.stride())] for x in (k, v)]
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or strides[0] != strides[1]:
             raise ValueError("k and v must be [pages][page_size][kv_heads][head_dim] of equal shape, type and strides")
         if k.dtype not in _DTYPES or not k.is_cuda or k.device != v.device:
             raise ValueError("k and v must be fp32, bf16 or fp16 on one GPU")
@@ -226,10 +228,8 @@ class PagedKV:
         self.k, self.v, self.device, self.dtype = k, v, k.device, k.dtype
         self.page_size, self.kv_heads, self.head_dim = k.shape[1:]
         self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
-        # a stride over one element is never taken: any value in range will do
-        ts = k.stride(1) if k.shape[1] > 1 else max(k.stride(1), self.head_dim)
-        hs = k.stride(2) if k.shape[2] > 1 else self.head_dim
-        self.struct = _lib.PagedKv(k=k.data_ptr(), v=v.data_ptr(), page_stride=k.stride(0), token_stride=ts,
+        ps, ts, hs, _ = strides[0]
+        self.struct = _lib.PagedKv(k=k.data_ptr(), v=v.data_ptr(), page_stride=ps, token_stride=ts,
                                    head_stride=hs, dtype=_DTYPES[k.dtype], page_size=self.page_size,
                                    n_pages=k.shape[0], n_kv_heads=self.kv_heads, head_dim=self.head_dim)
         self._ref = C.byref(self.struct)

@@ -845,3 +845,24 @@ def test_windows_beyond_32_bits_see_everything():
     with pytest.raises(RuntimeError):
         b.cache.attend(b.chunks, q, window=-2 ** 32 + 5)
     b.cache.check_status()
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_strides_over_one_page_slot_or_head_do_not_count(n):
+    """They are never taken: any value will do, also one that is no multiple of 16 bytes, or another in v than in k."""
+    q = _rand(_gen(64), n, 4, 64).bfloat16()
+    for P, kv, Hkv in ((64, 50, 2), (1, 45, 2), (16, 60, 1)):  # one page, one slot a page, one head
+        b = Batch("bf16", 64, Hkv, P, [n], [kv], seed=63, spare=0)
+        want = b.cache.attend(b.chunks, q)
+        pools = []
+        for x, odd in ((b.cache.k, 77), (b.cache.v, 99)):
+            pools.append(torch.as_strided(x, x.shape, [odd if m == 1 else s for m, s in zip(x.shape, x.stride())]))
+        cache = paged.PagedKV(*pools)
+        assert torch.equal(cache.attend(b.chunks, q), want)
+        kn, vn = _rand(_gen(65), n, Hkv, 64).bfloat16(), _rand(_gen(66), n, Hkv, 64).bfloat16()
+        cache.append(b.chunks, kn, vn)
+        page, slot = b.slots(0, kv - n, kv)
+        assert torch.equal(b.cache.k[page, slot], kn) and torch.equal(b.cache.v[page, slot], vn)
+        cache.check_status()
+    with pytest.raises(ValueError):
+        paged.PagedKV(b.cache.k, b.cache.v.transpose(0, 1))
