@@ -396,13 +396,11 @@ class PageAllocator:
         if window == 0:
             return 0
         first = max(0, int(self.len[seq]) + 1 - window) // self.page_size  # block of the next token's first position
-        n = 0
-        for b in range(first):
-            if self.table[seq, b] >= 0:
-                self.free.append(int(self.table[seq, b]))
-                self.table[seq, b] = -1
-                n += 1
-        return n
+        behind = self.table[seq, :first]
+        back = behind[behind >= 0].tolist()
+        self.free += back
+        behind[:] = -1
+        return len(back)
 
     def release(self, seq: int) -> None:
         """Ends a stream: its pages are free again and its length is 0."""

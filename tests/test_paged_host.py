@@ -350,3 +350,25 @@ def test_attention_refuses_a_scale_that_is_not_finite(scale):
     rc = _lib.lib().altxs_paged_attention(C.byref(_kv()), C.byref(_ch(n_tokens=0)), 4, scale, 0, 4096, 256, 4096, 256, None, 0,
                                           0, None)
     assert rc == _lib.ALTXS_EINVAL
+
+
+def test_trim_of_long_streams():
+    """Block by block in their order, and a step of a stream of a million positions takes no longer for those that
+    have come back long ago (a table of 65536 blocks: a loop over them took 5 ms, this 20 us)."""
+    import time
+
+    a = paged.PageAllocator(2, 70000, 16, 1 << 20, "cpu")
+    rng = np.random.default_rng(1)
+    a.extend([1 << 19, 77])
+    for w in (300000, 5000, 64):
+        first = max(0, int(a.len[0]) + 1 - w) // 16
+        want = [int(p) for p in a.table[0, :first] if p >= 0]
+        free = list(a.free)
+        assert a.trim(0, w) == len(want) and a.free == free + want and (a.table[0, :first] == -1).all()
+        a.extend([int(rng.integers(1, 100)), 0])
+    a.extend([(1 << 20) - int(a.len[0]), 0])
+    a.trim(0, 64)
+    t = time.perf_counter()
+    for _ in range(50):
+        assert a.trim(0, 64) == 0
+    assert (time.perf_counter() - t) / 50 < 1e-3
