@@ -22,9 +22,10 @@
 // S = Q K^T, the online softmax and O += P V as m16n8k16 fragments with fp32
 // sums.  p is rounded to the type for P V (the fragments take no other), its sum
 // from the unrounded p: the error against 64 bits is 1.0 to 1.2 times that of the
-// plain form, which keeps p in fp32 and rounds the output once.  The tcgen05 tile is 128 rows for at most
-// 16 real ones.  More rows in groups of 16 read the keys again and lose to it:
-// 256 streams of up to 2048 keys, 20 rows a head, took 251 us against 137.
+// plain form, which keeps p in fp32 and rounds the output once.  The tcgen05 tile
+// is 128 rows for at most 16 real ones.  More rows in groups of 16 read the keys
+// again and lose to it: 256 streams of up to 2048 keys, 20 rows a head, took
+// 251 us against 137.
 // Measured: three contexts of 60000 to 100000 keys, 32 heads over 8, hd 128 in
 // bf16: 1.12 GB in 205 us (5.5 TB/s).
 // fp32 (k_paged_vec, below): 256 streams of up to 2048 keys, 8 heads of 64:
@@ -757,7 +758,6 @@ int launch_few(void (*k)(FewArgs), const FewArgs &f, unsigned grid, int threads,
     cfg.stream = st;
     cfg.attrs = &early;
     cfg.numAttrs = beside ? 1 : 0;
-    if (beside) cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
     ALTXS_LAUNCH(kKPaged, st, cudaLaunchKernelEx(&cfg, k, f));
     return ALTXS_OK;
 }

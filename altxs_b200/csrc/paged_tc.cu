@@ -28,20 +28,20 @@
 // 16-bit types: the tiles are the cache's own rows, p is rounded to the type for
 // P V (a second plane of p would double that product): the error against 64 bits
 // is 1.2 to 1.3 times the plain form's, which keeps p in fp32 and rounds the
-// output once (bf16 0.0022 and 0.0017, fp16 0.00026 and 0.00021 relative).  Warps 9 and 11 fetch every other tile, warp 10 draws and announces the
-// items and clears what must not meet a p = 0 in tiles that not every row sees
-// whole.
-// fp32: every operand is a pair of fp16 planes, hi = fp16(v 2^a) and lo =
-// fp16(v 2^a - hi), the power of two chosen per query row and per 2 KB of keys
-// and of values (per position in tiles that not every row sees whole) so that
-// the largest magnitude is at 2^14: hi + lo keeps 22 significant bits of
-// everything within 2^-18 of that magnitude, and 2^-40 of it below.  p carries
-// the values' powers, O their running largest per row.  A product is
-// hi hi + hi lo + lo hi with fp32 sums: three fp16 products instead of six with
-// bf16 planes or three at half the rate with tf32.  (An infinity has no low plane:
-// one among the keys or values that a row sees leaves it NaN.)  Warp 9 fetches raw rows to
-// a stage each for keys and values (and announces the items), warps 10 to 15
-// write the planes.
+// output once (bf16 0.0022 and 0.0017, fp16 0.00026 and 0.00021 relative).
+// Warps 9 and 11 fetch every other tile, warp 10 draws and announces the items
+// and clears what must not meet a p = 0 in tiles that not every row sees whole.
+// fp32: every operand is a pair of fp16 planes, hi = fp16(v 2^a) and lo = fp16(v
+// 2^a - hi), the power of two chosen per query row and per 2 KB of keys and of
+// values (per position in tiles that not every row sees whole) so that the
+// largest magnitude is at 2^14: hi + lo keeps 22 significant bits of everything
+// within 2^-18 of that magnitude, and 2^-40 of it below.  p carries the values'
+// powers, O their running largest per row.  A product is hi hi + hi lo + lo hi
+// with fp32 sums: three fp16 products instead of six with bf16 planes or three
+// at half the rate with tf32.  (An infinity has no low plane: one among the keys
+// or values that a row sees leaves it NaN.)  Warp 9 fetches raw rows to a stage
+// each for keys and values (and announces the items), warps 10 to 15 write the
+// planes.
 //
 // Bounds: at full tiles the softmax group's own chain (wait for S and the P V
 // before it, load and maximum, exponentials, store: about 4000 clocks for two
@@ -49,20 +49,22 @@
 // start and end (mostly cold code; with 64 channels about 4000 clocks to find
 // the first item, 2000 for the queries, 1500 for the last products and 7000 for
 // the outputs).  Items are drawn by ticket, longest first, one ahead: two or
-// three ahead the long piece took 743 us where it took 651.  (Found by every role
-// for itself instead of by one ahead of all: 5 tokens of 48 streams 35 us where
-// they took 31.)  A sequence is cut as if it were alone, so 16 streams of 8 pairs
-// are 256 items for 148 SMs, where uncut they are 128.  Pages whose size is not a multiple of 4 are fetched position by
-// position: 5 tokens of 48 streams 105 us with pages of 1 to 3, 47 with 4, 40 with
-// 8, 36 with 16 and more.
-// Measured per call: 4096 new tokens over 20000 positions, 16 heads over 8, hd 128
-// in fp16: 647 us at 1965 MHz (931 TFLOP/s), 708 us back to back, where the power
-// limit holds the SMs at 1765 MHz; nine ragged sequences of up to 1999 new tokens,
-// 16 heads over 4, bf16: 204 us (648 TFLOP/s); 5 new tokens of 48 streams in
-// windows of 1024, 16-token pages, fp16: 35 us; 64 new tokens of 16 streams over
-// windows of 2048, 8 heads of 64, fp32: 97 us.  (Of the last two 1 us is the empty
-// kernel for few rows behind this one, and in fp32 5 us more the code that it
-// drives out of the instruction cache, where nothing runs between two calls.)
+// three ahead the long piece took 743 us where it took 651.  (Found by every
+// role for itself instead of by one ahead of all: 5 tokens of 48 streams 35 us
+// where they took 31.)  A sequence is cut as if it were alone, so 16 streams of
+// 8 pairs are 256 items for 148 SMs, where uncut they are 128.  Pages whose size
+// is not a multiple of 4 are fetched position by position: 5 tokens of 48
+// streams 105 us with pages of 1 to 3, 47 with 4, 40 with 8, 36 with 16 and
+// more.
+// Measured per call: 4096 new tokens over 20000 positions, 16 heads over 8, hd
+// 128 in fp16: 647 us at 1965 MHz (931 TFLOP/s), 708 us back to back, where the
+// power limit holds the SMs at 1765 MHz; nine ragged sequences of up to 1999 new
+// tokens, 16 heads over 4, bf16: 204 us (648 TFLOP/s); 5 new tokens of 48
+// streams in windows of 1024, 16-token pages, fp16: 35 us; 64 new tokens of 16
+// streams over windows of 2048, 8 heads of 64, fp32: 97 us.  (Of the last two 1
+// us is the empty kernel for few rows behind this one, and in fp32 5 us more the
+// code that it drives out of the instruction cache, where nothing runs between
+// two calls.)
 //
 // Splits of a block go to the workspace as (m, l, O); the item that arrives
 // last joins them in split order.  Tiles, blocks and splits are functions of

@@ -16,9 +16,10 @@ reference's static cache and its encoder's multi-symbol windows
 (``StaticACEngine``, altxs ``src/xsa_ttt/incremental.py:203-1218``,
 ``run_window`` ``:1268-1290``).  All tensors of a call share one type (fp32,
 bf16 or fp16); work is enqueued on the current stream.  No call records a
-gradient (inputs that require one raise; ``rope_backward`` is ``rope``'s).  Errors of the arguments
-raise; errors of the device data (a position beyond the tables, a page out of
-range, lengths beyond their bounds) set bits that ``check_status`` raises on.
+gradient (inputs that require one raise; ``rope_backward`` is ``rope``'s).
+Errors of the arguments raise; errors of the device data (a position beyond the
+tables, a page out of range, lengths beyond their bounds) set bits that
+``check_status`` raises on.
 """
 
 from __future__ import annotations
@@ -252,8 +253,9 @@ class PagedKV:
 
     def _workspace_for(self, need: int, stream: int) -> torch.Tensor:
         """One workspace per stream, shared by the caches whose calls follow one another there and freed with the
-        last of them (a call that gives up spoils it for all of them: each then reports that).  A call that is captured has its own, from the graph's memory and cleared in
-        the graph: it lives as long as the graph does, and no other call, captured or not, meets its counters."""
+        last of them (a call that gives up spoils it for all of them: each then reports that).  A call that is
+        captured has its own, from the graph's memory and cleared in the graph: it lives as long as the graph does,
+        and no other call, captured or not, meets its counters."""
         if torch.cuda.is_current_stream_capturing():
             return _workspace(need, self.device)
         ws = self._ws.get(stream)

@@ -586,9 +586,9 @@ int altxs_paged_append(const altxs_paged_kv *kv, const altxs_chunks *c, const al
  * next one on the same stream, of any shape it is large enough for.  After
  * ALTXS_ST_TIMEOUT zero them again: until then every call that may split its rows
  * among blocks of the tensor-core kernel sets ALTXS_ST_TIMEOUT too, so caches
- * whose calls follow one another on a stream can share a workspace.  Results are finite where the inputs a row
- * sees are: NaN and infinities that its mask hides do not reach it; one that it
- * sees leaves its output infinite or NaN. */
+ * whose calls follow one another on a stream can share a workspace.  Results are
+ * finite where the inputs a row sees are: NaN and infinities that its mask hides
+ * do not reach it; one that it sees leaves its output infinite or NaN. */
 #define ALTXS_PAGED_COUNTER_BYTES 524288
 int64_t altxs_paged_attention_workspace_bytes(const altxs_paged_kv *kv, const altxs_chunks *c, int n_heads,
                                               int window);
