@@ -499,7 +499,10 @@ int altxs_split_params(const altxs_model_desc *desc, const float *params, const 
  * Types: activations and cache share one type, fp32, bf16 or fp16.  Sums, the
  * softmax's maximum and sum and the rotation are fp32, outputs rounded once at
  * the end; in the 16-bit types the probabilities are rounded to the type for
- * their product with the values.  Data errors
+ * their product with the values.  In fp32, sequences with more than 16 rows a
+ * key/value head keep 22 bits of a query, key or value within 2^-18 of the
+ * largest magnitude among its head's channels (for values: among those that a
+ * row sees), fewer below, none below 2^-40 of it.  Data errors
  * never fault: a position or a page out of range sets ALTXS_ST_BAD_POS in the
  * caller's status word (a device word, NULL = not wanted), the access is
  * skipped, and what depends on it is said at each call.  As everywhere here, the
